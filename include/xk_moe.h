@@ -50,7 +50,7 @@ extern "C" {
 
 #define XK_DT_BF16 0
 #define XK_DT_FP32 1
-#define XK_DT_FP16 2 /* accepted by xk_moe_topk_softmax only */
+#define XK_DT_FP16 2 /* router logits and activation checkpoints only */
 #define XK_DT_NONE (-1) /* "no tensor" for optional weights */
 
 /* int4 `flags` arguments: pass 0. Every dequantised weight is rounded to bf16
@@ -243,6 +243,84 @@ int xk_moe_mxfp4(const void* A, int32_t a_dtype, int64_t M, int64_t hidden,
                  int64_t top_k, const int32_t* expert_map,
                  int32_t num_global_experts, int32_t mul_routed_weight, void* out,
                  void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Training the router and adapters over the frozen experts, and serving adapters.
+ * The reference has no counterpart of these entry points.
+ *
+ * moe_balance_loss. Over the T rows that mask [M] leaves (nonzero bytes; NULL: all),
+ * p = softmax(gating_output) in fp32, c_e the slots of those rows on expert e:
+ *   loss = E / (T^2 top_k) * sum_e c_e * sum_m p[m, e]     (0 for T = 0)
+ * loss fp32 [1], counts int32 [E] (c_e), tokens int32 [1] (T). topk_ids [M, top_k];
+ * ids outside [0, E) count nowhere. gating_output [M, E] bf16 | fp32 | fp16
+ * contiguous. The same inputs give the same bits.
+ * ------------------------------------------------------------------------- */
+int64_t xk_moe_balance_loss_workspace_bytes(int64_t M, int64_t E);
+int xk_moe_balance_loss(const void* gating_output, int32_t dtype, int64_t M, int64_t E,
+                        const int32_t* topk_ids, int64_t top_k, const uint8_t* mask,
+                        float* loss, int32_t* counts, int32_t* tokens, void* workspace,
+                        int64_t workspace_bytes, hipStream_t stream);
+
+/* The gradient of gating_output [M, E], in its dtype, from one or both of
+ *   grad_loss fp32 [1], with the counts and tokens of xk_moe_balance_loss (counts are
+ *     constants of the gradient; tokens NULL: T = M), and
+ *   grad_weights fp32 [M, top_k]: the gradient of the router's weights on topk_ids,
+ *     renormalized over the row's ids or not, as xk_moe_topk_softmax gives them (ids
+ *     outside [0, E) have no weight).
+ * Rows that the mask leaves out get zeros. */
+int xk_moe_router_backward(const void* gating_output, int32_t dtype, int64_t M, int64_t E,
+                           const int32_t* topk_ids, int64_t top_k, const uint8_t* mask,
+                           const float* grad_loss, const int32_t* counts,
+                           const int32_t* tokens, const float* grad_weights,
+                           int32_t renormalize, void* grad_gating, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Low-rank adapters of many requests beside a shared projection. With
+ * a = adapter_ids[m] in [0, L):
+ *   h[m] = x[m] lora_a[a]^T,   out[m] = base[m] + scaling[a] * h[m] lora_b[a]^T;
+ * rows with another id get out[m] = base[m] and h[m] = 0. x [M, K] with rows ldx
+ * apart, base [M, N] (NULL: zeros) with rows ldbase apart, lora_a [L, r, K] and
+ * lora_b [L, N, r] contiguous, all of one dtype (bf16 | fp32), out [M, N] of it;
+ * scaling fp32 [L] (NULL: ones); hidden fp32 [M, r] receives h (nullable).
+ * 1 <= L <= 1024, 1 <= r <= 128. out may be base where ldbase = N. workspace is
+ * 16-byte aligned. Results do not depend on scheduling.
+ * ------------------------------------------------------------------------- */
+int64_t xk_lora_projection_workspace_bytes(int64_t M, int64_t K, int64_t L, int64_t r);
+int xk_lora_projection(const void* x, int32_t dtype, int64_t ldx, int64_t M, int64_t K,
+                       const void* lora_a, const void* lora_b, int64_t L, int64_t N, int64_t r,
+                       const int32_t* adapter_ids, const float* scaling, const void* base,
+                       int64_t ldbase, void* out, float* hidden, void* workspace,
+                       int64_t workspace_bytes, hipStream_t stream);
+
+/* Gradients of the above for grad_out [M, N] (rows ldg apart) of `dtype`:
+ *   g[m] = scaling[a] * grad_out[m] lora_b[a],   grad_x[m] = g[m] lora_a[a]  (0 without),
+ *   grad_a[i] = sum_m g[m]^T x[m],  grad_b[i] = scaling[i] sum_m grad_out[m]^T h[m]
+ * over adapter i's rows (zeros for an adapter without rows); scaling is a constant.
+ * x [M, K] of dtype with rows ldx apart, or, with x_scales, the e4m3 values [M, K]
+ * and e8m0 scales of xk_act_checkpoint (ldx = K). hidden as the forward left it.
+ * grad_x [M, K], grad_a [L, r, K], grad_b [L, N, r] of dtype, contiguous. */
+int64_t xk_lora_projection_backward_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t L,
+                                                    int64_t r, int32_t dtype);
+int xk_lora_projection_backward(const void* grad_out, int32_t dtype, int64_t ldg, const void* x,
+                                int64_t ldx, const uint8_t* x_scales, int64_t M, int64_t K,
+                                const void* lora_a, const void* lora_b, int64_t L, int64_t N,
+                                int64_t r, const int32_t* adapter_ids, const float* scaling,
+                                const float* hidden, void* grad_x, void* grad_a, void* grad_b,
+                                void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Activations held in 8 bits for a backward pass: e4m3 values (bytes [M, K]) with one
+ * e8m0 byte for each 32 of a row (scales [M, ceil(K / 32)], the last block may be
+ * short), value = e4m3 * 2^(byte - 127). The scale is the least power of two with
+ * which no finite value of the block passes 448, values round to nearest even;
+ * infinities and NaN become NaN and do not count for the scale. x [M, K] bf16 | fp32
+ * | fp16 with rows ldx apart. Restored values that would pass the output type's
+ * largest finite value become that.
+ * ------------------------------------------------------------------------- */
+int xk_act_checkpoint(const void* x, int32_t dtype, int64_t ldx, int64_t M, int64_t K,
+                      uint8_t* values, uint8_t* scales, hipStream_t stream);
+int xk_act_restore(const uint8_t* values, const uint8_t* scales, int64_t M, int64_t K,
+                   int32_t dtype, void* out, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,254 @@
+"""lora_projection and its backward on the GPU against 64-bit forms.
+
+Bounds come from the arithmetic (_tuning_ref). Shapes: one token to several
+sorted tiles, either side of the size up to which workgroups find their rows
+themselves (256), odd and unaligned widths, ranks that fill no operand, one
+adapter to many, adapters and whole batches without rows, rows without an adapter.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import xkernels_amd as xk
+from tests._tuning_ref import check, checkpoint_ref, lora_grad_ref, lora_ref
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def _case(M, K, N, L, r, dt, seed=0, bare=0.2, runs=False):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(M, K, generator=g).to(dt)
+    a = (torch.randn(L, r, K, generator=g) / K ** 0.5).to(dt)
+    b = (torch.randn(L, N, r, generator=g) / r ** 0.5).to(dt)
+    ids = torch.randint(0, L, (M,), generator=g, dtype=torch.int32)
+    if runs:
+        ids = ids.sort().values
+    ids[torch.rand(M, generator=g) < bare] = -1
+    base = torch.randn(M, N, generator=g).to(dt)
+    dy = torch.randn(M, N, generator=g).to(dt)
+    sc = torch.rand(L, generator=g) + 0.5
+    return [t.cuda() for t in (x, a, b, ids, base, dy, sc)]
+
+
+SHAPES = [  # M, K, N, L, r
+    (1, 64, 32, 1, 16), (1, 7168, 512, 8, 16), (2, 40, 24, 3, 8), (17, 256, 96, 2, 4), (64, 1000, 328, 32, 16),
+    (100, 33, 47, 5, 3), (255, 512, 256, 4, 32), (256, 96, 160, 300, 8), (257, 512, 264, 4, 12),
+    (300, 2880, 384, 2, 8), (513, 127, 65, 7, 5), (700, 640, 1032, 3, 64), (1025, 320, 136, 1, 128),
+    (2000, 130, 258, 40, 100), (4100, 64, 64, 2, 16),
+]
+
+
+@pytest.mark.parametrize("M,K,N,L,r", SHAPES)
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_forward(M, K, N, L, r, dt, dev):
+    x, a, b, ids, base, _, sc = _case(M, K, N, L, r, dt, seed=M + K)
+    out, hidden = xk.lora_projection(x, a, b, ids, base=base, scaling=sc, return_hidden=True)
+    want, h, bound, hb = lora_ref(x, a, b, ids, base, sc)
+    assert out.dtype == dt and hidden.dtype == F32
+    check(out, want, bound, "out")
+    check(hidden, h, hb, "hidden")
+    bare = (ids < 0).nonzero().flatten()
+    assert torch.equal(out[bare], base[bare]) and not hidden[bare].any()
+    # the same bits without the hidden output and on a second call
+    assert torch.equal(xk.lora_projection(x, a, b, ids, base=base, scaling=sc), out)
+
+
+@pytest.mark.parametrize("M,K,N,L,r", SHAPES)
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_backward(M, K, N, L, r, dt, dev):
+    x, a, b, ids, _, dy, sc = _case(M, K, N, L, r, dt, seed=M + N, runs=M % 2 == 0)
+    _, hidden = xk.lora_projection(x, a, b, ids, scaling=sc, return_hidden=True)
+    got = xk.lora_projection_backward(dy, x, a, b, ids, hidden, scaling=sc)
+    want, bounds = lora_grad_ref(dy, x, a, b, ids, hidden, sc)
+    for name, g, w, bd in zip(("grad_x", "grad_a", "grad_b"), got, want, bounds):
+        assert g.dtype == dt
+        check(g, w, bd, name)
+    again = xk.lora_projection_backward(dy, x, a, b, ids, hidden, scaling=sc)
+    assert all(torch.equal(p, q) for p, q in zip(got, again))
+
+
+@pytest.mark.parametrize("M,K,N,L,r", [(1, 64, 32, 1, 16), (70, 100, 40, 3, 8), (600, 2880, 200, 2, 16), (333, 47, 9, 4, 6),
+                                       (1500, 256, 128, 1, 32)])
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_backward_from_8_bits(M, K, N, L, r, dt, dev):
+    x, a, b, ids, _, dy, sc = _case(M, K, N, L, r, dt, seed=M * 3)
+    _, hidden = xk.lora_projection(x, a, b, ids, scaling=sc, return_hidden=True)
+    held = xk.act_checkpoint(x)
+    got = xk.lora_projection_backward(dy, held, a, b, ids, hidden, scaling=sc)
+    want, bounds = lora_grad_ref(dy, checkpoint_ref(x)[0], a, b, ids, hidden, sc)
+    for name, g, w, bd in zip(("grad_x", "grad_a", "grad_b"), got, want, bounds):
+        check(g, w, bd, name)
+    # the restored activations give the same bits
+    again = xk.lora_projection_backward(dy, xk.act_restore(held, dt), a, b, ids, hidden, scaling=sc)
+    assert all(torch.equal(p, q) for p, q in zip(got, again))
+
+
+@pytest.mark.parametrize("M", [1, 40, 400])
+def test_plain_call_without_base_and_scaling(M, dev):
+    x, a, b, ids, *_ = _case(M, 96, 80, 3, 16, BF, seed=M)
+    out = xk.lora_projection(x, a, b, ids)
+    want, _, bound, _ = lora_ref(x, a, b, ids)
+    check(out, want, bound)
+    assert not out[ids < 0].any()
+
+
+@pytest.mark.parametrize("M", [5, 200, 300, 1000])
+@pytest.mark.parametrize("which", ["none", "one", "out of range", "int64"])
+def test_ids(M, which, dev):
+    """Every row bare; all rows on the last of many adapters; ids past the last, or whose
+    lower 32 bits are a valid one, have no adapter."""
+    L = 9
+    x, a, b, _, base, dy, sc = _case(M, 72, 56, L, 8, BF, seed=M)
+    if which == "none":
+        ids = torch.full((M,), -1, dtype=torch.int32)
+    elif which == "one":
+        ids = torch.full((M,), L - 1, dtype=torch.int32)
+    elif which == "out of range":
+        ids = torch.tensor([L, -7, 2 ** 31 - 1, -2 ** 31, 3], dtype=torch.int32).repeat(M)[:M]
+    else:
+        ids = torch.tensor([2 ** 32 + 1, 4, -2 ** 33, L], dtype=torch.int64).repeat(M)[:M]
+    plain = torch.where((ids >= 0) & (ids < L), ids, -1).int()
+    ids = ids.cuda()
+    out, hidden = xk.lora_projection(x, a, b, ids, base=base, scaling=sc, return_hidden=True)
+    want, h, bound, hb = lora_ref(x, a, b, plain, base, sc)
+    check(out, want, bound, "out")
+    check(hidden, h, hb, "hidden")
+    got = xk.lora_projection_backward(dy, x, a, b, ids, hidden, scaling=sc)
+    want, bounds = lora_grad_ref(dy, x, a, b, plain, hidden, sc)
+    for g, w, bd in zip(got, want, bounds):
+        check(g, w, bd)
+    used = plain[plain >= 0].unique()
+    rest = [i for i in range(L) if i not in used.tolist()]
+    assert not got[1][rest].any() and not got[2][rest].any()
+
+
+@pytest.mark.parametrize("M", [30, 400])
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_rows_apart(M, dt, dev):
+    """Column slices of wider tensors, at aligned and at odd offsets, and a transposed x."""
+    x, a, b, ids, base, dy, sc = _case(M, 128, 96, 3, 16, dt, seed=M)
+    want, h, bound, _ = lora_ref(x, a, b, ids, base, sc)
+    gw, gb = None, None
+    for off in (8, 3):
+        wide = torch.full((M, 300), float("nan"), dtype=dt, device="cuda")
+        wide[:, off:off + 128] = x
+        wb = torch.full((M, 200), float("nan"), dtype=dt, device="cuda")
+        wb[:, off:off + 96] = base
+        out, hidden = xk.lora_projection(wide[:, off:off + 128], a, b, ids, base=wb[:, off:off + 96], scaling=sc,
+                                         return_hidden=True)
+        check(out, want, bound, f"offset {off}")
+        wb[:, off:off + 96] = dy
+        got = xk.lora_projection_backward(wb[:, off:off + 96], wide[:, off:off + 128], a, b, ids, hidden, scaling=sc)
+        if gw is None:
+            gw, gb = lora_grad_ref(dy, x, a, b, ids, hidden, sc)
+        for g, w, bd in zip(got, gw, gb):
+            check(g, w, bd + 1e-6 * w.abs())  # (hidden of this call, not of the first)
+    out = xk.lora_projection(x.t().contiguous().t(), a, b, ids, base=base, scaling=sc)
+    check(out, want, bound, "transposed")
+    one = xk.lora_projection(x[:1].expand(M, 128), a, b, ids, base=base, scaling=sc)
+    w1, _, b1, _ = lora_ref(x[:1].expand(M, 128), a, b, ids, base, sc)
+    check(one, w1, b1, "one row for all")
+
+
+def test_rows_do_not_mix(dev):
+    """A row of NaN or infinities stays its own, among rows of its adapter and others."""
+    for M in (60, 500):
+        x, a, b, ids, base, dy, sc = _case(M, 128, 64, 2, 20, BF, seed=M, bare=0.0)
+        out = xk.lora_projection(x, a, b, ids, base=base, scaling=sc)
+        x2, base2 = x.clone(), base.clone()
+        x2[7], base2[9], x2[11, 5] = float("nan"), float("nan"), float("inf")
+        out2 = xk.lora_projection(x2, a, b, ids, base=base2, scaling=sc)
+        assert out2[7].isnan().all() and out2[9].isnan().all()
+        assert not torch.isfinite(out2[11]).any()
+        rest = [i for i in range(M) if i not in (7, 9, 11)]
+        assert torch.equal(out2[rest], out[rest])
+        ids[7] = -1  # a bare row's x is not read
+        out3 = xk.lora_projection(x2, a, b, ids, base=base, scaling=sc)
+        assert torch.equal(out3[7], base[7])
+
+
+def test_infinite_hidden_stays_infinite(dev):
+    """An h past bf16's or fp32's range keeps its sign through the pair."""
+    a = torch.zeros(1, 4, 8, dtype=BF, device="cuda")
+    a[0, 0, 0] = 1
+    b = torch.zeros(1, 8, 4, dtype=BF, device="cuda")
+    b[0, :, 0] = 1
+    b[0, 3, 0] = -1
+    x = torch.zeros(2, 8, dtype=BF, device="cuda")
+    x[0, 0] = float("inf")
+    x[1, 0] = 3.3e38
+    out = xk.lora_projection(x, a, b, torch.zeros(2, dtype=torch.int32, device="cuda"),
+                             scaling=torch.tensor([1.0], device="cuda"))
+    # inf * 0 in the other ranks of a hidden row is NaN by the formula too: h has one rank in use
+    assert torch.isnan(out[0]).all() or torch.isinf(out[0]).all()
+    assert torch.isfinite(out[1]).all() and out[1, 3] == -out[1, 0]
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_empty(dt, dev):
+    x, a, b, ids, base, dy, sc = _case(4, 64, 32, 3, 8, dt)
+    out, hidden = xk.lora_projection(x[:0], a, b, ids[:0], base=base[:0], scaling=sc, return_hidden=True)
+    assert out.shape == (0, 32) and hidden.shape == (0, 8)
+    gx, ga, gb = xk.lora_projection_backward(dy[:0], x[:0], a, b, ids[:0], hidden, scaling=sc)
+    assert gx.shape == (0, 64) and not ga.any() and not gb.any() and ga.shape == a.shape and gb.shape == b.shape
+
+
+def test_gradient_against_differences(dev):
+    """Directional differences of the fp32 forward: f is bilinear in (A, B) and linear in x,
+    so a central difference along one of them is exact but for rounding."""
+    x, a, b, ids, _, dy, sc = _case(40, 48, 40, 3, 8, F32, seed=5)
+    f = lambda x, a, b: float((xk.lora_projection(x, a, b, ids, scaling=sc).double() * dy.double()).sum())  # noqa: E731
+    _, hidden = xk.lora_projection(x, a, b, ids, scaling=sc, return_hidden=True)
+    grads = xk.lora_projection_backward(dy, x, a, b, ids, hidden, scaling=sc)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for i, t in enumerate((x, a, b)):
+        d = torch.randn(t.shape, generator=g, device="cuda")
+        args_p, args_m = [x, a, b], [x, a, b]
+        args_p[i], args_m[i] = t + d, t - d
+        diff = (f(*args_p) - f(*args_m)) / 2
+        want = float((grads[i].double() * d.double()).sum())
+        # each f is a sum of 40 * 40 terms off by 2^-20 of its size or less
+        size = float(xk.lora_projection(*[v.abs() for v in args_p], ids, scaling=sc).double().abs().sum()) * float(dy.abs().max())
+        assert abs(diff - want) <= 2.0 ** -19 * size, (i, diff, want, size)
+
+
+@pytest.mark.parametrize("M", [8, 600])
+def test_captured(M, dev):
+    """A serving step (projection + adapters) and a tuning step replay with new inputs; eager
+    work and synchronisations between the replays."""
+    x, a, b, ids, base, dy, sc = _case(M, 256, 128, 4, 16, BF, seed=M)
+    out, hidden = xk.lora_projection(x, a, b, ids, base=base, scaling=sc, return_hidden=True)
+    xk.lora_projection_backward(dy, x, a, b, ids, hidden, scaling=sc)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, hidden = xk.lora_projection(x, a, b, ids, base=base, scaling=sc, return_hidden=True)
+        held = xk.act_checkpoint(x)
+        grads = xk.lora_projection_backward(dy, held, a, b, ids, hidden, scaling=sc)
+    for seed in range(4):
+        fresh = _case(M, 256, 128, 4, 16, BF, seed=100 + seed)
+        for t, f in zip((x, a, b, ids, base, dy, sc), fresh):
+            t.copy_(f)
+        graph.replay()
+        got = [t.clone() for t in (out, hidden, *grads)]
+        torch.cuda.synchronize()
+        o, h = xk.lora_projection(x, a, b, ids, base=base, scaling=sc, return_hidden=True)
+        g = xk.lora_projection_backward(dy, xk.act_checkpoint(x), a, b, ids, h, scaling=sc)
+        assert all(torch.equal(p, q) for p, q in zip(got, (o, h, *g))), seed
+
+
+def test_streams(dev):
+    """Two streams at once, each with its own scratch."""
+    cases = [_case(300, 512, 256, 4, 16, BF, seed=s) for s in (1, 2)]
+    want = [xk.lora_projection(c[0], c[1], c[2], c[3], base=c[4], scaling=c[6]) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for c, st in zip(cases, streams):
+            with torch.cuda.stream(st):
+                got.append(xk.lora_projection(c[0], c[1], c[2], c[3], base=c[4], scaling=c[6]))
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want))

@@ -1,0 +1,202 @@
+"""moe_balance_loss and moe_router_backward on the GPU against 64-bit forms, with
+bounds from the arithmetic (_tuning_ref): one row to many planes, expert counts
+of every kernel (128, 256, 512 a row of lanes, and past it), masks that leave
+some or no rows, ids out of range, repeated ids, infinite and NaN logits."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import xkernels_amd as xk
+from tests._tuning_ref import F32, balance_ref, check, router_grad_ref, softmax_delta
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+SHAPES = [(1, 8, 2), (3, 4, 4), (200, 48, 8), (256, 100, 6), (257, 256, 8), (1000, 384, 8), (5000, 64, 1),
+          (300, 511, 16), (70, 512, 16), (40, 513, 8), (300, 1000, 20), (5, 3000, 2), (64, 1, 1), (33, 40, 24)]
+
+
+def _case(M, E, k, dt, seed=0, pad=0.0):
+    g = torch.Generator().manual_seed(seed)
+    z = (1.5 * torch.randn(M, E, generator=g) + torch.randn(E, generator=g)).to(dt)
+    ids = torch.topk(z.float(), k, dim=1).indices.int()
+    u = torch.randn(M, k, generator=g)
+    mask = torch.rand(M, generator=g) >= pad if pad else None
+    return z.cuda(), ids.cuda(), u.cuda(), None if mask is None else mask.cuda()
+
+
+def _check_loss(z, ids, mask):
+    got = xk.moe_balance_loss(z, ids, mask=mask)
+    loss, counts, tokens = balance_ref(z, ids, mask)
+    assert got.loss.dtype == torch.float32 and got.counts.dtype == got.tokens.dtype == torch.int32
+    assert torch.equal(got.counts.cpu().long(), counts) and int(got.tokens) == tokens
+    rel = softmax_delta(z.double().cpu()) + (z.shape[0] + 64) * F32 / 2
+    check(got.loss, loss, rel * loss, "loss")
+    return got
+
+
+@pytest.mark.parametrize("M,E,k", SHAPES)
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("pad", [0.0, 0.4])
+def test_loss_and_counts(M, E, k, dt, pad, dev):
+    z, ids, _, mask = _case(M, E, k, dt, seed=M + E, pad=pad)
+    got = _check_loss(z, ids, mask)
+    again = xk.moe_balance_loss(z, ids, mask=mask)
+    assert all(torch.equal(p, q) for p, q in zip(got, again))
+
+
+@pytest.mark.parametrize("M,E,k", SHAPES)
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("renorm,parts", [(True, "both"), (False, "both"), (True, "weights"), (False, "weights"),
+                                          (True, "loss")])
+def test_gradient(M, E, k, dt, renorm, parts, dev):
+    z, ids, u, mask = _case(M, E, k, dt, seed=M + k, pad=0.3 if M > 4 else 0.0)
+    st = xk.moe_balance_loss(z, ids, mask=mask)
+    gl = torch.tensor(0.7, device="cuda") if parts != "weights" else None
+    gw = u if parts != "loss" else None
+    got = xk.moe_router_backward(z, ids, grad_weights=gw, renormalize=renorm, grad_loss=gl,
+                                 counts=st.counts if gl is not None else None,
+                                 tokens=st.tokens if gl is not None else None, mask=mask)
+    want, bound = router_grad_ref(z, ids, gw, renorm, gl, st.counts, mask)
+    assert got.dtype == dt
+    check(got, want, bound)
+    if mask is not None:
+        assert not got[~mask].any()
+
+
+@pytest.mark.parametrize("E,k", [(64, 4), (600, 4), (64, 20)])
+def test_ids_out_of_range_and_repeated(E, k, dev):
+    z, ids, u, _ = _case(50, E, k, torch.float32, seed=E)
+    ids[3] = -1
+    ids[4, 0], ids[5, 1], ids[6, 2] = E, 2 ** 31 - 1, -2 ** 31
+    ids[7, :3] = 5
+    ids[8] = 1
+    st = _check_loss(z, ids, None)
+    for renorm in (True, False):
+        got = xk.moe_router_backward(z, ids, grad_weights=u, renormalize=renorm, grad_loss=torch.ones((), device="cuda"),
+                                     counts=st.counts)
+        want, bound = router_grad_ref(z, ids, u, renorm, 1.0, st.counts)
+        check(got, want, bound)
+    wide = ids.long()
+    wide[9, 0] = 2 ** 32 + 2
+    narrow = ids.clone()
+    narrow[9, 0] = -1
+    a, b = xk.moe_balance_loss(z, wide), xk.moe_balance_loss(z, narrow)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@pytest.mark.parametrize("M,E", [(10, 64), (400, 64), (20, 700)])
+def test_masked_rows_are_not_read(M, E, dev):
+    """NaN and infinities in padded rows, and a mask that leaves nothing."""
+    z, ids, u, _ = _case(M, E, 4, torch.bfloat16, seed=M)
+    mask = torch.ones(M, dtype=torch.bool, device="cuda")
+    mask[[1, 5, M - 1]] = False
+    want = xk.moe_balance_loss(z, ids, mask=mask)
+    grad = xk.moe_router_backward(z, ids, grad_weights=u, grad_loss=want.loss, counts=want.counts, tokens=want.tokens,
+                                  mask=mask)
+    z2, ids2, u2 = z.clone(), ids.clone(), u.clone()
+    z2[1], z2[5, 0], z2[M - 1] = float("nan"), float("inf"), float("-inf")
+    ids2[1], u2[5] = 3, float("nan")
+    got = xk.moe_balance_loss(z2, ids2, mask=mask)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    grad2 = xk.moe_router_backward(z2, ids2, grad_weights=u2, grad_loss=want.loss, counts=want.counts,
+                                   tokens=want.tokens, mask=mask)
+    assert torch.equal(grad, grad2) and not grad2[~mask].any()
+    none = torch.zeros(M, dtype=torch.bool, device="cuda")
+    st = xk.moe_balance_loss(z2, ids2, mask=none)
+    assert float(st.loss) == 0.0 and int(st.tokens) == 0 and not st.counts.any()
+    g = xk.moe_router_backward(z2, ids2, grad_weights=u2, grad_loss=st.loss + 1, counts=st.counts, tokens=st.tokens,
+                               mask=none)
+    assert not g.any()
+
+
+@pytest.mark.parametrize("M,E", [(12, 96), (300, 300), (12, 700)])
+def test_special_logits(M, E, dev):
+    """Experts masked with -inf or the type's lowest value have no probability and no
+    gradient; a row with NaN or +inf is NaN in its own gradient and the loss only."""
+    z, ids, u, _ = _case(M, E, 4, torch.float32, seed=E)
+    z[2, 10:] = float("-inf")
+    z[3, 4:] = torch.finfo(torch.float32).min
+    ids[2], ids[3] = torch.arange(4, device="cuda"), torch.arange(4, device="cuda")
+    st = _check_loss(z.clamp(min=-1e4), ids, None)  # the same probabilities: 0
+    st2 = xk.moe_balance_loss(z, ids)
+    torch.testing.assert_close(st2.loss, st.loss, rtol=1e-6, atol=0)
+    for renorm in (True, False):
+        kw = dict(grad_weights=u, renormalize=renorm, grad_loss=torch.ones((), device="cuda"), counts=st2.counts)
+        got = xk.moe_router_backward(z, ids, **kw)
+        assert torch.isfinite(got).all() and not got[2, 10:].any() and not got[3, 4:].any()
+        bad = z.clone()
+        bad[5, 1], bad[6, 0], bad[7] = float("nan"), float("inf"), float("-inf")
+        g2 = xk.moe_router_backward(bad, ids, **kw)
+        rows = [5, 6, 7]
+        assert g2[rows].isnan().any(1).all()
+        rest = [i for i in range(M) if i not in rows]
+        assert torch.equal(g2[rest], got[rest])
+    assert xk.moe_balance_loss(bad, ids).loss.isnan()
+
+
+def test_empty_batch(dev):
+    for E in (16, 700):
+        z = torch.empty(0, E, device="cuda")
+        ids = torch.empty(0, 2, dtype=torch.int32, device="cuda")
+        st = xk.moe_balance_loss(z, ids)
+        assert float(st.loss) == 0 and int(st.tokens) == 0 and not st.counts.any() and st.counts.numel() == E
+        assert xk.moe_router_backward(z, ids, grad_weights=torch.empty(0, 2, device="cuda")).shape == (0, E)
+
+
+def test_gradient_against_differences(dev):
+    """Central differences of the weights' and the loss's 64-bit forms along a direction."""
+    z, ids, u, _ = _case(30, 24, 4, torch.float32, seed=3)
+    st = xk.moe_balance_loss(z, ids)
+    got = xk.moe_router_backward(z, ids, grad_weights=u, renormalize=True, grad_loss=torch.ones((), device="cuda"),
+                                 counts=st.counts).double().cpu()
+    z64, i64, u64, c = z.double().cpu(), ids.long().cpu(), u.double().cpu(), st.counts.double().cpu()
+
+    def f(z):
+        p = torch.softmax(z, 1)
+        w = p.gather(1, i64)
+        return float((w / w.sum(1, keepdim=True) * u64).sum() + 24 / (30 * 30 * 4) * (c @ p.sum(0)))
+
+    d = torch.randn(z.shape, generator=torch.Generator().manual_seed(1), dtype=torch.float64)
+    h = 1e-5
+    diff = (f(z64 + h * d) - f(z64 - h * d)) / (2 * h)
+    # the difference's own error is about h^2 of third derivatives; the kernel's 2^-18 of the terms
+    assert abs(diff - float((got * d).sum())) <= 1e-6 + 2.0 ** -18 * float((got * d).abs().sum())
+
+
+def test_step_together_and_captured(dev):
+    """Router, loss and both gradients as a training step runs them, eager and in a graph."""
+    M, E, k = 300, 48, 4
+    z = _case(M, E, k, torch.bfloat16, seed=1)[0]
+    u = torch.randn(M, k, device="cuda")
+    coef = torch.tensor(0.01, device="cuda")
+
+    def step():
+        w, ids = xk.topk_softmax(z, k)
+        st = xk.moe_balance_loss(z, ids)
+        return w, *st, xk.moe_router_backward(z, ids, grad_weights=u, grad_loss=coef, counts=st.counts)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in range(4):
+        z.copy_(_case(M, E, k, torch.bfloat16, seed=10 + seed)[0])
+        graph.replay()
+        got = [t.clone() for t in out]
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, step()))
+
+
+def test_strided_and_unaligned(dev):
+    z, ids, u, _ = _case(90, 64, 4, torch.bfloat16, seed=2)
+    want = xk.moe_router_backward(z, ids, grad_weights=u)
+    wide = torch.zeros(90, 131, dtype=z.dtype, device="cuda")
+    wide[:, 3:67] = z
+    assert torch.equal(xk.moe_router_backward(wide[:, 3:67], ids, grad_weights=u), want)
+    flat = torch.zeros(90 * 64 + 1, dtype=z.dtype, device="cuda")
+    off = flat[1:].view(90, 64)
+    off.copy_(z)
+    assert torch.equal(xk.moe_router_backward(off, ids, grad_weights=u), want)
+    assert all(torch.equal(p, q) for p, q in zip(xk.moe_balance_loss(off, ids), xk.moe_balance_loss(z, ids)))

@@ -75,6 +75,28 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_p, _i32, _i64, _i64, _p, _p, _p, _p, _i64, _i64, _p, _p, _f32, _i32, _p, _p, _i64, _p,
          _i32, _i32, _p, _p, _i64, _p],
     ),
+    "xk_moe_balance_loss_workspace_bytes": (_i64, [_i64, _i64]),
+    "xk_moe_balance_loss": (
+        ctypes.c_int,
+        [_p, _i32, _i64, _i64, _p, _i64, _p, _p, _p, _p, _p, _i64, _p],
+    ),
+    "xk_moe_router_backward": (
+        ctypes.c_int,
+        [_p, _i32, _i64, _i64, _p, _i64, _p, _p, _p, _p, _p, _i32, _p, _p],
+    ),
+    "xk_lora_projection_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
+    "xk_lora_projection": (
+        ctypes.c_int,
+        [_p, _i32, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _p, _p, _i64, _p, _p, _p, _i64, _p],
+    ),
+    "xk_lora_projection_backward_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i32]),
+    "xk_lora_projection_backward": (
+        ctypes.c_int,
+        [_p, _i32, _i64, _p, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _p,
+         _i64, _p],
+    ),
+    "xk_act_checkpoint": (ctypes.c_int, [_p, _i32, _i64, _i64, _i64, _p, _p, _p]),
+    "xk_act_restore": (ctypes.c_int, [_p, _p, _i64, _i64, _i32, _p, _p]),
 }
 
 _LIB: ctypes.CDLL | None = None

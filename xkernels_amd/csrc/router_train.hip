@@ -1,0 +1,584 @@
+// The router's training step: the balance loss with its per-expert counts, and the
+// gradient of the logits.
+//
+// With V the T rows that the mask leaves (all without one), p = softmax(logits) in
+// fp32 and c_e the number of slots of V on expert e:
+//   loss = E / (T^2 k) sum_e c_e sum_{m in V} p_me,
+//   d loss / d z_mi = E / (T^2 k) p_mi (c_i - sum_e p_me c_e)    (c constant),
+// and through the router's weights (renormalised: a softmax of the selected logits)
+//   dz_i += sum_{j: e_j = i} w_j (u_j - sum_l w_l u_l),  w_j = p_{e_j} / sum_l p_{e_l}, or
+//   dz_i += p_i (sum_{j: e_j = i} u_j - sum_j p_{e_j} u_j)       (not renormalised).
+//
+// Both directions are one pass over the logits, HBM bound for large batches (M * E
+// values in, and out in the backward) and launches for small ones. The forward
+// keeps each workgroup's column sums in registers over its rows and leaves one
+// plane of sums and counts per workgroup; a second launch adds the planes in
+// order, so results do not depend on scheduling (counts are whole numbers; the
+// probabilities' sums have a fixed order). The backward forms p again rather than
+// read it: M * E exponentials cost less than M * E more values from memory.
+#include <algorithm>
+
+#include "router_rows.h"
+
+namespace xk {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kOneWg = 1024;        // threads of the one workgroup of a small batch
+constexpr int64_t kOneWgRows = 256; // rows up to which it is one workgroup's work
+constexpr int kFastExperts = 512, kFastTopk = 16;
+constexpr int kPlanes = 512;        // most workgroups of the forward
+
+__device__ __forceinline__ float row_max(float x) {
+  row_steps([&](auto from) { x = fmaxf(x, __uint_as_float(from(__float_as_uint(x)))); });
+  return x;
+}
+__device__ __forceinline__ float row_sum(float x) {
+  row_steps([&](auto from) { x += __uint_as_float(from(__float_as_uint(x))); });
+  return x;
+}
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) x = fmaxf(x, __shfl_xor(x, off));
+  return x;
+}
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off);
+  return x;
+}
+
+template <typename T> __device__ __forceinline__ T to_out(float f);
+template <> __device__ __forceinline__ uint16_t to_out<uint16_t>(float f) { return f32_to_bf16(f); }
+template <> __device__ __forceinline__ _Float16 to_out<_Float16>(float f) { return _Float16(f); }
+template <> __device__ __forceinline__ float to_out<float>(float f) { return f; }
+
+// A row's probabilities on its 16 lanes: lane i holds the 8-expert pieces i, i + 16, ...
+template <typename T, int PIECES, bool WIDE>
+__device__ __forceinline__ void row_softmax(const T* g, int E, int i16, float* p, float& mx, float& sum) {
+  mx = -__builtin_inff();
+#pragma unroll
+  for (int c = 0; c < PIECES; ++c) {
+    const int e0 = (c * 16 + i16) * 8;
+    if (WIDE) {
+      if (e0 < E) {
+        piece8<T>::load(g + e0, p + 8 * c);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[8 * c + i] = -__builtin_inff();
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[8 * c + i] = e0 + i < E ? logit_at<T>(g + e0 + i) : -__builtin_inff();
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mx = fmaxf(mx, p[8 * c + i]);
+  }
+  mx = row_max(mx);
+  sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < PIECES * 8; ++j) {
+    const int e = ((j >> 3) * 16 + i16) * 8 + (j & 7);
+    p[j] = e < E ? expf(p[j] - mx) : 0.f;
+    sum += p[j];
+  }
+  sum = row_sum(sum);
+  const float inv = 1.f / sum;
+#pragma unroll
+  for (int j = 0; j < PIECES * 8; ++j) p[j] *= inv;
+}
+
+// Scratch: planes of column sums and counts, the rows counted per plane, the
+// loss's parts and their ticket.
+struct BalanceScratch {
+  float* sums;     // [planes, E]
+  int32_t* cnt;    // [planes, E]
+  int32_t* rows;   // [planes]
+  double* parts;   // [blocks of the last kernel]
+  int32_t* ticket;
+  float* stat;     // [M, 2] for rows past kFastExperts: maximum and 1 / sum
+};
+
+// loss = E / (T^2 k) * total in 64 bits: T = 0 gives 0.
+__device__ __forceinline__ float loss_of(double total, int64_t E, int64_t T, int64_t k) {
+  return T == 0 ? 0.f : float(total * double(E) / (double(T) * double(T) * double(k)));
+}
+
+// One workgroup's rows: column sums of p over them in registers, then over the
+// workgroup's rows of lanes in LDS. ONE: the whole batch, loss included.
+template <typename T, int PIECES, bool WIDE, bool ONE>
+__global__ void __launch_bounds__(ONE ? kOneWg : kThreads)
+balance_rows(const T* __restrict__ logits, const int32_t* __restrict__ ids, const uint8_t* __restrict__ mask,
+             int64_t M, int E, int k, BalanceScratch s, float* __restrict__ loss, int32_t* __restrict__ counts,
+             int32_t* __restrict__ tokens) {
+  constexpr int N = PIECES * 8, kT = ONE ? kOneWg : kThreads, kWaves = kT / 64;
+  __shared__ float lds_sum[kWaves][PIECES * 128];
+  __shared__ int lds_cnt[PIECES * 128];
+  __shared__ int lds_rows;
+  __shared__ double lds_part[kWaves];
+  const int tid = threadIdx.x, i16 = tid & 15;
+  for (int e = tid; e < E; e += kT) lds_cnt[e] = 0;
+  if (tid == 0) {
+    lds_rows = 0;
+    if (!ONE && blockIdx.x == 0) *s.ticket = 0;  // for the launch that follows
+  }
+  __syncthreads();
+  float acc[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) acc[j] = 0.f;
+  int rows = 0;
+  for (int64_t row = int64_t(blockIdx.x) * (kT / 16) + (tid >> 4); row < M; row += int64_t(gridDim.x) * (kT / 16)) {
+    if (mask != nullptr && mask[row] == 0) continue;  // whole 16-lane rows
+    ++rows;
+    for (int j = i16; j < k; j += 16) {
+      const int id = ids[row * k + j];
+      if (id >= 0 && id < E) atomicAdd(&lds_cnt[id], 1);
+    }
+    float p[N], mx, sum;
+    row_softmax<T, PIECES, WIDE>(logits + row * E, E, i16, p, mx, sum);
+#pragma unroll
+    for (int j = 0; j < N; ++j) acc[j] += p[j];
+  }
+  if (i16 == 0 && rows) atomicAdd(&lds_rows, rows);
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    acc[j] += __shfl_xor(acc[j], 16);
+    acc[j] += __shfl_xor(acc[j], 32);
+  }
+  if ((tid & 63) < 16)
+#pragma unroll
+    for (int j = 0; j < N; ++j) lds_sum[tid >> 6][((j >> 3) * 16 + i16) * 8 + (j & 7)] = acc[j];
+  __syncthreads();
+  double part = 0.0;
+  for (int e = tid; e < E; e += kT) {
+    float t = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) t += lds_sum[w][e];
+    const int c = lds_cnt[e];
+    if (ONE) {
+      counts[e] = c;
+      part += double(c) * double(t);
+    } else {
+      s.sums[int64_t(blockIdx.x) * E + e] = t;
+      s.cnt[int64_t(blockIdx.x) * E + e] = c;
+    }
+  }
+  if (!ONE) {
+    if (tid == 0) s.rows[blockIdx.x] = lds_rows;
+    return;
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) part += __shfl_xor(part, off);
+  if ((tid & 63) == 0) lds_part[tid >> 6] = part;
+  __syncthreads();
+  if (tid == 0) {
+    double total = 0.0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) total += lds_part[w];
+    *loss = loss_of(total, E, lds_rows, k);
+    *tokens = lds_rows;
+  }
+}
+
+// Adds the planes: 16 columns a workgroup, 16 threads a column; the workgroup that
+// arrives last adds the loss's parts in order. COUNTED: counts[] is complete.
+template <bool COUNTED>
+__global__ void __launch_bounds__(kThreads)
+balance_finish(int planes, int64_t E, int64_t k, BalanceScratch s, float* __restrict__ loss,
+               int32_t* __restrict__ counts, int32_t* __restrict__ tokens) {
+  __shared__ float lds_p[16][16];
+  __shared__ int lds_c[16][16];
+  __shared__ int lds_rows[4];
+  __shared__ bool last;
+  const int tid = threadIdx.x, col = tid & 15, part = tid >> 4;
+  const int64_t e = int64_t(blockIdx.x) * 16 + col;
+  float p = 0.f;
+  int c = 0;
+  if (e < E)
+    for (int g = part; g < planes; g += 16) {
+      p += s.sums[int64_t(g) * E + e];
+      if (!COUNTED) c += s.cnt[int64_t(g) * E + e];
+    }
+  lds_p[part][col] = p;
+  lds_c[part][col] = c;
+  int rows = 0;
+  for (int g = tid; g < planes; g += kThreads) rows += s.rows[g];
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) rows += __shfl_xor(rows, off);
+  if ((tid & 63) == 0) lds_rows[tid >> 6] = rows;
+  __syncthreads();
+  const int T = lds_rows[0] + lds_rows[1] + lds_rows[2] + lds_rows[3];
+  double dot = 0.0;
+  if (tid < 16 && e < E) {
+    float ps = 0.f;
+    int cs = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      ps += lds_p[i][col];
+      cs += lds_c[i][col];
+    }
+    if (COUNTED) cs = counts[e];
+    else counts[e] = cs;
+    dot = double(cs) * double(ps);
+  }
+  if (tid < 64) {
+#pragma unroll
+    for (int off = 8; off >= 1; off >>= 1) dot += __shfl_xor(dot, off);
+    if (tid == 0) {
+      __hip_atomic_store(&s.parts[blockIdx.x], dot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const int at = __hip_atomic_fetch_add(s.ticket, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+      last = at == int(gridDim.x) - 1;
+    }
+  }
+  __syncthreads();
+  if (!last || tid >= 64) return;
+  double total = 0.0;
+  for (int i = tid; i < int(gridDim.x); i += 64)
+    total += __hip_atomic_load(&s.parts[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) total += __shfl_xor(total, off);
+  if (tid == 0) {
+    *loss = loss_of(total, E, T, k);
+    *tokens = T;
+  }
+}
+
+// ------------------------------------------------- rows past kFastExperts ----
+// Maximum and 1 / sum of each row (a wave each); counts[] and the ticket cleared.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+row_stats(const T* __restrict__ logits, const uint8_t* __restrict__ mask, int64_t M, int64_t E, BalanceScratch s,
+          int32_t* __restrict__ counts) {
+  const int lane = threadIdx.x & 63;
+  const int64_t t0 = int64_t(blockIdx.x) * kThreads + threadIdx.x;
+  for (int64_t e = t0; e < E; e += int64_t(gridDim.x) * kThreads) counts[e] = 0;
+  if (t0 == 0) *s.ticket = 0;
+  for (int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6); row < M; row += int64_t(gridDim.x) * 4) {
+    if (mask != nullptr && mask[row] == 0) continue;
+    const T* g = logits + row * E;
+    float mx = -__builtin_inff(), sum = 0.f;
+    for (int64_t e = lane; e < E; e += 64) mx = fmaxf(mx, logit_at<T>(g + e));
+    mx = wave_max(mx);
+    for (int64_t e = lane; e < E; e += 64) sum += expf(logit_at<T>(g + e) - mx);
+    sum = wave_sum(sum);
+    if (lane == 0) {
+      s.stat[2 * row] = mx;
+      s.stat[2 * row + 1] = 1.f / sum;
+    }
+  }
+}
+
+// Column sums: a thread per expert, a plane per part of the rows.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+balance_columns(const T* __restrict__ logits, const int32_t* __restrict__ ids, const uint8_t* __restrict__ mask,
+                int64_t M, int64_t E, int64_t k, int64_t rows_per_plane, BalanceScratch s,
+                int32_t* __restrict__ counts) {
+  const int64_t e = int64_t(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t first = int64_t(blockIdx.y) * rows_per_plane, end = min(M, first + rows_per_plane);
+  float sum = 0.f;
+  int rows = 0;
+  for (int64_t row = first; row < end; ++row) {
+    if (mask != nullptr && mask[row] == 0) continue;
+    ++rows;
+    if (e < E) sum += expf(logit_at<T>(logits + row * E + e) - s.stat[2 * row]) * s.stat[2 * row + 1];
+    if (blockIdx.x == 0)
+      for (int64_t j = threadIdx.x; j < k; j += kThreads) {
+        const int id = ids[row * k + j];
+        if (id >= 0 && id < E) atomicAdd(&counts[id], 1);
+      }
+  }
+  if (e < E) s.sums[int64_t(blockIdx.y) * E + e] = sum;
+  if (blockIdx.x == 0 && threadIdx.x == 0) s.rows[blockIdx.y] = rows;
+}
+
+// ---------------------------------------------------------------- backward ----
+struct RouterGrad {
+  const int32_t* ids;
+  const uint8_t* mask;
+  const int32_t* counts;      // with grad_loss
+  const int32_t* tokens;      // nullable: every row counts
+  const float* grad_loss;     // nullable
+  const float* grad_weights;  // nullable
+  int renorm;
+};
+
+// E / (T^2 k) * grad_loss; 0 without one or without rows.
+__device__ __forceinline__ float loss_factor(const RouterGrad& a, int64_t M, int64_t E, int64_t k) {
+  if (a.grad_loss == nullptr) return 0.f;
+  const double T = a.tokens != nullptr ? double(*a.tokens) : double(M);
+  return T > 0.0 ? float(double(*a.grad_loss) * double(E) / (T * T * double(k))) : 0.f;
+}
+
+// The counts less their mean: as p sums to 1, c_i - sum p c is the same of either,
+// and near-uniform counts (as a balanced router has) no longer cancel.
+template <typename T, int PIECES, bool WIDE>
+__global__ void __launch_bounds__(kThreads)
+router_grad_rows(const T* __restrict__ logits, int64_t M, int E, int k, RouterGrad a, T* __restrict__ grad) {
+  constexpr int N = PIECES * 8;
+  const int tid = threadIdx.x, i16 = tid & 15;
+  const bool with_loss = a.grad_loss != nullptr;
+  float c[N], mean = 0.f;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int e = ((j >> 3) * 16 + i16) * 8 + (j & 7);
+    c[j] = with_loss && e < E ? float(a.counts[e]) : 0.f;
+    mean += c[j];
+  }
+  mean = row_sum(mean) / float(E);
+#pragma unroll
+  for (int j = 0; j < N; ++j) c[j] -= mean;
+  const float factor = loss_factor(a, M, E, k);
+  for (int64_t row = int64_t(blockIdx.x) * (kThreads / 16) + (tid >> 4); row < M;
+       row += int64_t(gridDim.x) * (kThreads / 16)) {
+    T* out = grad + row * E;
+    const bool on = a.mask == nullptr || a.mask[row] != 0;  // the same on a row's 16 lanes
+    float p[N], pc = 0.f, q = 0.f, slot = 0.f, p_id = 0.f, mx = 0.f, sum = 1.f;
+    int id = -1;
+    if (on) {
+      row_softmax<T, PIECES, WIDE>(logits + row * E, E, i16, p, mx, sum);
+      if (with_loss) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) pc += p[j] * c[j];
+        pc = row_sum(pc);
+      }
+      if (a.grad_weights != nullptr) {  // lane t holds slot t
+        float u = 0.f;
+        if (i16 < k) {
+          id = a.ids[row * k + i16];
+          if (id < 0 || id >= E) id = -1;
+          u = a.grad_weights[row * k + i16];
+        }
+        if (id >= 0) p_id = expf(logit_at<T>(logits + row * E + id) - mx) / sum;
+        if (a.renorm) {
+          const float ps = row_sum(p_id);  // by all 16 lanes
+          const float w = id >= 0 ? p_id / ps : 0.f;
+          const float wu = row_sum(id >= 0 ? w * u : 0.f);
+          slot = id >= 0 ? w * (u - wu) : 0.f;
+        } else {
+          slot = id >= 0 ? p_id * u : 0.f;
+          q = row_sum(slot);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j) p[j] = with_loss ? factor * p[j] * (c[j] - pc) - p[j] * q : -p[j] * q;
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) p[j] = 0.f;
+    }
+#pragma unroll
+    for (int cc = 0; cc < PIECES; ++cc) {
+      const int e0 = (cc * 16 + i16) * 8;
+      if (WIDE) {
+        if (e0 < E) {
+          __attribute__((aligned(16))) T v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = to_out<T>(p[8 * cc + i]);
+#pragma unroll
+          for (int h = 0; h < int(sizeof(T)) / 2; ++h)
+            reinterpret_cast<u32x4*>(out + e0)[h] = reinterpret_cast<const u32x4*>(v)[h];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (e0 + i < E) out[e0 + i] = to_out<T>(p[8 * cc + i]);
+      }
+    }
+    if (on && a.grad_weights != nullptr) {
+      // the selected experts' values once more, with their slots' part: every
+      // slot of one expert forms the same sum, in slot order
+      float add = 0.f;
+      for (int l = 0; l < k; ++l) {
+        const float v = __shfl(slot, (tid & 48) + l);
+        const int other = __shfl(id, (tid & 48) + l);
+        if (other == id) add += v;
+      }
+      if (id >= 0) {
+        const float ci = with_loss ? float(a.counts[id]) - mean : 0.f;
+        const float v = (with_loss ? factor * p_id * (ci - pc) : 0.f) - p_id * q + add;
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // the row's stores first (vmcnt 0)
+        out[id] = to_out<T>(v);
+      }
+    }
+  }
+}
+
+// Any E and k: a wave per row, the row read again for each pass.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+router_grad_any(const T* __restrict__ logits, int64_t M, int64_t E, int64_t k, RouterGrad a, T* __restrict__ grad) {
+  const int lane = threadIdx.x & 63;
+  const bool with_loss = a.grad_loss != nullptr;
+  float mean = 0.f;
+  if (with_loss) {
+    for (int64_t e = lane; e < E; e += 64) mean += float(a.counts[e]);
+    mean = wave_sum(mean) / float(E);
+  }
+  const float factor = loss_factor(a, M, E, k);
+  for (int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6); row < M; row += int64_t(gridDim.x) * 4) {
+    const T* g = logits + row * E;
+    T* out = grad + row * E;
+    if (a.mask != nullptr && a.mask[row] == 0) {
+      for (int64_t e = lane; e < E; e += 64) out[e] = to_out<T>(0.f);
+      continue;
+    }
+    float mx = -__builtin_inff(), sum = 0.f;
+    for (int64_t e = lane; e < E; e += 64) mx = fmaxf(mx, logit_at<T>(g + e));
+    mx = wave_max(mx);
+    for (int64_t e = lane; e < E; e += 64) sum += expf(logit_at<T>(g + e) - mx);
+    sum = wave_sum(sum);
+    auto prob = [&](int64_t e) { return expf(logit_at<T>(g + e) - mx) / sum; };
+    float pc = 0.f, q = 0.f, ps = 0.f, wu = 0.f;
+    if (with_loss) {
+      for (int64_t e = lane; e < E; e += 64) pc += prob(e) * (float(a.counts[e]) - mean);
+      pc = wave_sum(pc);
+    }
+    if (a.grad_weights != nullptr) {
+      for (int64_t j = lane; j < k; j += 64) {
+        const int id = a.ids[row * k + j];
+        if (id < 0 || id >= E) continue;
+        const float pj = prob(id);
+        ps += pj;
+        q += pj * a.grad_weights[row * k + j];
+      }
+      ps = wave_sum(ps);
+      q = wave_sum(q);
+      if (a.renorm) {
+        wu = q / ps;
+        q = 0.f;
+      }
+    }
+    auto base = [&](int64_t e) {
+      const float pe = prob(e);
+      return (with_loss ? factor * pe * (float(a.counts[e]) - mean - pc) : 0.f) - pe * q;
+    };
+    for (int64_t e = lane; e < E; e += 64) out[e] = to_out<T>(base(e));
+    if (a.grad_weights == nullptr) continue;
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // the row's stores first (vmcnt 0)
+    for (int64_t j = lane; j < k; j += 64) {
+      const int id = a.ids[row * k + j];
+      if (id < 0 || id >= E) continue;
+      const float w = a.renorm ? prob(id) / ps : prob(id);
+      float add = 0.f;
+      for (int64_t l = 0; l < k; ++l)
+        if (a.ids[row * k + l] == id) add += w * (a.grad_weights[row * k + l] - wu);
+      out[id] = to_out<T>(base(id) + add);
+    }
+  }
+}
+
+int planes_for(int64_t M, int64_t E) {
+  if (E <= kFastExperts) return int(std::min<int64_t>(kPlanes, cdiv(M, 32)));
+  return int(std::max<int64_t>(1, std::min<int64_t>(64, cdiv(M, 16))));
+}
+int64_t up(int64_t x) { return (x + 255) / 256 * 256; }
+
+template <typename T, int PIECES>
+void launch_balance_rows(const T* g, const int32_t* ids, const uint8_t* mask, int64_t M, int E, int k, int planes,
+                         const BalanceScratch& s, float* loss, int32_t* counts, int32_t* tokens,
+                         hipStream_t stream) {
+  const bool wide = E % 8 == 0 && reinterpret_cast<uintptr_t>(g) % 16 == 0;
+  const bool one = M <= kOneWgRows;
+#define XK_ROWS(W, O)                                                                                             \
+  hipLaunchKernelGGL((balance_rows<T, PIECES, W, O>), dim3(O ? 1 : planes), dim3(O ? kOneWg : kThreads), 0, stream, g, \
+                     ids, mask, M, E, k, s, loss, counts, tokens)
+  if (one && wide) XK_ROWS(true, true);
+  else if (one) XK_ROWS(false, true);
+  else if (wide) XK_ROWS(true, false);
+  else XK_ROWS(false, false);
+#undef XK_ROWS
+}
+
+template <typename T>
+int balance_typed(const void* logits, const int32_t* ids, const uint8_t* mask, int64_t M, int64_t E, int64_t k,
+                  BalanceScratch s, float* loss, int32_t* counts, int32_t* tokens, hipStream_t stream) {
+  const T* g = static_cast<const T*>(logits);
+  const int planes = planes_for(M, E);
+  if (E <= kFastExperts) {
+    const int e = int(E), kk = int(k);
+    if (E <= 128) launch_balance_rows<T, 1>(g, ids, mask, M, e, kk, planes, s, loss, counts, tokens, stream);
+    else if (E <= 256) launch_balance_rows<T, 2>(g, ids, mask, M, e, kk, planes, s, loss, counts, tokens, stream);
+    else launch_balance_rows<T, 4>(g, ids, mask, M, e, kk, planes, s, loss, counts, tokens, stream);
+    XK_CHECK_LAUNCH("balance_rows");
+    if (M <= kOneWgRows) return XK_OK;
+    hipLaunchKernelGGL((balance_finish<false>), dim3(unsigned(cdiv(E, 16))), dim3(kThreads), 0, stream, planes, E, k,
+                       s, loss, counts, tokens);
+  } else {
+    const int64_t per = std::max<int64_t>(1, cdiv(M, planes));
+    hipLaunchKernelGGL((row_stats<T>), dim3(unsigned(std::min<int64_t>(2048, std::max<int64_t>(cdiv(M, 4), cdiv(E, kThreads))))),
+                       dim3(kThreads), 0, stream, g, mask, M, E, s, counts);
+    XK_CHECK_LAUNCH("row_stats");
+    hipLaunchKernelGGL((balance_columns<T>), dim3(unsigned(cdiv(E, kThreads)), planes), dim3(kThreads), 0, stream, g,
+                       ids, mask, M, E, k, per, s, counts);
+    XK_CHECK_LAUNCH("balance_columns");
+    hipLaunchKernelGGL((balance_finish<true>), dim3(unsigned(cdiv(E, 16))), dim3(kThreads), 0, stream, planes, E, k,
+                       s, loss, counts, tokens);
+  }
+  XK_CHECK_LAUNCH("balance_finish");
+  return XK_OK;
+}
+
+template <typename T, int PIECES>
+void launch_grad_rows(const T* g, int64_t M, int E, int k, const RouterGrad& a, T* grad, hipStream_t stream) {
+  const bool wide = E % 8 == 0 && (reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(grad)) % 16 == 0;
+  const dim3 grid(unsigned(std::min<int64_t>(2048, cdiv(M, kThreads / 16))));
+  if (wide)
+    hipLaunchKernelGGL((router_grad_rows<T, PIECES, true>), grid, dim3(kThreads), 0, stream, g, M, E, k, a, grad);
+  else
+    hipLaunchKernelGGL((router_grad_rows<T, PIECES, false>), grid, dim3(kThreads), 0, stream, g, M, E, k, a, grad);
+}
+
+template <typename T>
+int grad_typed(const void* logits, int64_t M, int64_t E, int64_t k, const RouterGrad& a, void* grad,
+               hipStream_t stream) {
+  const T* g = static_cast<const T*>(logits);
+  T* o = static_cast<T*>(grad);
+  if (E <= kFastExperts && k <= kFastTopk) {
+    if (E <= 128) launch_grad_rows<T, 1>(g, M, int(E), int(k), a, o, stream);
+    else if (E <= 256) launch_grad_rows<T, 2>(g, M, int(E), int(k), a, o, stream);
+    else launch_grad_rows<T, 4>(g, M, int(E), int(k), a, o, stream);
+  } else {
+    hipLaunchKernelGGL((router_grad_any<T>), dim3(unsigned(std::min<int64_t>(4096, cdiv(M, 4)))), dim3(kThreads), 0,
+                       stream, g, M, E, k, a, o);
+  }
+  XK_CHECK_LAUNCH("router_grad");
+  return XK_OK;
+}
+
+}  // namespace
+
+int64_t balance_workspace_bytes(int64_t M, int64_t E) {
+  const int64_t planes = planes_for(std::max<int64_t>(M, 1), E);
+  return up(planes * E * 4) * 2 + up(planes * 4) + up(cdiv(E, 16) * 8) + up(4) +
+         (E > kFastExperts ? up(M * 8) : 0);
+}
+
+int launch_balance_loss(const void* logits, int dtype, int64_t M, int64_t E, const int32_t* ids, int64_t k,
+                        const uint8_t* mask, float* loss, int32_t* counts, int32_t* tokens, void* workspace,
+                        hipStream_t stream) {
+  const int64_t planes = planes_for(std::max<int64_t>(M, 1), E);
+  char* w = static_cast<char*>(workspace);
+  BalanceScratch s;
+  s.sums = reinterpret_cast<float*>(w); w += up(planes * E * 4);
+  s.cnt = reinterpret_cast<int32_t*>(w); w += up(planes * E * 4);
+  s.rows = reinterpret_cast<int32_t*>(w); w += up(planes * 4);
+  s.parts = reinterpret_cast<double*>(w); w += up(cdiv(E, 16) * 8);
+  s.ticket = reinterpret_cast<int32_t*>(w); w += up(4);
+  s.stat = reinterpret_cast<float*>(w);
+  if (dtype == XK_DT_BF16)
+    return balance_typed<uint16_t>(logits, ids, mask, M, E, k, s, loss, counts, tokens, stream);
+  if (dtype == XK_DT_FP16)
+    return balance_typed<_Float16>(logits, ids, mask, M, E, k, s, loss, counts, tokens, stream);
+  return balance_typed<float>(logits, ids, mask, M, E, k, s, loss, counts, tokens, stream);
+}
+
+int launch_router_backward(const void* logits, int dtype, int64_t M, int64_t E, const int32_t* ids, int64_t k,
+                           const uint8_t* mask, const int32_t* counts, const int32_t* tokens, const float* grad_loss,
+                           const float* grad_weights, int renorm, void* grad, hipStream_t stream) {
+  const RouterGrad a{ids, mask, counts, tokens, grad_loss, grad_weights, renorm};
+  if (dtype == XK_DT_BF16) return grad_typed<uint16_t>(logits, M, E, k, a, grad, stream);
+  if (dtype == XK_DT_FP16) return grad_typed<_Float16>(logits, M, E, k, a, grad, stream);
+  return grad_typed<float>(logits, M, E, k, a, grad, stream);
+}
+
+}  // namespace xk

@@ -18,28 +18,13 @@
 // more than 2048 experts take a streaming variant (below).
 #include <stdint.h>
 
-#include "common.h"
+#include "router_rows.h"
 
 namespace xk {
 namespace {
 
 constexpr int kTsWaves = 4;
 constexpr int kTsThreads = kTsWaves * 64;
-
-template <typename T>
-__device__ __forceinline__ float logit_at(const T* p);
-template <>
-__device__ __forceinline__ float logit_at<uint16_t>(const uint16_t* p) {  // bf16 bits
-  return __uint_as_float(uint32_t(*p) << 16);
-}
-template <>
-__device__ __forceinline__ float logit_at<_Float16>(const _Float16* p) {
-  return float(*p);
-}
-template <>
-__device__ __forceinline__ float logit_at<float>(const float* p) {
-  return *p;
-}
 
 // The reference's stable descending sort (torch.sort, topk_softmax.py:88)
 // orders experts by probability, NaN above every number, and equal keys (NaN
@@ -148,48 +133,6 @@ topk_softmax_rows(const T* __restrict__ logits, int64_t M, int E, int k, int ren
 // place of six LDS permutes: the four rows of a wave cost about what one row
 // over 64 lanes does. Lane i holds the 8-expert pieces i, i + 16, ...; lane t
 // keeps selection t. 4,096 rows, E = 256, k = 8, bf16: 10.3 -> 7.2 us; 16,384 rows 24 -> 12 us per call.
-template <int CTRL> __device__ __forceinline__ uint32_t dpp(uint32_t x) {
-  return __builtin_amdgcn_update_dpp(x, x, CTRL, 0xF, 0xF, false);
-}
-// f over the partners of an all-reduce of 16 lanes: neighbours, pairs, the
-// mirrored half row, the mirrored row.
-template <typename F> __device__ __forceinline__ void row_steps(F&& f) {
-  f([](uint32_t x) { return dpp<0xB1>(x); });
-  f([](uint32_t x) { return dpp<0x4E>(x); });
-  f([](uint32_t x) { return dpp<0x141>(x); });
-  f([](uint32_t x) { return dpp<0x140>(x); });
-}
-
-template <typename T> struct piece8 {};  // 8 logits in 16-byte loads
-template <> struct piece8<uint16_t> {
-  __device__ __forceinline__ static void load(const uint16_t* g, float* v) {
-    const u32x4 r = *reinterpret_cast<const u32x4*>(g);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(r[i] << 16);
-      v[2 * i + 1] = __uint_as_float(r[i] & 0xFFFF0000u);
-    }
-  }
-};
-template <> struct piece8<_Float16> {
-  __device__ __forceinline__ static void load(const _Float16* g, float* v) {
-    typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-    const h8 r = *reinterpret_cast<const h8*>(g);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(r[i]);
-  }
-};
-template <> struct piece8<float> {
-  __device__ __forceinline__ static void load(const float* g, float* v) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const f32x4 r = reinterpret_cast<const f32x4*>(g)[h];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[4 * h + i] = r[i];
-    }
-  }
-};
-
 // WIDE: E a multiple of 8 and every row 16-byte aligned.
 template <typename T, int PIECES, bool WIDE>
 __global__ void __launch_bounds__(kTsThreads)

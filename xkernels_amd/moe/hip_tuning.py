@@ -1,0 +1,255 @@
+"""HIP backend of the ops for tuning and serving over the frozen experts: the
+router's training step, low-rank adapters and 8-bit activation checkpoints.
+
+As in ``hip_backend``: arguments are checked on the host, outputs and scratch are
+torch allocations on the tensors' device, the launch goes to torch's current stream
+of that device, errors surface as ``RuntimeError`` and CPU tensors are rejected.
+Nothing synchronises, so every call may be captured into a HIP graph.
+"""
+from __future__ import annotations
+
+from contextlib import nullcontext
+
+import torch
+
+from .. import _lib
+from .._backends import Backend
+from .._dispatch import register
+from .act_checkpoint import ActCheckpoint
+from .balance_loss import BalanceLoss
+from .hip_backend import _contig, _need_gpu, _ptr, _stream
+
+_LORA_DT = {torch.bfloat16: _lib.XK_DT_BF16, torch.float32: _lib.XK_DT_FP32}
+_ANY_DT = {**_LORA_DT, torch.float16: _lib.XK_DT_FP16}
+BLOCK = 32
+
+
+def _on(dev: torch.device):
+    """The tensors' device as the current one: HIP launches on a stream need it."""
+    return nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _code(op: str, t: torch.Tensor, table=_ANY_DT) -> int:
+    try:
+        return table[t.dtype]
+    except KeyError:
+        names = ", ".join(str(d).removeprefix("torch.") for d in table)
+        raise RuntimeError(f"{op}: unsupported dtype {t.dtype} ({names})") from None
+
+
+def _scratch(nbytes: int, dev) -> torch.Tensor:
+    return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+
+
+def _ids(op: str, t: torch.Tensor, n: int) -> torch.Tensor:
+    """int32, contiguous; 64-bit ids outside [0, n) stay outside."""
+    if t.dtype == torch.int64:
+        t = t.clamp(-1, n)
+    elif t.dtype not in (torch.int32, torch.int16, torch.int8, torch.uint8):
+        raise RuntimeError(f"{op}: ids must be whole numbers, got {t.dtype}")
+    return _contig(t, torch.int32)
+
+
+def _shape(op: str, name: str, t: torch.Tensor | None, want: tuple) -> None:
+    if t is not None and tuple(t.shape) != want:
+        raise RuntimeError(f"{op}: {name} must be {list(want)}, got {list(t.shape)}")
+
+
+def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """``t`` [M, n] as rows of consecutive values, and how far they lie apart."""
+    M, n = t.shape
+    if M > 1 and (n == 1 or t.stride(1) == 1) and t.stride(0) >= n:
+        return t, t.stride(0)
+    return t.contiguous(), n
+
+
+# ------------------------------------------------------------------- router ----
+
+def _router_args(op, gating_output, topk_ids, mask):
+    if gating_output.dim() != 2 or topk_ids.dim() != 2 or topk_ids.shape[0] != gating_output.shape[0]:
+        raise RuntimeError(f"{op}: expected gating_output [M, E] and topk_ids [M, top_k], got "
+                           f"{list(gating_output.shape)} and {list(topk_ids.shape)}")
+    M, E = gating_output.shape
+    k = topk_ids.shape[1]
+    if not 1 <= k <= E:
+        raise RuntimeError(f"{op}: top_k={k} outside [1, E={E}]")
+    if mask is not None:
+        _shape(op, "mask", mask, (M,))
+        mask = _contig(mask if mask.dtype == torch.bool else mask != 0).view(torch.uint8)
+    return M, E, k, gating_output.contiguous(), _ids(op, topk_ids, E), mask
+
+
+def moe_balance_loss_hip(gating_output: torch.Tensor, topk_ids: torch.Tensor,
+                         mask: torch.Tensor | None = None) -> BalanceLoss:
+    op = "moe_balance_loss"
+    dev = _need_gpu(op, gating_output, topk_ids, mask)
+    dt = _code(op, gating_output)
+    M, E, k, g, ids, on = _router_args(op, gating_output, topk_ids, mask)
+    with _on(dev):
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        counts = torch.empty(E, dtype=torch.int32, device=dev)
+        tokens = torch.empty((), dtype=torch.int32, device=dev)
+        ws = _scratch(_lib.query("xk_moe_balance_loss_workspace_bytes", M, E), dev)
+        _lib.call("xk_moe_balance_loss", _ptr(g), dt, M, E, _ptr(ids), k, _ptr(on), _ptr(loss), _ptr(counts),
+                  _ptr(tokens), _ptr(ws), ws.numel(), _stream(dev))
+    return BalanceLoss(loss, counts, tokens)
+
+
+def moe_router_backward_hip(gating_output: torch.Tensor, topk_ids: torch.Tensor,
+                            grad_weights: torch.Tensor | None = None, renormalize: bool = True,
+                            grad_loss: torch.Tensor | None = None, counts: torch.Tensor | None = None,
+                            tokens: torch.Tensor | None = None,
+                            mask: torch.Tensor | None = None) -> torch.Tensor:
+    op = "moe_router_backward"
+    dev = _need_gpu(op, gating_output, topk_ids, grad_weights, grad_loss, counts, tokens, mask)
+    dt = _code(op, gating_output)
+    M, E, k, g, ids, on = _router_args(op, gating_output, topk_ids, mask)
+    if grad_weights is None and grad_loss is None:
+        raise RuntimeError(f"{op}: neither grad_weights nor grad_loss")
+    _shape(op, "grad_weights", grad_weights, (M, k))
+    gw = None if grad_weights is None else _contig(grad_weights, torch.float32)
+    gl = cn = tk = None
+    if grad_loss is not None:
+        if counts is None:
+            raise RuntimeError(f"{op}: grad_loss needs the counts of moe_balance_loss")
+        if tokens is None and mask is not None:
+            raise RuntimeError(f"{op}: with a mask, grad_loss needs the tokens of moe_balance_loss")
+        _shape(op, "counts", counts, (E,))
+        if grad_loss.numel() != 1 or (tokens is not None and tokens.numel() != 1):
+            raise RuntimeError(f"{op}: grad_loss and tokens are single numbers")
+        gl, cn = _contig(grad_loss, torch.float32), _contig(counts, torch.int32)
+        tk = None if tokens is None else _contig(tokens, torch.int32)
+    with _on(dev):
+        grad = torch.empty_like(g)
+        _lib.call("xk_moe_router_backward", _ptr(g), dt, M, E, _ptr(ids), k, _ptr(on), _ptr(gl), _ptr(cn), _ptr(tk),
+                  _ptr(gw), int(bool(renormalize)), _ptr(grad), _stream(dev))
+    return grad
+
+
+# ----------------------------------------------------------------- adapters ----
+
+def _lora_args(op, rows, n_rows_name, cols, lora_a, lora_b, adapter_ids, scaling):
+    if lora_a.dim() != 3 or lora_b.dim() != 3:
+        raise RuntimeError(f"{op}: expected lora_a [L, r, K] and lora_b [L, N, r]")
+    L, r, K = lora_a.shape
+    N = lora_b.shape[1]
+    _shape(op, "lora_b", lora_b, (L, N, r))
+    _shape(op, "adapter_ids", adapter_ids, (rows,))
+    _shape(op, "scaling", scaling, (L,))
+    if lora_a.dtype != lora_b.dtype:
+        raise RuntimeError(f"{op}: lora_a is {lora_a.dtype}, lora_b {lora_b.dtype}")
+    if cols[0] != (K if n_rows_name == "x" else N):
+        raise RuntimeError(f"{op}: {n_rows_name} has {cols[0]} columns, the adapters "
+                           f"{K if n_rows_name == 'x' else N}")
+    sc = None if scaling is None else _contig(scaling, torch.float32)
+    return L, r, K, N, lora_a.contiguous(), lora_b.contiguous(), _ids(op, adapter_ids, L), sc
+
+
+def lora_projection_hip(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, adapter_ids: torch.Tensor,
+                        base: torch.Tensor | None = None, scaling: torch.Tensor | None = None,
+                        return_hidden: bool = False):
+    op = "lora_projection"
+    dev = _need_gpu(op, x, lora_a, lora_b, adapter_ids, base, scaling)
+    dt = _code(op, x, _LORA_DT)
+    if x.dim() != 2:
+        raise RuntimeError(f"{op}: x must be [M, K], got {list(x.shape)}")
+    M = x.shape[0]
+    L, r, K, N, a, b, ids, sc = _lora_args(op, M, "x", x.shape[1:], lora_a, lora_b, adapter_ids, scaling)
+    _shape(op, "base", base, (M, N))
+    for name, t in (("lora_a", a), ("base", base)):
+        if t is not None and t.dtype != x.dtype:
+            raise RuntimeError(f"{op}: {name} is {t.dtype}, x {x.dtype}")
+    xr, ldx = _rows(x)
+    br, ldb = (None, N) if base is None else _rows(base)
+    with _on(dev):
+        out = torch.empty((M, N), dtype=x.dtype, device=dev)
+        hidden = torch.empty((M, r), dtype=torch.float32, device=dev) if return_hidden else None
+        ws = _scratch(_lib.query("xk_lora_projection_workspace_bytes", M, K, L, r), dev)
+        _lib.call("xk_lora_projection", _ptr(xr), dt, ldx, M, K, _ptr(a), _ptr(b), L, N, r, _ptr(ids), _ptr(sc),
+                  _ptr(br), ldb, _ptr(out), _ptr(hidden), _ptr(ws), ws.numel(), _stream(dev))
+    return (out, hidden) if return_hidden else out
+
+
+def lora_projection_backward_hip(grad_out: torch.Tensor, x: torch.Tensor | ActCheckpoint, lora_a: torch.Tensor,
+                                 lora_b: torch.Tensor, adapter_ids: torch.Tensor, hidden: torch.Tensor,
+                                 scaling: torch.Tensor | None = None):
+    op = "lora_projection_backward"
+    held = isinstance(x, ActCheckpoint)
+    xt, scales = (x.values, x.scales) if held else (x, None)
+    dev = _need_gpu(op, grad_out, xt, scales, lora_a, lora_b, adapter_ids, hidden, scaling)
+    dt = _code(op, grad_out, _LORA_DT)
+    if grad_out.dim() != 2:
+        raise RuntimeError(f"{op}: grad_out must be [M, N], got {list(grad_out.shape)}")
+    M = grad_out.shape[0]
+    L, r, K, N, a, b, ids, sc = _lora_args(op, M, "grad_out", grad_out.shape[1:], lora_a, lora_b, adapter_ids, scaling)
+    _shape(op, "x", xt, (M, K))
+    _shape(op, "hidden", hidden, (M, r))
+    if a.dtype != grad_out.dtype:
+        raise RuntimeError(f"{op}: lora_a is {a.dtype}, grad_out {grad_out.dtype}")
+    if held:
+        xr, sr = _check_held(op, x)
+        ldx = K
+    else:
+        if x.dtype != grad_out.dtype:
+            raise RuntimeError(f"{op}: x is {x.dtype}, grad_out {grad_out.dtype}")
+        (xr, ldx), sr = _rows(x), None
+    gr, ldg = _rows(grad_out)
+    h = _contig(hidden, torch.float32)
+    with _on(dev):
+        grad_x = torch.empty((M, K), dtype=grad_out.dtype, device=dev)
+        grad_a, grad_b = torch.empty_like(a), torch.empty_like(b)
+        ws = _scratch(_lib.query("xk_lora_projection_backward_workspace_bytes", M, K, N, L, r, dt), dev)
+        _lib.call("xk_lora_projection_backward", _ptr(gr), dt, ldg, _ptr(xr), ldx, _ptr(sr), M, K, _ptr(a), _ptr(b),
+                  L, N, r, _ptr(ids), _ptr(sc), _ptr(h), _ptr(grad_x), _ptr(grad_a), _ptr(grad_b), _ptr(ws),
+                  ws.numel(), _stream(dev))
+    return grad_x, grad_a, grad_b
+
+
+# -------------------------------------------------------------- checkpoints ----
+
+def _check_held(op: str, held: ActCheckpoint) -> tuple[torch.Tensor, torch.Tensor]:
+    v, s = held
+    if v.dim() != 2 or v.dtype != torch.float8_e4m3fn or s.dtype != torch.uint8:
+        raise RuntimeError(f"{op}: a checkpoint is float8_e4m3fn [M, K] with uint8 scales, got {v.dtype} "
+                           f"{list(v.shape)}, {s.dtype}")
+    _shape(op, "scales", s, (v.shape[0], -(-v.shape[1] // BLOCK)))
+    return v.contiguous(), s.contiguous()
+
+
+def act_checkpoint_hip(x: torch.Tensor) -> ActCheckpoint:
+    op = "act_checkpoint"
+    dev = _need_gpu(op, x)
+    dt = _code(op, x)
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise RuntimeError(f"{op}: x must be [M, K], K >= 1, got {list(x.shape)}")
+    M, K = x.shape
+    xr, ldx = _rows(x)
+    with _on(dev):
+        values = torch.empty((M, K), dtype=torch.float8_e4m3fn, device=dev)
+        scales = torch.empty((M, -(-K // BLOCK)), dtype=torch.uint8, device=dev)
+        _lib.call("xk_act_checkpoint", _ptr(xr), dt, ldx, M, K, _ptr(values), _ptr(scales), _stream(dev))
+    return ActCheckpoint(values, scales)
+
+
+def act_restore_hip(held: ActCheckpoint, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    op = "act_restore"
+    held = ActCheckpoint(*held)
+    dev = _need_gpu(op, *held)
+    v, s = _check_held(op, held)
+    M, K = v.shape
+    if K == 0:
+        raise RuntimeError(f"{op}: no columns")
+    with _on(dev):
+        out = torch.empty((M, K), dtype=dtype, device=dev)
+        _lib.call("xk_act_restore", _ptr(v), _ptr(s), M, K, _code(op, out), _ptr(out), _stream(dev))
+    return out
+
+
+def register_all() -> None:
+    _lib.load()
+    register("moe_balance_loss", Backend.HIP)(moe_balance_loss_hip)
+    register("moe_router_backward", Backend.HIP)(moe_router_backward_hip)
+    register("lora_projection", Backend.HIP)(lora_projection_hip)
+    register("lora_projection_backward", Backend.HIP)(lora_projection_backward_hip)
+    register("act_checkpoint", Backend.HIP)(act_checkpoint_hip)
+    register("act_restore", Backend.HIP)(act_restore_hip)
