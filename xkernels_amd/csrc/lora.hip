@@ -41,7 +41,6 @@ constexpr int kTile = 64;      // rows of a sorted tile
 constexpr int kFewTile = 16;   // rows of a tile that a workgroup finds itself
 constexpr int kFew = 256;      // rows up to which they do (a thread per row)
 constexpr int kMaxRank = 128;
-constexpr int kCols = 128;     // columns of a wgrad workgroup
 
 // ------------------------------------------------------------- operands ----
 // frag: 8 contraction values of one operand row. half: 16 ranks as an operand, of
@@ -165,79 +164,88 @@ __device__ __forceinline__ int few_tile(const Rows& a, int j, int* rows) {
 }
 
 // --------------------------------------------------------------- shrink ----
-// acc[t] += 16 ranks x 16 rows over [k0, k1): lane's row x + (row lane & 15).
-template <typename T, int RT, bool VEC>
-__device__ __forceinline__ void shrink_range(const T* xr, bool valid, const T* ar, int64_t K, int r, int64_t k0,
-                                             int64_t k1, int lane, f32x4 (&acc)[RT]) {
-  const int g8 = (lane >> 4) * 8, rank = lane & 15;
-  int64_t k = k0;
-#pragma unroll 4
-  for (; k + 32 <= k1; k += 32) {
-    const typename mm<T>::frag xf = valid ? load_frag<T, VEC>(xr + k + g8, 8) : zero_frag<T>();
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const bool in = 16 * t + rank < r;
-      const typename mm<T>::frag af = in ? load_frag<T, VEC>(ar + int64_t(16 * t + rank) * K + k + g8, 8) : zero_frag<T>();
-      acc[t] = mm<T>::mma(af, xf, acc[t]);
-    }
-  }
-  if (k < k1) {
-    const int n = int(min(int64_t(8), max(int64_t(0), k1 - k - g8)));
-    const typename mm<T>::frag xf = valid ? load_frag<T, VEC>(xr + k + g8, n) : zero_frag<T>();
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const bool in = 16 * t + rank < r;
-      const typename mm<T>::frag af = in ? load_frag<T, VEC>(ar + int64_t(16 * t + rank) * K + k + g8, n) : zero_frag<T>();
-      acc[t] = mm<T>::mma(af, xf, acc[t]);
-    }
-  }
-}
-
-// planes[s, m, 0 .. 16 RT): the sums over slice s of K. Sorted tiles: a wave per 16
-// rows. Few rows: the waves share a tile and a quarter of the slice each.
+// planes[s, m, 0 .. 16 RT): the sums over slice s of K for a tile's rows. The waves
+// split the slice, a quarter each for the whole tile: the weights' operands, which
+// come from L2, serve all of a sorted tile's four 16-row products (with 16 rows a
+// wave, rank 64 read four times the bytes of x in weights), and the four partial
+// sums meet in LDS. Few rows: one 16-row product, the tile found here.
 template <typename T, int RT, bool VEC, bool FEW>
 __global__ void __launch_bounds__(kThreads)
 lora_shrink(Rows rows, const T* __restrict__ x, int64_t ldx, int64_t K, const T* __restrict__ a, int r,
             int64_t slice, float* __restrict__ planes) {
-  constexpr int RP = RT * 16;
+  constexpr int RP = RT * 16, BT = FEW ? 1 : kTile / 16;
+  __shared__ int tile_rows[BT * 16];
+  __shared__ f32x4 red[2][BT * RT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t k0 = int64_t(blockIdx.y) * slice, k1 = min(K, k0 + slice);
-  f32x4 acc[RT];
-#pragma unroll
-  for (int t = 0; t < RT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float* plane = planes + int64_t(blockIdx.y) * rows.M * RP;
+  int adapter;
+  int64_t m[BT];
   if (FEW) {
-    __shared__ int tile_rows[kFewTile];
-    __shared__ f32x4 red[3][RT][64];
-    const int adapter = few_tile(rows, blockIdx.x, tile_rows);
+    adapter = few_tile(rows, blockIdx.x, tile_rows);
     if (adapter < 0) return;
-    const int64_t m = tile_rows[lane & 15];
-    const bool valid = m < rows.M;
-    const int64_t quarter = slice / 4, w0 = min(k1, k0 + wave * quarter), w1 = min(k1, w0 + quarter);
-    shrink_range<T, RT, VEC>(valid ? x + m * ldx : x, valid, a + int64_t(adapter) * r * K, K, r, w0, w1, lane, acc);
-    if (wave > 0)
-#pragma unroll
-      for (int t = 0; t < RT; ++t) red[wave - 1][t][lane] = acc[t];
-    __syncthreads();
-    if (wave > 0 || !valid) return;
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const f32x4 v = ((acc[t] + red[0][t][lane]) + red[1][t][lane]) + red[2][t][lane];
-      *reinterpret_cast<f32x4*>(plane + m * RP + 16 * t + (lane >> 4) * 4) = v;
-    }
+    m[0] = tile_rows[lane & 15];
   } else {
     const int64_t pos = int64_t(blockIdx.x) * kTile;
     if (pos >= *rows.num_post) return;
-    const int adapter = rows.tile_adapter[blockIdx.x];
-    const int64_t m = rows.sorted[pos + wave * 16 + (lane & 15)];
-    const bool valid = m < rows.M;
-    if (__ballot(valid) == 0) return;
-    shrink_range<T, RT, VEC>(valid ? x + m * ldx : x, valid, a + int64_t(adapter) * r * K, K, r, k0, k1, lane, acc);
-    if (!valid) return;
+    adapter = rows.tile_adapter[blockIdx.x];
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
-      *reinterpret_cast<f32x4*>(plane + m * RP + 16 * t + (lane >> 4) * 4) = acc[t];
+    for (int i = 0; i < BT; ++i) m[i] = rows.sorted[pos + 16 * i + (lane & 15)];
   }
+  const int g8 = (lane >> 4) * 8, rank = lane & 15;
+  const T* xr[BT];
+  bool valid[BT];
+#pragma unroll
+  for (int i = 0; i < BT; ++i) {
+    valid[i] = m[i] < rows.M;
+    xr[i] = x + (valid[i] ? m[i] : 0) * ldx + g8;
+  }
+  const T* ar = a + int64_t(adapter) * r * K + g8;
+  f32x4 acc[BT][RT];
+#pragma unroll
+  for (int i = 0; i < BT; ++i)
+#pragma unroll
+    for (int t = 0; t < RT; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int64_t quarter = slice / 4, w0 = min(k1, k0 + wave * quarter), w1 = min(k1, w0 + quarter);
+  auto step = [&](int64_t k, int n) {
+    typename mm<T>::frag xf[BT];
+#pragma unroll
+    for (int i = 0; i < BT; ++i) xf[i] = valid[i] ? load_frag<T, VEC>(xr[i] + k, n) : zero_frag<T>();
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const typename mm<T>::frag af =
+          16 * t + rank < r ? load_frag<T, VEC>(ar + int64_t(16 * t + rank) * K + k, n) : zero_frag<T>();
+#pragma unroll
+      for (int i = 0; i < BT; ++i) acc[i][t] = mm<T>::mma(af, xf[i], acc[i][t]);
+    }
+  };
+  int64_t k = w0;
+#pragma unroll(FEW ? 4 : 2)
+  for (; k + 32 <= w1; k += 32) step(k, 8);
+  if (k < w1) step(k, int(min(int64_t(8), max(int64_t(0), w1 - k - g8))));
+  // waves 2 and 3 hand theirs to 0 and 1, then 1 to 0
+#pragma unroll
+  for (int half = 2; half >= 1; half >>= 1) {
+    if (wave >= half && wave < 2 * half)
+#pragma unroll
+      for (int i = 0; i < BT; ++i)
+#pragma unroll
+        for (int t = 0; t < RT; ++t) red[wave - half][i * RT + t][lane] = acc[i][t];
+    __syncthreads();
+    if (wave < half)
+#pragma unroll
+      for (int i = 0; i < BT; ++i)
+#pragma unroll
+        for (int t = 0; t < RT; ++t) acc[i][t] += red[wave][i * RT + t][lane];
+    __syncthreads();
+  }
+  if (wave > 0) return;
+  float* plane = planes + int64_t(blockIdx.y) * rows.M * RP;
+#pragma unroll
+  for (int i = 0; i < BT; ++i)
+    if (valid[i])
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+        *reinterpret_cast<f32x4*>(plane + m[i] * RP + 16 * t + (lane >> 4) * 4) = acc[i][t];
 }
 
 // Ranks [0, 16 RT) of row m: the planes' sum in order, zeros from r on. pitch: the
@@ -251,7 +259,15 @@ __device__ __forceinline__ f32x4 ranks4(const Ranks& u, int64_t m, int rank) {
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
   const float* p = u.planes + m * u.pitch + rank;
   if (u.pitch % 4 == 0 && rank + 4 <= u.pitch && (reinterpret_cast<uintptr_t>(u.planes) & 15) == 0) {
-    for (int s = 0; s < u.count; ++s) v += *reinterpret_cast<const f32x4*>(p + s * u.plane_stride);
+    int s = 0;
+    for (; s + 8 <= u.count; s += 8) {  // 8 loads in flight, added in order
+      f32x4 w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = *reinterpret_cast<const f32x4*>(p + (s + i) * u.plane_stride);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v += w[i];
+    }
+    for (; s < u.count; ++s) v += *reinterpret_cast<const f32x4*>(p + s * u.plane_stride);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (rank + i >= u.r) v[i] = 0.f;  // the planes hold 0 * x there: NaN for an infinite x
@@ -361,14 +377,26 @@ lora_expand(Rows rows, int64_t tiles, Ranks h, const T* __restrict__ b, const fl
   }
   const T* bw = b + int64_t(adapter) * N * h.r;
   const int nr = 8 * ((lane & 15) >> 2) + (lane & 3);  // this lane's weight row among 32, less 4 for the second product
-  for (int64_t n0 = c0 + wave * 32; n0 < c1; n0 += kThreads / 64 * 32) {
+  // a wave's columns lie together; the next 32 of the base are on their way while
+  // these are finished
+  const int64_t w0 = c0 + wave * (chunk / 4), w1 = min(c1, w0 + chunk / 4);
+  typename mm<T>::frag next[BT];
+  auto fetch = [&](int64_t n0) {
     const int64_t nb = n0 + g * 8;
-    const int cnt = int(min(int64_t(8), max(int64_t(0), c1 - nb)));
-    typename mm<T>::frag bs[BT];
+    const int cnt = int(min(int64_t(8), max(int64_t(0), w1 - nb)));
 #pragma unroll
     for (int i = 0; i < BT; ++i)
-      bs[i] = base != nullptr && m[i] < rows.M && cnt > 0 ? load_frag<T, VEC>(base + m[i] * ldbase + nb, cnt)
-                                                           : zero_frag<T>();
+      next[i] = base != nullptr && m[i] < rows.M && cnt > 0 ? load_frag<T, VEC>(base + m[i] * ldbase + nb, cnt)
+                                                             : zero_frag<T>();
+  };
+  if (w0 < w1) fetch(w0);
+  for (int64_t n0 = w0; n0 < w1; n0 += 32) {
+    const int64_t nb = n0 + g * 8;
+    const int cnt = int(min(int64_t(8), max(int64_t(0), w1 - nb)));
+    typename mm<T>::frag bs[BT];
+#pragma unroll
+    for (int i = 0; i < BT; ++i) bs[i] = next[i];
+    if (n0 + 32 < w1) fetch(n0 + 32);
     f32x4 acc[BT][2];
 #pragma unroll
     for (int i = 0; i < BT; ++i) acc[i][0] = acc[i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -377,7 +405,7 @@ lora_expand(Rows rows, int64_t tiles, Ranks h, const T* __restrict__ b, const fl
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int64_t n = n0 + nr + 4 * e;
-        const int left = n < c1 ? h.r - 16 * t - rank0 : 0;
+        const int left = n < w1 ? h.r - 16 * t - rank0 : 0;
         const typename mm<T>::half wf = load_half<T, VEC>(bw + n * h.r + 16 * t + rank0, left);
 #pragma unroll
         for (int i = 0; i < BT; ++i) acc[i][e] = mm<T>::mma_half(wf, hf[i][t], acc[i][e]);
@@ -429,12 +457,20 @@ transpose_used(const T* __restrict__ in, int64_t R, int64_t C, int64_t col_tiles
 // ---------------------------------------------------------------- wgrad ----
 // out[i] = sum over adapter i's rows of u[m, :]^T v[m, :]: u the ranks (r of them), v a
 // long row (C columns). Positions of the sorted order are cut into windows; a
-// workgroup takes one adapter's part of one window and kCols columns. An adapter
+// workgroup takes one adapter's part of one window and a strip of columns. An adapter
 // inside one window writes its gradient; one over several leaves a plane for each,
 // which wgrad_reduce adds in order (and which writes zeros for adapters without rows).
+//
+// The contraction runs over rows, along which neither operand is contiguous. u comes
+// packed as MFMA operands (lora_pack). v goes through LDS: a wave takes 32 rows at a
+// time into registers, the next 32 on their way meanwhile, writes them row by row
+// and reads them back transposed (ds_read_b64_tr_b16: 4 rows of a lane's column). A
+// wave's tile is its own, so the loop has no barrier; the waves' sums meet at the end.
+// Contraction place 8 g + j is row 4 g + j for j < 4, else 16 + 4 g + j - 4: with a
+// row pitch of 32 bytes past a multiple of 256 the transposed reads of half a wave then
+// fall on distinct banks.
 struct Side {
-  Ranks u;
-  const float* scaling;    // per adapter, nullable
+  const void* packed;      // [positions / 32, parts, 16 RT, 32] of T: u as operands
   const void* v;           // [M, C] of T, or e4m3 bytes with `scales`
   const uint8_t* scales;
   int64_t ldv, C;
@@ -443,45 +479,208 @@ struct Side {
   float* partial;          // [2 windows, 16 RT, C]
 };
 
+template <typename T> constexpr int kParts = std::is_same<T, float>::value ? 1 : 2;
+
+// Packs 64 positions' ranks: blockIdx.y 0 sums g's planes, scales them, keeps the sum
+// for the expansion and packs it; 1 packs scaling * hidden.
+template <typename T, int RT>
+__global__ void __launch_bounds__(kThreads)
+lora_pack(Rows rows, Ranks g, Ranks h, const float* __restrict__ scaling, float* __restrict__ g_sum,
+          T* __restrict__ packed_g, T* __restrict__ packed_h) {
+  constexpr int RP = RT * 16, PITCH = RP + 1;
+  __shared__ float u[kTile * PITCH];
+  const int64_t pos = int64_t(blockIdx.x) * kTile;
+  if (pos >= *rows.num_post) return;
+  const bool is_g = blockIdx.y == 0;
+  const float s = scaling != nullptr ? scaling[rows.tile_adapter[blockIdx.x]] : 1.f;
+  for (int q = threadIdx.x; q < kTile * (RP / 4); q += kThreads) {
+    const int i = q / (RP / 4), rank = (q % (RP / 4)) * 4;
+    const int64_t m = rows.sorted[pos + i];
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (m < rows.M) {
+      v = ranks4(is_g ? g : h, m, rank) * s;
+      if (is_g) *reinterpret_cast<f32x4*>(g_sum + m * RP + rank) = v;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) u[i * PITCH + rank + j] = v[j];
+  }
+  __syncthreads();
+  T* out = (is_g ? packed_g : packed_h) + pos * RP * kParts<T>;
+  for (int q = threadIdx.x; q < 2 * RP * 4; q += kThreads) {  // a lane's 8 places of a rank, of 2 x 32 rows
+    const int p8 = q & 3, rank = (q >> 2) % RP, tile = (q >> 2) / RP;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = u[(32 * tile + 4 * p8 + (j & 3) + (j >> 2) * 16) * PITCH + rank];
+    T* o = out + ((tile * kParts<T>) * RP + rank) * 32 + 8 * p8;
+    if constexpr (std::is_same<T, float>::value) {
+      *reinterpret_cast<f32x4*>(o) = f32x4{v[0], v[1], v[2], v[3]};
+      *reinterpret_cast<f32x4*>(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    } else {
+      *reinterpret_cast<bf16x8*>(o) = split_part(v, false);
+      *reinterpret_cast<bf16x8*>(o + RP * 32) = split_part(v, true);
+    }
+  }
+}
+
 // Window j's plane for adapter range [off0, off1): at most one adapter that goes
 // on past a window starts in it, and at most one comes in from the window before.
 __device__ __forceinline__ int64_t plane_of(int64_t off0, int64_t window, int64_t seg) {
   return 2 * window + (off0 >= window * seg ? 1 : 0);
 }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ typename mm<T>::frag load_row_piece(const Side& sd, int64_t m, int64_t c, int n) {
-  if (sd.scales == nullptr) return load_frag<T, VEC>(static_cast<const T*>(sd.v) + m * sd.ldv + c, n);
-  typename mm<T>::frag f = zero_frag<T>();
-  if (n <= 0) return f;
-  const uint8_t* q = static_cast<const uint8_t*>(sd.v) + m * sd.ldv + c;
-  __attribute__((aligned(8))) uint8_t b[8];
-  if (VEC && n >= 8) {
-    *reinterpret_cast<uint64_t*>(b) = *reinterpret_cast<const uint64_t*>(q);
-  } else {
+// 16 e4m3 bytes (n of them a row's) and their block's scale.
+struct Piece8 {
+  u32x4 q;
+  uint32_t scale;
+};
+
+// Column tiles of a wgrad workgroup: 128 accumulators a lane at most.
+template <typename T, int RT> constexpr int kColTiles = (std::is_same<T, float>::value ? 4 : 8) / (RT == 8 ? 2 : 1);
+
+template <typename T, int RT, bool VEC, bool Q8>
+__device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t* __restrict__ sorted, int64_t M,
+                                            int64_t c0, int64_t p0, int64_t p1, int64_t out_at, float* plane,
+                                            unsigned char* lds) {
+  constexpr int RP = RT * 16, CT = kColTiles<T, RT>, BC = CT * 16, PITCH = BC + 32 / sizeof(T), PARTS = kParts<T>;
+  constexpr bool F32 = std::is_same<T, float>::value;
+  constexpr int PER = Q8 ? 16 : 8, PIECES = BC / PER, RPI = 64 / PIECES, NI = 32 / RPI;  // rows an instruction, instructions a tile
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
+  T* vt = reinterpret_cast<T*>(lds) + wave * 32 * PITCH;
+  f32x4 acc[CT][RT];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) b[i] = i < n ? q[i] : 0;
+  for (int e = 0; e < CT; ++e)
+#pragma unroll
+    for (int t = 0; t < RT; ++t) acc[e][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  typedef typename std::conditional<Q8, Piece8, typename mm<T>::frag>::type piece;
+  piece v[NI];
+  const int64_t col = c0 + (lane % PIECES) * PER;
+  const int n = int(min(int64_t(PER), max(int64_t(0), sd.C - col)));
+  auto fetch = [&](int64_t p) {  // the 32 rows from p on
+    const int row = sorted[p + (lane & 31)];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int64_t m = __shfl(row, i * RPI + lane / PIECES);
+      if constexpr (Q8) {
+        v[i].q = u32x4{0, 0, 0, 0};
+        v[i].scale = 127;
+        if (m < M && n > 0) {
+          const uint8_t* q = static_cast<const uint8_t*>(sd.v) + m * sd.ldv + col;
+          if (VEC && n == PER) {
+            v[i].q = *reinterpret_cast<const u32x4*>(q);
+          } else {
+            uint8_t* b = reinterpret_cast<uint8_t*>(&v[i].q);
+#pragma unroll
+            for (int j = 0; j < PER; ++j) b[j] = j < n ? q[j] : 0;
+          }
+          v[i].scale = sd.scales[m * cdiv(sd.C, kMx8Block) + col / kMx8Block];
+        }
+      } else {
+        v[i] = m < M ? load_frag<T, VEC>(static_cast<const T*>(sd.v) + m * sd.ldv + col, n) : zero_frag<T>();
+      }
+    }
+  };
+  int64_t p = p0 + wave * 32;
+  bool more = p < p1 && sorted[p] < M;  // padding ends an adapter's positions
+  if (more) fetch(p);
+  while (more) {
+    // u's operands of these rows, then the rows themselves to LDS
+    typename mm<T>::frag uf[PARTS][RT];
+    const T* up = static_cast<const T*>(sd.packed) + p * RP * PARTS + (lane & 15) * 32 + 8 * g;
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+      for (int t = 0; t < RT; ++t) uf[part][t] = load_frag<T, true>(up + (part * RP + 16 * t) * 32, 8);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      T* at = vt + (i * RPI + lane / PIECES) * PITCH + (lane % PIECES) * PER;
+      if constexpr (Q8) {
+        const float s = mx8_scale(v[i].scale);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float w[8];
+          mx8_unpack4(v[i].q[2 * h], w);
+          mx8_unpack4(v[i].q[2 * h + 1], w + 4);
+          typename mm<T>::frag f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) io<T>::store(reinterpret_cast<T*>(&f) + j, w[j] * s);
+#pragma unroll
+          for (int j = 0; j < int(sizeof(T)) / 2; ++j)
+            reinterpret_cast<u32x4*>(at + 8 * h)[j] = reinterpret_cast<const u32x4*>(&f)[j];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < int(sizeof(T)) / 2; ++j)
+          reinterpret_cast<u32x4*>(at)[j] = reinterpret_cast<const u32x4*>(&v[i])[j];
+      }
+    }
+    p += 32 * (kThreads / 64);
+    more = p < p1 && sorted[p] < M;
+    if (more) fetch(p);
+#pragma unroll
+    for (int e = 0; e < CT; ++e) {
+      typename mm<T>::frag vf;
+      if constexpr (F32) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) vf.v[j] = vt[(4 * g + (j & 3) + (j >> 2) * 16) * PITCH + e * 16 + (lane & 15)];
+      } else {
+        typedef short s4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s4 lds_s4;
+        T* at = vt + (4 * g + ((lane & 15) >> 2)) * PITCH + e * 16 + (lane & 3) * 4;
+        const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)at);
+        const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + 16 * PITCH));
+        vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+      }
+#pragma unroll
+      for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+        for (int t = 0; t < RT; ++t) acc[e][t] = mm<T>::mma(uf[part][t], vf, acc[e][t]);
+    }
   }
-  const float s = mx8_scale(sd.scales[m * cdiv(sd.C, kMx8Block) + c / kMx8Block]);
-  float w[8];
-  mx8_unpack4(reinterpret_cast<const uint32_t*>(b)[0], w);
-  mx8_unpack4(reinterpret_cast<const uint32_t*>(b)[1], w + 4);
+  // the waves' sums: a quarter of the column tiles at a time, which one wave adds in
+  // wave order and writes
+  constexpr int CQ = CT / 4 > 0 ? CT / 4 : 1;
+  f32x4* red = reinterpret_cast<f32x4*>(lds);  // [4 waves][CQ][RT][64]
 #pragma unroll
-  for (int i = 0; i < 8; ++i) io<T>::store(reinterpret_cast<T*>(&f) + i, i < n ? w[i] * s : 0.f);
-  return f;
+  for (int q = 0; q < CT / CQ; ++q) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < CQ; ++e)
+#pragma unroll
+      for (int t = 0; t < RT; ++t) red[((wave * CQ + e) * RT + t) * 64 + lane] = acc[q * CQ + e][t];
+    __syncthreads();
+    if (wave != q) continue;
+#pragma unroll
+    for (int e = 0; e < CQ; ++e) {
+      const int64_t c = c0 + (q * CQ + e) * 16 + (lane & 15);
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kThreads / 64; ++w) sum += red[((w * CQ + e) * RT + t) * 64 + lane];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int rank = 16 * t + 4 * g + i;
+          if (rank >= r || c >= sd.C) continue;
+          if (plane == nullptr)
+            io<T>::store(static_cast<T*>(sd.out) + out_at + (sd.by_rank ? rank * sd.C + c : c * r + rank), sum[i]);
+          else
+            plane[rank * sd.C + c] = sum[i];
+        }
+      }
+    }
+  }
 }
 
-template <typename T, int RT, bool VEC>
+template <typename T, int RT, bool VEC, bool Q8>
 __global__ void __launch_bounds__(kThreads)
-lora_wgrad(Side side_a, Side side_b, int a_chunks, const int32_t* __restrict__ sorted,
+lora_wgrad(Side side_a, Side side_b, int r, int a_strips, const int32_t* __restrict__ sorted,
            const int32_t* __restrict__ offsets, int L, int64_t M, int64_t seg) {
-  constexpr int RP = RT * 16, KB = 32, VP = kCols + 8, UP = KB + 8;
-  constexpr bool F32 = std::is_same<T, float>::value;
-  __shared__ __attribute__((aligned(16))) T vt[KB * VP];
-  __shared__ __attribute__((aligned(16))) T ut[(F32 ? 1 : 2) * RP * UP];  // [part][rank][row]
-  const bool is_a = int(blockIdx.y) < a_chunks;
+  constexpr int RP = RT * 16, BC = kColTiles<T, RT> * 16, PITCH = BC + 32 / sizeof(T);
+  constexpr int kTileBytes = 4 * 32 * PITCH * sizeof(T), kRedBytes = 4 * (BC / 64 > 0 ? BC / 64 : 1) * RT * 64 * 16;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[kTileBytes > kRedBytes ? kTileBytes : kRedBytes];
+  const bool is_a = int(blockIdx.y) < a_strips;
   const Side& sd = is_a ? side_a : side_b;
-  const int64_t c0 = int64_t(is_a ? blockIdx.y : blockIdx.y - a_chunks) * kCols;
+  const int64_t c0 = int64_t(is_a ? blockIdx.y : blockIdx.y - a_strips) * BC;
   // pair (adapter, window) number blockIdx.x: adapter i takes the numbers from
   // offsets[i] / seg + i, one per window that it touches
   const int64_t want = blockIdx.x;
@@ -493,84 +692,17 @@ lora_wgrad(Side side_a, Side side_b, int a_chunks, const int32_t* __restrict__ s
   const int64_t off0 = offsets[lo], off1 = offsets[lo + 1], window = want - lo;
   if (off0 == off1 || window < off0 / seg || window > (off1 - 1) / seg) return;
   const int64_t p0 = max(off0, window * seg), p1 = min(off1, (window + 1) * seg);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
-  const float s = sd.scaling != nullptr ? sd.scaling[lo] : 1.f;
-  f32x4 acc[2][RT];
-#pragma unroll
-  for (int e = 0; e < 2; ++e)
-#pragma unroll
-    for (int t = 0; t < RT; ++t) acc[e][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int64_t p = p0; p < p1; p += KB) {
-    if (sorted[p] >= M) break;  // padding ends an adapter's positions
-    for (int q = tid; q < KB * (kCols / 8); q += kThreads) {
-      const int row = q / (kCols / 8), c = (q % (kCols / 8)) * 8;
-      const int64_t m = sorted[p + row];
-      const int n = int(min(int64_t(8), max(int64_t(0), sd.C - c0 - c)));
-      const typename mm<T>::frag f = m < M ? load_row_piece<T, VEC>(sd, m, c0 + c, n) : zero_frag<T>();
-#pragma unroll
-      for (int i = 0; i < int(sizeof(T)) / 2; ++i)
-        reinterpret_cast<u32x4*>(vt + row * VP + c)[i] = reinterpret_cast<const u32x4*>(&f)[i];
-    }
-    for (int q = tid; q < KB * (RP / 4); q += kThreads) {
-      const int row = q / (RP / 4), rank = (q % (RP / 4)) * 4;
-      const int64_t m = sorted[p + row];
-      f32x4 v = {0.f, 0.f, 0.f, 0.f};
-      if (m < M) v = ranks4(sd.u, m, rank) * s;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (F32) {
-          ut[(rank + i) * UP + row] = v[i];
-        } else {
-          const uint16_t hi16 = f32_to_bf16(v[i]);
-          ut[(rank + i) * UP + row] = hi16;
-          ut[(RP + rank + i) * UP + row] = f32_to_bf16(rest_of(v[i], bf16_to_f32(hi16)));
-        }
-      }
-    }
-    __syncthreads();
-    typename mm<T>::frag vf[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        reinterpret_cast<T*>(&vf[e])[j] = vt[(8 * g + j) * VP + wave * 32 + e * 16 + (lane & 15)];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-#pragma unroll
-      for (int part = 0; part < (F32 ? 1 : 2); ++part) {
-        const typename mm<T>::frag uf = load_frag<T, true>(ut + (part * RP + 16 * t + (lane & 15)) * UP + 8 * g, 8);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) acc[e][t] = mm<T>::mma(uf, vf[e], acc[e][t]);
-      }
-    }
-    __syncthreads();
-  }
   const bool whole = off0 / seg == (off1 - 1) / seg;
   float* plane = whole ? nullptr : sd.partial + plane_of(off0, window, seg) * RP * sd.C;
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int64_t c = c0 + wave * 32 + e * 16 + (lane & 15);
-    if (c >= sd.C) continue;
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int rank = 16 * t + 4 * g + i;
-        if (rank >= sd.u.r) continue;
-        if (whole) {
-          T* o = static_cast<T*>(sd.out) + int64_t(lo) * sd.u.r * sd.C;
-          io<T>::store(o + (sd.by_rank ? rank * sd.C + c : c * sd.u.r + rank), acc[e][t][i]);
-        } else {
-          plane[rank * sd.C + c] = acc[e][t][i];
-        }
-      }
-  }
+  const int64_t out_at = int64_t(lo) * r * sd.C;
+  if (is_a) wgrad_strip<T, RT, VEC, Q8>(sd, r, sorted, M, c0, p0, p1, out_at, plane, lds);
+  else wgrad_strip<T, RT, VEC, false>(sd, r, sorted, M, c0, p0, p1, out_at, plane, lds);
 }
 
 // Adds the planes of adapters over several windows; zeros for adapters without rows.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-wgrad_reduce(Side side_a, Side side_b, int a_blocks, int RP, const int32_t* __restrict__ offsets, int64_t seg) {
+wgrad_reduce(Side side_a, Side side_b, int r, int a_blocks, int RP, const int32_t* __restrict__ offsets, int64_t seg) {
   const bool is_a = int(blockIdx.x) < a_blocks;
   const Side& sd = is_a ? side_a : side_b;
   const int i = blockIdx.y;
@@ -578,7 +710,6 @@ wgrad_reduce(Side side_a, Side side_b, int a_blocks, int RP, const int32_t* __re
   const int64_t w0 = off0 / seg, w1 = off1 > off0 ? (off1 - 1) / seg : w0 - 1;
   if (w1 == w0) return;
   const int64_t q = int64_t(is_a ? blockIdx.x : blockIdx.x - a_blocks) * kThreads + threadIdx.x;
-  const int r = sd.u.r;
   if (q >= r * sd.C) return;
   const int64_t rank = q / sd.C, c = q % sd.C;
   float v = 0.f;
@@ -613,10 +744,10 @@ struct Slices {
   int64_t len;
   int count;
   Slices(int64_t C, int64_t tiles, bool few) {
-    const int64_t want = std::max<int64_t>(1, cdiv(few ? 512 : 1024, std::max<int64_t>(tiles, 1)));
+    const int64_t want = std::max<int64_t>(1, cdiv(few ? 512 : 768, std::max<int64_t>(tiles, 1)));
     const int64_t least = few ? 256 : 512;
     const int64_t n = std::max<int64_t>(1, std::min(want, cdiv(C, least)));
-    const int64_t unit = few ? 128 : 32;
+    const int64_t unit = 128;
     len = cdiv(cdiv(C, n), unit) * unit;
     count = int(cdiv(C, len));
   }
@@ -716,19 +847,25 @@ struct Windows {
 struct BackwardPlan {
   Sort sort;
   Slices slices;
-  int64_t a_chunks, b_chunks;
+  int64_t a_strips, b_strips;
   Windows win;
-  int64_t at, bt, planes, part_a, part_b, total;
+  int64_t at, bt, planes, g_sum, packed_g, packed_h, part_a, part_b, total;
   BackwardPlan(int64_t M, int64_t K, int64_t N, int L, int r, int64_t elem)
-      : sort(M, L), slices(N, sort.tiles, false), a_chunks(cdiv(K, kCols)), b_chunks(cdiv(N, kCols)),
-        win(M, L, a_chunks + b_chunks) {
-    const int64_t RP = rank_tiles(r) * 16;
+      : sort(M, L), slices(N, sort.tiles, false), a_strips(cdiv(K, strip(r, elem))), b_strips(cdiv(N, strip(r, elem))),
+        win(M, L, a_strips + b_strips) {
+    const int64_t RP = rank_tiles(r) * 16, packed = sort.tiles * kTile * RP * 4;  // two bf16 or one fp32
     at = sort.total;
     bt = at + up(int64_t(L) * r * K * elem);
     planes = bt + up(int64_t(L) * r * N * elem);
-    part_a = planes + up(int64_t(slices.count) * M * RP * 4);
+    g_sum = planes + up(int64_t(slices.count) * M * RP * 4);
+    packed_g = g_sum + up(M * RP * 4);
+    packed_h = packed_g + up(packed);
+    part_a = packed_h + up(packed);
     part_b = part_a + (win.count > 1 ? up(2 * win.count * RP * K * 4) : 0);
     total = part_b + (win.count > 1 ? up(2 * win.count * RP * N * 4) : 0);
+  }
+  static int64_t strip(int r, int64_t elem) {
+    return 16 * (rank_tiles(r) == 8 ? 2 : 4) * (elem == 2 ? 2 : 1);
   }
 };
 
@@ -768,11 +905,15 @@ int backward_typed(const T* dy, int64_t lddy, const void* x, int64_t ldx, const 
                        offsets, out);
   };
   const Ranks g{planes, M * RP, plan.slices.count, RP, r};
-  const Side sa{g, scaling, x, x_scales, ldx, K, da, 1, reinterpret_cast<float*>(ws + plan.part_a)};
-  const Side sb{Ranks{hidden, 0, 1, r, r}, scaling, dy, nullptr, lddy, N, db, 0, reinterpret_cast<float*>(ws + plan.part_b)};
+  const Ranks h{hidden, 0, 1, r, r};
+  float* g_sum = reinterpret_cast<float*>(ws + plan.g_sum);
+  T* packed_g = reinterpret_cast<T*>(ws + plan.packed_g);
+  T* packed_h = reinterpret_cast<T*>(ws + plan.packed_h);
+  const Side sa{packed_g, x, x_scales, ldx, K, da, 1, reinterpret_cast<float*>(ws + plan.part_a)};
+  const Side sb{packed_h, dy, nullptr, lddy, N, db, 0, reinterpret_cast<float*>(ws + plan.part_b)};
   const int64_t ab = cdiv(r * K, kThreads), bb = cdiv(r * N, kThreads);
   const auto reduce = [&]() {
-    hipLaunchKernelGGL((wgrad_reduce<T>), dim3(unsigned(ab + bb), L), dim3(kThreads), 0, stream, sa, sb, int(ab), RP,
+    hipLaunchKernelGGL((wgrad_reduce<T>), dim3(unsigned(ab + bb), L), dim3(kThreads), 0, stream, sa, sb, r, int(ab), RP,
                        offsets, plan.win.seg);
     XK_CHECK_LAUNCH("wgrad_reduce");
     return XK_OK;
@@ -784,20 +925,28 @@ int backward_typed(const T* dy, int64_t lddy, const void* x, int64_t ldx, const 
   XK_CHECK_LAUNCH("lora transpose");
   run_shrink<T>(rows, plan.sort.tiles, false, dy, lddy, N, bt, r, plan.slices, planes, stream);
   XK_CHECK_LAUNCH("lora_shrink");
-  run_expand<T>(rows, plan.sort.tiles, false, g, at, scaling, static_cast<const T*>(nullptr), 0, K, dx,
-                static_cast<float*>(nullptr), stream);
-  XK_CHECK_LAUNCH("lora_expand");
-  // (8-byte pieces of 8-bit rows are aligned where 16-byte ones of T are)
-  const bool vec = K % 8 == 0 && N % 8 == 0 && ldx % 8 == 0 && lddy % 8 == 0 && aligned16({dy, x});
-  const dim3 grid(unsigned(plan.win.count + L), unsigned(plan.a_chunks + plan.b_chunks));
   with_ranks(r, [&](auto rt) {
     constexpr int RT = decltype(rt)::value;
-    if (vec)
-      hipLaunchKernelGGL((lora_wgrad<T, RT, true>), grid, dim3(kThreads), 0, stream, sa, sb, int(plan.a_chunks),
-                         rows.sorted, offsets, L, M, plan.win.seg);
-    else
-      hipLaunchKernelGGL((lora_wgrad<T, RT, false>), grid, dim3(kThreads), 0, stream, sa, sb, int(plan.a_chunks),
-                         rows.sorted, offsets, L, M, plan.win.seg);
+    hipLaunchKernelGGL((lora_pack<T, RT>), dim3(unsigned(plan.sort.tiles), 2), dim3(kThreads), 0, stream, rows, g, h,
+                       scaling, g_sum, packed_g, packed_h);
+  });
+  XK_CHECK_LAUNCH("lora_pack");
+  run_expand<T>(rows, plan.sort.tiles, false, Ranks{g_sum, 0, 1, RP, r}, at, static_cast<const float*>(nullptr),
+                static_cast<const T*>(nullptr), 0, K, dx, static_cast<float*>(nullptr), stream);
+  XK_CHECK_LAUNCH("lora_expand");
+  const int64_t unit = x_scales != nullptr ? 16 : 8;  // values of a piece of x
+  const bool vec = K % unit == 0 && ldx % unit == 0 && N % 8 == 0 && lddy % 8 == 0 && aligned16({dy, x});
+  const dim3 grid(unsigned(plan.win.count + L), unsigned(plan.a_strips + plan.b_strips));
+  with_ranks(r, [&](auto rt) {
+    constexpr int RT = decltype(rt)::value;
+#define XK_WGRAD(V, Q)                                                                                           \
+  hipLaunchKernelGGL((lora_wgrad<T, RT, V, Q>), grid, dim3(kThreads), 0, stream, sa, sb, r, int(plan.a_strips), \
+                     rows.sorted, offsets, L, M, plan.win.seg)
+    if (vec && x_scales != nullptr) XK_WGRAD(true, true);
+    else if (vec) XK_WGRAD(true, false);
+    else if (x_scales != nullptr) XK_WGRAD(false, true);
+    else XK_WGRAD(false, false);
+#undef XK_WGRAD
   });
   XK_CHECK_LAUNCH("lora_wgrad");
   return reduce();
