@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(kThreads)
 lora_expand(Rows rows, int64_t tiles, Ranks h, const T* __restrict__ b, const float* __restrict__ scaling,
             const T* __restrict__ base, int64_t ldbase, int64_t N, int64_t chunk, T* __restrict__ out,
             float* __restrict__ hidden) {
-  constexpr int RP = RT * 16, BM = FEW ? kFewTile : kTile, BT = BM / 16, PITCH = RP + 4;
+  constexpr int RP = RT * 16, BM = FEW ? kFewTile : kTile, PITCH = RP + 4;
   __shared__ int tile_rows[BM];
   __shared__ __attribute__((aligned(16))) float hs[BM * PITCH];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
@@ -356,15 +356,22 @@ lora_expand(Rows rows, int64_t tiles, Ranks h, const T* __restrict__ b, const fl
     *reinterpret_cast<f32x4*>(hs + i * PITCH + rank) = v * s;
   }
   __syncthreads();
+  // Sorted tiles: a wave takes 32 of the rows and half of the chunk's columns; few
+  // rows: all 16 and a quarter. The weights and the base of the next 32 columns are on
+  // their way while these are finished: loads and stores leave a wave's counter in
+  // order, so a load that is waited for right after a store waits for the store too.
+  constexpr int BW = FEW ? 1 : 2, CW = FEW ? 4 : 2;
+  const int row0 = FEW ? 0 : (wave & 1) * 32, cw = FEW ? wave : wave >> 1;
   const int rank0 = mm<T>::rank0(lane);
-  typename mm<T>::half hf[BT][RT];
-  int64_t m[BT];
+  typename mm<T>::half hf[BW][RT];
+  int64_t m[BW];
 #pragma unroll
-  for (int i = 0; i < BT; ++i) {
-    m[i] = tile_rows[16 * i + (lane & 15)];
+  for (int i = 0; i < BW; ++i) {
+    const int at = row0 + 16 * i + (lane & 15);
+    m[i] = tile_rows[at];
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      const float* p = hs + (16 * i + (lane & 15)) * PITCH + 16 * t + rank0;
+      const float* p = hs + at * PITCH + 16 * t + rank0;
       if constexpr (std::is_same<T, float>::value) {
         hf[i][t] = *reinterpret_cast<const f32x4*>(p);
       } else {
@@ -375,60 +382,63 @@ lora_expand(Rows rows, int64_t tiles, Ranks h, const T* __restrict__ b, const fl
       }
     }
   }
-  const T* bw = b + int64_t(adapter) * N * h.r;
+  const T* bw = b + int64_t(adapter) * N * h.r + rank0;
   const int nr = 8 * ((lane & 15) >> 2) + (lane & 3);  // this lane's weight row among 32, less 4 for the second product
-  // a wave's columns lie together; the next 32 of the base are on their way while
-  // these are finished
-  const int64_t w0 = c0 + wave * (chunk / 4), w1 = min(c1, w0 + chunk / 4);
-  typename mm<T>::frag next[BT];
+  const int64_t w0 = c0 + cw * (chunk / CW), w1 = min(c1, w0 + chunk / CW);
+  typename mm<T>::half wf[RT][2];
+  typename mm<T>::frag bs[BW];
   auto fetch = [&](int64_t n0) {
-    const int64_t nb = n0 + g * 8;
-    const int cnt = int(min(int64_t(8), max(int64_t(0), w1 - nb)));
 #pragma unroll
-    for (int i = 0; i < BT; ++i)
-      next[i] = base != nullptr && m[i] < rows.M && cnt > 0 ? load_frag<T, VEC>(base + m[i] * ldbase + nb, cnt)
-                                                             : zero_frag<T>();
-  };
-  if (w0 < w1) fetch(w0);
-  for (int64_t n0 = w0; n0 < w1; n0 += 32) {
-    const int64_t nb = n0 + g * 8;
-    const int cnt = int(min(int64_t(8), max(int64_t(0), w1 - nb)));
-    typename mm<T>::frag bs[BT];
-#pragma unroll
-    for (int i = 0; i < BT; ++i) bs[i] = next[i];
-    if (n0 + 32 < w1) fetch(n0 + 32);
-    f32x4 acc[BT][2];
-#pragma unroll
-    for (int i = 0; i < BT; ++i) acc[i][0] = acc[i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
+    for (int t = 0; t < RT; ++t)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int64_t n = n0 + nr + 4 * e;
-        const int left = n < w1 ? h.r - 16 * t - rank0 : 0;
-        const typename mm<T>::half wf = load_half<T, VEC>(bw + n * h.r + 16 * t + rank0, left);
-#pragma unroll
-        for (int i = 0; i < BT; ++i) acc[i][e] = mm<T>::mma_half(wf, hf[i][t], acc[i][e]);
+        wf[t][e] = load_half<T, VEC>(bw + n * h.r + 16 * t, n < w1 ? h.r - 16 * t - rank0 : 0);
       }
-    }
+    const int64_t nb = n0 + g * 8;
+    const int cnt = int(min(int64_t(8), max(int64_t(0), w1 - nb)));
 #pragma unroll
-    for (int i = 0; i < BT; ++i) {
-      if (m[i] >= rows.M || cnt == 0) continue;
-      typename mm<T>::frag o;
+    for (int i = 0; i < BW; ++i)
+      bs[i] = base != nullptr && m[i] < rows.M && cnt > 0 ? load_frag<T, VEC>(base + m[i] * ldbase + nb, cnt)
+                                                           : zero_frag<T>();
+  };
+  if (w0 >= w1) return;
+  fetch(w0);
+  for (int64_t n0 = w0; n0 < w1; n0 += 32) {
+    const int64_t nb = n0 + g * 8;
+    const int cnt = int(min(int64_t(8), max(int64_t(0), w1 - nb)));
+    f32x4 acc[BW][2];
+#pragma unroll
+    for (int i = 0; i < BW; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) acc[i][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int i = 0; i < BW; ++i) acc[i][e] = mm<T>::mma_half(wf[t][e], hf[i][t], acc[i][e]);
+    typename mm<T>::frag o[BW];
+#pragma unroll
+    for (int i = 0; i < BW; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const T bv = reinterpret_cast<const T*>(&bs[i])[j];
-        io<T>::store(reinterpret_cast<T*>(&o) + j, io<T>::load(&bv) + acc[i][j >> 2][j & 3]);
+        io<T>::store(reinterpret_cast<T*>(&o[i]) + j, io<T>::load(&bv) + acc[i][j >> 2][j & 3]);
       }
+    if (n0 + 32 < w1) fetch(n0 + 32);
+#pragma unroll
+    for (int i = 0; i < BW; ++i) {
+      if (m[i] >= rows.M || cnt == 0) continue;
       T* p = out + m[i] * N + nb;
       if (VEC && cnt == 8) {
 #pragma unroll
         for (int j = 0; j < int(sizeof(T)) / 2; ++j)
-          reinterpret_cast<u32x4*>(p)[j] = reinterpret_cast<const u32x4*>(&o)[j];
+          reinterpret_cast<u32x4*>(p)[j] = reinterpret_cast<const u32x4*>(&o[i])[j];
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (j < cnt) p[j] = reinterpret_cast<const T*>(&o)[j];
+          if (j < cnt) p[j] = reinterpret_cast<const T*>(&o[i])[j];
       }
     }
   }
@@ -555,8 +565,7 @@ __device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t
   piece v[NI];
   const int64_t col = c0 + (lane % PIECES) * PER;
   const int n = int(min(int64_t(PER), max(int64_t(0), sd.C - col)));
-  auto fetch = [&](int64_t p) {  // the 32 rows from p on
-    const int row = sorted[p + (lane & 31)];
+  auto fetch = [&](int row) {  // the 32 rows whose numbers lanes 0 .. 31 hold
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int64_t m = __shfl(row, i * RPI + lane / PIECES);
@@ -579,9 +588,14 @@ __device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t
       }
     }
   };
+  // row numbers are read a tile ahead of the rows; padding (M) ends an adapter's positions
+  constexpr int kStep = 32 * (kThreads / 64);
   int64_t p = p0 + wave * 32;
-  bool more = p < p1 && sorted[p] < M;  // padding ends an adapter's positions
-  if (more) fetch(p);
+  auto row_at = [&](int64_t p) { return p < p1 ? int64_t(sorted[p + (lane & 31)]) : M; };
+  auto any = [&](int64_t row) { return __builtin_amdgcn_readfirstlane(int(row)) < M; };
+  int64_t row = row_at(p), next = row_at(p + kStep);
+  bool more = any(row);
+  if (more) fetch(int(row));
   while (more) {
     // u's operands of these rows, then the rows themselves to LDS
     typename mm<T>::frag uf[PARTS][RT];
@@ -613,9 +627,11 @@ __device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t
           reinterpret_cast<u32x4*>(at)[j] = reinterpret_cast<const u32x4*>(&v[i])[j];
       }
     }
-    p += 32 * (kThreads / 64);
-    more = p < p1 && sorted[p] < M;
-    if (more) fetch(p);
+    p += kStep;
+    row = next;
+    more = any(row);
+    if (more) fetch(int(row));
+    next = row_at(p + kStep);
 #pragma unroll
     for (int e = 0; e < CT; ++e) {
       typename mm<T>::frag vf;
