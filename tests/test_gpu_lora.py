@@ -69,6 +69,21 @@ def test_backward(M, K, N, L, r, dt, dev):
     assert all(torch.equal(p, q) for p, q in zip(got, again))
 
 
+@pytest.mark.parametrize("M,L,runs", [(70001, 1000, False), (70001, 1, False), (65536, 7, True), (66000, 1024, True),
+                                     (1500, 1024, False)])
+def test_many_rows(M, L, runs, dev):
+    """The sort's sizes: batches that are counted apart, and the most adapters."""
+    x, a, b, ids, base, dy, sc = _case(M, 32, 16, L, 4, BF, seed=L, runs=runs)
+    out, hidden = xk.lora_projection(x, a, b, ids, base=base, scaling=sc, return_hidden=True)
+    want, h, bound, hb = lora_ref(x, a, b, ids, base, sc)
+    check(out, want, bound, "out")
+    check(hidden, h, hb, "hidden")
+    got = xk.lora_projection_backward(dy, x, a, b, ids, hidden, scaling=sc)
+    want, bounds = lora_grad_ref(dy, x, a, b, ids, hidden, sc)
+    for name, g, w, bd in zip(("grad_x", "grad_a", "grad_b"), got, want, bounds):
+        check(g, w, bd, name)
+
+
 @pytest.mark.parametrize("M,K,N,L,r", [(1, 64, 32, 1, 16), (70, 100, 40, 3, 8), (600, 2880, 200, 2, 16), (333, 47, 9, 4, 6),
                                        (1500, 256, 128, 1, 32)])
 @pytest.mark.parametrize("dt", [BF, F32])

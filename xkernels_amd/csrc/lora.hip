@@ -12,9 +12,8 @@
 // once, in 16-byte pieces straight into MFMA operands, and the adapters' weights,
 // which many rows share, come from L2.
 //
-// Rows are sorted by adapter into tiles of 64 (the library's align); batches of up to
-// kFew rows instead let each workgroup find its tile of 16 itself, one launch
-// less. Contractions over a long axis are split over workgroups into planes, which
+// Rows are sorted by adapter into tiles of 64 (lora_prepare); batches of up to kFew
+// rows instead let each workgroup find its tile of 16 itself, one launch less. Contractions over a long axis are split over workgroups into planes, which
 // the next kernel adds in order: no atomics, results do not depend on scheduling.
 //
 // Precision: bf16 operands, fp32 sums. What stands between two products (h, g) is
@@ -28,12 +27,6 @@
 
 namespace xk {
 
-int64_t align_workspace_bytes(int64_t numel, int num_experts);
-int launch_align(const int32_t* ids, int64_t numel, int num_experts, int block_size, const int32_t* emap,
-                 int num_global, int32_t* sorted_ids, int32_t* expert_ids, int32_t* num_post,
-                 int32_t* expert_offsets, void* workspace, int64_t workspace_bytes, hipStream_t stream,
-                 int* clear = nullptr, int nclear = 0, int clear_stride = 1);
-
 namespace {
 
 constexpr int kThreads = 256;
@@ -41,37 +34,27 @@ constexpr int kTile = 64;      // rows of a sorted tile
 constexpr int kFewTile = 16;   // rows of a tile that a workgroup finds itself
 constexpr int kFew = 256;      // rows up to which they do (a thread per row)
 constexpr int kMaxRank = 128;
+constexpr int kMaxAdapters = 1024;
+constexpr int kSortThreads = 1024;             // and rows a round of the sort
+constexpr int64_t kOneLaunchRows = 65536;      // rows up to which each sorting workgroup counts the whole batch
+constexpr int kMostChunks = 512;               // else a launch counts first, for at most so many workgroups
 
 // ------------------------------------------------------------- operands ----
-// frag: 8 contraction values of one operand row. half: 16 ranks as an operand, of
-// which a lane holds 8 (bf16: lanes 32..63 once more, for the pair's other part) or
-// 4 (fp32).
+// frag: 8 contraction values of one operand row.
 template <typename T> struct mm;
 template <> struct mm<uint16_t> {
   typedef bf16x8 frag;
-  typedef bf16x8 half;
-  static constexpr int kHalf = 8;
   __device__ __forceinline__ static f32x4 mma(frag a, frag b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
-  __device__ __forceinline__ static f32x4 mma_half(half a, half b, f32x4 c) { return mma(a, b, c); }
-  __device__ __forceinline__ static int rank0(int lane) { return ((lane >> 4) & 1) * 8; }
 };
 template <> struct mm<float> {
   struct alignas(16) frag { float v[8]; };
-  typedef f32x4 half;
-  static constexpr int kHalf = 4;
   __device__ __forceinline__ static f32x4 mma(const frag& a, const frag& b, f32x4 c) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[j], b.v[j], c, 0, 0, 0);
     return c;
   }
-  __device__ __forceinline__ static f32x4 mma_half(half a, half b, f32x4 c) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
-    return c;
-  }
-  __device__ __forceinline__ static int rank0(int lane) { return (lane >> 4) * 4; }
 };
 
 // n values at p (n <= 8; the rest zero). VEC: whole ones are 16-byte aligned.
@@ -96,20 +79,6 @@ __device__ __forceinline__ typename mm<T>::frag zero_frag() {
   for (int i = 0; i < int(sizeof(T)) / 2; ++i) reinterpret_cast<u32x4*>(&f)[i] = u32x4{0, 0, 0, 0};
   return f;
 }
-// n of a lane's ranks of a half operand at p.
-template <typename T, bool VEC>
-__device__ __forceinline__ typename mm<T>::half load_half(const T* p, int n) {
-  typename mm<T>::half f;
-  if (VEC && n >= mm<T>::kHalf) {
-    *reinterpret_cast<u32x4*>(&f) = *reinterpret_cast<const u32x4*>(p);
-  } else {
-    T* v = reinterpret_cast<T*>(&f);
-#pragma unroll
-    for (int i = 0; i < mm<T>::kHalf; ++i) v[i] = i < n ? p[i] : T(0);
-  }
-  return f;
-}
-
 // What hi leaves of v; 0 where hi is infinite or NaN and says it all.
 __device__ __forceinline__ float rest_of(float v, float hi) {
   const float rest = v - hi;
@@ -126,14 +95,66 @@ __device__ __forceinline__ bf16x8 split_part(const float* v, bool low) {
   return f;
 }
 
+// The expansion's contraction, over ranks. bf16, up to 16 of them: one MFMA takes the
+// weights twice, against hi and lo. More: blocks of 32 ranks, the weights' operand
+// serves an MFMA with hi and one with lo (half the loads). fp32: blocks of 16.
+template <typename T, int RT> struct rank_blocks {
+  static constexpr bool kBoth = RT == 1;
+  static constexpr int kRanks = kBoth ? 16 : 32, kBlocks = kBoth ? 1 : RT / 2;
+  typedef bf16x8 weight;
+  struct hidden { bf16x8 part[kBoth ? 1 : 2]; };
+  __device__ __forceinline__ static int rank0(int lane) { return (kBoth ? (lane >> 4) & 1 : lane >> 4) * 8; }
+  __device__ __forceinline__ static hidden make(const float* p, int lane) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = p[j];
+    hidden h;
+    if constexpr (kBoth) {
+      h.part[0] = split_part(v, lane >= 32);
+    } else {
+      h.part[0] = split_part(v, false);
+      h.part[1] = split_part(v, true);
+    }
+    return h;
+  }
+  template <bool VEC> __device__ __forceinline__ static weight load(const uint16_t* p, int n) {
+    return load_frag<uint16_t, VEC>(p, n);
+  }
+  __device__ __forceinline__ static f32x4 mma(const weight& w, const hidden& h, f32x4 c) {
+    c = mm<uint16_t>::mma(w, h.part[0], c);
+    if constexpr (!kBoth) c = mm<uint16_t>::mma(w, h.part[1], c);
+    return c;
+  }
+};
+template <int RT> struct rank_blocks<float, RT> {
+  static constexpr int kRanks = 16, kBlocks = RT;
+  typedef f32x4 weight;
+  typedef f32x4 hidden;
+  __device__ __forceinline__ static int rank0(int lane) { return (lane >> 4) * 4; }
+  __device__ __forceinline__ static hidden make(const float* p, int) { return *reinterpret_cast<const f32x4*>(p); }
+  template <bool VEC> __device__ __forceinline__ static weight load(const float* p, int n) {
+    if (VEC && n >= 4) return *reinterpret_cast<const f32x4*>(p);
+    weight w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = i < n ? p[i] : 0.f;
+    return w;
+  }
+  __device__ __forceinline__ static f32x4 mma(const weight& w, const hidden& h, f32x4 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(w[j], h[j], c, 0, 0, 0);
+    return c;
+  }
+};
+
 // ----------------------------------------------------------------- rows ----
-struct Rows {  // sorted tiles, or (sorted == nullptr) at most kFew rows unsorted
+struct Rows {
   const int32_t* ids;
   int64_t M;
   int L;
-  const int32_t* sorted;
-  const int32_t* tile_adapter;
-  const int32_t* num_post;
+  // more than kFew rows: sorted by adapter, the rows without one last, each group
+  // filled up with M to whole tiles
+  const int32_t* sorted;        // [tiles, 64] row numbers
+  const int32_t* tile_adapter;  // [tiles]: L for rows without an adapter, -1 for unused tiles
 };
 
 // The tile of up to 16 rows that row j leads: rows of one adapter in ascending
@@ -163,6 +184,211 @@ __device__ __forceinline__ int few_tile(const Rows& a, int j, int* rows) {
   return want;
 }
 
+// ----------------------------------------------------------------- sort ----
+// A stable sort of the rows by adapter into tiles. Group L holds the rows without an
+// adapter. A workgroup places rounds of 1,024 rows of its part of the batch; what
+// lies before it, and the groups' sizes, it counts itself over the whole batch (64 KB
+// of ids at 16,384 rows, from L2: one launch where counting apart needs two) up to
+// kOneLaunchRows, past which lora_count leaves counts of every part.
+struct SortOut {
+  int32_t* sorted;
+  int32_t* tile_adapter;
+  int32_t* offsets;  // [L + 1]: where the groups' positions begin
+  int32_t* counts;   // [chunks, L + 1], with lora_count
+  int64_t tiles;
+};
+
+__device__ __forceinline__ int group_of(int id, int L) { return id >= 0 && id < L ? id : L; }
+
+// cnt[g] += lanes of group g; runs of one group, as requests' rows are, cost one add.
+__device__ __forceinline__ void count_groups(int* cnt, int g, bool in) {
+  const uint64_t active = __ballot(in);
+  if (active == 0) return;
+  const int first = __shfl(g, __ffsll(static_cast<unsigned long long>(active)) - 1);
+  const uint64_t same = __ballot(in && g == first);
+  if (same == active) {
+    if ((threadIdx.x & 63) == 0) atomicAdd(&cnt[first], __popcll(active));
+  } else if (in) {
+    atomicAdd(&cnt[g], 1);
+  }
+}
+
+__global__ void __launch_bounds__(kSortThreads)
+lora_count(const int32_t* __restrict__ ids, int64_t M, int L, int64_t part, int32_t* __restrict__ counts) {
+  __shared__ int cnt[kMaxAdapters + 1];
+  for (int g = threadIdx.x; g <= L; g += kSortThreads) cnt[g] = 0;
+  __syncthreads();
+  const int64_t first = int64_t(blockIdx.x) * part, end = min(M, first + part);
+  for (int64_t i = first; i < end; i += kSortThreads) {
+    const bool in = i + threadIdx.x < end;
+    count_groups(cnt, in ? group_of(ids[i + threadIdx.x], L) : 0, in);
+  }
+  __syncthreads();
+  for (int g = threadIdx.x; g <= L; g += kSortThreads) counts[int64_t(blockIdx.x) * (L + 1) + g] = cnt[g];
+}
+
+__device__ __forceinline__ void sort_part(const int32_t* __restrict__ ids, int64_t M, int L, int64_t part, int chunks,
+                                          bool counted, SortOut o) {
+  __shared__ int total[kMaxAdapters + 1], before[kMaxAdapters + 1], off[kMaxAdapters + 2];
+  __shared__ int wave_sum[kSortThreads / 64];
+  __shared__ __attribute__((aligned(16))) uint8_t in_wave[(kMaxAdapters + 1) * 16];  // [group][wave]
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, G = L + 1;
+  const int64_t first = int64_t(blockIdx.x) * part, end = min(M, first + part);
+  for (int g = tid; g < G; g += kSortThreads) total[g] = before[g] = 0;
+  __syncthreads();
+  if (counted) {
+    for (int64_t q = tid; q < int64_t(chunks) * G; q += kSortThreads) {
+      const int c = int(q / G), g = int(q - int64_t(c) * G), n = o.counts[q];
+      if (n == 0) continue;
+      atomicAdd(&total[g], n);
+      if (c < int(blockIdx.x)) atomicAdd(&before[g], n);
+    }
+  } else {
+    // (part is a multiple of kSortThreads, so a round is before it or not as a whole)
+    constexpr int kAhead = 8;
+    for (int64_t i0 = 0; i0 < M; i0 += kAhead * kSortThreads) {
+      int id[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int64_t i = i0 + j * kSortThreads + tid;
+        id[j] = i < M ? ids[i] : 0;
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int64_t i = i0 + j * kSortThreads + tid;
+        const int g = group_of(id[j], L);
+        count_groups(total, g, i < M);
+        if (i - tid < first) count_groups(before, g, i < M);
+      }
+    }
+  }
+  __syncthreads();
+  // positions of the groups: a prefix sum of the sizes in whole tiles (at most 1,025
+  // of them: the last thread takes two)
+  int mine = 0;
+  const int per = G > kSortThreads ? 2 : 1;
+  for (int j = 0; j < per; ++j)
+    if (tid * per + j < G) mine += (total[tid * per + j] + kTile - 1) / kTile * kTile;
+  int sum = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int v = __shfl_up(sum, d);
+    if (lane >= d) sum += v;
+  }
+  if (lane == 63) wave_sum[wave] = sum;
+  __syncthreads();
+  int at = sum - mine;
+  for (int w = 0; w < wave; ++w) at += wave_sum[w];
+  for (int j = 0; j < per; ++j) {
+    const int g = tid * per + j;
+    if (g > G) break;
+    off[g] = at;
+    if (g < G) at += (total[g] + kTile - 1) / kTile * kTile;
+  }
+  if (per == 1 && tid == G - 1) off[G] = at;
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int g = tid; g < G; g += kSortThreads) o.offsets[g] = off[g];
+  // this part's rows
+  const int bits = 32 - __clz(L);
+  for (int64_t i = first; i < end; i += kSortThreads) {
+    for (int q = tid; q < G * 4; q += kSortThreads) reinterpret_cast<uint32_t*>(in_wave)[q] = 0;
+    __syncthreads();
+    const int64_t row = i + tid;
+    const bool in = row < end;
+    const int g = in ? group_of(ids[row], L) : 0;
+    uint64_t peers = __ballot(in);
+    for (int b = 0; b < bits; ++b) {
+      const uint64_t set = __ballot((g >> b) & 1);
+      peers &= (g >> b) & 1 ? set : ~set;
+    }
+    const int rank = __popcll(peers & ((uint64_t(1) << lane) - 1));
+    if (in && rank == 0) in_wave[g * 16 + wave] = uint8_t(__popcll(peers));
+    __syncthreads();
+    if (in) {
+      const uint8_t* c = in_wave + g * 16;
+      int ahead = 0;
+      for (int w = 0; w < wave; ++w) ahead += c[w];
+      o.sorted[off[g] + before[g] + ahead + rank] = int(row);
+    }
+    __syncthreads();
+    for (int q = tid; q < G; q += kSortThreads) {
+      int n = 0;
+      for (int w = 0; w < 16; ++w) n += in_wave[q * 16 + w];
+      before[q] += n;
+    }
+    __syncthreads();
+  }
+  // the tiles' adapters and what fills them up, the tiles dealt out to the workgroups
+  for (int64_t t = int64_t(blockIdx.x) * (kSortThreads / kTile) + tid / kTile; t < o.tiles;
+       t += int64_t(chunks) * (kSortThreads / kTile)) {
+    const int64_t pos = t * kTile + tid % kTile;
+    int g = -1;
+    if (pos < off[G]) {
+      int lo = 0, hi = G - 1;  // the last group that begins at or before pos holds it (empty ones end there)
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (off[mid] <= pos) lo = mid; else hi = mid - 1;
+      }
+      g = lo;
+    }
+    if (tid % kTile == 0) o.tile_adapter[t] = g;
+    if (g < 0 || pos - off[g] >= total[g]) o.sorted[pos] = int(M);
+  }
+}
+
+// out[l, c, r] = in[l, r, c]. A thread takes 8 values along r, which it writes as 16
+// bytes (bf16) where rows of `out` are whole pieces.
+template <typename T>
+__device__ __forceinline__ void transpose_part(const T* __restrict__ in, int64_t L, int64_t R, int64_t C,
+                                               T* __restrict__ out, int64_t first, int64_t threads) {
+  const int64_t pieces = cdiv(R, 8), total = L * pieces * C;
+  for (int64_t q = first; q < total; q += threads) {
+    // neighbouring threads: along the shorter of the two, so that the wide side's
+    // accesses run through whole lines
+    int64_t l = q / (pieces * C), rest = q - l * (pieces * C), c, p;
+    if (R < C) {
+      c = rest / pieces;
+      p = rest - c * pieces;
+    } else {
+      p = rest / C;
+      c = rest - p * C;
+    }
+    const T* src = in + (l * R + p * 8) * C + c;
+    T* dst = out + (l * C + c) * R + p * 8;
+    const int n = int(min(int64_t(8), R - p * 8));
+    __attribute__((aligned(16))) T v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < n ? src[j * C] : T(0);
+    if (n == 8 && R % 8 == 0) {
+#pragma unroll
+      for (int j = 0; j < int(sizeof(T)) / 2; ++j) reinterpret_cast<u32x4*>(dst)[j] = reinterpret_cast<u32x4*>(v)[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < n) dst[j] = v[j];
+    }
+  }
+}
+
+// The sort, in `chunks` workgroups; for the backward more of them transpose the
+// weights, as the contractions there run along their other axis. (The gradients
+// of all adapters are written anyhow, as many bytes.)
+template <typename T>
+__global__ void __launch_bounds__(kSortThreads)
+lora_prepare(const int32_t* __restrict__ ids, int64_t M, int L, int64_t part, int chunks, int counted, SortOut o,
+             const T* __restrict__ a, const T* __restrict__ b, int64_t K, int64_t N, int r, T* __restrict__ at,
+             T* __restrict__ bt) {
+  if (int(blockIdx.x) < chunks) {
+    sort_part(ids, M, L, part, chunks, counted != 0, o);
+    return;
+  }
+  const int64_t first = int64_t(blockIdx.x - chunks) * kSortThreads + threadIdx.x;
+  const int64_t threads = int64_t(gridDim.x - chunks) * kSortThreads;
+  transpose_part<T>(a, L, r, K, at, first, threads);
+  transpose_part<T>(b, L, N, r, bt, first, threads);
+}
+
 // --------------------------------------------------------------- shrink ----
 // planes[s, m, 0 .. 16 RT): the sums over slice s of K for a tile's rows. The waves
 // split the slice, a quarter each for the whole tile: the weights' operands, which
@@ -185,11 +411,10 @@ lora_shrink(Rows rows, const T* __restrict__ x, int64_t ldx, int64_t K, const T*
     if (adapter < 0) return;
     m[0] = tile_rows[lane & 15];
   } else {
-    const int64_t pos = int64_t(blockIdx.x) * kTile;
-    if (pos >= *rows.num_post) return;
     adapter = rows.tile_adapter[blockIdx.x];
 #pragma unroll
-    for (int i = 0; i < BT; ++i) m[i] = rows.sorted[pos + 16 * i + (lane & 15)];
+    for (int i = 0; i < BT; ++i) m[i] = rows.sorted[int64_t(blockIdx.x) * kTile + 16 * i + (lane & 15)];
+    if (adapter < 0 || adapter >= rows.L) return;
   }
   const int g8 = (lane >> 4) * 8, rank = lane & 15;
   const T* xr[BT];
@@ -206,22 +431,29 @@ lora_shrink(Rows rows, const T* __restrict__ x, int64_t ldx, int64_t K, const T*
 #pragma unroll
     for (int t = 0; t < RT; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int64_t quarter = slice / 4, w0 = min(k1, k0 + wave * quarter), w1 = min(k1, w0 + quarter);
-  auto step = [&](int64_t k, int n) {
-    typename mm<T>::frag xf[BT];
+  typename mm<T>::frag xf[BT], af[RT];
+  auto fetch = [&](int64_t k) {
+    const int n = int(min(int64_t(8), max(int64_t(0), w1 - k - g8)));
 #pragma unroll
     for (int i = 0; i < BT; ++i) xf[i] = valid[i] ? load_frag<T, VEC>(xr[i] + k, n) : zero_frag<T>();
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const typename mm<T>::frag af =
-          16 * t + rank < r ? load_frag<T, VEC>(ar + int64_t(16 * t + rank) * K + k, n) : zero_frag<T>();
-#pragma unroll
-      for (int i = 0; i < BT; ++i) acc[i][t] = mm<T>::mma(af, xf[i], acc[i][t]);
-    }
+    for (int t = 0; t < RT; ++t)
+      af[t] = 16 * t + rank < r ? load_frag<T, VEC>(ar + int64_t(16 * t + rank) * K + k, n) : zero_frag<T>();
   };
-  int64_t k = w0;
-#pragma unroll(FEW ? 4 : 2)
-  for (; k + 32 <= w1; k += 32) step(k, 8);
-  if (k < w1) step(k, int(min(int64_t(8), max(int64_t(0), w1 - k - g8))));
+  if (w0 < w1) fetch(w0);
+#pragma unroll 2
+  for (int64_t k = w0; k < w1; k += 32) {
+    typename mm<T>::frag xc[BT], ac[RT];
+#pragma unroll
+    for (int i = 0; i < BT; ++i) xc[i] = xf[i];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) ac[t] = af[t];
+    if (k + 32 < w1) fetch(k + 32);
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int i = 0; i < BT; ++i) acc[i][t] = mm<T>::mma(ac[t], xc[i], acc[i][t]);
+  }
   // waves 2 and 3 hand theirs to 0 and 1, then 1 to 0
 #pragma unroll
   for (int half = 2; half >= 1; half >>= 1) {
@@ -287,7 +519,7 @@ __device__ __forceinline__ f32x4 ranks4(const Ranks& u, int64_t m, int rank) {
 // interleaved fours give it 8 of them, 16 bytes of bf16.
 template <typename T, int RT, bool VEC, bool FEW>
 __global__ void __launch_bounds__(kThreads)
-lora_expand(Rows rows, int64_t tiles, Ranks h, const T* __restrict__ b, const float* __restrict__ scaling,
+lora_expand(Rows rows, Ranks h, const T* __restrict__ b, const float* __restrict__ scaling,
             const T* __restrict__ base, int64_t ldbase, int64_t N, int64_t chunk, T* __restrict__ out,
             float* __restrict__ hidden) {
   constexpr int RP = RT * 16, BM = FEW ? kFewTile : kTile, PITCH = RP + 4;
@@ -298,26 +530,18 @@ lora_expand(Rows rows, int64_t tiles, Ranks h, const T* __restrict__ b, const fl
   int adapter;
   if (FEW) {
     adapter = few_tile(rows, blockIdx.x, tile_rows);
-    if (tid == 0 && adapter < 0) {  // a row without an adapter is its own workgroup's
+    if (adapter < 0) {  // a row without an adapter is its own workgroup's
       const int id = rows.ids[blockIdx.x];
-      tile_rows[0] = id < 0 || id >= rows.L ? int(blockIdx.x) : int(rows.M);
+      if (id >= 0 && id < rows.L) return;
+      if (tid == 0) tile_rows[0] = int(blockIdx.x);
     }
-    __syncthreads();
-  } else if (int64_t(blockIdx.x) < tiles) {
-    const int64_t pos = int64_t(blockIdx.x) * kTile;
-    if (pos >= *rows.num_post) return;
+  } else {
     adapter = rows.tile_adapter[blockIdx.x];
-    if (tid < BM) tile_rows[tid] = rows.sorted[pos + tid];
-    __syncthreads();
-  } else {  // the rows without an adapter among 64 in the batch's order
-    adapter = -1;
-    if (tid < BM) {
-      const int64_t m = (int64_t(blockIdx.x) - tiles) * kTile + tid;
-      const int id = m < rows.M ? rows.ids[m] : 0;
-      tile_rows[tid] = m < rows.M && (id < 0 || id >= rows.L) ? int(m) : int(rows.M);
-    }
-    __syncthreads();
+    if (tid < BM) tile_rows[tid] = rows.sorted[int64_t(blockIdx.x) * kTile + tid];
+    if (adapter < 0) return;
+    if (adapter == rows.L) adapter = -1;
   }
+  __syncthreads();
   if (adapter < 0) {
     for (int i = 0; i < (FEW ? 1 : BM); ++i) {
       const int64_t m = tile_rows[i];
@@ -357,53 +581,49 @@ lora_expand(Rows rows, int64_t tiles, Ranks h, const T* __restrict__ b, const fl
   }
   __syncthreads();
   // Sorted tiles: a wave takes 32 of the rows and half of the chunk's columns; few
-  // rows: all 16 and a quarter. The weights and the base of the next 32 columns are on
-  // their way while these are finished: loads and stores leave a wave's counter in
-  // order, so a load that is waited for right after a store waits for the store too.
+  // rows: all 16 and a quarter. The weights of the next 32 columns and the base of
+  // those after them are on their way while these are finished: loads and stores
+  // leave a wave's counter in order, so a load that is waited for right after a store
+  // waits for the store too.
   constexpr int BW = FEW ? 1 : 2, CW = FEW ? 4 : 2;
+  typedef rank_blocks<T, RT> rb;
   const int row0 = FEW ? 0 : (wave & 1) * 32, cw = FEW ? wave : wave >> 1;
-  const int rank0 = mm<T>::rank0(lane);
-  typename mm<T>::half hf[BW][RT];
+  const int rank0 = rb::rank0(lane);
+  typename rb::hidden hf[BW][rb::kBlocks];
   int64_t m[BW];
 #pragma unroll
   for (int i = 0; i < BW; ++i) {
     const int at = row0 + 16 * i + (lane & 15);
     m[i] = tile_rows[at];
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const float* p = hs + at * PITCH + 16 * t + rank0;
-      if constexpr (std::is_same<T, float>::value) {
-        hf[i][t] = *reinterpret_cast<const f32x4*>(p);
-      } else {
-        float v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = p[j];
-        hf[i][t] = split_part(v, g >= 2);
-      }
-    }
+    for (int t = 0; t < rb::kBlocks; ++t) hf[i][t] = rb::make(hs + at * PITCH + rb::kRanks * t + rank0, lane);
   }
   const T* bw = b + int64_t(adapter) * N * h.r + rank0;
   const int nr = 8 * ((lane & 15) >> 2) + (lane & 3);  // this lane's weight row among 32, less 4 for the second product
   const int64_t w0 = c0 + cw * (chunk / CW), w1 = min(c1, w0 + chunk / CW);
-  typename mm<T>::half wf[RT][2];
-  typename mm<T>::frag bs[BW];
-  auto fetch = [&](int64_t n0) {
+  if (w0 >= w1) return;
+  typename rb::weight wf[rb::kBlocks][2];
+  typename mm<T>::frag bs[2][BW];
+  auto fetch_weights = [&](int64_t n0) {
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
+    for (int t = 0; t < rb::kBlocks; ++t)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int64_t n = n0 + nr + 4 * e;
-        wf[t][e] = load_half<T, VEC>(bw + n * h.r + 16 * t, n < w1 ? h.r - 16 * t - rank0 : 0);
+        wf[t][e] = rb::template load<VEC>(bw + n * h.r + rb::kRanks * t, n < w1 ? h.r - rb::kRanks * t - rank0 : 0);
       }
+  };
+  auto fetch_base = [&](int64_t n0, typename mm<T>::frag (&to)[BW]) {
     const int64_t nb = n0 + g * 8;
     const int cnt = int(min(int64_t(8), max(int64_t(0), w1 - nb)));
 #pragma unroll
     for (int i = 0; i < BW; ++i)
-      bs[i] = base != nullptr && m[i] < rows.M && cnt > 0 ? load_frag<T, VEC>(base + m[i] * ldbase + nb, cnt)
+      to[i] = base != nullptr && m[i] < rows.M && cnt > 0 ? load_frag<T, VEC>(base + m[i] * ldbase + nb, cnt)
                                                            : zero_frag<T>();
   };
-  if (w0 >= w1) return;
-  fetch(w0);
+  fetch_base(w0, bs[0]);
+  fetch_weights(w0);
+  fetch_base(w0 + 32, bs[1]);
   for (int64_t n0 = w0; n0 < w1; n0 += 32) {
     const int64_t nb = n0 + g * 8;
     const int cnt = int(min(int64_t(8), max(int64_t(0), w1 - nb)));
@@ -413,20 +633,23 @@ lora_expand(Rows rows, int64_t tiles, Ranks h, const T* __restrict__ b, const fl
 #pragma unroll
       for (int e = 0; e < 2; ++e) acc[i][e] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
+    for (int t = 0; t < rb::kBlocks; ++t)
 #pragma unroll
       for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int i = 0; i < BW; ++i) acc[i][e] = mm<T>::mma_half(wf[t][e], hf[i][t], acc[i][e]);
+        for (int i = 0; i < BW; ++i) acc[i][e] = rb::mma(wf[t][e], hf[i][t], acc[i][e]);
     typename mm<T>::frag o[BW];
 #pragma unroll
     for (int i = 0; i < BW; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const T bv = reinterpret_cast<const T*>(&bs[i])[j];
+        const T bv = reinterpret_cast<const T*>(&bs[0][i])[j];
         io<T>::store(reinterpret_cast<T*>(&o[i]) + j, io<T>::load(&bv) + acc[i][j >> 2][j & 3]);
       }
-    if (n0 + 32 < w1) fetch(n0 + 32);
+    if (n0 + 32 < w1) fetch_weights(n0 + 32);
+#pragma unroll
+    for (int i = 0; i < BW; ++i) bs[0][i] = bs[1][i];
+    fetch_base(n0 + 64, bs[1]);
 #pragma unroll
     for (int i = 0; i < BW; ++i) {
       if (m[i] >= rows.M || cnt == 0) continue;
@@ -442,26 +665,6 @@ lora_expand(Rows rows, int64_t tiles, Ranks h, const T* __restrict__ b, const fl
       }
     }
   }
-}
-
-// ------------------------------------------------------------ transpose ----
-// out[l, c, r] = in[l, r, c] for the adapters that rows use (offsets differ).
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-transpose_used(const T* __restrict__ in, int64_t R, int64_t C, int64_t col_tiles, const int32_t* __restrict__ offsets,
-               T* __restrict__ out) {
-  __shared__ T tile[64][65];
-  const int l = blockIdx.y;
-  if (offsets[l] == offsets[l + 1]) return;
-  const int64_t r0 = int64_t(blockIdx.x) / col_tiles * 64, c0 = int64_t(blockIdx.x) % col_tiles * 64;
-  const T* src = in + int64_t(l) * R * C;
-  T* dst = out + int64_t(l) * R * C;
-  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-  for (int i = ty; i < 64; i += 4)
-    if (r0 + i < R && c0 + tx < C) tile[i][tx] = src[(r0 + i) * C + c0 + tx];
-  __syncthreads();
-  for (int i = ty; i < 64; i += 4)
-    if (c0 + i < C && r0 + tx < R) dst[(c0 + i) * R + r0 + tx] = tile[tx][i];
 }
 
 // ---------------------------------------------------------------- wgrad ----
@@ -500,9 +703,10 @@ lora_pack(Rows rows, Ranks g, Ranks h, const float* __restrict__ scaling, float*
   constexpr int RP = RT * 16, PITCH = RP + 1;
   __shared__ float u[kTile * PITCH];
   const int64_t pos = int64_t(blockIdx.x) * kTile;
-  if (pos >= *rows.num_post) return;
+  const int adapter = rows.tile_adapter[blockIdx.x];
+  if (adapter < 0 || adapter >= rows.L) return;
   const bool is_g = blockIdx.y == 0;
-  const float s = scaling != nullptr ? scaling[rows.tile_adapter[blockIdx.x]] : 1.f;
+  const float s = scaling != nullptr ? scaling[adapter] : 1.f;
   for (int q = threadIdx.x; q < kTile * (RP / 4); q += kThreads) {
     const int i = q / (RP / 4), rank = (q % (RP / 4)) * 4;
     const int64_t m = rows.sorted[pos + i];
@@ -739,17 +943,22 @@ int rank_tiles(int r) { return r <= 16 ? 1 : r <= 32 ? 2 : r <= 64 ? 4 : 8; }
 
 // Scratch of the sort by adapter.
 struct Sort {
-  int64_t sorted, tile_adapter, num_post, offsets, inner, inner_bytes, tiles, total;
+  int64_t tiles, part;
+  int chunks;
+  bool counted;
+  int64_t sorted, tile_adapter, offsets, counts, total;
   Sort(int64_t M, int L) {
-    const int64_t most = M + int64_t(L + 1) * (kTile - 1);
-    // a tile holds a row, and all but an adapter's last are full
-    tiles = std::min<int64_t>(M / kTile + L, M);
+    // the groups' last tiles hold a row at least, the others are full
+    tiles = std::min<int64_t>(M / kTile + L + 1, M);
+    counted = M > kOneLaunchRows;
+    part = cdiv(cdiv(M, counted ? kMostChunks : kOneLaunchRows / kSortThreads), kSortThreads) * kSortThreads;
+    part = std::max<int64_t>(part, kSortThreads);
+    chunks = int(std::max<int64_t>(1, cdiv(M, part)));
     int64_t o = 0;
-    sorted = o; o += up(most * 4);
-    tile_adapter = o; o += up(cdiv(most, kTile) * 4);
-    num_post = o; o += up(4);
+    sorted = o; o += up(tiles * kTile * 4);
+    tile_adapter = o; o += up(tiles * 4);
     offsets = o; o += up(int64_t(L + 1) * 4);
-    inner = o; inner_bytes = align_workspace_bytes(M, L); o += up(inner_bytes);
+    counts = o; o += counted ? up(int64_t(chunks) * (L + 1) * 4) : 0;
     total = o;
   }
 };
@@ -808,15 +1017,15 @@ void run_shrink(const Rows& rows, int64_t tiles, bool few, const T* x, int64_t l
 }
 
 template <typename T>
-void run_expand(const Rows& rows, int64_t tiles, bool few, const Ranks& h, const T* b, const float* scaling,
+void run_expand(const Rows& rows, int64_t tiles, bool few,  const Ranks& h, const T* b, const float* scaling,
                 const T* base, int64_t ldbase, int64_t N, T* out, float* hidden, hipStream_t stream) {
   const bool vec = N % 8 == 0 && h.r % 8 == 0 && (base == nullptr || ldbase % 8 == 0) && aligned16({b, base, out});
   const int64_t chunk = chunk_of(N, tiles, few);
-  const dim3 grid(unsigned(few ? rows.M : tiles + cdiv(rows.M, kTile)), unsigned(cdiv(N, chunk)));
+  const dim3 grid(unsigned(few ? rows.M : tiles), unsigned(cdiv(N, chunk)));
   with_ranks(h.r, [&](auto rt) {
     constexpr int RT = decltype(rt)::value;
 #define XK_EXPAND(V, F)                                                                                          \
-  hipLaunchKernelGGL((lora_expand<T, RT, V, F>), grid, dim3(kThreads), 0, stream, rows, tiles, h, b, scaling, base, \
+  hipLaunchKernelGGL((lora_expand<T, RT, V, F>), grid, dim3(kThreads), 0, stream, rows, h, b, scaling, base, \
                      ldbase, N, chunk, out, hidden)
     if (vec && few) XK_EXPAND(true, true);
     else if (vec) XK_EXPAND(true, false);
@@ -826,13 +1035,24 @@ void run_expand(const Rows& rows, int64_t tiles, bool few, const Ranks& h, const
   });
 }
 
-int sort_rows(const int32_t* ids, int64_t M, int L, const Sort& so, char* ws, Rows* rows, hipStream_t stream) {
-  rows->sorted = reinterpret_cast<int32_t*>(ws + so.sorted);
-  rows->tile_adapter = reinterpret_cast<int32_t*>(ws + so.tile_adapter);
-  rows->num_post = reinterpret_cast<int32_t*>(ws + so.num_post);
-  return launch_align(ids, M, L, kTile, nullptr, 0, reinterpret_cast<int32_t*>(ws + so.sorted),
-                      reinterpret_cast<int32_t*>(ws + so.tile_adapter), reinterpret_cast<int32_t*>(ws + so.num_post),
-                      reinterpret_cast<int32_t*>(ws + so.offsets), ws + so.inner, so.inner_bytes, stream);
+// Sorts the rows and, with a and b, transposes the weights.
+template <typename T>
+int prepare(const int32_t* ids, int64_t M, int L, const Sort& so, char* ws, Rows* rows, const T* a, const T* b, int64_t K,
+            int64_t N, int r, T* at, T* bt, hipStream_t stream) {
+  const SortOut o{reinterpret_cast<int32_t*>(ws + so.sorted), reinterpret_cast<int32_t*>(ws + so.tile_adapter),
+                  reinterpret_cast<int32_t*>(ws + so.offsets), reinterpret_cast<int32_t*>(ws + so.counts), so.tiles};
+  rows->sorted = o.sorted;
+  rows->tile_adapter = o.tile_adapter;
+  if (so.counted) {
+    hipLaunchKernelGGL(lora_count, dim3(so.chunks), dim3(kSortThreads), 0, stream, ids, M, L, so.part, o.counts);
+    XK_CHECK_LAUNCH("lora_count");
+  }
+  const int64_t pieces = a == nullptr ? 0 : int64_t(L) * (cdiv(r, 8) * K + cdiv(N, 8) * r);
+  const int64_t more = std::min<int64_t>(512, cdiv(pieces, 2 * kSortThreads));
+  hipLaunchKernelGGL((lora_prepare<T>), dim3(unsigned(so.chunks + more)), dim3(kSortThreads), 0, stream, ids, M, L,
+                     so.part, so.chunks, int(so.counted), o, a, b, K, N, r, at, bt);
+  XK_CHECK_LAUNCH("lora_prepare");
+  return XK_OK;
 }
 
 struct ForwardPlan {
@@ -890,9 +1110,10 @@ int forward_typed(const T* x, int64_t ldx, int64_t M, int64_t K, const T* a, con
                   const int32_t* ids, const float* scaling, const T* base, int64_t ldbase, T* out, float* hidden,
                   char* ws, hipStream_t stream) {
   const ForwardPlan plan(M, K, L, r);
-  Rows rows{ids, M, L, nullptr, nullptr, nullptr};
+  Rows rows{ids, M, L, nullptr, nullptr};
   if (!plan.few)
-    if (int rc = sort_rows(ids, M, L, plan.sort, ws, &rows, stream)) return rc;
+    if (int rc = prepare<T>(ids, M, L, plan.sort, ws, &rows, nullptr, nullptr, K, N, r, nullptr, nullptr, stream))
+      return rc;
   float* planes = reinterpret_cast<float*>(ws + plan.planes);
   run_shrink<T>(rows, plan.tiles, plan.few, x, ldx, K, a, r, plan.slices, planes, stream);
   XK_CHECK_LAUNCH("lora_shrink");
@@ -909,17 +1130,12 @@ int backward_typed(const T* dy, int64_t lddy, const void* x, int64_t ldx, const 
                    const float* hidden, T* dx, T* da, T* db, char* ws, hipStream_t stream) {
   const BackwardPlan plan(M, K, N, L, r, sizeof(T));
   const int RP = rank_tiles(r) * 16;
-  Rows rows{ids, M, L, nullptr, nullptr, nullptr};
-  if (int rc = sort_rows(ids, M, L, plan.sort, ws, &rows, stream)) return rc;
+  Rows rows{ids, M, L, nullptr, nullptr};
   const int32_t* offsets = reinterpret_cast<const int32_t*>(ws + plan.sort.offsets);
   T* at = reinterpret_cast<T*>(ws + plan.at);
   T* bt = reinterpret_cast<T*>(ws + plan.bt);
   float* planes = reinterpret_cast<float*>(ws + plan.planes);
-  const auto transpose = [&](const T* in, int64_t R, int64_t C, T* out) {
-    const int64_t ct = cdiv(C, 64);
-    hipLaunchKernelGGL((transpose_used<T>), dim3(unsigned(cdiv(R, 64) * ct), L), dim3(kThreads), 0, stream, in, R, C, ct,
-                       offsets, out);
-  };
+  if (int rc = prepare<T>(ids, M, L, plan.sort, ws, &rows, a, b, K, N, r, at, bt, stream)) return rc;
   const Ranks g{planes, M * RP, plan.slices.count, RP, r};
   const Ranks h{hidden, 0, 1, r, r};
   float* g_sum = reinterpret_cast<float*>(ws + plan.g_sum);
@@ -935,10 +1151,6 @@ int backward_typed(const T* dy, int64_t lddy, const void* x, int64_t ldx, const 
     return XK_OK;
   };
   if (M == 0) return reduce();  // no adapter has rows: zeros
-  transpose(b, N, r, bt);
-  XK_CHECK_LAUNCH("lora transpose");
-  transpose(a, r, K, at);
-  XK_CHECK_LAUNCH("lora transpose");
   run_shrink<T>(rows, plan.sort.tiles, false, dy, lddy, N, bt, r, plan.slices, planes, stream);
   XK_CHECK_LAUNCH("lora_shrink");
   with_ranks(r, [&](auto rt) {
