@@ -57,20 +57,32 @@ template <> struct mm<float> {
   }
 };
 
-// n values at p (n <= 8; the rest zero). VEC: whole ones are 16-byte aligned.
+// 8 values at p. VEC: widths are whole aligned pieces, one load and no condition, so
+// that loads stay in flight: the caller moves a pointer past the end to one that
+// can be read and drops or blanks what comes of it. Else n values and zeros.
 template <typename T, bool VEC>
-__device__ __forceinline__ typename mm<T>::frag load_frag(const T* p, int n) {
+__device__ __forceinline__ typename mm<T>::frag load_frag(const T* p, int64_t n) {
   typename mm<T>::frag f;
-  T* v = reinterpret_cast<T*>(&f);
-  if (VEC && n >= 8) {
+  if constexpr (VEC) {
 #pragma unroll
     for (int i = 0; i < int(sizeof(T)) / 2; ++i)
       reinterpret_cast<u32x4*>(&f)[i] = reinterpret_cast<const u32x4*>(p)[i];
   } else {
+    T* v = reinterpret_cast<T*>(&f);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : T(0);
   }
   return f;
+}
+template <typename T>
+__device__ __forceinline__ void blank_unless_frag(bool keep, typename mm<T>::frag& f) {
+#pragma unroll
+  for (int i = 0; i < int(sizeof(T)) / 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      u32x4& w = reinterpret_cast<u32x4*>(&f)[i];
+      w[j] = keep ? w[j] : 0u;
+    }
 }
 template <typename T>
 __device__ __forceinline__ typename mm<T>::frag zero_frag() {
@@ -120,6 +132,7 @@ template <typename T, int RT> struct rank_blocks {
   template <bool VEC> __device__ __forceinline__ static weight load(const uint16_t* p, int n) {
     return load_frag<uint16_t, VEC>(p, n);
   }
+  __device__ __forceinline__ static void blank_unless(bool keep, weight& w) { blank_unless_frag<uint16_t>(keep, w); }
   __device__ __forceinline__ static f32x4 mma(const weight& w, const hidden& h, f32x4 c) {
     c = mm<uint16_t>::mma(w, h.part[0], c);
     if constexpr (!kBoth) c = mm<uint16_t>::mma(w, h.part[1], c);
@@ -132,8 +145,12 @@ template <int RT> struct rank_blocks<float, RT> {
   typedef f32x4 hidden;
   __device__ __forceinline__ static int rank0(int lane) { return (lane >> 4) * 4; }
   __device__ __forceinline__ static hidden make(const float* p, int) { return *reinterpret_cast<const f32x4*>(p); }
+  __device__ __forceinline__ static void blank_unless(bool keep, weight& w) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = keep ? w[i] : 0.f;
+  }
   template <bool VEC> __device__ __forceinline__ static weight load(const float* p, int n) {
-    if (VEC && n >= 4) return *reinterpret_cast<const f32x4*>(p);
+    if constexpr (VEC) return *reinterpret_cast<const f32x4*>(p);
     weight w;
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = i < n ? p[i] : 0.f;
@@ -416,15 +433,15 @@ lora_shrink(Rows rows, const T* __restrict__ x, int64_t ldx, int64_t K, const T*
     for (int i = 0; i < BT; ++i) m[i] = rows.sorted[int64_t(blockIdx.x) * kTile + 16 * i + (lane & 15)];
     if (adapter < 0 || adapter >= rows.L) return;
   }
+  // Rows past the batch and ranks past r read others' values in their place: what
+  // comes of them stays in their own products, which are not used.
   const int g8 = (lane >> 4) * 8, rank = lane & 15;
   const T* xr[BT];
-  bool valid[BT];
+  const T* ar[RT];
 #pragma unroll
-  for (int i = 0; i < BT; ++i) {
-    valid[i] = m[i] < rows.M;
-    xr[i] = x + (valid[i] ? m[i] : 0) * ldx + g8;
-  }
-  const T* ar = a + int64_t(adapter) * r * K + g8;
+  for (int i = 0; i < BT; ++i) xr[i] = x + min(m[i], rows.M - 1) * ldx + g8;
+#pragma unroll
+  for (int t = 0; t < RT; ++t) ar[t] = a + (int64_t(adapter) * r + min(16 * t + rank, r - 1)) * K + g8;
   f32x4 acc[BT][RT];
 #pragma unroll
   for (int i = 0; i < BT; ++i)
@@ -433,26 +450,42 @@ lora_shrink(Rows rows, const T* __restrict__ x, int64_t ldx, int64_t K, const T*
   const int64_t quarter = slice / 4, w0 = min(k1, k0 + wave * quarter), w1 = min(k1, w0 + quarter);
   typename mm<T>::frag xf[BT], af[RT];
   auto fetch = [&](int64_t k) {
-    const int n = int(min(int64_t(8), max(int64_t(0), w1 - k - g8)));
 #pragma unroll
-    for (int i = 0; i < BT; ++i) xf[i] = valid[i] ? load_frag<T, VEC>(xr[i] + k, n) : zero_frag<T>();
+    for (int i = 0; i < BT; ++i) xf[i] = load_frag<T, VEC>(xr[i] + k, 8);
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
-      af[t] = 16 * t + rank < r ? load_frag<T, VEC>(ar + int64_t(16 * t + rank) * K + k, n) : zero_frag<T>();
+    for (int t = 0; t < RT; ++t) af[t] = load_frag<T, VEC>(ar[t] + k, 8);
   };
-  if (w0 < w1) fetch(w0);
+  const int64_t whole = w0 + (w1 - w0) / 32 * 32;
+  if (w0 < whole) fetch(w0);
 #pragma unroll 2
-  for (int64_t k = w0; k < w1; k += 32) {
+  for (int64_t k = w0; k < whole; k += 32) {
     typename mm<T>::frag xc[BT], ac[RT];
 #pragma unroll
     for (int i = 0; i < BT; ++i) xc[i] = xf[i];
 #pragma unroll
     for (int t = 0; t < RT; ++t) ac[t] = af[t];
-    if (k + 32 < w1) fetch(k + 32);
+    fetch(min(k + 32, whole - 32));  // (the last one again at the end: a load less to decide on)
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
       for (int i = 0; i < BT; ++i) acc[i][t] = mm<T>::mma(ac[t], xc[i], acc[i][t]);
+  }
+  if (whole < w1) {  // K's last, not whole 32
+    const int64_t n = w1 - whole - g8, back = VEC && n <= 0 ? whole + g8 : 0;
+#pragma unroll
+    for (int i = 0; i < BT; ++i) {
+      xf[i] = load_frag<T, VEC>(xr[i] + whole - back, n);
+      if (VEC) blank_unless_frag<T>(n > 0, xf[i]);
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      af[t] = load_frag<T, VEC>(ar[t] + whole - back, n);
+      if (VEC) blank_unless_frag<T>(n > 0, af[t]);
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int i = 0; i < BT; ++i) acc[i][t] = mm<T>::mma(af[t], xf[i], acc[i][t]);
   }
   // waves 2 and 3 hand theirs to 0 and 1, then 1 to 0
 #pragma unroll
@@ -474,7 +507,7 @@ lora_shrink(Rows rows, const T* __restrict__ x, int64_t ldx, int64_t K, const T*
   float* plane = planes + int64_t(blockIdx.y) * rows.M * RP;
 #pragma unroll
   for (int i = 0; i < BT; ++i)
-    if (valid[i])
+    if (m[i] < rows.M)
 #pragma unroll
       for (int t = 0; t < RT; ++t)
         *reinterpret_cast<f32x4*>(plane + m[i] * RP + 16 * t + (lane >> 4) * 4) = acc[i][t];
@@ -552,7 +585,7 @@ lora_expand(Rows rows, Ranks h, const T* __restrict__ b, const float* __restrict
         const int cnt = int(min(int64_t(8), c1 - n));
         const typename mm<T>::frag v = base != nullptr ? load_frag<T, VEC>(base + m * ldbase + n, cnt) : zero_frag<T>();
         T* o = out + m * N + n;
-        if (VEC && cnt == 8) {
+        if (VEC) {
 #pragma unroll
           for (int j = 0; j < int(sizeof(T)) / 2; ++j)
             reinterpret_cast<u32x4*>(o)[j] = reinterpret_cast<const u32x4*>(&v)[j];
@@ -604,22 +637,30 @@ lora_expand(Rows rows, Ranks h, const T* __restrict__ b, const float* __restrict
   if (w0 >= w1) return;
   typename rb::weight wf[rb::kBlocks][2];
   typename mm<T>::frag bs[2][BW];
+  const T* br[BW];
+#pragma unroll
+  for (int i = 0; i < BW; ++i) {
+    br[i] = base != nullptr ? base + min(m[i], rows.M - 1) * ldbase : nullptr;
+    bs[0][i] = bs[1][i] = zero_frag<T>();
+  }
+  // (VEC: columns past N read the last ones again, for columns that are not written)
   auto fetch_weights = [&](int64_t n0) {
 #pragma unroll
     for (int t = 0; t < rb::kBlocks; ++t)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int64_t n = n0 + nr + 4 * e;
-        wf[t][e] = rb::template load<VEC>(bw + n * h.r + rb::kRanks * t, n < w1 ? h.r - rb::kRanks * t - rank0 : 0);
+        const int left = h.r - rb::kRanks * t - rank0;
+        if (VEC) wf[t][e] = rb::template load<true>(bw + min(n, N - 1) * h.r + (left > 0 ? rb::kRanks * t : -rank0), 0);
+        else wf[t][e] = rb::template load<false>(bw + n * h.r + rb::kRanks * t, n < w1 ? left : 0);
       }
   };
   auto fetch_base = [&](int64_t n0, typename mm<T>::frag (&to)[BW]) {
+    if (base == nullptr) return;
     const int64_t nb = n0 + g * 8;
-    const int cnt = int(min(int64_t(8), max(int64_t(0), w1 - nb)));
 #pragma unroll
     for (int i = 0; i < BW; ++i)
-      to[i] = base != nullptr && m[i] < rows.M && cnt > 0 ? load_frag<T, VEC>(base + m[i] * ldbase + nb, cnt)
-                                                           : zero_frag<T>();
+      to[i] = load_frag<T, VEC>(br[i] + (VEC ? min(nb, N - 8) : nb), m[i] < rows.M ? w1 - nb : 0);
   };
   fetch_base(w0, bs[0]);
   fetch_weights(w0);
@@ -635,9 +676,11 @@ lora_expand(Rows rows, Ranks h, const T* __restrict__ b, const float* __restrict
 #pragma unroll
     for (int t = 0; t < rb::kBlocks; ++t)
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
+      for (int e = 0; e < 2; ++e) {
+        if (VEC) rb::blank_unless(rb::kRanks * t + rank0 < h.r, wf[t][e]);
 #pragma unroll
         for (int i = 0; i < BW; ++i) acc[i][e] = rb::mma(wf[t][e], hf[i][t], acc[i][e]);
+      }
     typename mm<T>::frag o[BW];
 #pragma unroll
     for (int i = 0; i < BW; ++i)
@@ -654,7 +697,7 @@ lora_expand(Rows rows, Ranks h, const T* __restrict__ b, const float* __restrict
     for (int i = 0; i < BW; ++i) {
       if (m[i] >= rows.M || cnt == 0) continue;
       T* p = out + m[i] * N + nb;
-      if (VEC && cnt == 8) {
+      if (VEC) {
 #pragma unroll
         for (int j = 0; j < int(sizeof(T)) / 2; ++j)
           reinterpret_cast<u32x4*>(p)[j] = reinterpret_cast<const u32x4*>(&o[i])[j];
@@ -769,26 +812,29 @@ __device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t
   piece v[NI];
   const int64_t col = c0 + (lane % PIECES) * PER;
   const int n = int(min(int64_t(PER), max(int64_t(0), sd.C - col)));
+  const int64_t col_at = VEC ? min(col, sd.C - PER) : col;  // (columns past C are not written)
+  const int64_t blocks = cdiv(sd.C, kMx8Block);
+  uint32_t held;  // bit i: v[i] is a row of the batch's
   auto fetch = [&](int row) {  // the 32 rows whose numbers lanes 0 .. 31 hold
+    held = 0;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int64_t m = __shfl(row, i * RPI + lane / PIECES);
+      held |= m < M ? 1u << i : 0u;
+      const int64_t at = min(m, M - 1);
       if constexpr (Q8) {
-        v[i].q = u32x4{0, 0, 0, 0};
-        v[i].scale = 127;
-        if (m < M && n > 0) {
-          const uint8_t* q = static_cast<const uint8_t*>(sd.v) + m * sd.ldv + col;
-          if (VEC && n == PER) {
-            v[i].q = *reinterpret_cast<const u32x4*>(q);
-          } else {
-            uint8_t* b = reinterpret_cast<uint8_t*>(&v[i].q);
+        const uint8_t* q = static_cast<const uint8_t*>(sd.v) + at * sd.ldv + col_at;
+        if constexpr (VEC) {
+          v[i].q = *reinterpret_cast<const u32x4*>(q);
+          v[i].scale = sd.scales[at * blocks + col_at / kMx8Block];
+        } else {
+          uint8_t* b = reinterpret_cast<uint8_t*>(&v[i].q);
 #pragma unroll
-            for (int j = 0; j < PER; ++j) b[j] = j < n ? q[j] : 0;
-          }
-          v[i].scale = sd.scales[m * cdiv(sd.C, kMx8Block) + col / kMx8Block];
+          for (int j = 0; j < PER; ++j) b[j] = j < n ? q[j] : 0;
+          v[i].scale = n > 0 ? sd.scales[at * blocks + col / kMx8Block] : 127;
         }
       } else {
-        v[i] = m < M ? load_frag<T, VEC>(static_cast<const T*>(sd.v) + m * sd.ldv + col, n) : zero_frag<T>();
+        v[i] = load_frag<T, VEC>(static_cast<const T*>(sd.v) + at * sd.ldv + col_at, n);
       }
     }
   };
@@ -810,6 +856,8 @@ __device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t
       for (int t = 0; t < RT; ++t) uf[part][t] = load_frag<T, true>(up + (part * RP + 16 * t) * 32, 8);
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
+      // (rows that fill a tile up have ranks of 0, which an infinity must not meet)
+      const bool keep = held >> i & 1;
       T* at = vt + (i * RPI + lane / PIECES) * PITCH + (lane % PIECES) * PER;
       if constexpr (Q8) {
         const float s = mx8_scale(v[i].scale);
@@ -821,11 +869,13 @@ __device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t
           typename mm<T>::frag f;
 #pragma unroll
           for (int j = 0; j < 8; ++j) io<T>::store(reinterpret_cast<T*>(&f) + j, w[j] * s);
+          blank_unless_frag<T>(keep, f);
 #pragma unroll
           for (int j = 0; j < int(sizeof(T)) / 2; ++j)
             reinterpret_cast<u32x4*>(at + 8 * h)[j] = reinterpret_cast<const u32x4*>(&f)[j];
         }
       } else {
+        blank_unless_frag<T>(keep, v[i]);
 #pragma unroll
         for (int j = 0; j < int(sizeof(T)) / 2; ++j)
           reinterpret_cast<u32x4*>(at)[j] = reinterpret_cast<const u32x4*>(&v[i])[j];
