@@ -23,6 +23,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "int4_common.h"
 #include "mx8.h"
 
 namespace xk {
@@ -136,6 +137,11 @@ template <typename T, int RT> struct rank_blocks {
   __device__ __forceinline__ static f32x4 mma(const weight& w, const hidden& h, f32x4 c) {
     c = mm<uint16_t>::mma(w, h.part[0], c);
     if constexpr (!kBoth) c = mm<uint16_t>::mma(w, h.part[1], c);
+    return c;
+  }
+  __device__ __forceinline__ static f32x4 mma(const hidden& h, const weight& w, f32x4 c) {
+    c = mm<uint16_t>::mma(h.part[0], w, c);
+    if constexpr (!kBoth) c = mm<uint16_t>::mma(h.part[1], w, c);
     return c;
   }
 };
@@ -407,110 +413,136 @@ lora_prepare(const int32_t* __restrict__ ids, int64_t M, int L, int64_t part, in
 }
 
 // --------------------------------------------------------------- shrink ----
-// planes[s, m, 0 .. 16 RT): the sums over slice s of K for a tile's rows. The waves
-// split the slice, a quarter each for the whole tile: the weights' operands, which
-// come from L2, serve all of a sorted tile's four 16-row products (with 16 rows a
-// wave, rank 64 read four times the bytes of x in weights), and the four partial
-// sums meet in LDS. Few rows: one 16-row product, the tile found here.
-template <typename T, int RT, bool VEC, bool FEW>
+// planes[s, m, 0 .. 16 RT): the sums over slice s of K for a tile's rows.
+//
+// An operand loaded straight from memory has its 16 bytes a lane in 16 rows, and the
+// vector cache serves 16 bytes of such a load a cycle where neighbouring lanes' 64
+// bytes could be one: 9.8 TB/s over the chip. x can be read that way (it is read
+// once), the weights beside it, which every 16 rows read again, cannot. So they go
+// through LDS, whole rows at a time, for the 16 rows of each of the four waves.
+template <typename T> constexpr int kStepK = 256 / sizeof(T);  // contraction values a round
+
+template <typename T, int RT, bool VEC>
 __global__ void __launch_bounds__(kThreads)
 lora_shrink(Rows rows, const T* __restrict__ x, int64_t ldx, int64_t K, const T* __restrict__ a, int r,
             int64_t slice, float* __restrict__ planes) {
-  constexpr int RP = RT * 16, BT = FEW ? 1 : kTile / 16;
-  __shared__ int tile_rows[BT * 16];
-  __shared__ f32x4 red[2][BT * RT][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int RP = RT * 16, KS = kStepK<T>, PER = 16 / sizeof(T), PPR = KS / PER;  // pieces of 16 bytes a row
+  constexpr int NA = RP * PPR / kThreads, PITCH = KS + PER, NX = KS / 32;
+  __shared__ __attribute__((aligned(16))) T as[2][RP * PITCH];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g8 = (lane >> 4) * 8;
+  const int adapter = rows.tile_adapter[blockIdx.x];
+  const int64_t m = rows.sorted[int64_t(blockIdx.x) * kTile + 16 * wave + (lane & 15)];
+  if (adapter < 0 || adapter >= rows.L) return;
   const int64_t k0 = int64_t(blockIdx.y) * slice, k1 = min(K, k0 + slice);
-  int adapter;
-  int64_t m[BT];
-  if (FEW) {
-    adapter = few_tile(rows, blockIdx.x, tile_rows);
-    if (adapter < 0) return;
-    m[0] = tile_rows[lane & 15];
-  } else {
-    adapter = rows.tile_adapter[blockIdx.x];
+  // rows past the batch and ranks past r read others' values in their place: what
+  // comes of them stays in their own sums, which are not used
+  const T* xr = x + min(m, rows.M - 1) * ldx;
+  const T* ar[NA];
 #pragma unroll
-    for (int i = 0; i < BT; ++i) m[i] = rows.sorted[int64_t(blockIdx.x) * kTile + 16 * i + (lane & 15)];
-    if (adapter < 0 || adapter >= rows.L) return;
-  }
-  // Rows past the batch and ranks past r read others' values in their place: what
-  // comes of them stays in their own products, which are not used.
-  const int g8 = (lane >> 4) * 8, rank = lane & 15;
-  const T* xr[BT];
-  const T* ar[RT];
-#pragma unroll
-  for (int i = 0; i < BT; ++i) xr[i] = x + min(m[i], rows.M - 1) * ldx + g8;
-#pragma unroll
-  for (int t = 0; t < RT; ++t) ar[t] = a + (int64_t(adapter) * r + min(16 * t + rank, r - 1)) * K + g8;
-  f32x4 acc[BT][RT];
-#pragma unroll
-  for (int i = 0; i < BT; ++i)
-#pragma unroll
-    for (int t = 0; t < RT; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int64_t quarter = slice / 4, w0 = min(k1, k0 + wave * quarter), w1 = min(k1, w0 + quarter);
-  typename mm<T>::frag xf[BT], af[RT];
+  for (int j = 0; j < NA; ++j)
+    ar[j] = a + (int64_t(adapter) * r + min((tid + j * kThreads) / PPR, r - 1)) * K;
+  const int ap = (tid % PPR) * PER;  // this thread's piece of a row (kThreads is a multiple of PPR)
+  u32x4 an[NA];
+  typename mm<T>::frag xn[NX];
   auto fetch = [&](int64_t k) {
 #pragma unroll
-    for (int i = 0; i < BT; ++i) xf[i] = load_frag<T, VEC>(xr[i] + k, 8);
+    for (int j = 0; j < NA; ++j) {
+      if constexpr (VEC) {
+        an[j] = *reinterpret_cast<const u32x4*>(ar[j] + min(k + ap, K - PER));
+        if (k + ap >= k1) an[j] = u32x4{0, 0, 0, 0};
+      } else {
+        T* v = reinterpret_cast<T*>(&an[j]);
 #pragma unroll
-    for (int t = 0; t < RT; ++t) af[t] = load_frag<T, VEC>(ar[t] + k, 8);
+        for (int i = 0; i < PER; ++i) v[i] = k + ap + i < k1 ? ar[j][k + ap + i] : T(0);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NX; ++j) {
+      const int64_t at = k + 32 * j + g8;
+      xn[j] = load_frag<T, VEC>(xr + (VEC ? min(at, K - 8) : at), k1 - at);
+    }
   };
+  auto put = [&](int buf) {
+#pragma unroll
+    for (int j = 0; j < NA; ++j)
+      *reinterpret_cast<u32x4*>(&as[buf][((tid + j * kThreads) / PPR) * PITCH + ap]) = an[j];
+  };
+  f32x4 acc[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  fetch(k0);
+  for (int64_t k = k0, buf = 0; k < k1; k += KS, buf ^= 1) {
+    put(int(buf));
+    typename mm<T>::frag xc[NX];
+#pragma unroll
+    for (int j = 0; j < NX; ++j) {
+      xc[j] = xn[j];
+      if (VEC && k + KS > k1) blank_unless_frag<T>(k + 32 * j + g8 < k1, xc[j]);  // (the weights there are 0)
+    }
+    if (k + KS < k1) fetch(k + KS);
+    lds_sync();  // one a round: a buffer is written again two rounds on
+#pragma unroll
+    for (int j = 0; j < NX; ++j)
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        const typename mm<T>::frag af = load_frag<T, true>(&as[buf][(16 * t + (lane & 15)) * PITCH + 32 * j + g8], 8);
+        acc[t] = mm<T>::mma(af, xc[j], acc[t]);
+      }
+  }
+  if (m >= rows.M) return;
+  float* plane = planes + (int64_t(blockIdx.y) * rows.M + m) * RP + (lane >> 4) * 4;
+#pragma unroll
+  for (int t = 0; t < RT; ++t) *reinterpret_cast<f32x4*>(plane + 16 * t) = acc[t];
+}
+
+// The same for few rows: a 16-row tile, found here, a quarter of the slice a wave,
+// weights straight to operands (they are read once); the quarters meet in LDS.
+template <typename T, int RT, bool VEC>
+__global__ void __launch_bounds__(kThreads)
+lora_shrink_few(Rows rows, const T* __restrict__ x, int64_t ldx, int64_t K, const T* __restrict__ a, int r,
+                int64_t slice, float* __restrict__ planes) {
+  constexpr int RP = RT * 16;
+  __shared__ int tile_rows[kFewTile];
+  __shared__ f32x4 red[3][RT][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g8 = (lane >> 4) * 8, rank = lane & 15;
+  const int adapter = few_tile(rows, blockIdx.x, tile_rows);
+  if (adapter < 0) return;
+  const int64_t m = tile_rows[rank], k0 = int64_t(blockIdx.y) * slice, k1 = min(K, k0 + slice);
+  const T* xr = x + min(m, rows.M - 1) * ldx + g8;
+  const T* ar[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) ar[t] = a + (int64_t(adapter) * r + min(16 * t + rank, r - 1)) * K + g8;
+  f32x4 acc[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int64_t quarter = slice / 4, w0 = min(k1, k0 + wave * quarter), w1 = min(k1, w0 + quarter);
   const int64_t whole = w0 + (w1 - w0) / 32 * 32;
-  if (w0 < whole) fetch(w0);
-#pragma unroll 2
+#pragma unroll 4
   for (int64_t k = w0; k < whole; k += 32) {
-    typename mm<T>::frag xc[BT], ac[RT];
+    const typename mm<T>::frag xf = load_frag<T, VEC>(xr + k, 8);
 #pragma unroll
-    for (int i = 0; i < BT; ++i) xc[i] = xf[i];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) ac[t] = af[t];
-    fetch(min(k + 32, whole - 32));  // (the last one again at the end: a load less to decide on)
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int i = 0; i < BT; ++i) acc[i][t] = mm<T>::mma(ac[t], xc[i], acc[i][t]);
+    for (int t = 0; t < RT; ++t) acc[t] = mm<T>::mma(load_frag<T, VEC>(ar[t] + k, 8), xf, acc[t]);
   }
   if (whole < w1) {  // K's last, not whole 32
-    const int64_t n = w1 - whole - g8, back = VEC && n <= 0 ? whole + g8 : 0;
-#pragma unroll
-    for (int i = 0; i < BT; ++i) {
-      xf[i] = load_frag<T, VEC>(xr[i] + whole - back, n);
-      if (VEC) blank_unless_frag<T>(n > 0, xf[i]);
-    }
+    const int64_t n = w1 - whole - g8, at = VEC && n <= 0 ? -g8 : whole;
+    typename mm<T>::frag xf = load_frag<T, VEC>(xr + at, n);
+    if (VEC) blank_unless_frag<T>(n > 0, xf);
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      af[t] = load_frag<T, VEC>(ar[t] + whole - back, n);
-      if (VEC) blank_unless_frag<T>(n > 0, af[t]);
+      typename mm<T>::frag af = load_frag<T, VEC>(ar[t] + at, n);
+      if (VEC) blank_unless_frag<T>(n > 0, af);
+      acc[t] = mm<T>::mma(af, xf, acc[t]);
     }
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int i = 0; i < BT; ++i) acc[i][t] = mm<T>::mma(af[t], xf[i], acc[i][t]);
   }
-  // waves 2 and 3 hand theirs to 0 and 1, then 1 to 0
+  if (wave > 0)
 #pragma unroll
-  for (int half = 2; half >= 1; half >>= 1) {
-    if (wave >= half && wave < 2 * half)
+    for (int t = 0; t < RT; ++t) red[wave - 1][t][lane] = acc[t];
+  __syncthreads();
+  if (wave > 0 || m >= rows.M) return;
+  float* plane = planes + (int64_t(blockIdx.y) * rows.M + m) * RP + (lane >> 4) * 4;
 #pragma unroll
-      for (int i = 0; i < BT; ++i)
-#pragma unroll
-        for (int t = 0; t < RT; ++t) red[wave - half][i * RT + t][lane] = acc[i][t];
-    __syncthreads();
-    if (wave < half)
-#pragma unroll
-      for (int i = 0; i < BT; ++i)
-#pragma unroll
-        for (int t = 0; t < RT; ++t) acc[i][t] += red[wave][i * RT + t][lane];
-    __syncthreads();
-  }
-  if (wave > 0) return;
-  float* plane = planes + int64_t(blockIdx.y) * rows.M * RP;
-#pragma unroll
-  for (int i = 0; i < BT; ++i)
-    if (m[i] < rows.M)
-#pragma unroll
-      for (int t = 0; t < RT; ++t)
-        *reinterpret_cast<f32x4*>(plane + m[i] * RP + 16 * t + (lane >> 4) * 4) = acc[i][t];
+  for (int t = 0; t < RT; ++t)
+    *reinterpret_cast<f32x4*>(plane + 16 * t) = ((acc[t] + red[0][t][lane]) + red[1][t][lane]) + red[2][t][lane];
 }
 
 // Ranks [0, 16 RT) of row m: the planes' sum in order, zeros from r on. pitch: the
@@ -547,104 +579,215 @@ __device__ __forceinline__ f32x4 ranks4(const Ranks& u, int64_t m, int rank) {
 
 // --------------------------------------------------------------- expand ----
 // out[m, n] = base[m, n] + s sum_r h[m, r] b[n, r] for a tile of rows and a chunk of
-// columns. The weights are the MFMA's rows and the tile's rows its columns, so a
-// lane ends up with consecutive columns of one row; two 16-column products with
-// interleaved fours give it 8 of them, 16 bytes of bf16.
-template <typename T, int RT, bool VEC, bool FEW>
-__global__ void __launch_bounds__(kThreads)
-lora_expand(Rows rows, Ranks h, const T* __restrict__ b, const float* __restrict__ scaling,
-            const T* __restrict__ base, int64_t ldbase, int64_t N, int64_t chunk, T* __restrict__ out,
-            float* __restrict__ hidden) {
-  constexpr int RP = RT * 16, BM = FEW ? kFewTile : kTile, PITCH = RP + 4;
-  __shared__ int tile_rows[BM];
-  __shared__ __attribute__((aligned(16))) float hs[BM * PITCH];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
-  const int64_t c0 = int64_t(blockIdx.y) * chunk, c1 = min(N, c0 + chunk);
-  int adapter;
-  if (FEW) {
-    adapter = few_tile(rows, blockIdx.x, tile_rows);
-    if (adapter < 0) {  // a row without an adapter is its own workgroup's
-      const int id = rows.ids[blockIdx.x];
-      if (id >= 0 && id < rows.L) return;
-      if (tid == 0) tile_rows[0] = int(blockIdx.x);
-    }
-  } else {
-    adapter = rows.tile_adapter[blockIdx.x];
-    if (tid < BM) tile_rows[tid] = rows.sorted[int64_t(blockIdx.x) * kTile + tid];
-    if (adapter < 0) return;
-    if (adapter == rows.L) adapter = -1;
-  }
-  __syncthreads();
-  if (adapter < 0) {
-    for (int i = 0; i < (FEW ? 1 : BM); ++i) {
-      const int64_t m = tile_rows[i];
-      if (m >= rows.M) continue;
-      if (hidden != nullptr && blockIdx.y == 0)
-        for (int j = tid; j < h.r; j += kThreads) hidden[m * h.r + j] = 0.f;
-      for (int64_t n = c0 + tid * 8; n < c1; n += kThreads * 8) {
-        const int cnt = int(min(int64_t(8), c1 - n));
-        const typename mm<T>::frag v = base != nullptr ? load_frag<T, VEC>(base + m * ldbase + n, cnt) : zero_frag<T>();
-        T* o = out + m * N + n;
-        if (VEC) {
-#pragma unroll
-          for (int j = 0; j < int(sizeof(T)) / 2; ++j)
-            reinterpret_cast<u32x4*>(o)[j] = reinterpret_cast<const u32x4*>(&v)[j];
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (j < cnt) o[j] = reinterpret_cast<const T*>(&v)[j];
-        }
-      }
-    }
-    return;
-  }
-  const float s = scaling != nullptr ? scaling[adapter] : 1.f;
-  for (int q = tid; q < BM * (RP / 4); q += kThreads) {
+// columns.
+
+// s * h of a tile's rows into LDS, fp32; the first chunk's workgroup leaves h itself.
+template <int RP, int PITCH>
+__device__ __forceinline__ void stage_ranks(const Ranks& h, const int* tile_rows, int n, int64_t M, float s, float* hs,
+                                            float* hidden) {
+  for (int q = threadIdx.x; q < n * (RP / 4); q += kThreads) {
     const int i = q / (RP / 4), rank = (q % (RP / 4)) * 4;
     const int64_t m = tile_rows[i];
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (m < rows.M) {
+    if (m < M) {
       v = ranks4(h, m, rank);
-      if (hidden != nullptr && blockIdx.y == 0)
+      if (hidden != nullptr)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (rank + j < h.r) hidden[m * h.r + rank + j] = v[j];
     }
     *reinterpret_cast<f32x4*>(hs + i * PITCH + rank) = v * s;
   }
-  __syncthreads();
-  // Sorted tiles: a wave takes 32 of the rows and half of the chunk's columns; few
-  // rows: all 16 and a quarter. The weights of the next 32 columns and the base of
-  // those after them are on their way while these are finished: loads and stores
-  // leave a wave's counter in order, so a load that is waited for right after a store
-  // waits for the store too.
-  constexpr int BW = FEW ? 1 : 2, CW = FEW ? 4 : 2;
+}
+
+// Rows without an adapter: the base, or zeros.
+template <typename T, bool VEC>
+__device__ __forceinline__ void copy_rows(const int* tile_rows, int n_rows, int64_t M, const T* base, int64_t ldbase,
+                                          int64_t N, int64_t c0, int64_t c1, T* out, float* hidden, int r) {
+  for (int i = 0; i < n_rows; ++i) {
+    const int64_t m = tile_rows[i];
+    if (m >= M) continue;
+    if (hidden != nullptr)
+      for (int j = threadIdx.x; j < r; j += kThreads) hidden[m * r + j] = 0.f;
+    for (int64_t n = c0 + threadIdx.x * 8; n < c1; n += kThreads * 8) {
+      const int64_t cnt = c1 - n;
+      const typename mm<T>::frag v = base != nullptr ? load_frag<T, VEC>(base + m * ldbase + n, cnt) : zero_frag<T>();
+      T* o = out + m * N + n;
+      if constexpr (VEC) {
+#pragma unroll
+        for (int j = 0; j < int(sizeof(T)) / 2; ++j)
+          reinterpret_cast<u32x4*>(o)[j] = reinterpret_cast<const u32x4*>(&v)[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j < cnt) o[j] = reinterpret_cast<const T*>(&v)[j];
+      }
+    }
+  }
+}
+
+// Sorted tiles: 16 rows a wave. The rows are the MFMA's rows and the weights its
+// columns, column l of product t being 16 bytes' worth * l + t: a lane ends up with 16
+// bytes of consecutive columns of four rows, and 16 lanes with 256 of a row, so base
+// and output move in whole lines. The weights of a round go through LDS for all four
+// waves (product t's rows together), the next round's on their way meanwhile, as is
+// its base: loads and stores leave a wave's counter in order, so neither is waited
+// for right after a store.
+template <typename T, int RT, bool VEC>
+__global__ void __launch_bounds__(kThreads)
+lora_expand(Rows rows, Ranks h, const T* __restrict__ b, const float* __restrict__ scaling,
+            const T* __restrict__ base, int64_t ldbase, int64_t N, int64_t chunk, T* __restrict__ out,
+            float* __restrict__ hidden) {
+  constexpr int RP = RT * 16, HP = RP + 4, PER = 16 / sizeof(T), BN = 16 * PER;
+  constexpr int PPR = RP / PER, WP = RP + PER, NW = BN * PPR / kThreads;  // pieces of a weight row, its pitch, pieces a thread
+  constexpr int kWeightBytes = 2 * BN * WP * sizeof(T), kHiddenBytes = kTile * HP * 4;
   typedef rank_blocks<T, RT> rb;
-  const int row0 = FEW ? 0 : (wave & 1) * 32, cw = FEW ? wave : wave >> 1;
-  const int rank0 = rb::rank0(lane);
-  typename rb::hidden hf[BW][rb::kBlocks];
-  int64_t m[BW];
-#pragma unroll
-  for (int i = 0; i < BW; ++i) {
-    const int at = row0 + 16 * i + (lane & 15);
-    m[i] = tile_rows[at];
-#pragma unroll
-    for (int t = 0; t < rb::kBlocks; ++t) hf[i][t] = rb::make(hs + at * PITCH + rb::kRanks * t + rank0, lane);
+  __shared__ int tile_rows[kTile];
+  __shared__ __attribute__((aligned(16))) unsigned char lds[kWeightBytes > kHiddenBytes ? kWeightBytes : kHiddenBytes];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
+  const int64_t c0 = int64_t(blockIdx.y) * chunk, c1 = min(N, c0 + chunk);
+  const int adapter = rows.tile_adapter[blockIdx.x];
+  if (tid < kTile) tile_rows[tid] = rows.sorted[int64_t(blockIdx.x) * kTile + tid];
+  if (adapter < 0) return;
+  __syncthreads();
+  if (blockIdx.y != 0) hidden = nullptr;
+  if (adapter == rows.L) {
+    copy_rows<T, VEC>(tile_rows, kTile, rows.M, base, ldbase, N, c0, c1, out, hidden, h.r);
+    return;
   }
-  const T* bw = b + int64_t(adapter) * N * h.r + rank0;
-  const int nr = 8 * ((lane & 15) >> 2) + (lane & 3);  // this lane's weight row among 32, less 4 for the second product
-  const int64_t w0 = c0 + cw * (chunk / CW), w1 = min(c1, w0 + chunk / CW);
-  if (w0 >= w1) return;
-  typename rb::weight wf[rb::kBlocks][2];
-  typename mm<T>::frag bs[2][BW];
-  const T* br[BW];
-#pragma unroll
-  for (int i = 0; i < BW; ++i) {
-    br[i] = base != nullptr ? base + min(m[i], rows.M - 1) * ldbase : nullptr;
-    bs[0][i] = bs[1][i] = zero_frag<T>();
-  }
-  // (VEC: columns past N read the last ones again, for columns that are not written)
+  const T* bw = b + int64_t(adapter) * N * h.r;
+  u32x4 wn[NW];
   auto fetch_weights = [&](int64_t n0) {
+#pragma unroll
+    for (int j = 0; j < NW; ++j) {
+      const int q = tid + j * kThreads, rank = (q % PPR) * PER;
+      const int64_t n = min(n0 + q / PPR, N - 1);  // (columns past N are not written)
+      if constexpr (VEC) {
+        wn[j] = *reinterpret_cast<const u32x4*>(bw + n * h.r + (rank < h.r ? rank : 0));
+        if (rank >= h.r) wn[j] = u32x4{0, 0, 0, 0};
+      } else {
+        T* v = reinterpret_cast<T*>(&wn[j]);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) v[i] = rank + i < h.r ? bw[n * h.r + rank + i] : T(0);
+      }
+    }
+  };
+  T* ws = reinterpret_cast<T*>(lds);
+  auto put_weights = [&](int buf) {
+#pragma unroll
+    for (int j = 0; j < NW; ++j) {
+      const int q = tid + j * kThreads, row = q / PPR;
+      *reinterpret_cast<u32x4*>(ws + (buf * BN + (row % PER) * 16 + row / PER) * WP + (q % PPR) * PER) = wn[j];
+    }
+  };
+  fetch_weights(c0);
+  float* hs = reinterpret_cast<float*>(lds);
+  stage_ranks<RP, HP>(h, tile_rows, kTile, rows.M, scaling != nullptr ? scaling[adapter] : 1.f, hs, hidden);
+  __syncthreads();
+  typename rb::hidden hf[rb::kBlocks];
+#pragma unroll
+  for (int t = 0; t < rb::kBlocks; ++t)
+    hf[t] = rb::make(hs + (16 * wave + (lane & 15)) * HP + rb::kRanks * t + rb::rank0(lane), lane);
+  const int64_t col = PER * (lane & 15);
+  const T* br[4];
+  T* orow[4];
+  bool in[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t m = tile_rows[16 * wave + 4 * g + i];
+    in[i] = m < rows.M;
+    br[i] = base != nullptr ? base + min(m, rows.M - 1) * ldbase : nullptr;
+    orow[i] = out + min(m, rows.M - 1) * N + col;
+  }
+  u32x4 bn[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bn[i] = u32x4{0, 0, 0, 0};
+  auto fetch_base = [&](int64_t n0) {
+    if (base == nullptr) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (VEC) {
+        bn[i] = *reinterpret_cast<const u32x4*>(br[i] + min(n0 + col, N - PER));
+      } else {
+        T* v = reinterpret_cast<T*>(&bn[i]);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) v[j] = n0 + col + j < c1 ? br[i][n0 + col + j] : T(0);
+      }
+    }
+  };
+  fetch_base(c0);
+  __syncthreads();  // hs has been read
+  int buf = 0;
+  for (int64_t n0 = c0; n0 < c1; n0 += BN, buf ^= 1) {
+    put_weights(buf);
+    if (n0 + BN < c1) fetch_weights(n0 + BN);
+    lds_sync();  // one a round: a buffer is written again two rounds on
+    f32x4 acc[PER];
+#pragma unroll
+    for (int t = 0; t < PER; ++t) {
+      acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int q = 0; q < rb::kBlocks; ++q) {
+        const typename rb::weight wf = *reinterpret_cast<const typename rb::weight*>(
+            ws + (buf * BN + t * 16 + (lane & 15)) * WP + rb::kRanks * q + rb::rank0(lane));
+        acc[t] = rb::mma(hf[q], wf, acc[t]);
+      }
+    }
+    u32x4 o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int t = 0; t < PER; ++t) {
+        const T bv = reinterpret_cast<const T*>(&bn[i])[t];
+        io<T>::store(reinterpret_cast<T*>(&o[i]) + t, io<T>::load(&bv) + acc[t][i]);
+      }
+    if (n0 + BN < c1) fetch_base(n0 + BN);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (!in[i]) continue;
+      if constexpr (VEC) {
+        if (n0 + col < c1) *reinterpret_cast<u32x4*>(orow[i] + n0) = o[i];
+      } else {
+#pragma unroll
+        for (int t = 0; t < PER; ++t)
+          if (n0 + col + t < c1) orow[i][n0 + t] = reinterpret_cast<const T*>(&o[i])[t];
+      }
+    }
+  }
+}
+
+// Few rows: a 16-row tile, found here, the chunk's columns a quarter a wave, weights
+// (read once) straight to operands. They are the MFMA's rows here; two products with
+// interleaved fours give a lane 8 consecutive columns of a row.
+template <typename T, int RT, bool VEC>
+__global__ void __launch_bounds__(kThreads)
+lora_expand_few(Rows rows, Ranks h, const T* __restrict__ b, const float* __restrict__ scaling,
+                const T* __restrict__ base, int64_t ldbase, int64_t N, int64_t chunk, T* __restrict__ out,
+                float* __restrict__ hidden) {
+  constexpr int RP = RT * 16, PITCH = RP + 4;
+  typedef rank_blocks<T, RT> rb;
+  __shared__ int tile_rows[kFewTile];
+  __shared__ __attribute__((aligned(16))) float hs[kFewTile * PITCH];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
+  const int64_t c0 = int64_t(blockIdx.y) * chunk, c1 = min(N, c0 + chunk);
+  if (blockIdx.y != 0) hidden = nullptr;
+  const int adapter = few_tile(rows, blockIdx.x, tile_rows);
+  if (adapter < 0) {  // a row without an adapter is its own workgroup's
+    const int id = rows.ids[blockIdx.x];
+    if (id >= 0 && id < rows.L) return;
+    const int mine = int(blockIdx.x);
+    copy_rows<T, VEC>(&mine, 1, rows.M, base, ldbase, N, c0, c1, out, hidden, h.r);
+    return;
+  }
+  const int64_t w0 = c0 + wave * (chunk / 4), w1 = min(c1, w0 + chunk / 4);
+  const int64_t m = tile_rows[lane & 15];
+  const int rank0 = rb::rank0(lane);
+  const T* bw = b + int64_t(adapter) * N * h.r + rank0;
+  const T* br = base != nullptr ? base + min(m, rows.M - 1) * ldbase : nullptr;
+  const int nr = 8 * ((lane & 15) >> 2) + (lane & 3);  // this lane's weight row among 32, less 4 for the second product
+  typename rb::weight wf[rb::kBlocks][2];
+  typename mm<T>::frag bs = zero_frag<T>();
+  auto fetch = [&](int64_t n0) {  // (VEC: columns past N read the last ones again, for columns that are not written)
 #pragma unroll
     for (int t = 0; t < rb::kBlocks; ++t)
 #pragma unroll
@@ -654,58 +797,42 @@ lora_expand(Rows rows, Ranks h, const T* __restrict__ b, const float* __restrict
         if (VEC) wf[t][e] = rb::template load<true>(bw + min(n, N - 1) * h.r + (left > 0 ? rb::kRanks * t : -rank0), 0);
         else wf[t][e] = rb::template load<false>(bw + n * h.r + rb::kRanks * t, n < w1 ? left : 0);
       }
-  };
-  auto fetch_base = [&](int64_t n0, typename mm<T>::frag (&to)[BW]) {
-    if (base == nullptr) return;
     const int64_t nb = n0 + g * 8;
-#pragma unroll
-    for (int i = 0; i < BW; ++i)
-      to[i] = load_frag<T, VEC>(br[i] + (VEC ? min(nb, N - 8) : nb), m[i] < rows.M ? w1 - nb : 0);
+    if (base != nullptr) bs = load_frag<T, VEC>(br + (VEC ? min(nb, N - 8) : nb), w1 - nb);
   };
-  fetch_base(w0, bs[0]);
-  fetch_weights(w0);
-  fetch_base(w0 + 32, bs[1]);
+  if (w0 < w1) fetch(w0);  // on their way while the ranks are summed
+  stage_ranks<RP, PITCH>(h, tile_rows, kFewTile, rows.M, scaling != nullptr ? scaling[adapter] : 1.f, hs, hidden);
+  __syncthreads();
+  typename rb::hidden hf[rb::kBlocks];
+#pragma unroll
+  for (int t = 0; t < rb::kBlocks; ++t) hf[t] = rb::make(hs + (lane & 15) * PITCH + rb::kRanks * t + rank0, lane);
   for (int64_t n0 = w0; n0 < w1; n0 += 32) {
-    const int64_t nb = n0 + g * 8;
-    const int cnt = int(min(int64_t(8), max(int64_t(0), w1 - nb)));
-    f32x4 acc[BW][2];
-#pragma unroll
-    for (int i = 0; i < BW; ++i)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) acc[i][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (int t = 0; t < rb::kBlocks; ++t)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         if (VEC) rb::blank_unless(rb::kRanks * t + rank0 < h.r, wf[t][e]);
-#pragma unroll
-        for (int i = 0; i < BW; ++i) acc[i][e] = rb::mma(wf[t][e], hf[i][t], acc[i][e]);
+        acc[e] = rb::mma(wf[t][e], hf[t], acc[e]);
       }
-    typename mm<T>::frag o[BW];
+    typename mm<T>::frag o;
 #pragma unroll
-    for (int i = 0; i < BW; ++i)
+    for (int j = 0; j < 8; ++j) {
+      const T bv = reinterpret_cast<const T*>(&bs)[j];
+      io<T>::store(reinterpret_cast<T*>(&o) + j, io<T>::load(&bv) + acc[j >> 2][j & 3]);
+    }
+    if (n0 + 32 < w1) fetch(n0 + 32);
+    const int64_t nb = n0 + g * 8, cnt = w1 - nb;
+    if (m >= rows.M || cnt <= 0) continue;
+    T* p = out + m * N + nb;
+    if constexpr (VEC) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const T bv = reinterpret_cast<const T*>(&bs[0][i])[j];
-        io<T>::store(reinterpret_cast<T*>(&o[i]) + j, io<T>::load(&bv) + acc[i][j >> 2][j & 3]);
-      }
-    if (n0 + 32 < w1) fetch_weights(n0 + 32);
+      for (int j = 0; j < int(sizeof(T)) / 2; ++j)
+        reinterpret_cast<u32x4*>(p)[j] = reinterpret_cast<const u32x4*>(&o)[j];
+    } else {
 #pragma unroll
-    for (int i = 0; i < BW; ++i) bs[0][i] = bs[1][i];
-    fetch_base(n0 + 64, bs[1]);
-#pragma unroll
-    for (int i = 0; i < BW; ++i) {
-      if (m[i] >= rows.M || cnt == 0) continue;
-      T* p = out + m[i] * N + nb;
-      if (VEC) {
-#pragma unroll
-        for (int j = 0; j < int(sizeof(T)) / 2; ++j)
-          reinterpret_cast<u32x4*>(p)[j] = reinterpret_cast<const u32x4*>(&o[i])[j];
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (j < cnt) p[j] = reinterpret_cast<const T*>(&o[i])[j];
-      }
+      for (int j = 0; j < 8; ++j)
+        if (j < cnt) p[j] = reinterpret_cast<const T*>(&o)[j];
     }
   }
 }
@@ -726,7 +853,7 @@ lora_expand(Rows rows, Ranks h, const T* __restrict__ b, const float* __restrict
 // row pitch of 32 bytes past a multiple of 256 the transposed reads of half a wave then
 // fall on distinct banks.
 struct Side {
-  const void* packed;      // [positions / 32, parts, 16 RT, 32] of T: u as operands
+  const void* packed;      // [positions / 32, parts, RT, 64 lanes, 8] of T: u as operands
   const void* v;           // [M, C] of T, or e4m3 bytes with `scales`
   const uint8_t* scales;
   int64_t ldv, C;
@@ -768,7 +895,7 @@ lora_pack(Rows rows, Ranks g, Ranks h, const float* __restrict__ scaling, float*
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = u[(32 * tile + 4 * p8 + (j & 3) + (j >> 2) * 16) * PITCH + rank];
-    T* o = out + ((tile * kParts<T>) * RP + rank) * 32 + 8 * p8;
+    T* o = out + tile * kParts<T> * RP * 32 + ((rank >> 4) * 64 + 16 * p8 + (rank & 15)) * 8;  // lane 16 p8 + rank % 16
     if constexpr (std::is_same<T, float>::value) {
       *reinterpret_cast<f32x4*>(o) = f32x4{v[0], v[1], v[2], v[3]};
       *reinterpret_cast<f32x4*>(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
@@ -849,11 +976,11 @@ __device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t
   while (more) {
     // u's operands of these rows, then the rows themselves to LDS
     typename mm<T>::frag uf[PARTS][RT];
-    const T* up = static_cast<const T*>(sd.packed) + p * RP * PARTS + (lane & 15) * 32 + 8 * g;
+    const T* up = static_cast<const T*>(sd.packed) + p * RP * PARTS + lane * 8;
 #pragma unroll
     for (int part = 0; part < PARTS; ++part)
 #pragma unroll
-      for (int t = 0; t < RT; ++t) uf[part][t] = load_frag<T, true>(up + (part * RP + 16 * t) * 32, 8);
+      for (int t = 0; t < RT; ++t) uf[part][t] = load_frag<T, true>(up + (part * RT + t) * 512, 8);
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       // (rows that fill a tile up have ranks of 0, which an infinity must not meet)
@@ -1020,7 +1147,7 @@ struct Slices {
   int count;
   Slices(int64_t C, int64_t tiles, bool few) {
     const int64_t want = std::max<int64_t>(1, cdiv(few ? 512 : 768, std::max<int64_t>(tiles, 1)));
-    const int64_t least = few ? 256 : 512;
+    const int64_t least = few ? 256 : 1024;
     const int64_t n = std::max<int64_t>(1, std::min(want, cdiv(C, least)));
     const int64_t unit = 128;
     len = cdiv(cdiv(C, n), unit) * unit;
@@ -1056,12 +1183,12 @@ void run_shrink(const Rows& rows, int64_t tiles, bool few, const T* x, int64_t l
   const dim3 grid(unsigned(few ? rows.M : tiles), sl.count);
   with_ranks(r, [&](auto rt) {
     constexpr int RT = decltype(rt)::value;
-#define XK_SHRINK(V, F) \
-  hipLaunchKernelGGL((lora_shrink<T, RT, V, F>), grid, dim3(kThreads), 0, stream, rows, x, ldx, K, a, r, sl.len, planes)
-    if (vec && few) XK_SHRINK(true, true);
-    else if (vec) XK_SHRINK(true, false);
-    else if (few) XK_SHRINK(false, true);
-    else XK_SHRINK(false, false);
+#define XK_SHRINK(NAME, V) \
+  hipLaunchKernelGGL((NAME<T, RT, V>), grid, dim3(kThreads), 0, stream, rows, x, ldx, K, a, r, sl.len, planes)
+    if (vec && few) XK_SHRINK(lora_shrink_few, true);
+    else if (vec) XK_SHRINK(lora_shrink, true);
+    else if (few) XK_SHRINK(lora_shrink_few, false);
+    else XK_SHRINK(lora_shrink, false);
 #undef XK_SHRINK
   });
 }
@@ -1074,13 +1201,13 @@ void run_expand(const Rows& rows, int64_t tiles, bool few,  const Ranks& h, cons
   const dim3 grid(unsigned(few ? rows.M : tiles), unsigned(cdiv(N, chunk)));
   with_ranks(h.r, [&](auto rt) {
     constexpr int RT = decltype(rt)::value;
-#define XK_EXPAND(V, F)                                                                                          \
-  hipLaunchKernelGGL((lora_expand<T, RT, V, F>), grid, dim3(kThreads), 0, stream, rows, h, b, scaling, base, \
-                     ldbase, N, chunk, out, hidden)
-    if (vec && few) XK_EXPAND(true, true);
-    else if (vec) XK_EXPAND(true, false);
-    else if (few) XK_EXPAND(false, true);
-    else XK_EXPAND(false, false);
+#define XK_EXPAND(NAME, V)                                                                                       \
+  hipLaunchKernelGGL((NAME<T, RT, V>), grid, dim3(kThreads), 0, stream, rows, h, b, scaling, base, ldbase, N, chunk, \
+                     out, hidden)
+    if (vec && few) XK_EXPAND(lora_expand_few, true);
+    else if (vec) XK_EXPAND(lora_expand, true);
+    else if (few) XK_EXPAND(lora_expand_few, false);
+    else XK_EXPAND(lora_expand, false);
 #undef XK_EXPAND
   });
 }
