@@ -30,6 +30,8 @@ namespace xk {
 
 namespace {
 
+// Kernels of MFMAs ask for two waves a SIMD at least (the second launch bound), with
+// which their sums stay in registers that other instructions reach.
 constexpr int kThreads = 256;
 constexpr int kTile = 64;      // rows of a sorted tile
 constexpr int kFewTile = 16;   // rows of a tile that a workgroup finds itself
@@ -423,7 +425,7 @@ lora_prepare(const int32_t* __restrict__ ids, int64_t M, int L, int64_t part, in
 template <typename T> constexpr int kStepK = 256 / sizeof(T);  // contraction values a round
 
 template <typename T, int RT, bool VEC>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
 lora_shrink(Rows rows, const T* __restrict__ x, int64_t ldx, int64_t K, const T* __restrict__ a, int r,
             int64_t slice, float* __restrict__ planes) {
   constexpr int RP = RT * 16, KS = kStepK<T>, PER = 16 / sizeof(T), PPR = KS / PER;  // pieces of 16 bytes a row
@@ -498,7 +500,7 @@ lora_shrink(Rows rows, const T* __restrict__ x, int64_t ldx, int64_t K, const T*
 // The same for few rows: a 16-row tile, found here, a quarter of the slice a wave,
 // weights straight to operands (they are read once); the quarters meet in LDS.
 template <typename T, int RT, bool VEC>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
 lora_shrink_few(Rows rows, const T* __restrict__ x, int64_t ldx, int64_t K, const T* __restrict__ a, int r,
                 int64_t slice, float* __restrict__ planes) {
   constexpr int RP = RT * 16;
@@ -634,7 +636,7 @@ __device__ __forceinline__ void copy_rows(const int* tile_rows, int n_rows, int6
 // its base: loads and stores leave a wave's counter in order, so neither is waited
 // for right after a store.
 template <typename T, int RT, bool VEC>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
 lora_expand(Rows rows, Ranks h, const T* __restrict__ b, const float* __restrict__ scaling,
             const T* __restrict__ base, int64_t ldbase, int64_t N, int64_t chunk, T* __restrict__ out,
             float* __restrict__ hidden) {
@@ -722,35 +724,36 @@ lora_expand(Rows rows, Ranks h, const T* __restrict__ b, const float* __restrict
     put_weights(buf);
     if (n0 + BN < c1) fetch_weights(n0 + BN);
     lds_sync();  // one a round: a buffer is written again two rounds on
-    f32x4 acc[PER];
+    f32x4 acc[PER];  // from the base on
 #pragma unroll
     for (int t = 0; t < PER; ++t) {
-      acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const T bv = reinterpret_cast<const T*>(&bn[i])[t];
+        acc[t][i] = io<T>::load(&bv);
+      }
+    }
+    if (n0 + BN < c1) fetch_base(n0 + BN);
+#pragma unroll
+    for (int t = 0; t < PER; ++t)
 #pragma unroll
       for (int q = 0; q < rb::kBlocks; ++q) {
         const typename rb::weight wf = *reinterpret_cast<const typename rb::weight*>(
             ws + (buf * BN + t * 16 + (lane & 15)) * WP + rb::kRanks * q + rb::rank0(lane));
         acc[t] = rb::mma(hf[q], wf, acc[t]);
       }
-    }
-    u32x4 o[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int t = 0; t < PER; ++t) {
-        const T bv = reinterpret_cast<const T*>(&bn[i])[t];
-        io<T>::store(reinterpret_cast<T*>(&o[i]) + t, io<T>::load(&bv) + acc[t][i]);
-      }
-    if (n0 + BN < c1) fetch_base(n0 + BN);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (!in[i]) continue;
+      u32x4 o;
+#pragma unroll
+      for (int t = 0; t < PER; ++t) io<T>::store(reinterpret_cast<T*>(&o) + t, acc[t][i]);
       if constexpr (VEC) {
-        if (n0 + col < c1) *reinterpret_cast<u32x4*>(orow[i] + n0) = o[i];
+        if (n0 + col < c1) *reinterpret_cast<u32x4*>(orow[i] + n0) = o;
       } else {
 #pragma unroll
         for (int t = 0; t < PER; ++t)
-          if (n0 + col + t < c1) orow[i][n0 + t] = reinterpret_cast<const T*>(&o[i])[t];
+          if (n0 + col + t < c1) orow[i][n0 + t] = reinterpret_cast<const T*>(&o)[t];
       }
     }
   }
@@ -760,7 +763,7 @@ lora_expand(Rows rows, Ranks h, const T* __restrict__ b, const float* __restrict
 // (read once) straight to operands. They are the MFMA's rows here; two products with
 // interleaved fours give a lane 8 consecutive columns of a row.
 template <typename T, int RT, bool VEC>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
 lora_expand_few(Rows rows, Ranks h, const T* __restrict__ b, const float* __restrict__ scaling,
                 const T* __restrict__ base, int64_t ldbase, int64_t N, int64_t chunk, T* __restrict__ out,
                 float* __restrict__ hidden) {
@@ -1069,7 +1072,7 @@ __device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t
 }
 
 template <typename T, int RT, bool VEC, bool Q8>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
 lora_wgrad(Side side_a, Side side_b, int r, int a_strips, const int32_t* __restrict__ sorted,
            const int32_t* __restrict__ offsets, int L, int64_t M, int64_t seg) {
   constexpr int RP = RT * 16, BC = kColTiles<T, RT> * 16, PITCH = BC + 32 / sizeof(T);
