@@ -225,13 +225,13 @@ struct SortOut {
 
 __device__ __forceinline__ int group_of(int id, int L) { return id >= 0 && id < L ? id : L; }
 
-// cnt[g] += lanes of group g; runs of one group, as requests' rows are, cost one add.
+// cnt[g] += lanes of group g (those with `in`, the wave's first lane among them if
+// any is); runs of one group, as requests' rows are, cost one add.
 __device__ __forceinline__ void count_groups(int* cnt, int g, bool in) {
   const uint64_t active = __ballot(in);
   if (active == 0) return;
-  const int first = __shfl(g, __ffsll(static_cast<unsigned long long>(active)) - 1);
-  const uint64_t same = __ballot(in && g == first);
-  if (same == active) {
+  const int first = __builtin_amdgcn_readfirstlane(g);
+  if (__ballot(in && g == first) == active) {
     if ((threadIdx.x & 63) == 0) atomicAdd(&cnt[first], __popcll(active));
   } else if (in) {
     atomicAdd(&cnt[g], 1);
@@ -281,13 +281,15 @@ __device__ __forceinline__ void sort_part(const int32_t* __restrict__ ids, int64
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
         const int64_t i = i0 + j * kSortThreads + tid;
-        const int g = group_of(id[j], L);
-        count_groups(total, g, i < M);
-        if (i - tid < first) count_groups(before, g, i < M);
+        count_groups(i - tid < first ? before : total, group_of(id[j], L), i < M);
       }
     }
   }
   __syncthreads();
+  if (!counted) {  // total: what lies before too
+    for (int g = tid; g < G; g += kSortThreads) total[g] += before[g];
+    __syncthreads();
+  }
   // positions of the groups: a prefix sum of the sizes in whole tiles (at most 1,025
   // of them: the last thread takes two)
   int mine = 0;
@@ -336,6 +338,7 @@ __device__ __forceinline__ void sort_part(const int32_t* __restrict__ ids, int64
       for (int w = 0; w < wave; ++w) ahead += c[w];
       o.sorted[off[g] + before[g] + ahead + rank] = int(row);
     }
+    if (i + kSortThreads >= end) break;
     __syncthreads();
     for (int q = tid; q < G; q += kSortThreads) {
       int n = 0;
@@ -606,23 +609,35 @@ __device__ __forceinline__ void stage_ranks(const Ranks& h, const int* tile_rows
 template <typename T, bool VEC>
 __device__ __forceinline__ void copy_rows(const int* tile_rows, int n_rows, int64_t M, const T* base, int64_t ldbase,
                                           int64_t N, int64_t c0, int64_t c1, T* out, float* hidden, int r) {
-  for (int i = 0; i < n_rows; ++i) {
-    const int64_t m = tile_rows[i];
-    if (m >= M) continue;
-    if (hidden != nullptr)
-      for (int j = threadIdx.x; j < r; j += kThreads) hidden[m * r + j] = 0.f;
-    for (int64_t n = c0 + threadIdx.x * 8; n < c1; n += kThreads * 8) {
-      const int64_t cnt = c1 - n;
-      const typename mm<T>::frag v = base != nullptr ? load_frag<T, VEC>(base + m * ldbase + n, cnt) : zero_frag<T>();
+  if (hidden != nullptr)
+    for (int q = threadIdx.x; q < n_rows * r; q += kThreads)
+      if (tile_rows[q / r] < M) hidden[int64_t(tile_rows[q / r]) * r + q % r] = 0.f;
+  const int pieces = int(cdiv(c1 - c0, 8)), total = n_rows * pieces;
+  for (int q0 = threadIdx.x; q0 < total; q0 += 4 * kThreads) {  // 4 pieces in flight
+    typename mm<T>::frag v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int q = q0 + j * kThreads;
+      v[j] = zero_frag<T>();
+      if (q >= total || base == nullptr) continue;
+      const int64_t m = tile_rows[q / pieces], n = c0 + int64_t(q % pieces) * 8;
+      if (m < M) v[j] = load_frag<T, VEC>(base + m * ldbase + n, c1 - n);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int q = q0 + j * kThreads;
+      if (q >= total) continue;
+      const int64_t m = tile_rows[q / pieces], n = c0 + int64_t(q % pieces) * 8;
+      if (m >= M) continue;
       T* o = out + m * N + n;
       if constexpr (VEC) {
 #pragma unroll
-        for (int j = 0; j < int(sizeof(T)) / 2; ++j)
-          reinterpret_cast<u32x4*>(o)[j] = reinterpret_cast<const u32x4*>(&v)[j];
+        for (int i = 0; i < int(sizeof(T)) / 2; ++i)
+          reinterpret_cast<u32x4*>(o)[i] = reinterpret_cast<const u32x4*>(&v[j])[i];
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (j < cnt) o[j] = reinterpret_cast<const T*>(&v)[j];
+        for (int i = 0; i < 8; ++i)
+          if (n + i < c1) o[i] = reinterpret_cast<const T*>(&v[j])[i];
       }
     }
   }
@@ -911,7 +926,7 @@ lora_pack(Rows rows, Ranks g, Ranks h, const float* __restrict__ scaling, float*
 
 // Window j's plane for adapter range [off0, off1): at most one adapter that goes
 // on past a window starts in it, and at most one comes in from the window before.
-__device__ __forceinline__ int64_t plane_of(int64_t off0, int64_t window, int64_t seg) {
+__device__ __forceinline__ int plane_of(int off0, int window, int seg) {
   return 2 * window + (off0 >= window * seg ? 1 : 0);
 }
 
@@ -926,7 +941,7 @@ template <typename T, int RT> constexpr int kColTiles = (std::is_same<T, float>:
 
 template <typename T, int RT, bool VEC, bool Q8>
 __device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t* __restrict__ sorted, int64_t M,
-                                            int64_t c0, int64_t p0, int64_t p1, int64_t out_at, float* plane,
+                                            int64_t c0, int p0, int p1, int64_t out_at, float* plane,
                                             unsigned char* lds) {
   constexpr int RP = RT * 16, CT = kColTiles<T, RT>, BC = CT * 16, PITCH = BC + 32 / sizeof(T), PARTS = kParts<T>;
   constexpr bool F32 = std::is_same<T, float>::value;
@@ -970,35 +985,35 @@ __device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t
   };
   // row numbers are read a tile ahead of the rows; padding (M) ends an adapter's positions
   constexpr int kStep = 32 * (kThreads / 64);
-  int64_t p = p0 + wave * 32;
-  auto row_at = [&](int64_t p) { return p < p1 ? int64_t(sorted[p + (lane & 31)]) : M; };
-  auto any = [&](int64_t row) { return __builtin_amdgcn_readfirstlane(int(row)) < M; };
-  int64_t row = row_at(p), next = row_at(p + kStep);
+  int p = p0 + __builtin_amdgcn_readfirstlane(wave) * 32;
+  auto row_at = [&](int p) { return p < p1 ? sorted[p + (lane & 31)] : int(M); };
+  auto any = [&](int row) { return __builtin_amdgcn_readfirstlane(row) < M; };
+  int row = row_at(p), next = row_at(p + kStep);
   bool more = any(row);
-  if (more) fetch(int(row));
-  while (more) {
-    // u's operands of these rows, then the rows themselves to LDS
-    typename mm<T>::frag uf[PARTS][RT];
-    const T* up = static_cast<const T*>(sd.packed) + p * RP * PARTS + lane * 8;
+  // u's operands of the rows, which up to 32 ranks leave registers to read ahead
+  constexpr bool kAhead = PARTS * RT <= 4;
+  typename mm<T>::frag uf[PARTS][RT];
+  auto fetch_u = [&](int p) {
+    const T* up = static_cast<const T*>(sd.packed) + int64_t(p) * RP * PARTS + lane * 8;
 #pragma unroll
     for (int part = 0; part < PARTS; ++part)
 #pragma unroll
       for (int t = 0; t < RT; ++t) uf[part][t] = load_frag<T, true>(up + (part * RT + t) * 512, 8);
+  };
+  if (more) fetch(row);
+  if (more && kAhead) fetch_u(p);
+  while (more) {
+    if (!kAhead) fetch_u(p);
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       // (rows that fill a tile up have ranks of 0, which an infinity must not meet)
       const bool keep = held >> i & 1;
       T* at = vt + (i * RPI + lane / PIECES) * PITCH + (lane % PIECES) * PER;
       if constexpr (Q8) {
-        const float s = mx8_scale(v[i].scale);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float w[8];
-          mx8_unpack4(v[i].q[2 * h], w);
-          mx8_unpack4(v[i].q[2 * h + 1], w + 4);
           typename mm<T>::frag f;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) io<T>::store(reinterpret_cast<T*>(&f) + j, w[j] * s);
+          mx8_unpack8(v[i].q[2 * h], v[i].q[2 * h + 1], v[i].scale, reinterpret_cast<T*>(&f));
           blank_unless_frag<T>(keep, f);
 #pragma unroll
           for (int j = 0; j < int(sizeof(T)) / 2; ++j)
@@ -1011,10 +1026,16 @@ __device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t
           reinterpret_cast<u32x4*>(at)[j] = reinterpret_cast<const u32x4*>(&v[i])[j];
       }
     }
+    typename mm<T>::frag uc[PARTS][RT];
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+      for (int t = 0; t < RT; ++t) uc[part][t] = uf[part][t];
     p += kStep;
     row = next;
     more = any(row);
-    if (more) fetch(int(row));
+    if (more) fetch(row);
+    if (more && kAhead) fetch_u(p);
     next = row_at(p + kStep);
 #pragma unroll
     for (int e = 0; e < CT; ++e) {
@@ -1033,7 +1054,7 @@ __device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t
 #pragma unroll
       for (int part = 0; part < PARTS; ++part)
 #pragma unroll
-        for (int t = 0; t < RT; ++t) acc[e][t] = mm<T>::mma(uf[part][t], vf, acc[e][t]);
+        for (int t = 0; t < RT; ++t) acc[e][t] = mm<T>::mma(uc[part][t], vf, acc[e][t]);
     }
   }
   // the waves' sums: a quarter of the column tiles at a time, which one wave adds in
@@ -1074,7 +1095,7 @@ __device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t
 template <typename T, int RT, bool VEC, bool Q8>
 __global__ void __launch_bounds__(kThreads, 2)
 lora_wgrad(Side side_a, Side side_b, int r, int a_strips, const int32_t* __restrict__ sorted,
-           const int32_t* __restrict__ offsets, int L, int64_t M, int64_t seg) {
+           const int32_t* __restrict__ offsets, int L, int64_t M, int seg) {
   constexpr int RP = RT * 16, BC = kColTiles<T, RT> * 16, PITCH = BC + 32 / sizeof(T);
   constexpr int kTileBytes = 4 * 32 * PITCH * sizeof(T), kRedBytes = 4 * (BC / 64 > 0 ? BC / 64 : 1) * RT * 64 * 16;
   __shared__ __attribute__((aligned(16))) unsigned char lds[kTileBytes > kRedBytes ? kTileBytes : kRedBytes];
@@ -1083,17 +1104,17 @@ lora_wgrad(Side side_a, Side side_b, int r, int a_strips, const int32_t* __restr
   const int64_t c0 = int64_t(is_a ? blockIdx.y : blockIdx.y - a_strips) * BC;
   // pair (adapter, window) number blockIdx.x: adapter i takes the numbers from
   // offsets[i] / seg + i, one per window that it touches
-  const int64_t want = blockIdx.x;
+  const int want = blockIdx.x;
   int lo = 0, hi = L - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (offsets[mid] / seg + mid <= want) lo = mid; else hi = mid - 1;
   }
-  const int64_t off0 = offsets[lo], off1 = offsets[lo + 1], window = want - lo;
+  const int off0 = offsets[lo], off1 = offsets[lo + 1], window = want - lo;
   if (off0 == off1 || window < off0 / seg || window > (off1 - 1) / seg) return;
-  const int64_t p0 = max(off0, window * seg), p1 = min(off1, (window + 1) * seg);
+  const int p0 = max(off0, window * seg), p1 = min(off1, (window + 1) * seg);
   const bool whole = off0 / seg == (off1 - 1) / seg;
-  float* plane = whole ? nullptr : sd.partial + plane_of(off0, window, seg) * RP * sd.C;
+  float* plane = whole ? nullptr : sd.partial + int64_t(plane_of(off0, window, seg)) * RP * sd.C;
   const int64_t out_at = int64_t(lo) * r * sd.C;
   if (is_a) wgrad_strip<T, RT, VEC, Q8>(sd, r, sorted, M, c0, p0, p1, out_at, plane, lds);
   else wgrad_strip<T, RT, VEC, false>(sd, r, sorted, M, c0, p0, p1, out_at, plane, lds);
@@ -1102,18 +1123,18 @@ lora_wgrad(Side side_a, Side side_b, int r, int a_strips, const int32_t* __restr
 // Adds the planes of adapters over several windows; zeros for adapters without rows.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-wgrad_reduce(Side side_a, Side side_b, int r, int a_blocks, int RP, const int32_t* __restrict__ offsets, int64_t seg) {
+wgrad_reduce(Side side_a, Side side_b, int r, int a_blocks, int RP, const int32_t* __restrict__ offsets, int seg) {
   const bool is_a = int(blockIdx.x) < a_blocks;
   const Side& sd = is_a ? side_a : side_b;
   const int i = blockIdx.y;
-  const int64_t off0 = offsets[i], off1 = offsets[i + 1];
-  const int64_t w0 = off0 / seg, w1 = off1 > off0 ? (off1 - 1) / seg : w0 - 1;
+  const int off0 = offsets[i], off1 = offsets[i + 1];
+  const int w0 = off0 / seg, w1 = off1 > off0 ? (off1 - 1) / seg : w0 - 1;
   if (w1 == w0) return;
   const int64_t q = int64_t(is_a ? blockIdx.x : blockIdx.x - a_blocks) * kThreads + threadIdx.x;
   if (q >= r * sd.C) return;
   const int64_t rank = q / sd.C, c = q % sd.C;
   float v = 0.f;
-  for (int64_t w = w0; w <= w1; ++w) v += sd.partial[(plane_of(off0, w, seg) * RP + rank) * sd.C + c];
+  for (int w = w0; w <= w1; ++w) v += sd.partial[(int64_t(plane_of(off0, w, seg)) * RP + rank) * sd.C + c];
   io<T>::store(static_cast<T*>(sd.out) + int64_t(i) * r * sd.C + (sd.by_rank ? q : c * r + rank), v);
 }
 
@@ -1158,8 +1179,12 @@ struct Slices {
   }
 };
 
-int64_t chunk_of(int64_t N, int64_t tiles, bool few) {
-  const int64_t want = std::max<int64_t>(1, cdiv(few ? 512 : 1024, std::max<int64_t>(tiles, 1)));
+// Columns of an expansion's workgroup: as many workgroups as the chip holds at once
+// (a tile's registers and LDS: 4, 3 or 2 a CU), so that none waits for a second round.
+// M = 16,384, N = 7,168, r = 64, 3 a CU: 99 us with 3 chunks, 119 with 4, 112 with 8.
+int64_t chunk_of(int64_t N, int64_t tiles, bool few, int r) {
+  const int64_t places = 256 * (rank_tiles(r) <= 2 ? 4 : rank_tiles(r) == 4 ? 3 : 2);
+  const int64_t want = std::max<int64_t>(1, cdiv(few ? 512 : places, std::max<int64_t>(tiles, 1)));
   const int64_t n = std::max<int64_t>(1, std::min(want, cdiv(N, few ? 128 : 256)));
   return cdiv(cdiv(N, n), 128) * 128;
 }
@@ -1200,7 +1225,7 @@ template <typename T>
 void run_expand(const Rows& rows, int64_t tiles, bool few,  const Ranks& h, const T* b, const float* scaling,
                 const T* base, int64_t ldbase, int64_t N, T* out, float* hidden, hipStream_t stream) {
   const bool vec = N % 8 == 0 && h.r % 8 == 0 && (base == nullptr || ldbase % 8 == 0) && aligned16({b, base, out});
-  const int64_t chunk = chunk_of(N, tiles, few);
+  const int64_t chunk = chunk_of(N, tiles, few, h.r);
   const dim3 grid(unsigned(few ? rows.M : tiles), unsigned(cdiv(N, chunk)));
   with_ranks(h.r, [&](auto rt) {
     constexpr int RT = decltype(rt)::value;
@@ -1251,11 +1276,12 @@ struct ForwardPlan {
 
 // Windows of the sorted positions: enough for the CUs, none shorter than 256 rows.
 struct Windows {
-  int64_t seg, count;
+  int seg;
+  int64_t count;
   Windows(int64_t M, int L, int64_t chunks) {
     const int64_t most = M + int64_t(L) * (kTile - 1);
     const int64_t n = std::max<int64_t>(1, std::min(cdiv(1024, chunks), cdiv(most, 256)));
-    seg = cdiv(cdiv(most, n), kTile) * kTile;
+    seg = int(cdiv(cdiv(most, n), kTile) * kTile);
     count = cdiv(most, seg);
   }
 };

@@ -35,4 +35,25 @@ __device__ __forceinline__ void mx8_unpack4(uint32_t w, float* v) {
   v[3] = b[1];
 }
 
+// 8 scaled values of two words. bf16: v_cvt_scalef32_pk_bf16_fp8, which applies the
+// exponent field of its scale operand (byte 0: 2^-127); a reserved byte 255 makes
+// every value NaN first.
+__device__ __forceinline__ void mx8_unpack8(uint32_t w0, uint32_t w1, uint32_t byte, float* v) {
+  const float s = mx8_scale(byte);
+  mx8_unpack4(w0, v);
+  mx8_unpack4(w1, v + 4);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] *= s;
+}
+__device__ __forceinline__ void mx8_unpack8(uint32_t w0, uint32_t w1, uint32_t byte, uint16_t* v) {
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  if (byte == 255u) w0 = w1 = 0x7F7F7F7Fu;
+  const float s = __uint_as_float((byte == 255u ? 127u : byte) << 23);
+  b2* o = reinterpret_cast<b2*>(v);
+  o[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, s, false);
+  o[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, s, true);
+  o[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, s, false);
+  o[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, s, true);
+}
+
 }  // namespace xk
