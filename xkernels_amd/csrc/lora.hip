@@ -37,6 +37,9 @@ constexpr int kTile = 64;      // rows of a sorted tile
 constexpr int kFewTile = 16;   // rows of a tile that a workgroup finds itself
 constexpr int kFew = 256;      // rows up to which they do (a thread per row)
 constexpr int kMaxRank = 128;
+// Workgroups of a CU that the registers and LDS of their ranks' tiles of 16 allow.
+template <int RT> constexpr int kExpandPlaces = RT == 1 ? 4 : RT <= 4 ? 3 : 2;
+constexpr int kWgradPlaces = 2;
 constexpr int kMaxAdapters = 1024;
 constexpr int kSortThreads = 1024;             // and rows a round of the sort
 constexpr int64_t kOneLaunchRows = 65536;      // rows up to which each sorting workgroup counts the whole batch
@@ -180,6 +183,7 @@ struct Rows {
   // filled up with M to whole tiles
   const int32_t* sorted;        // [tiles, 64] row numbers
   const int32_t* tile_adapter;  // [tiles]: L for rows without an adapter, -1 for unused tiles
+  const int32_t* end;           // positions in use
 };
 
 // The tile of up to 16 rows that row j leads: rows of one adapter in ascending
@@ -218,7 +222,7 @@ __device__ __forceinline__ int few_tile(const Rows& a, int j, int* rows) {
 struct SortOut {
   int32_t* sorted;
   int32_t* tile_adapter;
-  int32_t* offsets;  // [L + 1]: where the groups' positions begin
+  int32_t* offsets;  // [L + 2]: where the groups' positions begin, and their end
   int32_t* counts;   // [chunks, L + 1], with lora_count
   int64_t tiles;
 };
@@ -315,7 +319,7 @@ __device__ __forceinline__ void sort_part(const int32_t* __restrict__ ids, int64
   if (per == 1 && tid == G - 1) off[G] = at;
   __syncthreads();
   if (blockIdx.x == 0)
-    for (int g = tid; g < G; g += kSortThreads) o.offsets[g] = off[g];
+    for (int g = tid; g <= G; g += kSortThreads) o.offsets[g] = off[g];
   // this part's rows
   const int bits = 32 - __clz(L);
   for (int64_t i = first; i < end; i += kSortThreads) {
@@ -522,8 +526,21 @@ lora_shrink_few(Rows rows, const T* __restrict__ x, int64_t ldx, int64_t K, cons
   for (int t = 0; t < RT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int64_t quarter = slice / 4, w0 = min(k1, k0 + wave * quarter), w1 = min(k1, w0 + quarter);
   const int64_t whole = w0 + (w1 - w0) / 32 * 32;
-#pragma unroll 4
-  for (int64_t k = w0; k < whole; k += 32) {
+  int64_t k = w0;
+  for (; k + 128 <= whole; k += 128) {  // four steps' loads in flight
+    typename mm<T>::frag xf[4], af[4][RT];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      xf[j] = load_frag<T, VEC>(xr + k + 32 * j, 8);
+#pragma unroll
+      for (int t = 0; t < RT; ++t) af[j][t] = load_frag<T, VEC>(ar[t] + k + 32 * j, 8);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int t = 0; t < RT; ++t) acc[t] = mm<T>::mma(af[j][t], xf[j], acc[t]);
+  }
+  for (; k < whole; k += 32) {
     const typename mm<T>::frag xf = load_frag<T, VEC>(xr + k, 8);
 #pragma unroll
     for (int t = 0; t < RT; ++t) acc[t] = mm<T>::mma(load_frag<T, VEC>(ar[t] + k, 8), xf, acc[t]);
@@ -651,10 +668,10 @@ __device__ __forceinline__ void copy_rows(const int* tile_rows, int n_rows, int6
 // its base: loads and stores leave a wave's counter in order, so neither is waited
 // for right after a store.
 template <typename T, int RT, bool VEC>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, kExpandPlaces<RT>)
 lora_expand(Rows rows, Ranks h, const T* __restrict__ b, const float* __restrict__ scaling,
-            const T* __restrict__ base, int64_t ldbase, int64_t N, int64_t chunk, T* __restrict__ out,
-            float* __restrict__ hidden) {
+            const T* __restrict__ base, int64_t ldbase, int64_t N, int chunks, T* __restrict__ out,
+            float* __restrict__ hidden_out) {
   constexpr int RP = RT * 16, HP = RP + 4, PER = 16 / sizeof(T), BN = 16 * PER;
   constexpr int PPR = RP / PER, WP = RP + PER, NW = BN * PPR / kThreads;  // pieces of a weight row, its pitch, pieces a thread
   constexpr int kWeightBytes = 2 * BN * WP * sizeof(T), kHiddenBytes = kTile * HP * 4;
@@ -662,116 +679,130 @@ lora_expand(Rows rows, Ranks h, const T* __restrict__ b, const float* __restrict
   __shared__ int tile_rows[kTile];
   __shared__ __attribute__((aligned(16))) unsigned char lds[kWeightBytes > kHiddenBytes ? kWeightBytes : kHiddenBytes];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
-  const int64_t c0 = int64_t(blockIdx.y) * chunk, c1 = min(N, c0 + chunk);
-  const int adapter = rows.tile_adapter[blockIdx.x];
-  if (tid < kTile) tile_rows[tid] = rows.sorted[int64_t(blockIdx.x) * kTile + tid];
-  if (adapter < 0) return;
-  __syncthreads();
-  if (blockIdx.y != 0) hidden = nullptr;
-  if (adapter == rows.L) {
-    copy_rows<T, VEC>(tile_rows, kTile, rows.M, base, ldbase, N, c0, c1, out, hidden, h.r);
-    return;
+  const int64_t per_tile = cdiv(N, BN), rounds = int64_t(*rows.end / kTile) * per_tile;
+  int64_t at, until;
+  if (chunks > 0) {  // a tile's chunk
+    const int64_t tile = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+    at = tile * per_tile + per_tile * chunk / chunks;
+    until = min(rounds, tile * per_tile + per_tile * (chunk + 1) / chunks);
+  } else {
+    at = rounds * blockIdx.x / gridDim.x;
+    until = rounds * (blockIdx.x + 1) / gridDim.x;
   }
-  const T* bw = b + int64_t(adapter) * N * h.r;
-  u32x4 wn[NW];
-  auto fetch_weights = [&](int64_t n0) {
+  for (int64_t step; at < until; at += step) {
+    const int64_t tile = at / per_tile, c0 = (at - tile * per_tile) * BN;
+    step = min(until - at, per_tile - (at - tile * per_tile));
+    const int64_t c1 = min(N, c0 + step * BN);
+    const int adapter = rows.tile_adapter[tile];
+    float* hidden = c0 == 0 ? hidden_out : nullptr;
+    __syncthreads();  // the tile before
+    if (tid < kTile) tile_rows[tid] = rows.sorted[tile * kTile + tid];
+    __syncthreads();
+    if (adapter >= rows.L) {
+      copy_rows<T, VEC>(tile_rows, kTile, rows.M, base, ldbase, N, c0, c1, out, hidden, h.r);
+      continue;
+    }
+    const T* bw = b + int64_t(adapter) * N * h.r;
+    u32x4 wn[NW];
+    auto fetch_weights = [&](int64_t n0) {
 #pragma unroll
-    for (int j = 0; j < NW; ++j) {
-      const int q = tid + j * kThreads, rank = (q % PPR) * PER;
-      const int64_t n = min(n0 + q / PPR, N - 1);  // (columns past N are not written)
-      if constexpr (VEC) {
-        wn[j] = *reinterpret_cast<const u32x4*>(bw + n * h.r + (rank < h.r ? rank : 0));
-        if (rank >= h.r) wn[j] = u32x4{0, 0, 0, 0};
-      } else {
-        T* v = reinterpret_cast<T*>(&wn[j]);
+      for (int j = 0; j < NW; ++j) {
+        const int q = tid + j * kThreads, rank = (q % PPR) * PER;
+        const int64_t n = min(n0 + q / PPR, N - 1);  // (columns past N are not written)
+        if constexpr (VEC) {
+          wn[j] = *reinterpret_cast<const u32x4*>(bw + n * h.r + (rank < h.r ? rank : 0));
+          if (rank >= h.r) wn[j] = u32x4{0, 0, 0, 0};
+        } else {
+          T* v = reinterpret_cast<T*>(&wn[j]);
 #pragma unroll
-        for (int i = 0; i < PER; ++i) v[i] = rank + i < h.r ? bw[n * h.r + rank + i] : T(0);
+          for (int i = 0; i < PER; ++i) v[i] = rank + i < h.r ? bw[n * h.r + rank + i] : T(0);
+        }
       }
-    }
-  };
-  T* ws = reinterpret_cast<T*>(lds);
-  auto put_weights = [&](int buf) {
+    };
+    T* ws = reinterpret_cast<T*>(lds);
+    auto put_weights = [&](int buf) {
 #pragma unroll
-    for (int j = 0; j < NW; ++j) {
-      const int q = tid + j * kThreads, row = q / PPR;
-      *reinterpret_cast<u32x4*>(ws + (buf * BN + (row % PER) * 16 + row / PER) * WP + (q % PPR) * PER) = wn[j];
-    }
-  };
-  fetch_weights(c0);
-  float* hs = reinterpret_cast<float*>(lds);
-  stage_ranks<RP, HP>(h, tile_rows, kTile, rows.M, scaling != nullptr ? scaling[adapter] : 1.f, hs, hidden);
-  __syncthreads();
-  typename rb::hidden hf[rb::kBlocks];
+      for (int j = 0; j < NW; ++j) {
+        const int q = tid + j * kThreads, row = q / PPR;
+        *reinterpret_cast<u32x4*>(ws + (buf * BN + (row % PER) * 16 + row / PER) * WP + (q % PPR) * PER) = wn[j];
+      }
+    };
+    fetch_weights(c0);
+    float* hs = reinterpret_cast<float*>(lds);
+    stage_ranks<RP, HP>(h, tile_rows, kTile, rows.M, scaling != nullptr ? scaling[adapter] : 1.f, hs, hidden);
+    __syncthreads();
+    typename rb::hidden hf[rb::kBlocks];
 #pragma unroll
-  for (int t = 0; t < rb::kBlocks; ++t)
-    hf[t] = rb::make(hs + (16 * wave + (lane & 15)) * HP + rb::kRanks * t + rb::rank0(lane), lane);
-  const int64_t col = PER * (lane & 15);
-  const T* br[4];
-  T* orow[4];
-  bool in[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t m = tile_rows[16 * wave + 4 * g + i];
-    in[i] = m < rows.M;
-    br[i] = base != nullptr ? base + min(m, rows.M - 1) * ldbase : nullptr;
-    orow[i] = out + min(m, rows.M - 1) * N + col;
-  }
-  u32x4 bn[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) bn[i] = u32x4{0, 0, 0, 0};
-  auto fetch_base = [&](int64_t n0) {
-    if (base == nullptr) return;
+    for (int t = 0; t < rb::kBlocks; ++t)
+      hf[t] = rb::make(hs + (16 * wave + (lane & 15)) * HP + rb::kRanks * t + rb::rank0(lane), lane);
+    const int64_t col = PER * (lane & 15);
+    const T* br[4];
+    T* orow[4];
+    bool in[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if constexpr (VEC) {
-        bn[i] = *reinterpret_cast<const u32x4*>(br[i] + min(n0 + col, N - PER));
-      } else {
-        T* v = reinterpret_cast<T*>(&bn[i]);
-#pragma unroll
-        for (int j = 0; j < PER; ++j) v[j] = n0 + col + j < c1 ? br[i][n0 + col + j] : T(0);
-      }
+      const int64_t m = tile_rows[16 * wave + 4 * g + i];
+      in[i] = m < rows.M;
+      br[i] = base != nullptr ? base + min(m, rows.M - 1) * ldbase : nullptr;
+      orow[i] = out + min(m, rows.M - 1) * N + col;
     }
-  };
-  fetch_base(c0);
-  __syncthreads();  // hs has been read
-  int buf = 0;
-  for (int64_t n0 = c0; n0 < c1; n0 += BN, buf ^= 1) {
-    put_weights(buf);
-    if (n0 + BN < c1) fetch_weights(n0 + BN);
-    lds_sync();  // one a round: a buffer is written again two rounds on
-    f32x4 acc[PER];  // from the base on
+    u32x4 bn[4];
 #pragma unroll
-    for (int t = 0; t < PER; ++t) {
+    for (int i = 0; i < 4; ++i) bn[i] = u32x4{0, 0, 0, 0};
+    auto fetch_base = [&](int64_t n0) {
+      if (base == nullptr) return;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const T bv = reinterpret_cast<const T*>(&bn[i])[t];
-        acc[t][i] = io<T>::load(&bv);
+        if constexpr (VEC) {
+          bn[i] = *reinterpret_cast<const u32x4*>(br[i] + min(n0 + col, N - PER));
+        } else {
+          T* v = reinterpret_cast<T*>(&bn[i]);
+#pragma unroll
+          for (int j = 0; j < PER; ++j) v[j] = n0 + col + j < c1 ? br[i][n0 + col + j] : T(0);
+        }
+      }
+    };
+    fetch_base(c0);
+    __syncthreads();  // hs has been read
+    int buf = 0;
+    for (int64_t n0 = c0; n0 < c1; n0 += BN, buf ^= 1) {
+      put_weights(buf);
+      if (n0 + BN < c1) fetch_weights(n0 + BN);
+      lds_sync();  // one a round: a buffer is written again two rounds on
+      f32x4 acc[PER];  // from the base on
+#pragma unroll
+      for (int t = 0; t < PER; ++t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const T bv = reinterpret_cast<const T*>(&bn[i])[t];
+          acc[t][i] = io<T>::load(&bv);
+        }
+      }
+      if (n0 + BN < c1) fetch_base(n0 + BN);
+#pragma unroll
+      for (int t = 0; t < PER; ++t)
+#pragma unroll
+        for (int q = 0; q < rb::kBlocks; ++q) {
+          const typename rb::weight wf = *reinterpret_cast<const typename rb::weight*>(
+              ws + (buf * BN + t * 16 + (lane & 15)) * WP + rb::kRanks * q + rb::rank0(lane));
+          acc[t] = rb::mma(hf[q], wf, acc[t]);
+        }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (!in[i]) continue;
+        u32x4 o;
+#pragma unroll
+        for (int t = 0; t < PER; ++t) io<T>::store(reinterpret_cast<T*>(&o) + t, acc[t][i]);
+        if constexpr (VEC) {
+          if (n0 + col < c1) *reinterpret_cast<u32x4*>(orow[i] + n0) = o;
+        } else {
+#pragma unroll
+          for (int t = 0; t < PER; ++t)
+            if (n0 + col + t < c1) orow[i][n0 + t] = reinterpret_cast<const T*>(&o)[t];
+        }
       }
     }
-    if (n0 + BN < c1) fetch_base(n0 + BN);
-#pragma unroll
-    for (int t = 0; t < PER; ++t)
-#pragma unroll
-      for (int q = 0; q < rb::kBlocks; ++q) {
-        const typename rb::weight wf = *reinterpret_cast<const typename rb::weight*>(
-            ws + (buf * BN + t * 16 + (lane & 15)) * WP + rb::kRanks * q + rb::rank0(lane));
-        acc[t] = rb::mma(hf[q], wf, acc[t]);
-      }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (!in[i]) continue;
-      u32x4 o;
-#pragma unroll
-      for (int t = 0; t < PER; ++t) io<T>::store(reinterpret_cast<T*>(&o) + t, acc[t][i]);
-      if constexpr (VEC) {
-        if (n0 + col < c1) *reinterpret_cast<u32x4*>(orow[i] + n0) = o;
-      } else {
-#pragma unroll
-        for (int t = 0; t < PER; ++t)
-          if (n0 + col + t < c1) orow[i][n0 + t] = reinterpret_cast<const T*>(&o)[t];
-      }
     }
-  }
 }
 
 // Few rows: a 16-row tile, found here, the chunk's columns a quarter a wave, weights
@@ -857,10 +888,11 @@ lora_expand_few(Rows rows, Ranks h, const T* __restrict__ b, const float* __rest
 
 // ---------------------------------------------------------------- wgrad ----
 // out[i] = sum over adapter i's rows of u[m, :]^T v[m, :]: u the ranks (r of them), v a
-// long row (C columns). Positions of the sorted order are cut into windows; a
-// workgroup takes one adapter's part of one window and a strip of columns. An adapter
-// inside one window writes its gradient; one over several leaves a plane for each,
-// which wgrad_reduce adds in order (and which writes zeros for adapters without rows).
+// long row (C columns). Positions of the sorted order are cut into even windows, as
+// many as make one workgroup for each place on the chip; a workgroup takes a window,
+// adapter by adapter, and a strip of columns. An adapter inside one window writes
+// its gradient; one over several leaves a plane for each, which wgrad_reduce adds in
+// order (and which writes zeros for adapters without rows).
 //
 // The contraction runs over rows, along which neither operand is contiguous. u comes
 // packed as MFMA operands (lora_pack). v goes through LDS: a wave takes 32 rows at a
@@ -946,7 +978,11 @@ __device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t
   constexpr int RP = RT * 16, CT = kColTiles<T, RT>, BC = CT * 16, PITCH = BC + 32 / sizeof(T), PARTS = kParts<T>;
   constexpr bool F32 = std::is_same<T, float>::value;
   constexpr int PER = Q8 ? 16 : 8, PIECES = BC / PER, RPI = 64 / PIECES, NI = 32 / RPI;  // rows an instruction, instructions a tile
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
+  // (opaque: else what every adapter's pass has alike is formed before the loop over
+  // them and held in registers through it)
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  const int lane = tid & 63, wave = tid >> 6, g = lane >> 4;
   T* vt = reinterpret_cast<T*>(lds) + wave * 32 * PITCH;
   f32x4 acc[CT][RT];
 #pragma unroll
@@ -954,13 +990,14 @@ __device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t
 #pragma unroll
     for (int t = 0; t < RT; ++t) acc[e][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   typedef typename std::conditional<Q8, Piece8, typename mm<T>::frag>::type piece;
-  piece v[NI];
+  constexpr int DEPTH = RT <= 2 ? 2 : 1;  // tiles on their way
+  piece vs[DEPTH][NI];
   const int64_t col = c0 + (lane % PIECES) * PER;
   const int n = int(min(int64_t(PER), max(int64_t(0), sd.C - col)));
   const int64_t col_at = VEC ? min(col, sd.C - PER) : col;  // (columns past C are not written)
   const int64_t blocks = cdiv(sd.C, kMx8Block);
-  uint32_t held;  // bit i: v[i] is a row of the batch's
-  auto fetch = [&](int row) {  // the 32 rows whose numbers lanes 0 .. 31 hold
+  uint32_t helds[DEPTH];  // bit i: piece i is a row of the batch's
+  auto fetch = [&](int row, piece (&v)[NI], uint32_t& held) __attribute__((always_inline)) {  // the 32 rows whose numbers lanes 0 .. 31 hold
     held = 0;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
@@ -988,21 +1025,27 @@ __device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t
   int p = p0 + __builtin_amdgcn_readfirstlane(wave) * 32;
   auto row_at = [&](int p) { return p < p1 ? sorted[p + (lane & 31)] : int(M); };
   auto any = [&](int row) { return __builtin_amdgcn_readfirstlane(row) < M; };
-  int row = row_at(p), next = row_at(p + kStep);
-  bool more = any(row);
   // u's operands of the rows, which up to 32 ranks leave registers to read ahead
   constexpr bool kAhead = PARTS * RT <= 4;
   typename mm<T>::frag uf[PARTS][RT];
-  auto fetch_u = [&](int p) {
+  auto fetch_u = [&](int p) __attribute__((always_inline)) {
     const T* up = static_cast<const T*>(sd.packed) + int64_t(p) * RP * PARTS + lane * 8;
 #pragma unroll
     for (int part = 0; part < PARTS; ++part)
 #pragma unroll
       for (int t = 0; t < RT; ++t) uf[part][t] = load_frag<T, true>(up + (part * RT + t) * 512, 8);
   };
-  if (more) fetch(row);
-  if (more && kAhead) fetch_u(p);
-  while (more) {
+  // tile d of the DEPTH next: its rows are fetched if there are any
+  bool more[DEPTH];
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d) {
+    const int row = row_at(p + d * kStep);
+    more[d] = any(row);
+    if (more[d]) fetch(row, vs[d], helds[d]);
+  }
+  int next = row_at(p + DEPTH * kStep);
+  if (more[0] && kAhead) fetch_u(p);
+  auto tile = [&](piece (&v)[NI], uint32_t& held, bool& again, bool follows) __attribute__((always_inline)) {
     if (!kAhead) fetch_u(p);
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
@@ -1032,11 +1075,10 @@ __device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t
 #pragma unroll
       for (int t = 0; t < RT; ++t) uc[part][t] = uf[part][t];
     p += kStep;
-    row = next;
-    more = any(row);
-    if (more) fetch(row);
-    if (more && kAhead) fetch_u(p);
-    next = row_at(p + kStep);
+    again = any(next);
+    if (again) fetch(next, v, held);
+    if (follows && kAhead) fetch_u(p);
+    next = row_at(p + DEPTH * kStep);
 #pragma unroll
     for (int e = 0; e < CT; ++e) {
       typename mm<T>::frag vf;
@@ -1055,6 +1097,17 @@ __device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t
       for (int part = 0; part < PARTS; ++part)
 #pragma unroll
         for (int t = 0; t < RT; ++t) acc[e][t] = mm<T>::mma(uc[part][t], vf, acc[e][t]);
+    }
+  };
+  while (more[0]) {
+    if constexpr (DEPTH == 1) {
+      bool again;
+      tile(vs[0], helds[0], again, any(next));
+      more[0] = again;
+    } else {
+      tile(vs[0], helds[0], more[0], more[1]);
+      if (!more[1]) break;
+      tile(vs[1], helds[1], more[1], more[0]);
     }
   }
   // the waves' sums: a quarter of the column tiles at a time, which one wave adds in
@@ -1093,31 +1146,33 @@ __device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t
 }
 
 template <typename T, int RT, bool VEC, bool Q8>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, kWgradPlaces)
 lora_wgrad(Side side_a, Side side_b, int r, int a_strips, const int32_t* __restrict__ sorted,
            const int32_t* __restrict__ offsets, int L, int64_t M, int seg) {
   constexpr int RP = RT * 16, BC = kColTiles<T, RT> * 16, PITCH = BC + 32 / sizeof(T);
   constexpr int kTileBytes = 4 * 32 * PITCH * sizeof(T), kRedBytes = 4 * (BC / 64 > 0 ? BC / 64 : 1) * RT * 64 * 16;
   __shared__ __attribute__((aligned(16))) unsigned char lds[kTileBytes > kRedBytes ? kTileBytes : kRedBytes];
   const bool is_a = int(blockIdx.y) < a_strips;
-  const Side& sd = is_a ? side_a : side_b;
+  const Side sd = is_a ? side_a : side_b;
   const int64_t c0 = int64_t(is_a ? blockIdx.y : blockIdx.y - a_strips) * BC;
-  // pair (adapter, window) number blockIdx.x: adapter i takes the numbers from
-  // offsets[i] / seg + i, one per window that it touches
-  const int want = blockIdx.x;
-  int lo = 0, hi = L - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (offsets[mid] / seg + mid <= want) lo = mid; else hi = mid - 1;
+  const int window = blockIdx.x, first = window * seg, end = min(offsets[L], first + seg);
+  if (first >= end) return;
+  int i = 0, hi = L - 1;  // the last adapter that begins at or before the window
+  while (i < hi) {
+    const int mid = (i + hi + 1) >> 1;
+    if (offsets[mid] <= first) i = mid; else hi = mid - 1;
   }
-  const int off0 = offsets[lo], off1 = offsets[lo + 1], window = want - lo;
-  if (off0 == off1 || window < off0 / seg || window > (off1 - 1) / seg) return;
-  const int p0 = max(off0, window * seg), p1 = min(off1, (window + 1) * seg);
-  const bool whole = off0 / seg == (off1 - 1) / seg;
-  float* plane = whole ? nullptr : sd.partial + int64_t(plane_of(off0, window, seg)) * RP * sd.C;
-  const int64_t out_at = int64_t(lo) * r * sd.C;
-  if (is_a) wgrad_strip<T, RT, VEC, Q8>(sd, r, sorted, M, c0, p0, p1, out_at, plane, lds);
-  else wgrad_strip<T, RT, VEC, false>(sd, r, sorted, M, c0, p0, p1, out_at, plane, lds);
+  for (int off0 = offsets[i], off1; i < L && off0 < end; ++i, off0 = off1) {
+    off1 = offsets[i + 1];
+    if (off0 == off1) continue;
+    const bool whole = off0 >= first && off1 <= first + seg;
+    float* plane = whole ? nullptr : sd.partial + int64_t(plane_of(off0, window, seg)) * RP * sd.C;
+    const int64_t out_at = int64_t(i) * r * sd.C;
+    const int p0 = max(off0, first), p1 = min(off1, end);
+    if (Q8 && is_a) wgrad_strip<T, RT, VEC, Q8>(sd, r, sorted, M, c0, p0, p1, out_at, plane, lds);
+    else wgrad_strip<T, RT, VEC, false>(sd, r, sorted, M, c0, p0, p1, out_at, plane, lds);
+    __syncthreads();  // the LDS of the sums is the next one's tiles
+  }
 }
 
 // Adds the planes of adapters over several windows; zeros for adapters without rows.
@@ -1158,7 +1213,7 @@ struct Sort {
     int64_t o = 0;
     sorted = o; o += up(tiles * kTile * 4);
     tile_adapter = o; o += up(tiles * 4);
-    offsets = o; o += up(int64_t(L + 1) * 4);
+    offsets = o; o += up(int64_t(L + 2) * 4);
     counts = o; o += counted ? up(int64_t(chunks) * (L + 1) * 4) : 0;
     total = o;
   }
@@ -1179,15 +1234,28 @@ struct Slices {
   }
 };
 
-// Columns of an expansion's workgroup: as many workgroups as the chip holds at once
-// (a tile's registers and LDS: 4, 3 or 2 a CU), so that none waits for a second round.
-// M = 16,384, N = 7,168, r = 64, 3 a CU: 99 us with 3 chunks, 119 with 4, 112 with 8.
-int64_t chunk_of(int64_t N, int64_t tiles, bool few, int r) {
-  const int64_t places = 256 * (rank_tiles(r) <= 2 ? 4 : rank_tiles(r) == 4 ? 3 : 2);
-  const int64_t want = std::max<int64_t>(1, cdiv(few ? 512 : places, std::max<int64_t>(tiles, 1)));
-  const int64_t n = std::max<int64_t>(1, std::min(want, cdiv(N, few ? 128 : 256)));
+// Columns of a few rows' expansion workgroup.
+int64_t chunk_of(int64_t N, int64_t tiles) {
+  const int64_t n = std::max<int64_t>(1, std::min(cdiv(512, std::max<int64_t>(tiles, 1)), cdiv(N, 128)));
   return cdiv(cdiv(N, n), 128) * 128;
 }
+
+// Workgroups of an expansion. The chip has places for 4, 3 or 2 a CU (a tile's
+// registers and LDS). Six tiles' worth of them or more: each tile in that many
+// chunks, of two rounds at least (a workgroup begins with 3 to 4 us of reading
+// its ranks). Else one even share for each place: a second round of workgroups for a
+// few left over costs as much as the first (M = 16,384, N = 7,168, r = 64, 265 tiles
+// of ragged requests: 128 us in 3 chunks, 109 us in shares).
+struct Shares {
+  int chunks;
+  unsigned grid;
+  Shares(int64_t N, int64_t tiles, int r, int64_t elem) {
+    const int64_t places = 256 * (rank_tiles(r) == 1 ? 4 : rank_tiles(r) <= 4 ? 3 : 2), per_tile = cdiv(N, 256 / elem);
+    const int64_t each = places / tiles;
+    chunks = each >= 6 ? int(std::min(each, cdiv(per_tile, 2))) : 0;
+    grid = unsigned(chunks > 0 ? tiles * chunks : places);
+  }
+};
 
 template <typename F> void with_ranks(int r, F&& f) {
   switch (rank_tiles(r)) {
@@ -1225,17 +1293,22 @@ template <typename T>
 void run_expand(const Rows& rows, int64_t tiles, bool few,  const Ranks& h, const T* b, const float* scaling,
                 const T* base, int64_t ldbase, int64_t N, T* out, float* hidden, hipStream_t stream) {
   const bool vec = N % 8 == 0 && h.r % 8 == 0 && (base == nullptr || ldbase % 8 == 0) && aligned16({b, base, out});
-  const int64_t chunk = chunk_of(N, tiles, few, h.r);
-  const dim3 grid(unsigned(few ? rows.M : tiles), unsigned(cdiv(N, chunk)));
+  const int64_t chunk = chunk_of(N, tiles);
+  const dim3 grid(unsigned(rows.M), unsigned(cdiv(N, chunk)));
+  const Shares sh(N, tiles, h.r, sizeof(T));
   with_ranks(h.r, [&](auto rt) {
     constexpr int RT = decltype(rt)::value;
-#define XK_EXPAND(NAME, V)                                                                                       \
-  hipLaunchKernelGGL((NAME<T, RT, V>), grid, dim3(kThreads), 0, stream, rows, h, b, scaling, base, ldbase, N, chunk, \
-                     out, hidden)
-    if (vec && few) XK_EXPAND(lora_expand_few, true);
-    else if (vec) XK_EXPAND(lora_expand, true);
-    else if (few) XK_EXPAND(lora_expand_few, false);
-    else XK_EXPAND(lora_expand, false);
+#define XK_EXPAND_FEW(V)                                                                                          \
+  hipLaunchKernelGGL((lora_expand_few<T, RT, V>), grid, dim3(kThreads), 0, stream, rows, h, b, scaling, base, ldbase, \
+                     N, chunk, out, hidden)
+#define XK_EXPAND(V)                                                                                               \
+  hipLaunchKernelGGL((lora_expand<T, RT, V>), dim3(sh.grid), dim3(kThreads), 0, stream, rows, h, b, scaling, base, \
+                     ldbase, N, sh.chunks, out, hidden)
+    if (vec && few) XK_EXPAND_FEW(true);
+    else if (vec) XK_EXPAND(true);
+    else if (few) XK_EXPAND_FEW(false);
+    else XK_EXPAND(false);
+#undef XK_EXPAND_FEW
 #undef XK_EXPAND
   });
 }
@@ -1248,6 +1321,7 @@ int prepare(const int32_t* ids, int64_t M, int L, const Sort& so, char* ws, Rows
                   reinterpret_cast<int32_t*>(ws + so.offsets), reinterpret_cast<int32_t*>(ws + so.counts), so.tiles};
   rows->sorted = o.sorted;
   rows->tile_adapter = o.tile_adapter;
+  rows->end = o.offsets + L + 1;
   if (so.counted) {
     hipLaunchKernelGGL(lora_count, dim3(so.chunks), dim3(kSortThreads), 0, stream, ids, M, L, so.part, o.counts);
     XK_CHECK_LAUNCH("lora_count");
@@ -1274,15 +1348,16 @@ struct ForwardPlan {
   }
 };
 
-// Windows of the sorted positions: enough for the CUs, none shorter than 256 rows.
+// Windows of the sorted positions: one workgroup for each place that registers and
+// LDS leave on the chip, so that all run at once and for as long.
 struct Windows {
   int seg;
   int64_t count;
-  Windows(int64_t M, int L, int64_t chunks) {
-    const int64_t most = M + int64_t(L) * (kTile - 1);
-    const int64_t n = std::max<int64_t>(1, std::min(cdiv(1024, chunks), cdiv(most, 256)));
-    seg = int(cdiv(cdiv(most, n), kTile) * kTile);
-    count = cdiv(most, seg);
+  Windows(int64_t tiles, int64_t strips) {
+    const int64_t places = 256 * kWgradPlaces;
+    const int64_t n = std::max<int64_t>(1, std::min(places / strips, cdiv(tiles, 2)));
+    seg = int(std::max<int64_t>(1, cdiv(tiles, n)) * kTile);
+    count = std::max<int64_t>(1, cdiv(tiles * kTile, seg));
   }
 };
 
@@ -1294,7 +1369,7 @@ struct BackwardPlan {
   int64_t at, bt, planes, g_sum, packed_g, packed_h, part_a, part_b, total;
   BackwardPlan(int64_t M, int64_t K, int64_t N, int L, int r, int64_t elem)
       : sort(M, L), slices(N, sort.tiles, false), a_strips(cdiv(K, strip(r, elem))), b_strips(cdiv(N, strip(r, elem))),
-        win(M, L, a_strips + b_strips) {
+        win(sort.tiles, a_strips + b_strips) {
     const int64_t RP = rank_tiles(r) * 16, packed = sort.tiles * kTile * RP * 4;  // two bf16 or one fp32
     at = sort.total;
     bt = at + up(int64_t(L) * r * K * elem);
@@ -1316,7 +1391,7 @@ int forward_typed(const T* x, int64_t ldx, int64_t M, int64_t K, const T* a, con
                   const int32_t* ids, const float* scaling, const T* base, int64_t ldbase, T* out, float* hidden,
                   char* ws, hipStream_t stream) {
   const ForwardPlan plan(M, K, L, r);
-  Rows rows{ids, M, L, nullptr, nullptr};
+  Rows rows{ids, M, L, nullptr, nullptr, nullptr};
   if (!plan.few)
     if (int rc = prepare<T>(ids, M, L, plan.sort, ws, &rows, nullptr, nullptr, K, N, r, nullptr, nullptr, stream))
       return rc;
@@ -1336,7 +1411,7 @@ int backward_typed(const T* dy, int64_t lddy, const void* x, int64_t ldx, const 
                    const float* hidden, T* dx, T* da, T* db, char* ws, hipStream_t stream) {
   const BackwardPlan plan(M, K, N, L, r, sizeof(T));
   const int RP = rank_tiles(r) * 16;
-  Rows rows{ids, M, L, nullptr, nullptr};
+  Rows rows{ids, M, L, nullptr, nullptr, nullptr};
   const int32_t* offsets = reinterpret_cast<const int32_t*>(ws + plan.sort.offsets);
   T* at = reinterpret_cast<T*>(ws + plan.at);
   T* bt = reinterpret_cast<T*>(ws + plan.bt);
@@ -1370,7 +1445,7 @@ int backward_typed(const T* dy, int64_t lddy, const void* x, int64_t ldx, const 
   XK_CHECK_LAUNCH("lora_expand");
   const int64_t unit = x_scales != nullptr ? 16 : 8;  // values of a piece of x
   const bool vec = K % unit == 0 && ldx % unit == 0 && N % 8 == 0 && lddy % 8 == 0 && aligned16({dy, x});
-  const dim3 grid(unsigned(plan.win.count + L), unsigned(plan.a_strips + plan.b_strips));
+  const dim3 grid(unsigned(plan.win.count), unsigned(plan.a_strips + plan.b_strips));
   with_ranks(r, [&](auto rt) {
     constexpr int RT = decltype(rt)::value;
 #define XK_WGRAD(V, Q)                                                                                           \
