@@ -603,16 +603,36 @@ __device__ __forceinline__ f32x4 ranks4(const Ranks& u, int64_t m, int rank) {
 // out[m, n] = base[m, n] + s sum_r h[m, r] b[n, r] for a tile of rows and a chunk of
 // columns.
 
-// s * h of a tile's rows into LDS, fp32; the first chunk's workgroup leaves h itself.
-template <int RP, int PITCH>
-__device__ __forceinline__ void stage_ranks(const Ranks& h, const int* tile_rows, int n, int64_t M, float s, float* hs,
+// s * h of a tile's N rows into LDS, fp32; the first chunk's workgroup leaves h itself.
+// With fewer values than threads the planes are dealt out in PARTS, added in order.
+template <int RP, int PITCH, int N>
+__device__ __forceinline__ void stage_ranks(const Ranks& h, const int* tile_rows, int64_t M, float s, float* hs,
                                             float* hidden) {
-  for (int q = threadIdx.x; q < n * (RP / 4); q += kThreads) {
+  constexpr int VALUES = N * (RP / 4), PARTS = VALUES < kThreads ? kThreads / VALUES : 1;
+  __shared__ f32x4 part_sums[PARTS > 1 ? PARTS - 1 : 1][PARTS > 1 ? VALUES : 1];
+  f32x4 first = {0.f, 0.f, 0.f, 0.f};
+  if (PARTS > 1) {
+    const int q = threadIdx.x % VALUES, part = threadIdx.x / VALUES;
+    const int64_t m = tile_rows[q / (RP / 4)];
+    Ranks mine = h;
+    mine.planes += part * h.count / PARTS * h.plane_stride;
+    mine.count = (part + 1) * h.count / PARTS - part * h.count / PARTS;
+    if (m < M) first = ranks4(mine, m, (q % (RP / 4)) * 4);
+    if (part > 0) part_sums[part - 1][q] = first;
+    __syncthreads();
+  }
+  for (int q = threadIdx.x; q < VALUES; q += kThreads) {
     const int i = q / (RP / 4), rank = (q % (RP / 4)) * 4;
     const int64_t m = tile_rows[i];
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     if (m < M) {
-      v = ranks4(h, m, rank);
+      if (PARTS > 1) {
+        v = first;
+#pragma unroll
+        for (int j = 1; j < PARTS; ++j) v += part_sums[j - 1][q];
+      } else {
+        v = ranks4(h, m, rank);
+      }
       if (hidden != nullptr)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -729,7 +749,7 @@ lora_expand(Rows rows, Ranks h, const T* __restrict__ b, const float* __restrict
     };
     fetch_weights(c0);
     float* hs = reinterpret_cast<float*>(lds);
-    stage_ranks<RP, HP>(h, tile_rows, kTile, rows.M, scaling != nullptr ? scaling[adapter] : 1.f, hs, hidden);
+    stage_ranks<RP, HP, kTile>(h, tile_rows, rows.M, scaling != nullptr ? scaling[adapter] : 1.f, hs, hidden);
     __syncthreads();
     typename rb::hidden hf[rb::kBlocks];
 #pragma unroll
@@ -850,7 +870,7 @@ lora_expand_few(Rows rows, Ranks h, const T* __restrict__ b, const float* __rest
     if (base != nullptr) bs = load_frag<T, VEC>(br + (VEC ? min(nb, N - 8) : nb), w1 - nb);
   };
   if (w0 < w1) fetch(w0);  // on their way while the ranks are summed
-  stage_ranks<RP, PITCH>(h, tile_rows, kFewTile, rows.M, scaling != nullptr ? scaling[adapter] : 1.f, hs, hidden);
+  stage_ranks<RP, PITCH, kFewTile>(h, tile_rows, rows.M, scaling != nullptr ? scaling[adapter] : 1.f, hs, hidden);
   __syncthreads();
   typename rb::hidden hf[rb::kBlocks];
 #pragma unroll
@@ -1226,7 +1246,7 @@ struct Slices {
   int count;
   Slices(int64_t C, int64_t tiles, bool few) {
     const int64_t want = std::max<int64_t>(1, cdiv(few ? 512 : 768, std::max<int64_t>(tiles, 1)));
-    const int64_t least = few ? 256 : 1024;
+    const int64_t least = few ? 512 : tiles < 64 ? 256 : 1024;
     const int64_t n = std::max<int64_t>(1, std::min(want, cdiv(C, least)));
     const int64_t unit = 128;
     len = cdiv(cdiv(C, n), unit) * unit;

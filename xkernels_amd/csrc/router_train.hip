@@ -24,10 +24,11 @@ namespace xk {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kOneWg = 1024;        // threads of the one workgroup of a small batch
+constexpr int kRowThreads = 512;    // of a forward's workgroup: few planes, many rows on their way
+constexpr int kOneWg = 1024;        // threads of the one workgroup of a small batch, and of the sums
 constexpr int64_t kOneWgRows = 256; // rows up to which it is one workgroup's work
 constexpr int kFastExperts = 512, kFastTopk = 16;
-constexpr int kPlanes = 512;        // most workgroups of the forward
+constexpr int kPlanes = 512;        // most workgroups of the forward: 16 waves a CU
 
 __device__ __forceinline__ float row_max(float x) {
   row_steps([&](auto from) { x = fmaxf(x, __uint_as_float(from(__float_as_uint(x)))); });
@@ -53,39 +54,51 @@ template <> __device__ __forceinline__ uint16_t to_out<uint16_t>(float f) { retu
 template <> __device__ __forceinline__ _Float16 to_out<_Float16>(float f) { return _Float16(f); }
 template <> __device__ __forceinline__ float to_out<float>(float f) { return f; }
 
-// A row's probabilities on its 16 lanes: lane i holds the 8-expert pieces i, i + 16, ...
+// e^x for x <= 0 or NaN, to 2 steps of fp32: 2^(x log2 e) by v_exp_f32, what the
+// product and log2 e in 24 bits leave over (c, and 1.33e-8 x after the factor ln 2)
+// carried over as a factor. Results below the least normal number are 0.
+__device__ __forceinline__ float exp_neg(float x) {
+  x = x < -104.f ? -104.f : x;
+  const float a = x * 1.44269502f;
+  const float c = fmaf(x, 1.44269502f, -a);
+  const float e = __builtin_amdgcn_exp2f(a);
+  return fmaf(e, fmaf(c, 0.693147181f, x * 1.33497587e-8f), e);
+}
+
+// A row on its 16 lanes: lane i holds the 8-expert pieces i, i + 16, ...; z the logits
+// (-inf past E).
 template <typename T, int PIECES, bool WIDE>
-__device__ __forceinline__ void row_softmax(const T* g, int E, int i16, float* p, float& mx, float& sum) {
-  mx = -__builtin_inff();
+__device__ __forceinline__ void load_row(const T* g, int E, int i16, float* z) {
 #pragma unroll
   for (int c = 0; c < PIECES; ++c) {
     const int e0 = (c * 16 + i16) * 8;
     if (WIDE) {
       if (e0 < E) {
-        piece8<T>::load(g + e0, p + 8 * c);
+        piece8<T>::load(g + e0, z + 8 * c);
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[8 * c + i] = -__builtin_inff();
+        for (int i = 0; i < 8; ++i) z[8 * c + i] = -__builtin_inff();
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) p[8 * c + i] = e0 + i < E ? logit_at<T>(g + e0 + i) : -__builtin_inff();
+      for (int i = 0; i < 8; ++i) z[8 * c + i] = e0 + i < E ? logit_at<T>(g + e0 + i) : -__builtin_inff();
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) mx = fmaxf(mx, p[8 * c + i]);
   }
+}
+// z becomes e^(z - mx); the sum over the row is returned. (Past E: e^-inf = 0 but where
+// mx is infinite, and then the row is NaN.)
+template <int N> __device__ __forceinline__ float row_exp(float* z, float& mx) {
+  mx = z[0];
+#pragma unroll
+  for (int j = 1; j < N; ++j) mx = fmaxf(mx, z[j]);
   mx = row_max(mx);
-  sum = 0.f;
+  float sum = 0.f;
 #pragma unroll
-  for (int j = 0; j < PIECES * 8; ++j) {
-    const int e = ((j >> 3) * 16 + i16) * 8 + (j & 7);
-    p[j] = e < E ? expf(p[j] - mx) : 0.f;
-    sum += p[j];
+  for (int j = 0; j < N; ++j) {
+    z[j] = exp_neg(z[j] - mx);
+    sum += z[j];
   }
-  sum = row_sum(sum);
-  const float inv = 1.f / sum;
-#pragma unroll
-  for (int j = 0; j < PIECES * 8; ++j) p[j] *= inv;
+  return row_sum(sum);
 }
 
 // Scratch: planes of column sums and counts, the rows counted per plane, the
@@ -107,11 +120,11 @@ __device__ __forceinline__ float loss_of(double total, int64_t E, int64_t T, int
 // One workgroup's rows: column sums of p over them in registers, then over the
 // workgroup's rows of lanes in LDS. ONE: the whole batch, loss included.
 template <typename T, int PIECES, bool WIDE, bool ONE>
-__global__ void __launch_bounds__(ONE ? kOneWg : kThreads)
+__global__ void __launch_bounds__(ONE ? kOneWg : kRowThreads)
 balance_rows(const T* __restrict__ logits, const int32_t* __restrict__ ids, const uint8_t* __restrict__ mask,
              int64_t M, int E, int k, BalanceScratch s, float* __restrict__ loss, int32_t* __restrict__ counts,
              int32_t* __restrict__ tokens) {
-  constexpr int N = PIECES * 8, kT = ONE ? kOneWg : kThreads, kWaves = kT / 64;
+  constexpr int N = PIECES * 8, kT = ONE ? kOneWg : kRowThreads, kWaves = kT / 64;
   __shared__ float lds_sum[kWaves][PIECES * 128];
   __shared__ int lds_cnt[PIECES * 128];
   __shared__ int lds_rows;
@@ -134,10 +147,11 @@ balance_rows(const T* __restrict__ logits, const int32_t* __restrict__ ids, cons
       const int id = ids[row * k + j];
       if (id >= 0 && id < E) atomicAdd(&lds_cnt[id], 1);
     }
-    float p[N], mx, sum;
-    row_softmax<T, PIECES, WIDE>(logits + row * E, E, i16, p, mx, sum);
+    float p[N], mx;
+    load_row<T, PIECES, WIDE>(logits + row * E, E, i16, p);
+    const float inv = 1.f / row_exp<N>(p, mx);
 #pragma unroll
-    for (int j = 0; j < N; ++j) acc[j] += p[j];
+    for (int j = 0; j < N; ++j) acc[j] = fmaf(p[j], inv, acc[j]);
   }
   if (i16 == 0 && rows) atomicAdd(&lds_rows, rows);
 #pragma unroll
@@ -180,40 +194,55 @@ balance_rows(const T* __restrict__ logits, const int32_t* __restrict__ ids, cons
   }
 }
 
-// Adds the planes: 16 columns a workgroup, 16 threads a column; the workgroup that
-// arrives last adds the loss's parts in order. COUNTED: counts[] is complete.
+// Adds the planes: 16 columns a workgroup, 64 threads a column, eight planes' loads in
+// flight each; the workgroup that arrives last adds the loss's parts in order.
+// COUNTED: counts[] is complete.
 template <bool COUNTED>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kOneWg)
 balance_finish(int planes, int64_t E, int64_t k, BalanceScratch s, float* __restrict__ loss,
                int32_t* __restrict__ counts, int32_t* __restrict__ tokens) {
-  __shared__ float lds_p[16][16];
-  __shared__ int lds_c[16][16];
-  __shared__ int lds_rows[4];
-  __shared__ bool last;
+  constexpr int kParts = kOneWg / 16, kAhead = 8;
+  __shared__ float lds_p[kParts][16];
+  __shared__ int lds_c[kParts][16];
+  __shared__ int lds_rows[kOneWg / 64];
   const int tid = threadIdx.x, col = tid & 15, part = tid >> 4;
   const int64_t e = int64_t(blockIdx.x) * 16 + col;
   float p = 0.f;
   int c = 0;
-  if (e < E)
-    for (int g = part; g < planes; g += 16) {
-      p += s.sums[int64_t(g) * E + e];
-      if (!COUNTED) c += s.cnt[int64_t(g) * E + e];
+  for (int g0 = part; g0 < planes; g0 += kParts * kAhead) {
+    float pv[kAhead];
+    int cv[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int g = g0 + j * kParts;
+      const bool in = g < planes && e < E;
+      pv[j] = in ? s.sums[int64_t(g) * E + e] : 0.f;
+      cv[j] = in && !COUNTED ? s.cnt[int64_t(g) * E + e] : 0;
     }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      p += pv[j];
+      c += cv[j];
+    }
+  }
   lds_p[part][col] = p;
   lds_c[part][col] = c;
   int rows = 0;
-  for (int g = tid; g < planes; g += kThreads) rows += s.rows[g];
+  for (int g = tid; g < planes; g += kOneWg) rows += s.rows[g];
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) rows += __shfl_xor(rows, off);
   if ((tid & 63) == 0) lds_rows[tid >> 6] = rows;
   __syncthreads();
-  const int T = lds_rows[0] + lds_rows[1] + lds_rows[2] + lds_rows[3];
+  if (tid >= 64) return;
+  int T = 0;
+#pragma unroll
+  for (int w = 0; w < kOneWg / 64; ++w) T += lds_rows[w];
   double dot = 0.0;
   if (tid < 16 && e < E) {
     float ps = 0.f;
     int cs = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
+#pragma unroll 16
+    for (int i = 0; i < kParts; ++i) {
       ps += lds_p[i][col];
       cs += lds_c[i][col];
     }
@@ -221,17 +250,14 @@ balance_finish(int planes, int64_t E, int64_t k, BalanceScratch s, float* __rest
     else counts[e] = cs;
     dot = double(cs) * double(ps);
   }
-  if (tid < 64) {
 #pragma unroll
-    for (int off = 8; off >= 1; off >>= 1) dot += __shfl_xor(dot, off);
-    if (tid == 0) {
-      __hip_atomic_store(&s.parts[blockIdx.x], dot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      const int at = __hip_atomic_fetch_add(s.ticket, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-      last = at == int(gridDim.x) - 1;
-    }
+  for (int off = 8; off >= 1; off >>= 1) dot += __shfl_xor(dot, off);
+  int at = 0;
+  if (tid == 0) {
+    __hip_atomic_store(&s.parts[blockIdx.x], dot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    at = __hip_atomic_fetch_add(s.ticket, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
   }
-  __syncthreads();
-  if (!last || tid >= 64) return;
+  if (__builtin_amdgcn_readfirstlane(at) != int(gridDim.x) - 1) return;
   double total = 0.0;
   for (int i = tid; i < int(gridDim.x); i += 64)
     total += __hip_atomic_load(&s.parts[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -311,13 +337,18 @@ __device__ __forceinline__ float loss_factor(const RouterGrad& a, int64_t M, int
 }
 
 // The counts less their mean: as p sums to 1, c_i - sum p c is the same of either,
-// and near-uniform counts (as a balanced router has) no longer cancel.
+// and near-uniform counts (as a balanced router has) no longer cancel. A row's
+// gradient goes through LDS on its way out: the selected experts' slots, on the lane
+// of their number, put their values there, and whole pieces leave.
 template <typename T, int PIECES, bool WIDE>
 __global__ void __launch_bounds__(kThreads)
 router_grad_rows(const T* __restrict__ logits, int64_t M, int E, int k, RouterGrad a, T* __restrict__ grad) {
-  constexpr int N = PIECES * 8;
+  constexpr int N = PIECES * 8, ROW = PIECES * 128;
+  __shared__ __attribute__((aligned(16))) T rows_lds[kThreads / 16][ROW];
+  __shared__ float centred[ROW];
   const int tid = threadIdx.x, i16 = tid & 15;
-  const bool with_loss = a.grad_loss != nullptr;
+  const bool with_loss = a.grad_loss != nullptr, with_weights = a.grad_weights != nullptr;
+  T* mine = rows_lds[tid >> 4];
   float c[N], mean = 0.f;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
@@ -327,79 +358,89 @@ router_grad_rows(const T* __restrict__ logits, int64_t M, int E, int k, RouterGr
   }
   mean = row_sum(mean) / float(E);
 #pragma unroll
-  for (int j = 0; j < N; ++j) c[j] -= mean;
+  for (int j = 0; j < N; ++j) {
+    c[j] -= mean;
+    if (tid < 16) centred[((j >> 3) * 16 + i16) * 8 + (j & 7)] = c[j];
+  }
+  __syncthreads();
   const float factor = loss_factor(a, M, E, k);
   for (int64_t row = int64_t(blockIdx.x) * (kThreads / 16) + (tid >> 4); row < M;
        row += int64_t(gridDim.x) * (kThreads / 16)) {
+    const T* g = logits + row * E;
     T* out = grad + row * E;
     const bool on = a.mask == nullptr || a.mask[row] != 0;  // the same on a row's 16 lanes
-    float p[N], pc = 0.f, q = 0.f, slot = 0.f, p_id = 0.f, mx = 0.f, sum = 1.f;
-    int id = -1;
+    float p[N];
     if (on) {
-      row_softmax<T, PIECES, WIDE>(logits + row * E, E, i16, p, mx, sum);
+      int id = -1;
+      float u = 0.f, z_id = -__builtin_inff();
+      if (with_weights && i16 < k) {  // lane t holds slot t
+        id = a.ids[row * k + i16];
+        if (id < 0 || id >= E) id = -1;
+        u = a.grad_weights[row * k + i16];
+      }
+      load_row<T, PIECES, WIDE>(g, E, i16, p);
+      if (id >= 0) z_id = logit_at<T>(g + id);
+      float mx, pc = 0.f, q = 0.f;
+      const float inv = 1.f / row_exp<N>(p, mx);
       if (with_loss) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) pc += p[j] * c[j];
-        pc = row_sum(pc);
+        for (int j = 0; j < N; ++j) pc = fmaf(p[j], c[j], pc);
+        pc = row_sum(pc) * inv;
       }
-      if (a.grad_weights != nullptr) {  // lane t holds slot t
-        float u = 0.f;
-        if (i16 < k) {
-          id = a.ids[row * k + i16];
-          if (id < 0 || id >= E) id = -1;
-          u = a.grad_weights[row * k + i16];
-        }
-        if (id >= 0) p_id = expf(logit_at<T>(logits + row * E + id) - mx) / sum;
-        if (a.renorm) {
-          const float ps = row_sum(p_id);  // by all 16 lanes
-          const float w = id >= 0 ? p_id / ps : 0.f;
-          const float wu = row_sum(id >= 0 ? w * u : 0.f);
-          slot = id >= 0 ? w * (u - wu) : 0.f;
+      float slot = 0.f, p_id = 0.f;
+      if (with_weights) {
+        p_id = id >= 0 ? exp_neg(z_id - mx) * inv : 0.f;
+        if (a.renorm) {  // a softmax of the slots' logits
+          const float top = row_max(z_id);
+          const float w = id >= 0 ? exp_neg(z_id - top) : 0.f;
+          const float scale = 1.f / row_sum(w);
+          const float wu = row_sum(id >= 0 ? w * u : 0.f) * scale;
+          slot = id >= 0 ? w * scale * (u - wu) : 0.f;
         } else {
           slot = id >= 0 ? p_id * u : 0.f;
           q = row_sum(slot);
         }
       }
+      const float f = factor * inv, qi = q * inv;
 #pragma unroll
-      for (int j = 0; j < N; ++j) p[j] = with_loss ? factor * p[j] * (c[j] - pc) - p[j] * q : -p[j] * q;
+      for (int j = 0; j < N; ++j) p[j] = with_loss ? p[j] * fmaf(f, c[j] - pc, -qi) : -p[j] * qi;
+#pragma unroll
+      for (int cc = 0; cc < PIECES; ++cc)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mine[(cc * 16 + i16) * 8 + i] = to_out<T>(p[8 * cc + i]);
+      if (with_weights) {
+        // every slot of one expert forms the same sum, in slot order
+        float add = 0.f;
+        for (int l = 0; l < k; ++l) {
+          const float v = __shfl(slot, (tid & 48) + l);
+          const int other = __shfl(id, (tid & 48) + l);
+          if (other == id) add += v;
+        }
+        if (id >= 0) mine[id] = to_out<T>((with_loss ? p_id * fmaf(factor, centred[id] - pc, -q) : -p_id * q) + add);
+      }
     } else {
 #pragma unroll
-      for (int j = 0; j < N; ++j) p[j] = 0.f;
+      for (int cc = 0; cc < PIECES; ++cc)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mine[(cc * 16 + i16) * 8 + i] = to_out<T>(0.f);
     }
+    // (a wave's LDS accesses are carried out in order; its rows are its own)
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int cc = 0; cc < PIECES; ++cc) {
       const int e0 = (cc * 16 + i16) * 8;
       if (WIDE) {
-        if (e0 < E) {
-          __attribute__((aligned(16))) T v[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = to_out<T>(p[8 * cc + i]);
+        if (e0 < E)
 #pragma unroll
           for (int h = 0; h < int(sizeof(T)) / 2; ++h)
-            reinterpret_cast<u32x4*>(out + e0)[h] = reinterpret_cast<const u32x4*>(v)[h];
-        }
+            reinterpret_cast<u32x4*>(out + e0)[h] = reinterpret_cast<const u32x4*>(mine + e0)[h];
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (e0 + i < E) out[e0 + i] = to_out<T>(p[8 * cc + i]);
+          if (e0 + i < E) out[e0 + i] = mine[e0 + i];
       }
     }
-    if (on && a.grad_weights != nullptr) {
-      // the selected experts' values once more, with their slots' part: every
-      // slot of one expert forms the same sum, in slot order
-      float add = 0.f;
-      for (int l = 0; l < k; ++l) {
-        const float v = __shfl(slot, (tid & 48) + l);
-        const int other = __shfl(id, (tid & 48) + l);
-        if (other == id) add += v;
-      }
-      if (id >= 0) {
-        const float ci = with_loss ? float(a.counts[id]) - mean : 0.f;
-        const float v = (with_loss ? factor * p_id * (ci - pc) : 0.f) - p_id * q + add;
-        __builtin_amdgcn_s_waitcnt(0x0F70);  // the row's stores first (vmcnt 0)
-        out[id] = to_out<T>(v);
-      }
-    }
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -428,16 +469,23 @@ router_grad_any(const T* __restrict__ logits, int64_t M, int64_t E, int64_t k, R
     for (int64_t e = lane; e < E; e += 64) sum += expf(logit_at<T>(g + e) - mx);
     sum = wave_sum(sum);
     auto prob = [&](int64_t e) { return expf(logit_at<T>(g + e) - mx) / sum; };
-    float pc = 0.f, q = 0.f, ps = 0.f, wu = 0.f;
+    float pc = 0.f, q = 0.f, ps = 0.f, wu = 0.f, top = -__builtin_inff();
     if (with_loss) {
       for (int64_t e = lane; e < E; e += 64) pc += prob(e) * (float(a.counts[e]) - mean);
       pc = wave_sum(pc);
     }
     if (a.grad_weights != nullptr) {
+      if (a.renorm) {  // a softmax of the slots' logits
+        for (int64_t j = lane; j < k; j += 64) {
+          const int id = a.ids[row * k + j];
+          if (id >= 0 && id < E) top = fmaxf(top, logit_at<T>(g + id));
+        }
+        top = wave_max(top);
+      }
       for (int64_t j = lane; j < k; j += 64) {
         const int id = a.ids[row * k + j];
         if (id < 0 || id >= E) continue;
-        const float pj = prob(id);
+        const float pj = a.renorm ? expf(logit_at<T>(g + id) - top) : prob(id);
         ps += pj;
         q += pj * a.grad_weights[row * k + j];
       }
@@ -458,7 +506,7 @@ router_grad_any(const T* __restrict__ logits, int64_t M, int64_t E, int64_t k, R
     for (int64_t j = lane; j < k; j += 64) {
       const int id = a.ids[row * k + j];
       if (id < 0 || id >= E) continue;
-      const float w = a.renorm ? prob(id) / ps : prob(id);
+      const float w = a.renorm ? expf(logit_at<T>(g + id) - top) / ps : prob(id);
       float add = 0.f;
       for (int64_t l = 0; l < k; ++l)
         if (a.ids[row * k + l] == id) add += w * (a.grad_weights[row * k + l] - wu);
@@ -468,7 +516,7 @@ router_grad_any(const T* __restrict__ logits, int64_t M, int64_t E, int64_t k, R
 }
 
 int planes_for(int64_t M, int64_t E) {
-  if (E <= kFastExperts) return int(std::min<int64_t>(kPlanes, cdiv(M, 32)));
+  if (E <= kFastExperts) return int(std::min<int64_t>(kPlanes, cdiv(M, kRowThreads / 16)));
   return int(std::max<int64_t>(1, std::min<int64_t>(64, cdiv(M, 16))));
 }
 int64_t up(int64_t x) { return (x + 255) / 256 * 256; }
@@ -480,7 +528,7 @@ void launch_balance_rows(const T* g, const int32_t* ids, const uint8_t* mask, in
   const bool wide = E % 8 == 0 && reinterpret_cast<uintptr_t>(g) % 16 == 0;
   const bool one = M <= kOneWgRows;
 #define XK_ROWS(W, O)                                                                                             \
-  hipLaunchKernelGGL((balance_rows<T, PIECES, W, O>), dim3(O ? 1 : planes), dim3(O ? kOneWg : kThreads), 0, stream, g, \
+  hipLaunchKernelGGL((balance_rows<T, PIECES, W, O>), dim3(O ? 1 : planes), dim3(O ? kOneWg : kRowThreads), 0, stream, g, \
                      ids, mask, M, E, k, s, loss, counts, tokens)
   if (one && wide) XK_ROWS(true, true);
   else if (one) XK_ROWS(false, true);
@@ -498,10 +546,11 @@ int balance_typed(const void* logits, const int32_t* ids, const uint8_t* mask, i
     const int e = int(E), kk = int(k);
     if (E <= 128) launch_balance_rows<T, 1>(g, ids, mask, M, e, kk, planes, s, loss, counts, tokens, stream);
     else if (E <= 256) launch_balance_rows<T, 2>(g, ids, mask, M, e, kk, planes, s, loss, counts, tokens, stream);
+    else if (E <= 384) launch_balance_rows<T, 3>(g, ids, mask, M, e, kk, planes, s, loss, counts, tokens, stream);
     else launch_balance_rows<T, 4>(g, ids, mask, M, e, kk, planes, s, loss, counts, tokens, stream);
     XK_CHECK_LAUNCH("balance_rows");
     if (M <= kOneWgRows) return XK_OK;
-    hipLaunchKernelGGL((balance_finish<false>), dim3(unsigned(cdiv(E, 16))), dim3(kThreads), 0, stream, planes, E, k,
+    hipLaunchKernelGGL((balance_finish<false>), dim3(unsigned(cdiv(E, 16))), dim3(kOneWg), 0, stream, planes, E, k,
                        s, loss, counts, tokens);
   } else {
     const int64_t per = std::max<int64_t>(1, cdiv(M, planes));
@@ -511,7 +560,7 @@ int balance_typed(const void* logits, const int32_t* ids, const uint8_t* mask, i
     hipLaunchKernelGGL((balance_columns<T>), dim3(unsigned(cdiv(E, kThreads)), planes), dim3(kThreads), 0, stream, g,
                        ids, mask, M, E, k, per, s, counts);
     XK_CHECK_LAUNCH("balance_columns");
-    hipLaunchKernelGGL((balance_finish<true>), dim3(unsigned(cdiv(E, 16))), dim3(kThreads), 0, stream, planes, E, k,
+    hipLaunchKernelGGL((balance_finish<true>), dim3(unsigned(cdiv(E, 16))), dim3(kOneWg), 0, stream, planes, E, k,
                        s, loss, counts, tokens);
   }
   XK_CHECK_LAUNCH("balance_finish");
@@ -536,6 +585,7 @@ int grad_typed(const void* logits, int64_t M, int64_t E, int64_t k, const Router
   if (E <= kFastExperts && k <= kFastTopk) {
     if (E <= 128) launch_grad_rows<T, 1>(g, M, int(E), int(k), a, o, stream);
     else if (E <= 256) launch_grad_rows<T, 2>(g, M, int(E), int(k), a, o, stream);
+    else if (E <= 384) launch_grad_rows<T, 3>(g, M, int(E), int(k), a, o, stream);
     else launch_grad_rows<T, 4>(g, M, int(E), int(k), a, o, stream);
   } else {
     hipLaunchKernelGGL((router_grad_any<T>), dim3(unsigned(std::min<int64_t>(4096, cdiv(M, 4)))), dim3(kThreads), 0,

@@ -8,7 +8,7 @@ Nothing synchronises, so every call may be captured into a HIP graph.
 """
 from __future__ import annotations
 
-from contextlib import nullcontext
+from functools import lru_cache
 
 import torch
 
@@ -17,47 +17,74 @@ from .._backends import Backend
 from .._dispatch import register
 from .act_checkpoint import ActCheckpoint
 from .balance_loss import BalanceLoss
-from .hip_backend import _contig, _need_gpu, _ptr, _stream
+from .hip_backend import _contig, _need_gpu, _ptr, _raw_stream
 
 _LORA_DT = {torch.bfloat16: _lib.XK_DT_BF16, torch.float32: _lib.XK_DT_FP32}
 _ANY_DT = {**_LORA_DT, torch.float16: _lib.XK_DT_FP16}
 BLOCK = 32
 
+# the current device's number without torch.cuda's lazy-initialisation checks (the
+# tensors at hand are on a device), where this torch has the call
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
-def _on(dev: torch.device):
-    """The tensors' device as the current one: HIP launches on a stream need it."""
-    return nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+def _device(op: str, first: torch.Tensor, *others: torch.Tensor | None) -> int:
+    """The number of the device that all of them are on."""
+    i = first.get_device()
+    if i < 0:
+        _need_gpu(op, first)
+    for t in others:
+        if t is not None and t.get_device() != i:
+            _need_gpu(op, first, t)
+    return i
+
+
+def _stream(i: int) -> int:
+    return _raw_stream(i) if _raw_stream is not None else torch.cuda.current_stream(i).cuda_stream
+
+
+def _elsewhere(i: int, fn, *args):
+    """``fn(*args)`` with device ``i``, which its tensors are on, as the current one: HIP
+    launches on a stream need it."""
+    with torch.cuda.device(i):
+        return fn(*args)
 
 
 def _code(op: str, t: torch.Tensor, table=_ANY_DT) -> int:
-    try:
-        return table[t.dtype]
-    except KeyError:
+    dt = table.get(t.dtype)
+    if dt is None:
         names = ", ".join(str(d).removeprefix("torch.") for d in table)
-        raise RuntimeError(f"{op}: unsupported dtype {t.dtype} ({names})") from None
+        raise RuntimeError(f"{op}: unsupported dtype {t.dtype} ({names})")
+    return dt
 
 
-def _scratch(nbytes: int, dev) -> torch.Tensor:
-    return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+@lru_cache(maxsize=4096)
+def _bytes(query: str, *sizes: int) -> int:
+    """A workspace's size, a function of the call's sizes alone."""
+    return max(_lib.query(query, *sizes), 1)
 
 
 def _ids(op: str, t: torch.Tensor, n: int) -> torch.Tensor:
     """int32, contiguous; 64-bit ids outside [0, n) stay outside."""
+    if t.dtype == torch.int32:
+        return t if t.is_contiguous() else t.contiguous()
     if t.dtype == torch.int64:
         t = t.clamp(-1, n)
-    elif t.dtype not in (torch.int32, torch.int16, torch.int8, torch.uint8):
+    elif t.dtype not in (torch.int16, torch.int8, torch.uint8):
         raise RuntimeError(f"{op}: ids must be whole numbers, got {t.dtype}")
     return _contig(t, torch.int32)
 
 
 def _shape(op: str, name: str, t: torch.Tensor | None, want: tuple) -> None:
-    if t is not None and tuple(t.shape) != want:
+    if t is not None and t.shape != want:
         raise RuntimeError(f"{op}: {name} must be {list(want)}, got {list(t.shape)}")
 
 
 def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     """``t`` [M, n] as rows of consecutive values, and how far they lie apart."""
     M, n = t.shape
+    if t.is_contiguous():
+        return t, n
     if M > 1 and (n == 1 or t.stride(1) == 1) and t.stride(0) >= n:
         return t, t.stride(0)
     return t.contiguous(), n
@@ -82,16 +109,18 @@ def _router_args(op, gating_output, topk_ids, mask):
 def moe_balance_loss_hip(gating_output: torch.Tensor, topk_ids: torch.Tensor,
                          mask: torch.Tensor | None = None) -> BalanceLoss:
     op = "moe_balance_loss"
-    dev = _need_gpu(op, gating_output, topk_ids, mask)
+    i = _device(op, gating_output, topk_ids, mask)
+    if i != _current_device():
+        return _elsewhere(i, moe_balance_loss_hip, gating_output, topk_ids, mask)
     dt = _code(op, gating_output)
     M, E, k, g, ids, on = _router_args(op, gating_output, topk_ids, mask)
-    with _on(dev):
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        counts = torch.empty(E, dtype=torch.int32, device=dev)
-        tokens = torch.empty((), dtype=torch.int32, device=dev)
-        ws = _scratch(_lib.query("xk_moe_balance_loss_workspace_bytes", M, E), dev)
-        _lib.call("xk_moe_balance_loss", _ptr(g), dt, M, E, _ptr(ids), k, _ptr(on), _ptr(loss), _ptr(counts),
-                  _ptr(tokens), _ptr(ws), ws.numel(), _stream(dev))
+    loss = g.new_empty((), dtype=torch.float32)
+    counts = g.new_empty(E, dtype=torch.int32)
+    tokens = g.new_empty((), dtype=torch.int32)
+    nbytes = _bytes("xk_moe_balance_loss_workspace_bytes", M, E)
+    ws = g.new_empty(nbytes, dtype=torch.uint8)
+    _lib.call("xk_moe_balance_loss", g.data_ptr(), dt, M, E, ids.data_ptr(), k, _ptr(on), loss.data_ptr(),
+              counts.data_ptr(), tokens.data_ptr(), ws.data_ptr(), nbytes, _stream(i))
     return BalanceLoss(loss, counts, tokens)
 
 
@@ -101,7 +130,10 @@ def moe_router_backward_hip(gating_output: torch.Tensor, topk_ids: torch.Tensor,
                             tokens: torch.Tensor | None = None,
                             mask: torch.Tensor | None = None) -> torch.Tensor:
     op = "moe_router_backward"
-    dev = _need_gpu(op, gating_output, topk_ids, grad_weights, grad_loss, counts, tokens, mask)
+    i = _device(op, gating_output, topk_ids, grad_weights, grad_loss, counts, tokens, mask)
+    if i != _current_device():
+        return _elsewhere(i, moe_router_backward_hip, gating_output, topk_ids, grad_weights, renormalize, grad_loss,
+                          counts, tokens, mask)
     dt = _code(op, gating_output)
     M, E, k, g, ids, on = _router_args(op, gating_output, topk_ids, mask)
     if grad_weights is None and grad_loss is None:
@@ -119,28 +151,27 @@ def moe_router_backward_hip(gating_output: torch.Tensor, topk_ids: torch.Tensor,
             raise RuntimeError(f"{op}: grad_loss and tokens are single numbers")
         gl, cn = _contig(grad_loss, torch.float32), _contig(counts, torch.int32)
         tk = None if tokens is None else _contig(tokens, torch.int32)
-    with _on(dev):
-        grad = torch.empty_like(g)
-        _lib.call("xk_moe_router_backward", _ptr(g), dt, M, E, _ptr(ids), k, _ptr(on), _ptr(gl), _ptr(cn), _ptr(tk),
-                  _ptr(gw), int(bool(renormalize)), _ptr(grad), _stream(dev))
+    grad = torch.empty_like(g)
+    _lib.call("xk_moe_router_backward", g.data_ptr(), dt, M, E, ids.data_ptr(), k, _ptr(on), _ptr(gl), _ptr(cn),
+              _ptr(tk), _ptr(gw), int(bool(renormalize)), grad.data_ptr(), _stream(i))
     return grad
 
 
 # ----------------------------------------------------------------- adapters ----
 
-def _lora_args(op, rows, n_rows_name, cols, lora_a, lora_b, adapter_ids, scaling):
+def _lora_args(op, M, name, cols, axis, lora_a, lora_b, adapter_ids, scaling):
+    """Checks the adapters against ``cols`` columns of ``name`` (axis 0: K, 1: N)."""
     if lora_a.dim() != 3 or lora_b.dim() != 3:
         raise RuntimeError(f"{op}: expected lora_a [L, r, K] and lora_b [L, N, r]")
     L, r, K = lora_a.shape
     N = lora_b.shape[1]
     _shape(op, "lora_b", lora_b, (L, N, r))
-    _shape(op, "adapter_ids", adapter_ids, (rows,))
+    _shape(op, "adapter_ids", adapter_ids, (M,))
     _shape(op, "scaling", scaling, (L,))
     if lora_a.dtype != lora_b.dtype:
         raise RuntimeError(f"{op}: lora_a is {lora_a.dtype}, lora_b {lora_b.dtype}")
-    if cols[0] != (K if n_rows_name == "x" else N):
-        raise RuntimeError(f"{op}: {n_rows_name} has {cols[0]} columns, the adapters "
-                           f"{K if n_rows_name == 'x' else N}")
+    if cols != (N if axis else K):
+        raise RuntimeError(f"{op}: {name} has {cols} columns, the adapters {N if axis else K}")
     sc = None if scaling is None else _contig(scaling, torch.float32)
     return L, r, K, N, lora_a.contiguous(), lora_b.contiguous(), _ids(op, adapter_ids, L), sc
 
@@ -149,24 +180,27 @@ def lora_projection_hip(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Ten
                         base: torch.Tensor | None = None, scaling: torch.Tensor | None = None,
                         return_hidden: bool = False):
     op = "lora_projection"
-    dev = _need_gpu(op, x, lora_a, lora_b, adapter_ids, base, scaling)
+    i = _device(op, x, lora_a, lora_b, adapter_ids, base, scaling)
+    if i != _current_device():
+        return _elsewhere(i, lora_projection_hip, x, lora_a, lora_b, adapter_ids, base, scaling, return_hidden)
     dt = _code(op, x, _LORA_DT)
     if x.dim() != 2:
         raise RuntimeError(f"{op}: x must be [M, K], got {list(x.shape)}")
-    M = x.shape[0]
-    L, r, K, N, a, b, ids, sc = _lora_args(op, M, "x", x.shape[1:], lora_a, lora_b, adapter_ids, scaling)
-    _shape(op, "base", base, (M, N))
-    for name, t in (("lora_a", a), ("base", base)):
-        if t is not None and t.dtype != x.dtype:
-            raise RuntimeError(f"{op}: {name} is {t.dtype}, x {x.dtype}")
+    M, cols = x.shape
+    L, r, K, N, a, b, ids, sc = _lora_args(op, M, "x", cols, 0, lora_a, lora_b, adapter_ids, scaling)
+    if a.dtype != x.dtype or (base is not None and base.dtype != x.dtype):
+        raise RuntimeError(f"{op}: x is {x.dtype}, the adapters {a.dtype}, base {None if base is None else base.dtype}")
     xr, ldx = _rows(x)
-    br, ldb = (None, N) if base is None else _rows(base)
-    with _on(dev):
-        out = torch.empty((M, N), dtype=x.dtype, device=dev)
-        hidden = torch.empty((M, r), dtype=torch.float32, device=dev) if return_hidden else None
-        ws = _scratch(_lib.query("xk_lora_projection_workspace_bytes", M, K, L, r), dev)
-        _lib.call("xk_lora_projection", _ptr(xr), dt, ldx, M, K, _ptr(a), _ptr(b), L, N, r, _ptr(ids), _ptr(sc),
-                  _ptr(br), ldb, _ptr(out), _ptr(hidden), _ptr(ws), ws.numel(), _stream(dev))
+    br, ldb = None, N
+    if base is not None:
+        _shape(op, "base", base, (M, N))
+        br, ldb = _rows(base)
+    out = x.new_empty((M, N))
+    hidden = x.new_empty((M, r), dtype=torch.float32) if return_hidden else None
+    nbytes = _bytes("xk_lora_projection_workspace_bytes", M, K, L, r)
+    ws = x.new_empty(nbytes, dtype=torch.uint8)
+    _lib.call("xk_lora_projection", xr.data_ptr(), dt, ldx, M, K, a.data_ptr(), b.data_ptr(), L, N, r, ids.data_ptr(),
+              _ptr(sc), _ptr(br), ldb, out.data_ptr(), _ptr(hidden), ws.data_ptr(), nbytes, _stream(i))
     return (out, hidden) if return_hidden else out
 
 
@@ -176,38 +210,37 @@ def lora_projection_backward_hip(grad_out: torch.Tensor, x: torch.Tensor | ActCh
     op = "lora_projection_backward"
     held = isinstance(x, ActCheckpoint)
     xt, scales = (x.values, x.scales) if held else (x, None)
-    dev = _need_gpu(op, grad_out, xt, scales, lora_a, lora_b, adapter_ids, hidden, scaling)
+    i = _device(op, grad_out, xt, scales, lora_a, lora_b, adapter_ids, hidden, scaling)
+    if i != _current_device():
+        return _elsewhere(i, lora_projection_backward_hip, grad_out, x, lora_a, lora_b, adapter_ids, hidden, scaling)
     dt = _code(op, grad_out, _LORA_DT)
     if grad_out.dim() != 2:
         raise RuntimeError(f"{op}: grad_out must be [M, N], got {list(grad_out.shape)}")
-    M = grad_out.shape[0]
-    L, r, K, N, a, b, ids, sc = _lora_args(op, M, "grad_out", grad_out.shape[1:], lora_a, lora_b, adapter_ids, scaling)
+    M, cols = grad_out.shape
+    L, r, K, N, a, b, ids, sc = _lora_args(op, M, "grad_out", cols, 1, lora_a, lora_b, adapter_ids, scaling)
     _shape(op, "x", xt, (M, K))
     _shape(op, "hidden", hidden, (M, r))
-    if a.dtype != grad_out.dtype:
-        raise RuntimeError(f"{op}: lora_a is {a.dtype}, grad_out {grad_out.dtype}")
+    if a.dtype != grad_out.dtype or (not held and x.dtype != grad_out.dtype):
+        raise RuntimeError(f"{op}: grad_out is {grad_out.dtype}, the adapters {a.dtype}, x {xt.dtype}")
     if held:
-        xr, sr = _check_held(op, x)
-        ldx = K
+        (xr, sr), ldx = _check_held(op, x), K
     else:
-        if x.dtype != grad_out.dtype:
-            raise RuntimeError(f"{op}: x is {x.dtype}, grad_out {grad_out.dtype}")
         (xr, ldx), sr = _rows(x), None
     gr, ldg = _rows(grad_out)
     h = _contig(hidden, torch.float32)
-    with _on(dev):
-        grad_x = torch.empty((M, K), dtype=grad_out.dtype, device=dev)
-        grad_a, grad_b = torch.empty_like(a), torch.empty_like(b)
-        ws = _scratch(_lib.query("xk_lora_projection_backward_workspace_bytes", M, K, N, L, r, dt), dev)
-        _lib.call("xk_lora_projection_backward", _ptr(gr), dt, ldg, _ptr(xr), ldx, _ptr(sr), M, K, _ptr(a), _ptr(b),
-                  L, N, r, _ptr(ids), _ptr(sc), _ptr(h), _ptr(grad_x), _ptr(grad_a), _ptr(grad_b), _ptr(ws),
-                  ws.numel(), _stream(dev))
+    grad_x = grad_out.new_empty((M, K))
+    grad_a, grad_b = torch.empty_like(a), torch.empty_like(b)
+    nbytes = _bytes("xk_lora_projection_backward_workspace_bytes", M, K, N, L, r, dt)
+    ws = grad_out.new_empty(nbytes, dtype=torch.uint8)
+    _lib.call("xk_lora_projection_backward", gr.data_ptr(), dt, ldg, xr.data_ptr(), ldx, _ptr(sr), M, K, a.data_ptr(),
+              b.data_ptr(), L, N, r, ids.data_ptr(), _ptr(sc), h.data_ptr(), grad_x.data_ptr(), grad_a.data_ptr(),
+              grad_b.data_ptr(), ws.data_ptr(), nbytes, _stream(i))
     return grad_x, grad_a, grad_b
 
 
 # -------------------------------------------------------------- checkpoints ----
 
-def _check_held(op: str, held: ActCheckpoint) -> tuple[torch.Tensor, torch.Tensor]:
+def _check_held(op: str, held) -> tuple[torch.Tensor, torch.Tensor]:
     v, s = held
     if v.dim() != 2 or v.dtype != torch.float8_e4m3fn or s.dtype != torch.uint8:
         raise RuntimeError(f"{op}: a checkpoint is float8_e4m3fn [M, K] with uint8 scales, got {v.dtype} "
@@ -218,30 +251,31 @@ def _check_held(op: str, held: ActCheckpoint) -> tuple[torch.Tensor, torch.Tenso
 
 def act_checkpoint_hip(x: torch.Tensor) -> ActCheckpoint:
     op = "act_checkpoint"
-    dev = _need_gpu(op, x)
+    i = _device(op, x)
+    if i != _current_device():
+        return _elsewhere(i, act_checkpoint_hip, x)
     dt = _code(op, x)
     if x.dim() != 2 or x.shape[1] == 0:
         raise RuntimeError(f"{op}: x must be [M, K], K >= 1, got {list(x.shape)}")
     M, K = x.shape
     xr, ldx = _rows(x)
-    with _on(dev):
-        values = torch.empty((M, K), dtype=torch.float8_e4m3fn, device=dev)
-        scales = torch.empty((M, -(-K // BLOCK)), dtype=torch.uint8, device=dev)
-        _lib.call("xk_act_checkpoint", _ptr(xr), dt, ldx, M, K, _ptr(values), _ptr(scales), _stream(dev))
+    values = x.new_empty((M, K), dtype=torch.float8_e4m3fn)
+    scales = x.new_empty((M, -(-K // BLOCK)), dtype=torch.uint8)
+    _lib.call("xk_act_checkpoint", xr.data_ptr(), dt, ldx, M, K, values.data_ptr(), scales.data_ptr(), _stream(i))
     return ActCheckpoint(values, scales)
 
 
 def act_restore_hip(held: ActCheckpoint, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     op = "act_restore"
-    held = ActCheckpoint(*held)
-    dev = _need_gpu(op, *held)
+    i = _device(op, *held)
+    if i != _current_device():
+        return _elsewhere(i, act_restore_hip, held, dtype)
     v, s = _check_held(op, held)
     M, K = v.shape
     if K == 0:
         raise RuntimeError(f"{op}: no columns")
-    with _on(dev):
-        out = torch.empty((M, K), dtype=dtype, device=dev)
-        _lib.call("xk_act_restore", _ptr(v), _ptr(s), M, K, _code(op, out), _ptr(out), _stream(dev))
+    out = v.new_empty((M, K), dtype=dtype)
+    _lib.call("xk_act_restore", v.data_ptr(), s.data_ptr(), M, K, _code(op, out), out.data_ptr(), _stream(i))
     return out
 
 
