@@ -28,6 +28,7 @@ constexpr int kRowThreads = 512;    // of a forward's workgroup: few planes, man
 constexpr int kOneWg = 1024;        // threads of the one workgroup of a small batch, and of the sums
 constexpr int64_t kOneWgRows = 256; // rows up to which it is one workgroup's work
 constexpr int kFastExperts = 512, kFastTopk = 16;
+constexpr int kGradWgs = 1024;      // most workgroups of the gradient: each forms the counts' mean once
 constexpr int kPlanes = 512;        // most workgroups of the forward: 16 waves a CU
 
 __device__ __forceinline__ float row_max(float x) {
@@ -336,6 +337,19 @@ __device__ __forceinline__ float loss_factor(const RouterGrad& a, int64_t M, int
   return T > 0.0 ? float(double(*a.grad_loss) * double(E) / (T * T * double(k))) : 0.f;
 }
 
+template <typename T, int PIECES>
+__device__ __forceinline__ void put_row(const float* p, T* row, int i16) {
+#pragma unroll
+  for (int cc = 0; cc < PIECES; ++cc) {
+    __attribute__((aligned(16))) T v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_out<T>(p[8 * cc + i]);
+#pragma unroll
+    for (int h = 0; h < int(sizeof(T)) / 2; ++h)
+      reinterpret_cast<u32x4*>(row + (cc * 16 + i16) * 8)[h] = reinterpret_cast<const u32x4*>(v)[h];
+  }
+}
+
 // The counts less their mean: as p sums to 1, c_i - sum p c is the same of either,
 // and near-uniform counts (as a balanced router has) no longer cancel. A row's
 // gradient goes through LDS on its way out: the selected experts' slots, on the lane
@@ -345,24 +359,21 @@ __global__ void __launch_bounds__(kThreads)
 router_grad_rows(const T* __restrict__ logits, int64_t M, int E, int k, RouterGrad a, T* __restrict__ grad) {
   constexpr int N = PIECES * 8, ROW = PIECES * 128;
   __shared__ __attribute__((aligned(16))) T rows_lds[kThreads / 16][ROW];
-  __shared__ float centred[ROW];
+  __shared__ __attribute__((aligned(16))) float counted[ROW];
   const int tid = threadIdx.x, i16 = tid & 15;
   const bool with_loss = a.grad_loss != nullptr, with_weights = a.grad_weights != nullptr;
   T* mine = rows_lds[tid >> 4];
+  for (int e = tid; e < ROW; e += kThreads) counted[e] = with_loss && e < E ? float(a.counts[e]) : 0.f;
+  __syncthreads();
   float c[N], mean = 0.f;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const int e = ((j >> 3) * 16 + i16) * 8 + (j & 7);
-    c[j] = with_loss && e < E ? float(a.counts[e]) : 0.f;
+    c[j] = counted[((j >> 3) * 16 + i16) * 8 + (j & 7)];
     mean += c[j];
   }
   mean = row_sum(mean) / float(E);
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    c[j] -= mean;
-    if (tid < 16) centred[((j >> 3) * 16 + i16) * 8 + (j & 7)] = c[j];
-  }
-  __syncthreads();
+  for (int j = 0; j < N; ++j) c[j] -= mean;
   const float factor = loss_factor(a, M, E, k);
   for (int64_t row = int64_t(blockIdx.x) * (kThreads / 16) + (tid >> 4); row < M;
        row += int64_t(gridDim.x) * (kThreads / 16)) {
@@ -404,10 +415,7 @@ router_grad_rows(const T* __restrict__ logits, int64_t M, int E, int k, RouterGr
       const float f = factor * inv, qi = q * inv;
 #pragma unroll
       for (int j = 0; j < N; ++j) p[j] = with_loss ? p[j] * fmaf(f, c[j] - pc, -qi) : -p[j] * qi;
-#pragma unroll
-      for (int cc = 0; cc < PIECES; ++cc)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) mine[(cc * 16 + i16) * 8 + i] = to_out<T>(p[8 * cc + i]);
+      put_row<T, PIECES>(p, mine, i16);
       if (with_weights) {
         // every slot of one expert forms the same sum, in slot order
         float add = 0.f;
@@ -416,13 +424,12 @@ router_grad_rows(const T* __restrict__ logits, int64_t M, int E, int k, RouterGr
           const int other = __shfl(id, (tid & 48) + l);
           if (other == id) add += v;
         }
-        if (id >= 0) mine[id] = to_out<T>((with_loss ? p_id * fmaf(factor, centred[id] - pc, -q) : -p_id * q) + add);
+        if (id >= 0) mine[id] = to_out<T>((with_loss ? p_id * fmaf(factor, counted[id] - mean - pc, -q) : -p_id * q) + add);
       }
     } else {
 #pragma unroll
-      for (int cc = 0; cc < PIECES; ++cc)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) mine[(cc * 16 + i16) * 8 + i] = to_out<T>(0.f);
+      for (int j = 0; j < N; ++j) p[j] = 0.f;
+      put_row<T, PIECES>(p, mine, i16);
     }
     // (a wave's LDS accesses are carried out in order; its rows are its own)
     __builtin_amdgcn_wave_barrier();
@@ -570,7 +577,7 @@ int balance_typed(const void* logits, const int32_t* ids, const uint8_t* mask, i
 template <typename T, int PIECES>
 void launch_grad_rows(const T* g, int64_t M, int E, int k, const RouterGrad& a, T* grad, hipStream_t stream) {
   const bool wide = E % 8 == 0 && (reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(grad)) % 16 == 0;
-  const dim3 grid(unsigned(std::min<int64_t>(2048, cdiv(M, kThreads / 16))));
+  const dim3 grid(unsigned(std::min<int64_t>(kGradWgs, cdiv(M, kThreads / 16))));
   if (wide)
     hipLaunchKernelGGL((router_grad_rows<T, PIECES, true>), grid, dim3(kThreads), 0, stream, g, M, E, k, a, grad);
   else
