@@ -26,7 +26,7 @@ def test_registered():
         assert name in xk.__all__
 
 
-def _balance(dtype=BF, M=8, E=16, k=2, logits=P, ids=P, loss=P, counts=P, tokens=P, ws=P, ws_bytes=1 << 40):
+def _balance(dtype=BF, M=800, E=16, k=2, logits=P, ids=P, loss=P, counts=P, tokens=P, ws=P, ws_bytes=1 << 40):
     return _rc("xk_moe_balance_loss", logits, dtype, M, E, ids, k, None, loss, counts, tokens, ws, ws_bytes, None)
 
 
@@ -106,6 +106,8 @@ def test_size_queries_take_any_numbers():
         assert _lib.query("xk_lora_projection_workspace_bytes", 8, 64, 2, bad) == 0
         assert _lib.query("xk_lora_projection_backward_workspace_bytes", 8, 64, 64, bad, 8, BF) == 0
         assert _lib.query("xk_moe_balance_loss_workspace_bytes", 8, bad) == 0
+    assert _lib.query("xk_moe_balance_loss_workspace_bytes", 256, 512) == 0  # one workgroup needs none
+    assert _lib.query("xk_moe_balance_loss_workspace_bytes", 257, 512) > 0
     assert _lib.query("xk_lora_projection_workspace_bytes", 8, 64, 2, 8) > 0
     assert _lib.query("xk_lora_projection_backward_workspace_bytes", 0, 64, 64, 2, 8, BF) > 0
 

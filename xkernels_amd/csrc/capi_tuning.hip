@@ -54,6 +54,7 @@ int check_lora(const char* op, int dtype, int64_t M, int64_t K, int64_t N, int64
 }
 
 int check_workspace(const char* op, const void* ws, int64_t bytes, int64_t need) {
+  if (need == 0) return XK_OK;
   if (ws == nullptr || bytes < need)
     return set_error(XK_ERR_WORKSPACE, "%s: workspace %lld B < %lld B", op, (long long)bytes, (long long)need);
   XK_REQUIRE(reinterpret_cast<uintptr_t>(ws) % 16 == 0, "%s: workspace is not 16-byte aligned", op);

@@ -1460,9 +1460,6 @@ int backward_typed(const T* dy, int64_t lddy, const void* x, int64_t ldx, const 
                        scaling, g_sum, packed_g, packed_h);
   });
   XK_CHECK_LAUNCH("lora_pack");
-  run_expand<T>(rows, plan.sort.tiles, false, Ranks{g_sum, 0, 1, RP, r}, at, static_cast<const float*>(nullptr),
-                static_cast<const T*>(nullptr), 0, K, dx, static_cast<float*>(nullptr), stream);
-  XK_CHECK_LAUNCH("lora_expand");
   const int64_t unit = x_scales != nullptr ? 16 : 8;  // values of a piece of x
   const bool vec = K % unit == 0 && ldx % unit == 0 && N % 8 == 0 && lddy % 8 == 0 && aligned16({dy, x});
   const dim3 grid(unsigned(plan.win.count), unsigned(plan.a_strips + plan.b_strips));
@@ -1478,6 +1475,11 @@ int backward_typed(const T* dy, int64_t lddy, const void* x, int64_t ldx, const 
 #undef XK_WGRAD
   });
   XK_CHECK_LAUNCH("lora_wgrad");
+  // (after the weights' gradients, which read grad_out while it is still in the last
+  // level's cache; dx would push it out)
+  run_expand<T>(rows, plan.sort.tiles, false, Ranks{g_sum, 0, 1, RP, r}, at, static_cast<const float*>(nullptr),
+                static_cast<const T*>(nullptr), 0, K, dx, static_cast<float*>(nullptr), stream);
+  XK_CHECK_LAUNCH("lora_expand");
   return reduce();
 }
 

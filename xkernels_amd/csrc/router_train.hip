@@ -605,6 +605,7 @@ int grad_typed(const void* logits, int64_t M, int64_t E, int64_t k, const Router
 }  // namespace
 
 int64_t balance_workspace_bytes(int64_t M, int64_t E) {
+  if (M <= kOneWgRows && E <= kFastExperts) return 0;  // one workgroup
   const int64_t planes = planes_for(std::max<int64_t>(M, 1), E);
   return up(planes * E * 4) * 2 + up(planes * 4) + up(cdiv(E, 16) * 8) + up(4) +
          (E > kFastExperts ? up(M * 8) : 0);

@@ -61,7 +61,7 @@ def _code(op: str, t: torch.Tensor, table=_ANY_DT) -> int:
 @lru_cache(maxsize=4096)
 def _bytes(query: str, *sizes: int) -> int:
     """A workspace's size, a function of the call's sizes alone."""
-    return max(_lib.query(query, *sizes), 1)
+    return _lib.query(query, *sizes)
 
 
 def _ids(op: str, t: torch.Tensor, n: int) -> torch.Tensor:
@@ -117,10 +117,10 @@ def moe_balance_loss_hip(gating_output: torch.Tensor, topk_ids: torch.Tensor,
     loss = g.new_empty((), dtype=torch.float32)
     counts = g.new_empty(E, dtype=torch.int32)
     tokens = g.new_empty((), dtype=torch.int32)
-    nbytes = _bytes("xk_moe_balance_loss_workspace_bytes", M, E)
-    ws = g.new_empty(nbytes, dtype=torch.uint8)
+    nbytes = _bytes("xk_moe_balance_loss_workspace_bytes", M, E)  # 0 for small batches
+    ws = g.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _lib.call("xk_moe_balance_loss", g.data_ptr(), dt, M, E, ids.data_ptr(), k, _ptr(on), loss.data_ptr(),
-              counts.data_ptr(), tokens.data_ptr(), ws.data_ptr(), nbytes, _stream(i))
+              counts.data_ptr(), tokens.data_ptr(), _ptr(ws), nbytes, _stream(i))
     return BalanceLoss(loss, counts, tokens)
 
 
