@@ -251,8 +251,9 @@ SPEC_REFERENCES = {
 
 
 def register_reference_backends() -> None:
-    """Install the oracle as the REFERENCE backend of the five kernels and as the
-    resolution of the Op Specs' reference paths (test harness only)."""
+    """Install the oracle as the REFERENCE backend of the five kernels (and of the
+    tuning ops) and as the resolution of the Op Specs' reference paths (test
+    harness only)."""
     from xkernels_amd._backends import Backend
     from xkernels_amd._dispatch import register
     from xkernels_amd.registry import bind_reference
@@ -264,3 +265,7 @@ def register_reference_backends() -> None:
     register("topk_softmax", Backend.REFERENCE)(topk_softmax_ref)
     for path, fn in SPEC_REFERENCES.items():
         bind_reference(path, fn)
+    from .tuning_ref import TUNING_REFERENCES
+
+    for kernel, fn in TUNING_REFERENCES.items():
+        register(kernel, Backend.REFERENCE)(fn)

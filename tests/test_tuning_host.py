@@ -8,7 +8,8 @@ import torch
 
 import xkernels_amd as xk
 from tests._tuning_ref import balance_ref, checkpoint_ref, e4m3_grid, lora_grad_ref, lora_ref, router_grad_ref
-from xkernels_amd import _dispatch, _lib
+from xkernels_amd import _dispatch, _lib, verify
+from xkernels_amd.registry import all_cards, all_specs, cost_model, input_gen, load_shape_sweep, reference_callable
 
 P = 0x1000  # a pointer that no refused call follows
 BF, FP32, FP16 = _lib.XK_DT_BF16, _lib.XK_DT_FP32, _lib.XK_DT_FP16
@@ -24,6 +25,57 @@ def test_registered():
                  "act_checkpoint", "act_restore"):
         assert xk.Backend.HIP in _dispatch.registered_backends(name)
         assert name in xk.__all__
+
+
+OPS = [f"{k}@1.0.0" for k in ("moe_balance_loss", "moe_router_backward", "lora_projection",
+                              "lora_projection_backward", "act_checkpoint", "act_restore")]
+
+
+@pytest.mark.parametrize("op", OPS)
+def test_registry(op):
+    assert {"HIP", "REFERENCE"} <= set(all_cards()[op])
+    points = load_shape_sweep(all_specs()[op].shape_sweep)
+    for p in points:
+        flops, nbytes = cost_model.cost_model(op, p)
+        assert flops > 0 and nbytes > 0
+        a, b = (input_gen.generate_inputs(op, p, 7, "cpu") for _ in range(2))
+        assert callable(reference_callable(op)) and a.keys() == b.keys()
+    r = verify(op.replace("@", ".reference@"), arch="any")
+    assert r["compiled"] and r["correctness"]["passed"], r
+    if not torch.cuda.is_available():
+        r = verify(op.replace("@", ".hip@"), arch="amd_cdna4")
+        assert r["compiled"] is False and "device" in r["artifacts"]["error"]
+
+
+def test_oracle_against_the_64_bit_forms():
+    from oracle import tuning_ref as o
+
+    f = input_gen.generate_inputs(OPS[2], load_shape_sweep("lora_projection")[3], 1, "cpu")
+    out, hidden, bound, _ = lora_ref(*(f[k] for k in ("x", "lora_a", "lora_b", "adapter_ids", "base", "scaling")))
+    got, gh = o.lora_projection_ref(**f, return_hidden=True)
+    torch.testing.assert_close(got.double(), out, rtol=1e-5, atol=1e-5)
+    torch.testing.assert_close(gh.double(), hidden, rtol=1e-5, atol=1e-5)
+    f = input_gen.generate_inputs(OPS[3], load_shape_sweep("lora_projection_backward")[2], 1, "cpu")
+    want, _ = lora_grad_ref(f["grad_out"], f["x"], f["lora_a"], f["lora_b"], f["adapter_ids"], f["hidden"], f["scaling"])
+    for p, q in zip(o.lora_projection_backward_ref(**f), want):
+        torch.testing.assert_close(p.double(), q, rtol=1e-5, atol=1e-4)
+    f = input_gen.generate_inputs(OPS[0], load_shape_sweep("moe_balance_loss")[1], 1, "cpu")
+    loss, counts, T = balance_ref(f["gating_output"], f["topk_ids"], f["mask"])
+    got = o.moe_balance_loss_ref(**f)
+    torch.testing.assert_close(got[0].double(), loss, rtol=1e-6, atol=0)
+    assert torch.equal(got[1].long(), counts) and int(got[2]) == T
+    for renorm in (True, False):
+        f = input_gen.generate_inputs(OPS[1], load_shape_sweep("moe_router_backward")[0], 1, "cpu")
+        f["renormalize"] = renorm
+        f["topk_ids"][3, 1] = -1
+        want, _ = router_grad_ref(f["gating_output"], f["topk_ids"], f["grad_weights"], renorm, 1.0, f["counts"])
+        torch.testing.assert_close(o.moe_router_backward_ref(**f).double(), want, rtol=1e-4, atol=1e-7)
+    x = torch.randn(9, 70) * 100
+    x[2, 3], x[4, 60] = float("inf"), float("nan")
+    want, scales = checkpoint_ref(x)
+    held = o.act_checkpoint_ref(x)
+    assert torch.equal(held[1], scales)
+    torch.testing.assert_close(o.act_restore_ref(held, torch.float32).double(), want, rtol=0, atol=0, equal_nan=True)
 
 
 def _balance(dtype=BF, M=800, E=16, k=2, logits=P, ids=P, loss=P, counts=P, tokens=P, ws=P, ws_bytes=1 << 40):

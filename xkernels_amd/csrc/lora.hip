@@ -689,7 +689,7 @@ __device__ __forceinline__ void copy_rows(const int* tile_rows, int n_rows, int6
 // for right after a store.
 template <typename T, int RT, bool VEC>
 __global__ void __launch_bounds__(kThreads, kExpandPlaces<RT>)
-lora_expand(Rows rows, Ranks h, const T* __restrict__ b, const float* __restrict__ scaling,
+lora_expand(Rows rows, Ranks h, const T* __restrict__ b, int wide, const float* __restrict__ scaling,
             const T* __restrict__ base, int64_t ldbase, int64_t N, int chunks, T* __restrict__ out,
             float* __restrict__ hidden_out) {
   constexpr int RP = RT * 16, HP = RP + 4, PER = 16 / sizeof(T), BN = 16 * PER;
@@ -729,7 +729,7 @@ lora_expand(Rows rows, Ranks h, const T* __restrict__ b, const float* __restrict
       for (int j = 0; j < NW; ++j) {
         const int q = tid + j * kThreads, rank = (q % PPR) * PER;
         const int64_t n = min(n0 + q / PPR, N - 1);  // (columns past N are not written)
-        if constexpr (VEC) {
+        if (wide) {  // (r a multiple of 8, the weights aligned)
           wn[j] = *reinterpret_cast<const u32x4*>(bw + n * h.r + (rank < h.r ? rank : 0));
           if (rank >= h.r) wn[j] = u32x4{0, 0, 0, 0};
         } else {
@@ -830,7 +830,7 @@ lora_expand(Rows rows, Ranks h, const T* __restrict__ b, const float* __restrict
 // interleaved fours give a lane 8 consecutive columns of a row.
 template <typename T, int RT, bool VEC>
 __global__ void __launch_bounds__(kThreads, 2)
-lora_expand_few(Rows rows, Ranks h, const T* __restrict__ b, const float* __restrict__ scaling,
+lora_expand_few(Rows rows, Ranks h, const T* __restrict__ b, int wide, const float* __restrict__ scaling,
                 const T* __restrict__ base, int64_t ldbase, int64_t N, int64_t chunk, T* __restrict__ out,
                 float* __restrict__ hidden) {
   constexpr int RP = RT * 16, PITCH = RP + 4;
@@ -863,7 +863,7 @@ lora_expand_few(Rows rows, Ranks h, const T* __restrict__ b, const float* __rest
       for (int e = 0; e < 2; ++e) {
         const int64_t n = n0 + nr + 4 * e;
         const int left = h.r - rb::kRanks * t - rank0;
-        if (VEC) wf[t][e] = rb::template load<true>(bw + min(n, N - 1) * h.r + (left > 0 ? rb::kRanks * t : -rank0), 0);
+        if (wide) wf[t][e] = rb::template load<true>(bw + min(n, N - 1) * h.r + (left > 0 ? rb::kRanks * t : -rank0), 0);
         else wf[t][e] = rb::template load<false>(bw + n * h.r + rb::kRanks * t, n < w1 ? left : 0);
       }
     const int64_t nb = n0 + g * 8;
@@ -881,7 +881,7 @@ lora_expand_few(Rows rows, Ranks h, const T* __restrict__ b, const float* __rest
     for (int t = 0; t < rb::kBlocks; ++t)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        if (VEC) rb::blank_unless(rb::kRanks * t + rank0 < h.r, wf[t][e]);
+        rb::blank_unless(rb::kRanks * t + rank0 < h.r, wf[t][e]);
         acc[e] = rb::mma(wf[t][e], hf[t], acc[e]);
       }
     typename mm<T>::frag o;
@@ -1312,17 +1312,18 @@ void run_shrink(const Rows& rows, int64_t tiles, bool few, const T* x, int64_t l
 template <typename T>
 void run_expand(const Rows& rows, int64_t tiles, bool few,  const Ranks& h, const T* b, const float* scaling,
                 const T* base, int64_t ldbase, int64_t N, T* out, float* hidden, hipStream_t stream) {
-  const bool vec = N % 8 == 0 && h.r % 8 == 0 && (base == nullptr || ldbase % 8 == 0) && aligned16({b, base, out});
+  const bool vec = N % 8 == 0 && (base == nullptr || ldbase % 8 == 0) && aligned16({base, out});
+  const int wide = h.r % 8 == 0 && aligned16({b});
   const int64_t chunk = chunk_of(N, tiles);
   const dim3 grid(unsigned(rows.M), unsigned(cdiv(N, chunk)));
   const Shares sh(N, tiles, h.r, sizeof(T));
   with_ranks(h.r, [&](auto rt) {
     constexpr int RT = decltype(rt)::value;
 #define XK_EXPAND_FEW(V)                                                                                          \
-  hipLaunchKernelGGL((lora_expand_few<T, RT, V>), grid, dim3(kThreads), 0, stream, rows, h, b, scaling, base, ldbase, \
-                     N, chunk, out, hidden)
+  hipLaunchKernelGGL((lora_expand_few<T, RT, V>), grid, dim3(kThreads), 0, stream, rows, h, b, wide, scaling, base, \
+                     ldbase, N, chunk, out, hidden)
 #define XK_EXPAND(V)                                                                                               \
-  hipLaunchKernelGGL((lora_expand<T, RT, V>), dim3(sh.grid), dim3(kThreads), 0, stream, rows, h, b, scaling, base, \
+  hipLaunchKernelGGL((lora_expand<T, RT, V>), dim3(sh.grid), dim3(kThreads), 0, stream, rows, h, b, wide, scaling, base, \
                      ldbase, N, sh.chunks, out, hidden)
     if (vec && few) XK_EXPAND_FEW(true);
     else if (vec) XK_EXPAND(true);

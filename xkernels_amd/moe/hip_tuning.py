@@ -208,8 +208,8 @@ def lora_projection_backward_hip(grad_out: torch.Tensor, x: torch.Tensor | ActCh
                                  lora_b: torch.Tensor, adapter_ids: torch.Tensor, hidden: torch.Tensor,
                                  scaling: torch.Tensor | None = None):
     op = "lora_projection_backward"
-    held = isinstance(x, ActCheckpoint)
-    xt, scales = (x.values, x.scales) if held else (x, None)
+    held = isinstance(x, tuple)
+    xt, scales = x if held else (x, None)
     i = _device(op, grad_out, xt, scales, lora_a, lora_b, adapter_ids, hidden, scaling)
     if i != _current_device():
         return _elsewhere(i, lora_projection_backward_hip, grad_out, x, lora_a, lora_b, adapter_ids, hidden, scaling)

@@ -72,11 +72,45 @@ def _moe_mxfp4(p: dict[str, Any]) -> tuple[int, int]:
     return flops, e_act * mxfp4_expert_bytes(hidden, ispp) + 2 * ab * M * hidden + 8 * M * k
 
 
+def _moe_balance_loss(p: dict[str, Any]) -> tuple[int, int]:
+    M, E, k = int(p["M"]), int(p["E"]), int(p["top_k"])
+    return 10 * M * E, dtype_bytes(p.get("dtype", "bf16")) * M * E + 4 * M * k + 4 * E
+
+
+def _moe_router_backward(p: dict[str, Any]) -> tuple[int, int]:
+    M, E, k = int(p["M"]), int(p["E"]), int(p["top_k"])
+    return 15 * M * E, 2 * dtype_bytes(p.get("dtype", "bf16")) * M * E + 8 * M * k + 4 * E
+
+
+def _lora_projection(p: dict[str, Any]) -> tuple[int, int]:
+    M, K, N, L, r = (int(p[x]) for x in ("M", "K", "N", "L", "r"))
+    ab = dtype_bytes(p.get("dtype", "bf16"))
+    return 2 * M * r * (K + N), ab * (M * (K + 2 * N) + min(L, M) * r * (K + N)) + 4 * M
+
+
+def _lora_projection_backward(p: dict[str, Any]) -> tuple[int, int]:
+    M, K, N, L, r = (int(p[x]) for x in ("M", "K", "N", "L", "r"))
+    ab = dtype_bytes(p.get("dtype", "bf16"))
+    x_bytes = M * (K + -(-K // 32)) if p.get("held") else ab * M * K
+    return 4 * M * r * (K + N), ab * (M * (K + N) + (min(L, M) + L) * r * (K + N)) + x_bytes + 4 * M * (r + 1)
+
+
+def _act_checkpoint(p: dict[str, Any]) -> tuple[int, int]:
+    M, K = int(p["M"]), int(p["K"])
+    return 2 * M * K, M * (K * (dtype_bytes(p.get("dtype", "bf16")) + 1) + -(-K // 32))
+
+
 _MODELS: dict[str, Callable[[dict[str, Any]], tuple[int, int]]] = {
     "moe_int4_w4a16@1.0.0": _moe_int4_w4a16,
     "moe_sum_reduce@1.0.0": _moe_sum_reduce,
     "moe_align_block_size@1.0.0": _moe_align,
     "moe_mxfp4@1.0.0": _moe_mxfp4,
+    "moe_balance_loss@1.0.0": _moe_balance_loss,
+    "moe_router_backward@1.0.0": _moe_router_backward,
+    "lora_projection@1.0.0": _lora_projection,
+    "lora_projection_backward@1.0.0": _lora_projection_backward,
+    "act_checkpoint@1.0.0": _act_checkpoint,
+    "act_restore@1.0.0": _act_checkpoint,
 }
 
 

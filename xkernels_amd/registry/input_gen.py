@@ -77,12 +77,71 @@ def _topk_softmax(p: dict[str, Any], seed: int, device: str) -> dict[str, Any]:
     return {"gating_output": gating, "topk": int(p["topk"]), "renormalize": bool(p["renormalize"])}
 
 
+def _moe_balance_loss(p: dict[str, Any], seed: int, device: str) -> dict[str, Any]:
+    z = _randn(device, torch.float32, p["M"], p["E"], seed=seed).to(to_torch_dtype(p["dtype"]))
+    g = torch.Generator(device=device).manual_seed(seed + 1)
+    mask = torch.rand(int(p["M"]), generator=g, device=device) >= p["padded"] if p["padded"] else None
+    return {"gating_output": z, "topk_ids": torch.topk(z.float(), int(p["top_k"]), dim=1).indices.int(), "mask": mask}
+
+
+def _moe_router_backward(p: dict[str, Any], seed: int, device: str) -> dict[str, Any]:
+    a = _moe_balance_loss({**p, "padded": 0.0}, seed, device)
+    ids = a["topk_ids"]
+    return {"gating_output": a["gating_output"], "topk_ids": ids,
+            "grad_weights": _randn(device, torch.float32, *ids.shape, seed=seed + 2),
+            "renormalize": bool(p["renormalize"]), "grad_loss": torch.ones((), device=device),
+            "counts": torch.bincount(ids.flatten().long(), minlength=int(p["E"])).int()}
+
+
+def _lora_projection(p: dict[str, Any], seed: int, device: str) -> dict[str, Any]:
+    dt = to_torch_dtype(p["dtype"])
+    M, K, N, L, r = (int(p[x]) for x in ("M", "K", "N", "L", "r"))
+    g = torch.Generator(device=device).manual_seed(seed + 3)
+    return {"x": _randn(device, torch.float32, M, K, seed=seed).to(dt),
+            "lora_a": (_randn(device, torch.float32, L, r, K, seed=seed + 1) / K ** 0.5).to(dt),
+            "lora_b": (_randn(device, torch.float32, L, N, r, seed=seed + 2) / r ** 0.5).to(dt),
+            "adapter_ids": torch.randint(-1, L, (M,), generator=g, device=device, dtype=torch.int32),
+            "base": _randn(device, torch.float32, M, N, seed=seed + 4).to(dt),
+            "scaling": torch.rand(L, generator=g, device=device) + 0.5}
+
+
+def _lora_projection_backward(p: dict[str, Any], seed: int, device: str) -> dict[str, Any]:
+    f = _lora_projection(p, seed, device)
+    hidden = _randn(device, torch.float32, int(p["M"]), int(p["r"]), seed=seed + 5)
+    x = _held(f["x"]) if p.get("held") else f["x"]
+    return {"grad_out": f["base"], "x": x, "lora_a": f["lora_a"], "lora_b": f["lora_b"],
+            "adapter_ids": f["adapter_ids"], "hidden": hidden, "scaling": f["scaling"]}
+
+
+def _held(x: torch.Tensor):
+    """Any valid checkpoint: the values' own e4m3 rounding with scales of 1."""
+    from ..moe.act_checkpoint import ActCheckpoint
+
+    scales = torch.full((x.shape[0], -(-x.shape[1] // 32)), 127, dtype=torch.uint8, device=x.device)
+    return ActCheckpoint(x.to(torch.float8_e4m3fn), scales)
+
+
+def _act_checkpoint(p: dict[str, Any], seed: int, device: str) -> dict[str, Any]:
+    return {"x": (8 * _randn(device, torch.float32, int(p["M"]), int(p["K"]), seed=seed)).to(to_torch_dtype(p["dtype"]))}
+
+
+def _act_restore(p: dict[str, Any], seed: int, device: str) -> dict[str, Any]:
+    x = _randn(device, torch.float32, int(p["M"]), int(p["K"]), seed=seed)
+    return {"held": _held(x), "dtype": to_torch_dtype(p["dtype"])}
+
+
 _GENERATORS: dict[str, Callable[[dict, int, str], dict[str, Any]]] = {
     "moe_sum_reduce@1.0.0": _moe_sum_reduce,
     "moe_align_block_size@1.0.0": _moe_align_block_size,
     "moe_int4_w4a16@1.0.0": _moe_int4_w4a16,
     "moe_mxfp4@1.0.0": _moe_mxfp4,
     "topk_softmax@1.0.0": _topk_softmax,
+    "moe_balance_loss@1.0.0": _moe_balance_loss,
+    "moe_router_backward@1.0.0": _moe_router_backward,
+    "lora_projection@1.0.0": _lora_projection,
+    "lora_projection_backward@1.0.0": _lora_projection_backward,
+    "act_checkpoint@1.0.0": _act_checkpoint,
+    "act_restore@1.0.0": _act_restore,
 }
 
 
