@@ -62,6 +62,17 @@ __device__ __forceinline__ int map_expert(int id, const int32_t* expert_map,
 
 __host__ __device__ __forceinline__ int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// A value of any size at an address aligned to its elements only: one wide access,
+// which the hardware takes at any alignment.
+template <typename V, typename E> __device__ __forceinline__ V load_unaligned(const E* p) {
+  V v;
+  __builtin_memcpy(&v, p, sizeof(V));
+  return v;
+}
+template <typename V, typename E> __device__ __forceinline__ void store_unaligned(E* p, const V& v) {
+  __builtin_memcpy(p, &v, sizeof(V));
+}
+
 // MFMA operand vector types.
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));

@@ -65,7 +65,8 @@ template <> struct mm<float> {
 
 // 8 values at p. VEC: widths are whole aligned pieces, one load and no condition, so
 // that loads stay in flight: the caller moves a pointer past the end to one that
-// can be read and drops or blanks what comes of it. Else n values and zeros.
+// can be read and drops or blanks what comes of it. Else n values and zeros: whole
+// pieces unaligned, a row's last one value by value.
 template <typename T, bool VEC>
 __device__ __forceinline__ typename mm<T>::frag load_frag(const T* p, int64_t n) {
   typename mm<T>::frag f;
@@ -73,12 +74,33 @@ __device__ __forceinline__ typename mm<T>::frag load_frag(const T* p, int64_t n)
 #pragma unroll
     for (int i = 0; i < int(sizeof(T)) / 2; ++i)
       reinterpret_cast<u32x4*>(&f)[i] = reinterpret_cast<const u32x4*>(p)[i];
+  } else if (n >= 8) {
+    f = load_unaligned<typename mm<T>::frag>(p);
   } else {
     T* v = reinterpret_cast<T*>(&f);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : T(0);
   }
   return f;
+}
+// 16 bytes the same way: n values of PER.
+template <typename T> __device__ __forceinline__ u32x4 load_piece(const T* p, int64_t n) {
+  constexpr int PER = 16 / sizeof(T);
+  if (n >= PER) return load_unaligned<u32x4>(p);
+  u32x4 w;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) reinterpret_cast<T*>(&w)[i] = i < n ? p[i] : T(0);
+  return w;
+}
+template <typename T, typename V> __device__ __forceinline__ void store_values(T* p, int64_t n, const V& v) {
+  constexpr int ALL = sizeof(V) / sizeof(T);
+  if (n >= ALL) {
+    store_unaligned(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < ALL; ++i)
+      if (i < n) p[i] = reinterpret_cast<const T*>(&v)[i];
+  }
 }
 template <typename T>
 __device__ __forceinline__ void blank_unless_frag(bool keep, typename mm<T>::frag& f) {
@@ -460,9 +482,7 @@ lora_shrink(Rows rows, const T* __restrict__ x, int64_t ldx, int64_t K, const T*
         an[j] = *reinterpret_cast<const u32x4*>(ar[j] + min(k + ap, K - PER));
         if (k + ap >= k1) an[j] = u32x4{0, 0, 0, 0};
       } else {
-        T* v = reinterpret_cast<T*>(&an[j]);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) v[i] = k + ap + i < k1 ? ar[j][k + ap + i] : T(0);
+        an[j] = load_piece(ar[j] + k + ap, k1 - k - ap);
       }
     }
 #pragma unroll
@@ -672,9 +692,7 @@ __device__ __forceinline__ void copy_rows(const int* tile_rows, int n_rows, int6
         for (int i = 0; i < int(sizeof(T)) / 2; ++i)
           reinterpret_cast<u32x4*>(o)[i] = reinterpret_cast<const u32x4*>(&v[j])[i];
       } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (n + i < c1) o[i] = reinterpret_cast<const T*>(&v[j])[i];
+        store_values(o, c1 - n, v[j]);
       }
     }
   }
@@ -733,9 +751,7 @@ lora_expand(Rows rows, Ranks h, const T* __restrict__ b, int wide, const float* 
           wn[j] = *reinterpret_cast<const u32x4*>(bw + n * h.r + (rank < h.r ? rank : 0));
           if (rank >= h.r) wn[j] = u32x4{0, 0, 0, 0};
         } else {
-          T* v = reinterpret_cast<T*>(&wn[j]);
-#pragma unroll
-          for (int i = 0; i < PER; ++i) v[i] = rank + i < h.r ? bw[n * h.r + rank + i] : T(0);
+          wn[j] = load_piece(bw + n * h.r + rank, h.r - rank);
         }
       }
     };
@@ -776,9 +792,7 @@ lora_expand(Rows rows, Ranks h, const T* __restrict__ b, int wide, const float* 
         if constexpr (VEC) {
           bn[i] = *reinterpret_cast<const u32x4*>(br[i] + min(n0 + col, N - PER));
         } else {
-          T* v = reinterpret_cast<T*>(&bn[i]);
-#pragma unroll
-          for (int j = 0; j < PER; ++j) v[j] = n0 + col + j < c1 ? br[i][n0 + col + j] : T(0);
+          bn[i] = load_piece(br[i] + n0 + col, c1 - n0 - col);
         }
       }
     };
@@ -816,9 +830,7 @@ lora_expand(Rows rows, Ranks h, const T* __restrict__ b, int wide, const float* 
         if constexpr (VEC) {
           if (n0 + col < c1) *reinterpret_cast<u32x4*>(orow[i] + n0) = o;
         } else {
-#pragma unroll
-          for (int t = 0; t < PER; ++t)
-            if (n0 + col + t < c1) orow[i][n0 + t] = reinterpret_cast<const T*>(&o)[t];
+          store_values(orow[i] + n0, c1 - n0 - col, o);
         }
       }
     }
@@ -899,9 +911,7 @@ lora_expand_few(Rows rows, Ranks h, const T* __restrict__ b, int wide, const flo
       for (int j = 0; j < int(sizeof(T)) / 2; ++j)
         reinterpret_cast<u32x4*>(p)[j] = reinterpret_cast<const u32x4*>(&o)[j];
     } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < cnt) p[j] = reinterpret_cast<const T*>(&o)[j];
+      store_values(p, cnt, o);
     }
   }
 }
@@ -1030,9 +1040,7 @@ __device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t
           v[i].q = *reinterpret_cast<const u32x4*>(q);
           v[i].scale = sd.scales[at * blocks + col_at / kMx8Block];
         } else {
-          uint8_t* b = reinterpret_cast<uint8_t*>(&v[i].q);
-#pragma unroll
-          for (int j = 0; j < PER; ++j) b[j] = j < n ? q[j] : 0;
+          v[i].q = load_piece(q, n);
           v[i].scale = n > 0 ? sd.scales[at * blocks + col / kMx8Block] : 127;
         }
       } else {

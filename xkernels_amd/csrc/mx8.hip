@@ -46,6 +46,8 @@ __device__ __forceinline__ void load_piece(const T* p, int n, T* v) {
     u32x4* d = reinterpret_cast<u32x4*>(v);
 #pragma unroll
     for (int i = 0; i < int(kPiece * sizeof(T) / 16); ++i) d[i] = s[i];
+  } else if (n == kPiece) {
+    __builtin_memcpy(v, p, kPiece * sizeof(T));  // wide accesses at any alignment
   } else {
 #pragma unroll
     for (int i = 0; i < kPiece; ++i) v[i] = i < n ? p[i] : T(0);
@@ -58,6 +60,8 @@ __device__ __forceinline__ void store_piece(T* p, int n, const T* v) {
     u32x4* d = reinterpret_cast<u32x4*>(p);
 #pragma unroll
     for (int i = 0; i < int(kPiece * sizeof(T) / 16); ++i) d[i] = s[i];
+  } else if (n == kPiece) {
+    __builtin_memcpy(p, v, kPiece * sizeof(T));
   } else {
 #pragma unroll
     for (int i = 0; i < kPiece; ++i)

@@ -80,6 +80,10 @@ __device__ __forceinline__ void load_row(const T* g, int E, int i16, float* z) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) z[8 * c + i] = -__builtin_inff();
       }
+    } else if (e0 + 8 <= E) {
+      __attribute__((aligned(16))) T v[8];
+      __builtin_memcpy(v, g + e0, sizeof(v));  // a wide access at any alignment
+      piece8<T>::load(v, z + 8 * c);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) z[8 * c + i] = e0 + i < E ? logit_at<T>(g + e0 + i) : -__builtin_inff();
@@ -441,6 +445,8 @@ router_grad_rows(const T* __restrict__ logits, int64_t M, int E, int k, RouterGr
 #pragma unroll
           for (int h = 0; h < int(sizeof(T)) / 2; ++h)
             reinterpret_cast<u32x4*>(out + e0)[h] = reinterpret_cast<const u32x4*>(mine + e0)[h];
+      } else if (e0 + 8 <= E) {
+        __builtin_memcpy(out + e0, mine + e0, 8 * sizeof(T));
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
