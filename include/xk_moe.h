@@ -246,7 +246,8 @@ int xk_moe_mxfp4(const void* A, int32_t a_dtype, int64_t M, int64_t hidden,
 
 /* ---------------------------------------------------------------------------
  * Training the router and adapters over the frozen experts, and serving adapters.
- * The reference has no counterpart of these entry points.
+ * The reference has no counterpart of these entry points. Outputs overlap neither
+ * inputs nor each other (but for xk_lora_projection's out and base).
  *
  * moe_balance_loss. Over the T rows that mask [M] leaves (nonzero bytes; NULL: all),
  * p = softmax(gating_output) in fp32, c_e the slots of those rows on expert e:
@@ -282,8 +283,10 @@ int xk_moe_router_backward(const void* gating_output, int32_t dtype, int64_t M, 
  * apart, base [M, N] (NULL: zeros) with rows ldbase apart, lora_a [L, r, K] and
  * lora_b [L, N, r] contiguous, all of one dtype (bf16 | fp32), out [M, N] of it;
  * scaling fp32 [L] (NULL: ones); hidden fp32 [M, r] receives h (nullable).
- * 1 <= L <= 1024, 1 <= r <= 128. out may be base where ldbase = N. workspace is
- * 16-byte aligned. Results do not depend on scheduling.
+ * 1 <= L <= 1024, 1 <= r <= 128, M < 2^29, K and N <= 1,000,000. out may be base where
+ * ldbase = N. workspace is 16-byte aligned. Results do not depend on scheduling.
+ * bf16 products take h and g as the sum of two bf16 values, so an infinite weight
+ * (in the gradients an infinite x or grad_out too) may come out as NaN.
  * ------------------------------------------------------------------------- */
 int64_t xk_lora_projection_workspace_bytes(int64_t M, int64_t K, int64_t L, int64_t r);
 int xk_lora_projection(const void* x, int32_t dtype, int64_t ldx, int64_t M, int64_t K,

@@ -11,6 +11,7 @@ import pytest
 import torch
 
 import xkernels_amd as xk
+from xkernels_amd import _lib
 from tests._tuning_ref import check, checkpoint_ref, lora_grad_ref, lora_ref
 
 pytestmark = pytest.mark.gpu
@@ -267,3 +268,107 @@ def test_streams(dev):
                 got.append(xk.lora_projection(c[0], c[1], c[2], c[3], base=c[4], scaling=c[6]))
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("M", [3, 250, 700])
+@pytest.mark.parametrize("N", [64, 47])
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_out_over_base(M, N, dt, dev):
+    """The C entry point may write the result over the base."""
+    x, a, b, ids, base, _, sc = _case(M, 96, N, 3, 12, dt, seed=M)
+    want = xk.lora_projection(x, a, b, ids, base=base, scaling=sc)
+    need = _lib.query("xk_lora_projection_workspace_bytes", M, 96, 3, 12)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    _lib.call("xk_lora_projection", x.data_ptr(), _lib.XK_DT_BF16 if dt == BF else _lib.XK_DT_FP32, 96, M, 96,
+              a.data_ptr(), b.data_ptr(), 3, N, 12, ids.data_ptr(), sc.data_ptr(), base.data_ptr(), N, base.data_ptr(),
+              None, ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(base, want)
+
+
+@pytest.mark.parametrize("M", [20, 500])
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_weights_at_odd_offsets(M, dt, dev):
+    """Adapters that begin between two 16-byte pieces, as slices of a bank do: the same values."""
+    x, a, b, ids, base, dy, sc = _case(M, 128, 64, 4, 16, dt, seed=M)
+    want = xk.lora_projection(x, a, b, ids, base=base, scaling=sc, return_hidden=True)
+    grads = xk.lora_projection_backward(dy, x, a, b, ids, want[1], scaling=sc)
+    bank = torch.full((a.numel() + b.numel() + 8,), float("nan"), dtype=dt, device="cuda")
+    a2 = bank[1:1 + a.numel()].view(a.shape)
+    b2 = bank[3 + a.numel():3 + a.numel() + b.numel()].view(b.shape)
+    a2.copy_(a)
+    b2.copy_(b)
+    got = xk.lora_projection(x, a2, b2, ids, base=base, scaling=sc, return_hidden=True)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    got = xk.lora_projection_backward(dy, x, a2, b2, ids, want[1], scaling=sc)
+    assert all(torch.equal(p, q) for p, q in zip(got, grads))
+
+
+@pytest.mark.parametrize("M", [200, 600])
+def test_bare_rows_hold_anything(M, dev):
+    """NaN in the x, grad_out and hidden of rows without an adapter reaches nothing."""
+    x, a, b, ids, base, dy, sc = _case(M, 64, 48, 3, 8, BF, seed=M, bare=0.4)
+    bare = ids < 0
+    _, hidden = xk.lora_projection(x, a, b, ids, base=base, scaling=sc, return_hidden=True)
+    want = xk.lora_projection_backward(dy, x, a, b, ids, hidden, scaling=sc)
+    for t in (x, dy, hidden):
+        t[bare] = float("nan")
+    got = xk.lora_projection_backward(dy, x, a, b, ids, hidden, scaling=sc)
+    assert all(torch.equal(p, q) for p, q in zip(got, want)) and not got[0][bare].any()
+
+
+@pytest.mark.parametrize("dt", [torch.int16, torch.int8, torch.uint8])
+def test_narrow_ids(dt, dev):
+    x, a, b, ids, base, _, sc = _case(90, 64, 48, 3, 8, BF, bare=0.0)
+    ids[5] = 100
+    want = xk.lora_projection(x, a, b, ids, base=base, scaling=sc)
+    assert torch.equal(xk.lora_projection(x, a, b, ids.to(dt), base=base, scaling=sc), want)
+    assert torch.equal(want[5], base[5])
+
+
+def test_more_than_32_bits_of_values(dev):
+    """x, base, out, grad_out and grad_x past 2^31 values: the last rows, whose adapter's
+    gradients come from them alone."""
+    M, W, r = 66000, 33000, 4
+    x = torch.zeros(M, W, dtype=BF, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x[-3:] = torch.randn(3, W, generator=g, device="cuda").to(BF)
+    a = (torch.randn(2, r, W, generator=g, device="cuda") / W ** 0.5).to(BF)
+    b = torch.randn(2, W, r, generator=g, device="cuda").to(BF)
+    ids = torch.zeros(M, dtype=torch.int32, device="cuda")
+    ids[-3:] = 1
+    out, hidden = xk.lora_projection(x, a, b, ids, base=x, return_hidden=True)
+    last = slice(M - 3, M)
+    want, h, bound, hb = lora_ref(x[last], a, b, ids[last], x[last], None)
+    check(out[last], want, bound, "out")
+    check(hidden[last], h, hb, "hidden")
+    assert not out[:-3].any() and not hidden[:-3].any()
+    got = xk.lora_projection_backward(out, x, a, b, ids, hidden)
+    want, bounds = lora_grad_ref(out[last], x[last], a, b, ids[last], hidden[last], None)
+    check(got[0][last], want[0], bounds[0], "grad_x")
+    assert not got[0][:-3].any()
+    for i in (1, 2):
+        check(got[i][1], want[i][1], bounds[i][1], "weights")
+        assert not got[i][0].any()
+
+
+def test_refusals(dev):
+    """Shapes and types that do not fit, before any launch."""
+    x, a, b, ids, base, dy, sc = _case(6, 64, 32, 3, 8, BF)
+    _, h = xk.lora_projection(x, a, b, ids, return_hidden=True)
+    bad = [lambda: xk.lora_projection(x[:, :60], a, b, ids), lambda: xk.lora_projection(x, a, b[:2], ids),
+           lambda: xk.lora_projection(x, a, b, ids[:5]), lambda: xk.lora_projection(x.float(), a, b, ids),
+           lambda: xk.lora_projection(x, a, b, ids, base=base.float()), lambda: xk.lora_projection(x, a, b, ids.float()),
+           lambda: xk.lora_projection(x, a, b, ids, base=base[:, :30]), lambda: xk.lora_projection(x[0], a, b, ids),
+           lambda: xk.lora_projection(x, a, b, ids, scaling=sc[:2]), lambda: xk.lora_projection(x, a[0], b, ids),
+           lambda: xk.lora_projection(x.half(), a.half(), b.half(), ids), lambda: xk.lora_projection(x, a, b.float(), ids),
+           lambda: xk.lora_projection(x, a.cpu(), b, ids),
+           lambda: xk.lora_projection_backward(dy[:, :30], x, a, b, ids, h),
+           lambda: xk.lora_projection_backward(dy, x[:5], a, b, ids, h),
+           lambda: xk.lora_projection_backward(dy, x, a, b, ids, h[:, :7]),
+           lambda: xk.lora_projection_backward(dy, x.float(), a, b, ids, h),
+           lambda: xk.lora_projection_backward(dy, xk.act_checkpoint(x)._replace(scales=ids[:, None]), a, b, ids, h),
+           lambda: xk.lora_projection_backward(dy, (x, xk.act_checkpoint(x).scales), a, b, ids, h)]
+    for i, call in enumerate(bad):
+        with pytest.raises(RuntimeError):
+            call()
+            pytest.fail(f"call {i} went through")

@@ -200,3 +200,85 @@ def test_strided_and_unaligned(dev):
     off.copy_(z)
     assert torch.equal(xk.moe_router_backward(off, ids, grad_weights=u), want)
     assert all(torch.equal(p, q) for p, q in zip(xk.moe_balance_loss(off, ids), xk.moe_balance_loss(z, ids)))
+
+
+@pytest.mark.parametrize("M", [40, 700])
+def test_mask_types(M, dev):
+    """Masks of whole numbers, of floats and of strided booleans: nonzero counts."""
+    z, ids, u, mask = _case(M, 96, 4, torch.bfloat16, seed=M, pad=0.4)
+    want = xk.moe_balance_loss(z, ids, mask=mask)
+    kw = dict(grad_weights=u, grad_loss=want.loss, counts=want.counts, tokens=want.tokens)
+    grad = xk.moe_router_backward(z, ids, mask=mask, **kw)
+    for other in (mask.to(torch.uint8) * 2, mask.long() << 40, mask.float() * 0.25, mask.repeat_interleave(2)[::2]):
+        got = xk.moe_balance_loss(z, ids, mask=other)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+        assert torch.equal(xk.moe_router_backward(z, ids, mask=other, **kw), grad)
+
+
+@pytest.mark.parametrize("M,E", [(80, 64), (900, 256), (60, 700)])
+def test_padded_batch_captured(M, E, dev):
+    """One graph for batches of any fill: the mask and what it leaves change between replays."""
+    z, ids, u, mask = _case(M, E, 4, torch.bfloat16, seed=1, pad=0.5)
+    coef = torch.tensor(0.01, device="cuda")
+
+    def step():
+        st = xk.moe_balance_loss(z, ids, mask=mask)
+        return *st, xk.moe_router_backward(z, ids, grad_weights=u, renormalize=False, grad_loss=coef, counts=st.counts,
+                                           tokens=st.tokens, mask=mask)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed, fill in enumerate((1.0, 0.3, 0.0, 0.8)):
+        fresh = _case(M, E, 4, torch.bfloat16, seed=20 + seed)
+        z.copy_(fresh[0])
+        ids.copy_(fresh[1])
+        mask.copy_(torch.rand(M, generator=torch.Generator().manual_seed(seed)) < fill)
+        graph.replay()
+        got = [t.clone() for t in out]
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, step())), seed
+        assert int(got[2]) == int(mask.sum())
+
+
+def test_more_than_32_bits_of_logits(dev):
+    """Rows past 2^31 logits; all but the last three padded."""
+    M, E, k = 4200000, 512, 2
+    z = torch.zeros(M, E, dtype=torch.float16, device="cuda")
+    few = _case(3, E, k, torch.float16, seed=9)
+    z[-3:] = few[0]
+    ids = torch.zeros(M, k, dtype=torch.int32, device="cuda")
+    ids[-3:] = few[1]
+    u = torch.ones(M, k, device="cuda")
+    u[-3:] = few[2]
+    mask = torch.zeros(M, dtype=torch.bool, device="cuda")
+    mask[-3:] = True
+    st = xk.moe_balance_loss(z, ids, mask=mask)
+    loss, counts, tokens = balance_ref(few[0], few[1], None)
+    assert torch.equal(st.counts.cpu().long(), counts) and int(st.tokens) == tokens == 3
+    check(st.loss, loss, (softmax_delta(few[0].double().cpu()) + 67 * F32 / 2) * loss, "loss")
+    gl = torch.tensor(0.7, device="cuda")
+    got = xk.moe_router_backward(z, ids, grad_weights=u, grad_loss=gl, counts=st.counts, tokens=st.tokens, mask=mask)
+    want, bound = router_grad_ref(few[0], few[1], few[2], True, gl, st.counts)
+    check(got[-3:], want, bound)
+    assert not got[:-3].any()
+
+
+def test_refusals(dev):
+    z, ids, u, mask = _case(6, 16, 2, torch.float32, pad=0.5)
+    st = xk.moe_balance_loss(z, ids)
+    bad = [lambda: xk.moe_balance_loss(z, ids[:5]), lambda: xk.moe_balance_loss(z, ids[:, :0]),
+           lambda: xk.moe_balance_loss(z, ids.float()), lambda: xk.moe_balance_loss(z.double(), ids),
+           lambda: xk.moe_balance_loss(z[0], ids), lambda: xk.moe_balance_loss(z, ids, mask=mask[:5]),
+           lambda: xk.moe_balance_loss(z[:, :1], ids), lambda: xk.moe_balance_loss(z, ids.cpu()),
+           lambda: xk.moe_router_backward(z, ids), lambda: xk.moe_router_backward(z, ids, grad_loss=st.loss),
+           lambda: xk.moe_router_backward(z, ids, grad_loss=st.loss, counts=st.counts, mask=mask),
+           lambda: xk.moe_router_backward(z, ids, grad_loss=st.loss, counts=st.counts[:5]),
+           lambda: xk.moe_router_backward(z, ids, grad_loss=u, counts=st.counts),
+           lambda: xk.moe_router_backward(z, ids, grad_weights=u[:, :1])]
+    for i, call in enumerate(bad):
+        with pytest.raises(RuntimeError):
+            call()
+            pytest.fail(f"call {i} went through")

@@ -223,3 +223,10 @@ def test_checkpoint_form():
     assert s.tolist() == [[127], [128]]
     assert q[0, :5].tolist() == [448.0, 1.0, -1.0, 0.0, 16.0]  # ties to the even code
     assert q[1, :2].tolist() == [448.0, 3.0]  # 449 is 224.5 scaled: 224
+
+
+@pytest.mark.parametrize("kw", [dict(M=1 << 29), dict(K=1000001, ldx=1 << 24), dict(N=1000001, ldb=1 << 24)])
+def test_lora_refuses_what_no_grid_holds(kw):
+    assert _lora(**kw) == INVALID and "bad sizes" in _lib.last_error()
+    grad = {{"ldb": "ldg"}.get(k, k): v for k, v in kw.items()}
+    assert _lora_grad(**grad) == INVALID and "bad sizes" in _lib.last_error()

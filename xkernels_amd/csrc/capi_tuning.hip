@@ -32,6 +32,8 @@ namespace {
 // Sizes past these do not occur and keep every product below in 64 bits.
 constexpr int64_t kMaxRows = int64_t(1) << 30, kMaxCols = int64_t(1) << 24;
 constexpr int kMaxAdapters = 1024;
+// of adapters: what the launches' grids hold at any rank and type
+constexpr int64_t kMaxLoraRows = int64_t(1) << 29, kMaxLoraCols = 1000000;
 
 bool any_dtype(int dt) { return dt == XK_DT_BF16 || dt == XK_DT_FP32 || dt == XK_DT_FP16; }
 
@@ -46,7 +48,7 @@ int check_router(const char* op, int dtype, int64_t M, int64_t E, int64_t k) {
 
 int check_lora(const char* op, int dtype, int64_t M, int64_t K, int64_t N, int64_t L, int64_t r) {
   XK_REQUIRE(dtype == XK_DT_BF16 || dtype == XK_DT_FP32, "%s: dtype code %d is neither bf16 nor fp32", op, dtype);
-  XK_REQUIRE(M >= 0 && M < kMaxRows && K >= 1 && K <= kMaxCols && N >= 1 && N <= kMaxCols,
+  XK_REQUIRE(M >= 0 && M < kMaxLoraRows && K >= 1 && K <= kMaxLoraCols && N >= 1 && N <= kMaxLoraCols,
              "%s: bad sizes M=%lld K=%lld N=%lld", op, (long long)M, (long long)K, (long long)N);
   XK_REQUIRE(L >= 1 && L <= kMaxAdapters, "%s: %lld adapters, outside [1, %d]", op, (long long)L, kMaxAdapters);
   XK_REQUIRE(r >= 1 && r <= lora_max_rank(), "%s: rank %lld outside [1, %d]", op, (long long)r, lora_max_rank());

@@ -73,6 +73,14 @@ template <typename V, typename E> __device__ __forceinline__ void store_unaligne
   __builtin_memcpy(p, &v, sizeof(V));
 }
 
+// Between LDS accesses of a wave's lanes to each other's places: the hardware carries
+// a wave's out in order, so this costs no instruction, but it keeps the compiler from
+// passing a lane its own value on or moving one access over the other.
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // MFMA operand vector types.
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));

@@ -704,12 +704,12 @@ __device__ __forceinline__ void copy_rows(const int* tile_rows, int n_rows, int6
 // and output move in whole lines. The weights of a round go through LDS for all four
 // waves (product t's rows together), the next round's on their way meanwhile, as is
 // its base: loads and stores leave a wave's counter in order, so neither is waited
-// for right after a store.
+// for right after a store. `out` may be `base`: a lane's values of it are read before
+// they are written, and no other lane uses them.
 template <typename T, int RT, bool VEC>
 __global__ void __launch_bounds__(kThreads, kExpandPlaces<RT>)
 lora_expand(Rows rows, Ranks h, const T* __restrict__ b, int wide, const float* __restrict__ scaling,
-            const T* __restrict__ base, int64_t ldbase, int64_t N, int chunks, T* __restrict__ out,
-            float* __restrict__ hidden_out) {
+            const T* base, int64_t ldbase, int64_t N, int chunks, T* out, float* __restrict__ hidden_out) {
   constexpr int RP = RT * 16, HP = RP + 4, PER = 16 / sizeof(T), BN = 16 * PER;
   constexpr int PPR = RP / PER, WP = RP + PER, NW = BN * PPR / kThreads;  // pieces of a weight row, its pitch, pieces a thread
   constexpr int kWeightBytes = 2 * BN * WP * sizeof(T), kHiddenBytes = kTile * HP * 4;
@@ -843,8 +843,7 @@ lora_expand(Rows rows, Ranks h, const T* __restrict__ b, int wide, const float* 
 template <typename T, int RT, bool VEC>
 __global__ void __launch_bounds__(kThreads, 2)
 lora_expand_few(Rows rows, Ranks h, const T* __restrict__ b, int wide, const float* __restrict__ scaling,
-                const T* __restrict__ base, int64_t ldbase, int64_t N, int64_t chunk, T* __restrict__ out,
-                float* __restrict__ hidden) {
+                const T* base, int64_t ldbase, int64_t N, int64_t chunk, T* out, float* __restrict__ hidden) {
   constexpr int RP = RT * 16, PITCH = RP + 4;
   typedef rank_blocks<T, RT> rb;
   __shared__ int tile_rows[kFewTile];
@@ -1097,6 +1096,7 @@ __device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t
           reinterpret_cast<u32x4*>(at)[j] = reinterpret_cast<const u32x4*>(&v[i])[j];
       }
     }
+    wave_lds_fence();
     typename mm<T>::frag uc[PARTS][RT];
 #pragma unroll
     for (int part = 0; part < PARTS; ++part)
@@ -1126,6 +1126,7 @@ __device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t
 #pragma unroll
         for (int t = 0; t < RT; ++t) acc[e][t] = mm<T>::mma(uc[part][t], vf, acc[e][t]);
     }
+    wave_lds_fence();
   };
   while (more[0]) {
     if constexpr (DEPTH == 1) {

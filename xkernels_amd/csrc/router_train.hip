@@ -420,6 +420,7 @@ router_grad_rows(const T* __restrict__ logits, int64_t M, int E, int k, RouterGr
 #pragma unroll
       for (int j = 0; j < N; ++j) p[j] = with_loss ? p[j] * fmaf(f, c[j] - pc, -qi) : -p[j] * qi;
       put_row<T, PIECES>(p, mine, i16);
+      wave_lds_fence();  // a slot's value replaces another lane's
       if (with_weights) {
         // every slot of one expert forms the same sum, in slot order
         float add = 0.f;
@@ -435,8 +436,7 @@ router_grad_rows(const T* __restrict__ logits, int64_t M, int E, int k, RouterGr
       for (int j = 0; j < N; ++j) p[j] = 0.f;
       put_row<T, PIECES>(p, mine, i16);
     }
-    // (a wave's LDS accesses are carried out in order; its rows are its own)
-    __builtin_amdgcn_wave_barrier();
+    wave_lds_fence();
 #pragma unroll
     for (int cc = 0; cc < PIECES; ++cc) {
       const int e0 = (cc * 16 + i16) * 8;
@@ -453,7 +453,7 @@ router_grad_rows(const T* __restrict__ logits, int64_t M, int E, int k, RouterGr
           if (e0 + i < E) out[e0 + i] = mine[e0 + i];
       }
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_lds_fence();
   }
 }
 
