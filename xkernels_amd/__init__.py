@@ -2,7 +2,10 @@
 
 Public ops (same names and signatures as ``xkernels``):
 ``fused_moe_int4_w4a16``, ``fused_moe_mxfp4``, ``moe_align_block_size``,
-``moe_sum_reduce``, ``topk_softmax``; harness: ``find_impl``, ``verify``, ``verify_parity``,
+``moe_sum_reduce``, ``topk_softmax``; without a counterpart there, for tuning and
+serving over the frozen experts: ``moe_balance_loss``, ``moe_router_backward``,
+``lora_projection``, ``lora_projection_backward``, ``act_checkpoint``,
+``act_restore``; harness: ``find_impl``, ``verify``, ``verify_parity``,
 ``backend_diagnostics``. The ops run hand-written HIP kernels from
 ``libxk_moe.so``; they raise if the library is missing or the tensors are not on
 the GPU.

@@ -16,6 +16,7 @@
 // order, so results do not depend on scheduling (counts are whole numbers; the
 // probabilities' sums have a fixed order). The backward forms p again rather than
 // read it: M * E exponentials cost less than M * E more values from memory.
+// Up to kOneWgRows rows the forward is one workgroup and one launch.
 #include <algorithm>
 
 #include "router_rows.h"
@@ -124,6 +125,10 @@ __device__ __forceinline__ float loss_of(double total, int64_t E, int64_t T, int
 
 // One workgroup's rows: column sums of p over them in registers, then over the
 // workgroup's rows of lanes in LDS. ONE: the whole batch, loss included.
+//
+// bf16, k = 8: M = 65,536, E = 384 19 us (50 MB and 2 of ids, 2.7 TB/s, and some 15
+// VALU operations for each of 25 M logits, about 12 us); 8,192 x 256 5.3; one
+// workgroup, 200 x 48 fp32, 6.7.
 template <typename T, int PIECES, bool WIDE, bool ONE>
 __global__ void __launch_bounds__(ONE ? kOneWg : kRowThreads)
 balance_rows(const T* __restrict__ logits, const int32_t* __restrict__ ids, const uint8_t* __restrict__ mask,
@@ -201,7 +206,8 @@ balance_rows(const T* __restrict__ logits, const int32_t* __restrict__ ids, cons
 
 // Adds the planes: 16 columns a workgroup, 64 threads a column, eight planes' loads in
 // flight each; the workgroup that arrives last adds the loss's parts in order.
-// COUNTED: counts[] is complete.
+// COUNTED: counts[] is complete. 5.2 to 5.5 us: a launch, two dependent rounds of loads
+// and the ticket.
 template <bool COUNTED>
 __global__ void __launch_bounds__(kOneWg)
 balance_finish(int planes, int64_t E, int64_t k, BalanceScratch s, float* __restrict__ loss,
@@ -358,6 +364,9 @@ __device__ __forceinline__ void put_row(const float* p, T* row, int i16) {
 // and near-uniform counts (as a balanced router has) no longer cancel. A row's
 // gradient goes through LDS on its way out: the selected experts' slots, on the lane
 // of their number, put their values there, and whole pieces leave.
+//
+// bf16, k = 8: M = 65,536, E = 384 30 us (100 MB and 4 of ids and weights, 3.5 TB/s,
+// and as much VALU work as the forward's beside it), 8,192 x 256 7.0.
 template <typename T, int PIECES, bool WIDE>
 __global__ void __launch_bounds__(kThreads)
 router_grad_rows(const T* __restrict__ logits, int64_t M, int E, int k, RouterGrad a, T* __restrict__ grad) {

@@ -1,5 +1,6 @@
 """Quantized fused-MoE ops on gfx950: router (topk_softmax) -> align -> INT4 / MXFP4
-grouped GEMM -> combine.
+grouped GEMM -> combine; and for tuning and serving over them the router's training
+step, low-rank adapters and 8-bit activation checkpoints.
 
 The HIP backend registers inside ``backend_registration_guard``: if the native
 library is missing the failure is recorded (``backend_diagnostics()``) and any

@@ -1,4 +1,4 @@
-"""HIP backend of the five MoE ops: thin wrappers over libxk_moe.so.
+"""HIP backend of the reference's five MoE ops: thin wrappers over libxk_moe.so.
 
 Each callable has the reference backend's exact signature (the kwargs splatted
 by ``verify``; src/xkernels/ops/moe/reference.py:22-33, w4a16.py:53-56,
