@@ -45,7 +45,7 @@ constexpr int kFew = 256;      // rows up to which they do (a thread per row)
 constexpr int kMaxRank = 128;
 // Workgroups of a CU that the registers and LDS of their ranks' tiles of 16 allow.
 template <int RT> constexpr int kExpandPlaces = RT == 1 ? 4 : RT <= 4 ? 3 : 2;
-constexpr int kWgradPlaces = 2;
+template <typename T, int RT> constexpr int kWgradPlaces = sizeof(T) == 4 && RT == 1 ? 3 : 2;
 constexpr int kMaxAdapters = 1024;
 constexpr int kSortThreads = 1024;             // and rows a round of the sort
 constexpr int64_t kOneLaunchRows = 65536;      // rows up to which each sorting workgroup counts the whole batch
@@ -407,8 +407,8 @@ __device__ __forceinline__ void sort_part(const int32_t* __restrict__ ids, int64
   }
 }
 
-// out[l, c, r] = in[l, r, c]. A thread takes 8 values along r, which it writes as 16
-// bytes (bf16) where rows of `out` are whole pieces.
+// out[l, c, r] = in[l, r, c]. A thread takes 8 values along r, which it writes in 16
+// bytes (bf16), unaligned where rows of `out` are no whole pieces.
 template <typename T>
 __device__ __forceinline__ void transpose_part(const T* __restrict__ in, int64_t L, int64_t R, int64_t C,
                                                T* __restrict__ out, int64_t first, int64_t threads) {
@@ -433,6 +433,9 @@ __device__ __forceinline__ void transpose_part(const T* __restrict__ in, int64_t
     if (n == 8 && R % 8 == 0) {
 #pragma unroll
       for (int j = 0; j < int(sizeof(T)) / 2; ++j) reinterpret_cast<u32x4*>(dst)[j] = reinterpret_cast<u32x4*>(v)[j];
+    } else if (n == 8) {
+#pragma unroll
+      for (int j = 0; j < int(sizeof(T)) / 2; ++j) store_unaligned(dst + j * 16 / sizeof(T), reinterpret_cast<u32x4*>(v)[j]);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -1171,47 +1174,65 @@ __device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t
       tile(vs[1], helds[1], more[1], more[0]);
     }
   }
-  // the waves' sums: a quarter of the column tiles at a time, which one wave adds in
-  // wave order and writes
-  constexpr int CQ = CT / 4 > 0 ? CT / 4 : 1;
-  f32x4* red = reinterpret_cast<f32x4*>(lds);  // [4 waves][CQ][RT][64]
+  // the waves' sums, 16 ranks at a time, added in wave order by all threads and written in
+  // 16 bytes: of a rank's columns, or (out [L, C, r]) of a column's ranks. (The code of a
+  // part is kept short: a short adapter's whole pass is one run through it.)
+  constexpr int ITEM = 65;  // f32x4s from one column tile's to the next: a rank's pieces fall on all banks
+  f32x4* red = reinterpret_cast<f32x4*>(lds);  // [4 waves][CT][ITEM]
+  const float* redf = reinterpret_cast<const float*>(lds);
 #pragma unroll
-  for (int q = 0; q < CT / CQ; ++q) {
+  for (int t = 0; t < RT; ++t) {
+    if (16 * t >= r) break;
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < CQ; ++e)
-#pragma unroll
-      for (int t = 0; t < RT; ++t) red[((wave * CQ + e) * RT + t) * 64 + lane] = acc[q * CQ + e][t];
+    for (int e = 0; e < CT; ++e) red[(wave * CT + e) * ITEM + lane] = acc[e][t];
     __syncthreads();
-    if (wave != q) continue;
+    if (plane != nullptr || sd.by_rank) {
+      constexpr int OUT = 16 / sizeof(T), ROW = BC / OUT;
+      const int k = tid / ROW, c_in = tid % ROW * OUT, rank = 16 * t + k;
+      const int64_t c = c0 + c_in, at = int64_t(rank) * sd.C + c;
+      if (k >= 16 || rank >= r || c >= sd.C) continue;
+      float v[OUT];
 #pragma unroll
-    for (int e = 0; e < CQ; ++e) {
-      const int64_t c = c0 + (q * CQ + e) * 16 + (lane & 15);
+      for (int x = 0; x < OUT; ++x) {
+        const int col = c_in + x, item = ((col >> 4) * ITEM + (k >> 2) * 16 + (col & 15)) * 4 + (k & 3);
+        v[x] = 0.f;
 #pragma unroll
-      for (int t = 0; t < RT; ++t) {
+        for (int w = 0; w < kThreads / 64; ++w) v[x] += redf[w * CT * ITEM * 4 + item];
+      }
+      if (plane != nullptr) {
+#pragma unroll
+        for (int x = 0; x < OUT; x += 4) store_values(plane + at + x, sd.C - c - x, f32x4{v[x], v[x + 1], v[x + 2], v[x + 3]});
+      } else {
+        u32x4 o;
+#pragma unroll
+        for (int x = 0; x < OUT; ++x) io<T>::store(reinterpret_cast<T*>(&o) + x, v[x]);
+        store_values(static_cast<T*>(sd.out) + out_at + at, sd.C - c, o);
+      }
+    } else {
+      struct four { T v[4]; };
+#pragma unroll 1
+      for (int e = wave; e < CT; e += kThreads / 64) {
         f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < kThreads / 64; ++w) sum += red[((w * CQ + e) * RT + t) * 64 + lane];
+        for (int w = 0; w < kThreads / 64; ++w) sum += red[(w * CT + e) * ITEM + lane];
+        const int64_t c = c0 + e * 16 + (lane & 15);
+        const int rank = 16 * t + 4 * g;
+        four o;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int rank = 16 * t + 4 * g + i;
-          if (rank >= r || c >= sd.C) continue;
-          if (plane == nullptr)
-            io<T>::store(static_cast<T*>(sd.out) + out_at + (sd.by_rank ? rank * sd.C + c : c * r + rank), sum[i]);
-          else
-            plane[rank * sd.C + c] = sum[i];
-        }
+        for (int x = 0; x < 4; ++x) io<T>::store(&o.v[x], sum[x]);
+        if (c < sd.C) store_values(static_cast<T*>(sd.out) + out_at + c * r + rank, r - rank, o);
       }
     }
   }
 }
 
 template <typename T, int RT, bool VEC, bool Q8>
-__global__ void __launch_bounds__(kThreads, kWgradPlaces)
+__global__ void __launch_bounds__(kThreads, (kWgradPlaces<T, RT>))
 lora_wgrad(Side side_a, Side side_b, int r, int a_strips, const int32_t* __restrict__ sorted,
            const int32_t* __restrict__ offsets, int L, int64_t M, int seg) {
   constexpr int RP = RT * 16, BC = kColTiles<T, RT> * 16, PITCH = BC + 32 / sizeof(T);
-  constexpr int kTileBytes = 4 * 32 * PITCH * sizeof(T), kRedBytes = 4 * (BC / 64 > 0 ? BC / 64 : 1) * RT * 64 * 16;
+  constexpr int kTileBytes = 4 * 32 * PITCH * sizeof(T), kRedBytes = 4 * (BC / 16) * 65 * 16;
   __shared__ __attribute__((aligned(16))) unsigned char lds[kTileBytes > kRedBytes ? kTileBytes : kRedBytes];
   const bool is_a = int(blockIdx.y) < a_strips;
   const Side sd = is_a ? side_a : side_b;
@@ -1391,7 +1412,7 @@ int prepare(const int32_t* ids, int64_t M, int L, const Sort& so, char* ws, Rows
     XK_CHECK_LAUNCH("lora_count");
   }
   const int64_t pieces = a == nullptr ? 0 : int64_t(L) * (cdiv(r, 8) * K + cdiv(N, 8) * r);
-  const int64_t more = std::min<int64_t>(512, cdiv(pieces, 2 * kSortThreads));
+  const int64_t more = std::min<int64_t>(512, cdiv(pieces, kSortThreads));
   hipLaunchKernelGGL((lora_prepare<T>), dim3(unsigned(so.chunks + more)), dim3(kSortThreads), 0, stream, ids, M, L,
                      so.part, so.chunks, int(so.counted), o, a, b, K, N, r, at, bt);
   XK_CHECK_LAUNCH("lora_prepare");
@@ -1417,9 +1438,9 @@ struct ForwardPlan {
 struct Windows {
   int seg;
   int64_t count;
-  Windows(int64_t tiles, int64_t strips) {
-    const int64_t places = 256 * kWgradPlaces;
-    const int64_t n = std::max<int64_t>(1, std::min(places / strips, cdiv(tiles, 2)));
+  Windows(int64_t tiles, int64_t strips, int each) {
+    const int64_t places = 256 * each;
+    const int64_t n = std::max<int64_t>(1, std::min(places / strips, tiles));
     seg = int(std::max<int64_t>(1, cdiv(tiles, n)) * kTile);
     count = std::max<int64_t>(1, cdiv(tiles * kTile, seg));
   }
@@ -1433,7 +1454,7 @@ struct BackwardPlan {
   int64_t at, bt, planes, g_sum, packed_g, packed_h, part_a, part_b, total;
   BackwardPlan(int64_t M, int64_t K, int64_t N, int L, int r, int64_t elem)
       : sort(M, L), slices(N, sort.tiles, false), a_strips(cdiv(K, strip(r, elem))), b_strips(cdiv(N, strip(r, elem))),
-        win(sort.tiles, a_strips + b_strips) {
+        win(sort.tiles, a_strips + b_strips, elem == 4 && r <= 16 ? kWgradPlaces<float, 1> : kWgradPlaces<uint16_t, 1>) {
     const int64_t RP = rank_tiles(r) * 16, packed = sort.tiles * kTile * RP * 4;  // two bf16 or one fp32
     at = sort.total;
     bt = at + up(int64_t(L) * r * K * elem);
