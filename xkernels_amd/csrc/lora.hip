@@ -45,6 +45,8 @@ constexpr int kFew = 256;      // rows up to which they do (a thread per row)
 constexpr int kMaxRank = 128;
 // Workgroups of a CU that the registers and LDS of their ranks' tiles of 16 allow.
 template <int RT> constexpr int kExpandPlaces = RT == 1 ? 4 : RT <= 4 ? 3 : 2;
+// The same of the weight gradients (fp32, 24 adapters of rank 8 on 2,422 rows, 6,552 and
+// 7,168 columns: 53 us with three, 65 with two).
 template <typename T, int RT> constexpr int kWgradPlaces = sizeof(T) == 4 && RT == 1 ? 3 : 2;
 constexpr int kMaxAdapters = 1024;
 constexpr int kSortThreads = 1024;             // and rows a round of the sort
@@ -963,8 +965,9 @@ lora_expand_few(Rows rows, Ranks h, const T* __restrict__ b, int wide, const flo
 // fall on distinct banks.
 //
 // Both gradients in one launch. HBM, two workgroups a CU (their sums and two tiles of
-// rows fill the registers): M = 8,192, K = 7,168, N = 4,096, r = 16 45 us (184 MB, 4.1 TB/s),
-// 16,384 x (7,168 of 8 bits + 2,048), r = 32 52 to 60 (184 MB, 3.1 to 3.5).
+// rows fill the registers): M = 8,192, K = 7,168, N = 4,096, r = 16 44 us (184 MB, 4.2 TB/s),
+// 16,384 x (7,168 of 8 bits + 2,048), r = 32 49 to 57 (184 MB, 3.2 to 3.8); 300 rows of
+// 2 x 2,880, r = 8 5.2.
 struct Side {
   const void* packed;      // [positions / 32, parts, RT, 64 lanes, 8] of T: u as operands
   const void* v;           // [M, C] of T, or e4m3 bytes with `scales`
@@ -1176,7 +1179,8 @@ __device__ __forceinline__ void wgrad_strip(const Side& sd, int r, const int32_t
   }
   // the waves' sums, 16 ranks at a time, added in wave order by all threads and written in
   // 16 bytes: of a rank's columns, or (out [L, C, r]) of a column's ranks. (The code of a
-  // part is kept short: a short adapter's whole pass is one run through it.)
+  // part is kept short: a short adapter's whole pass is one run through it. 59 rows,
+  // r = 64: 15 us, 30 with a quarter of the columns at a time, added by one wave.)
   constexpr int ITEM = 65;  // f32x4s from one column tile's to the next: a rank's pieces fall on all banks
   f32x4* red = reinterpret_cast<f32x4*>(lds);  // [4 waves][CT][ITEM]
   const float* redf = reinterpret_cast<const float*>(lds);
@@ -1258,8 +1262,7 @@ lora_wgrad(Side side_a, Side side_b, int r, int a_strips, const int32_t* __restr
 }
 
 // Adds the planes of adapters over several windows; zeros for adapters without rows
-// (4 adapters of 8,192 rows, r = 16: 4.7 us; one window for all would save it at
-// 300 rows but takes wgrad from 9.7 us to 13).
+// (4 adapters of 8,192 rows, r = 16: 4.8 us).
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 wgrad_reduce(Side side_a, Side side_b, int r, int a_blocks, int RP, const int32_t* __restrict__ offsets, int seg) {
@@ -1411,6 +1414,8 @@ int prepare(const int32_t* ids, int64_t M, int L, const Sort& so, char* ws, Rows
     hipLaunchKernelGGL(lora_count, dim3(so.chunks), dim3(kSortThreads), 0, stream, ids, M, L, so.part, o.counts);
     XK_CHECK_LAUNCH("lora_count");
   }
+  // a transposed piece a thread: latency (2 adapters 3,952 -> 6,867, r = 64: 7.4 us, with
+  // two pieces 9.1)
   const int64_t pieces = a == nullptr ? 0 : int64_t(L) * (cdiv(r, 8) * K + cdiv(N, 8) * r);
   const int64_t more = std::min<int64_t>(512, cdiv(pieces, kSortThreads));
   hipLaunchKernelGGL((lora_prepare<T>), dim3(unsigned(so.chunks + more)), dim3(kSortThreads), 0, stream, ids, M, L,
@@ -1434,7 +1439,9 @@ struct ForwardPlan {
 };
 
 // Windows of the sorted positions: one workgroup for each place that registers and
-// LDS leave on the chip, so that all run at once and for as long.
+// LDS leave on the chip, so that all run at once and for as long, a tile at least: short
+// adapters then lie in windows of their own rather than one after the other (80 rows of
+// 4 adapters, r = 64: 8.1 us, with two tiles at least 13.3).
 struct Windows {
   int seg;
   int64_t count;
