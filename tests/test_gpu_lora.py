@@ -372,3 +372,37 @@ def test_refusals(dev):
         with pytest.raises(RuntimeError):
             call()
             pytest.fail(f"call {i} went through")
+
+
+@pytest.mark.parametrize("r,dt", [(8, F32), (16, BF), (64, BF), (128, BF), (128, F32)])
+@pytest.mark.parametrize("K,N", [(520, 264), (2050, 77)])
+def test_short_adapters(r, dt, K, N, dev):
+    """Adapters of one row to a few tiles, in windows of their own and shared ones."""
+    sizes = [1, 64, 65, 0, 3, 200, 31, 0, 129]
+    ids = torch.tensor([i for i, n in enumerate(sizes) for _ in range(n)], dtype=torch.int32)
+    ids = ids[torch.randperm(len(ids), generator=torch.Generator().manual_seed(r))].cuda()
+    x, a, b, _, _, dy, sc = _case(len(ids), K, N, len(sizes), r, dt, seed=r)
+    _, hidden = xk.lora_projection(x, a, b, ids, scaling=sc, return_hidden=True)
+    got = xk.lora_projection_backward(dy, x, a, b, ids, hidden, scaling=sc)
+    want, bounds = lora_grad_ref(dy, x, a, b, ids, hidden, sc)
+    for name, g, w, bd in zip(("grad_x", "grad_a", "grad_b"), got, want, bounds):
+        check(g, w, bd, name)
+    for i in (3, 7):
+        assert not got[1][i].any() and not got[2][i].any()
+
+
+def test_gradients_on_streams(dev):
+    """Two backward passes at once."""
+    cases = [_case(500, 512, 264, 4, 16, BF, seed=s) for s in (1, 2)]
+    hs = [xk.lora_projection(c[0], c[1], c[2], c[3], return_hidden=True)[1] for c in cases]
+    run = lambda c, h: xk.lora_projection_backward(c[5], c[0], c[1], c[2], c[3], h, scaling=c[6])  # noqa: E731
+    want = [run(c, h) for c, h in zip(cases, hs)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for c, h, st in zip(cases, hs, streams):
+            with torch.cuda.stream(st):
+                got.append(run(c, h))
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for g, w in zip(got, want) for p, q in zip(g, w))

@@ -282,3 +282,19 @@ def test_refusals(dev):
         with pytest.raises(RuntimeError):
             call()
             pytest.fail(f"call {i} went through")
+
+
+@pytest.mark.parametrize("E", [48, 600])
+def test_counts_of_several_ranks(E, dev):
+    """Parts of a batch, each with the summed counts and rows: together the whole batch's gradient."""
+    z, ids, u, mask = _case(700, E, 4, torch.float32, seed=E, pad=0.2)
+    whole = xk.moe_balance_loss(z, ids, mask=mask)
+    gl = torch.tensor(0.3, device="cuda")
+    want, bound = router_grad_ref(z, ids, u, True, gl, whole.counts, mask)
+    parts = [slice(0, 100), slice(100, 420), slice(420, 700)]
+    sts = [xk.moe_balance_loss(z[p], ids[p], mask=mask[p]) for p in parts]
+    counts, tokens = sum(s.counts for s in sts), sum(s.tokens for s in sts)
+    assert torch.equal(counts, whole.counts) and int(tokens) == int(whole.tokens)
+    got = torch.cat([xk.moe_router_backward(z[p], ids[p], grad_weights=u[p], grad_loss=gl, counts=counts, tokens=tokens,
+                                            mask=mask[p]) for p in parts])
+    check(got, want, bound)
