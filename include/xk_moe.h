@@ -300,7 +300,8 @@ int xk_lora_projection(const void* x, int32_t dtype, int64_t ldx, int64_t M, int
  *   grad_a[i] = sum_m g[m]^T x[m],  grad_b[i] = scaling[i] sum_m grad_out[m]^T h[m]
  * over adapter i's rows (zeros for an adapter without rows); scaling is a constant.
  * x [M, K] of dtype with rows ldx apart, or, with x_scales, the e4m3 values [M, K]
- * and e8m0 scales of xk_act_checkpoint (ldx = K). hidden as the forward left it.
+ * and e8m0 scales of xk_act_checkpoint (ldx = K), taken as xk_act_restore gives them in
+ * dtype. hidden as the forward left it.
  * grad_x [M, K], grad_a [L, r, K], grad_b [L, N, r] of dtype, contiguous. */
 int64_t xk_lora_projection_backward_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t L,
                                                     int64_t r, int32_t dtype);

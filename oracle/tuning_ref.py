@@ -63,7 +63,7 @@ def lora_projection_ref(x, lora_a, lora_b, adapter_ids, base=None, scaling=None,
 
 
 def lora_projection_backward_ref(grad_out, x, lora_a, lora_b, adapter_ids, hidden, scaling=None):
-    x = act_restore_ref(x, torch.float32) if isinstance(x, tuple) else x.float()
+    x = act_restore_ref(x, grad_out.dtype).float() if isinstance(x, tuple) else x.float()
     gx = torch.zeros(x.shape, device=x.device)
     ga, gb = torch.zeros(lora_a.shape, device=x.device), torch.zeros(lora_b.shape, device=x.device)
     for i in range(lora_a.shape[0]):

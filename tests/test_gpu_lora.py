@@ -406,3 +406,46 @@ def test_gradients_on_streams(dev):
                 got.append(run(c, h))
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for g, w in zip(got, want) for p, q in zip(g, w))
+
+
+@pytest.mark.parametrize("K", [96, 70])
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_backward_from_8_bits_at_the_top(K, dt, dev):
+    """Activations whose 8-bit neighbour passes the type's range enter the gradients as they are
+    restored, the largest finite value: the same bits, and finite ones."""
+    x, a, b, _, _, dy, _ = _case(3, K, 16, 1, 4, dt, seed=K)
+    x[0, 3], x[1, 40], x[2, K - 1] = torch.finfo(dt).max, torch.finfo(dt).min, torch.finfo(dt).max
+    dy *= 2.0 ** -9
+    ids = torch.zeros(3, dtype=torch.int32, device="cuda")
+    hidden = torch.randn(3, 4, device="cuda")
+    held = xk.act_checkpoint(x)
+    back = xk.act_restore(held, dt)
+    assert torch.isfinite(back).all() and back[0, 3] == torch.finfo(dt).max
+    got = xk.lora_projection_backward(dy, held, a, b, ids, hidden)
+    want = xk.lora_projection_backward(dy, back, a, b, ids, hidden)
+    assert all(torch.isfinite(t).all() for t in got)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    ref, bounds = lora_grad_ref(dy, back, a, b, ids, hidden)
+    for name, g, w, bd in zip(("grad_x", "grad_a", "grad_b"), got, ref, bounds):
+        check(g, w, bd, name)
+
+
+@pytest.mark.parametrize("K", [8192, 8191])
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_backward_from_every_byte(K, dt, dev):
+    """Every e4m3 code at every scale byte, reserved ones among them, in a gradient of one row
+    and one rank (x itself times a power of two): as act_restore gives them."""
+    a, b = torch.ones(1, 1, K, dtype=dt, device="cuda"), torch.ones(1, 8, 1, dtype=dt, device="cuda")
+    ids, hidden = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.ones(1, 1, device="cuda")
+    scales = torch.arange(256, dtype=torch.uint8).view(1, 256).cuda()
+    dy = torch.zeros(1, 8, dtype=dt, device="cuda")
+    for power in (0, 40, -40):
+        dy[0, 3] = 2.0 ** power
+        for first in range(0, 256, 32):
+            codes = (torch.arange(32) + first).to(torch.uint8).repeat(256)[:K].view(1, K)
+            held = xk.ActCheckpoint(codes.cuda().view(torch.float8_e4m3fn), scales)
+            got = xk.lora_projection_backward(dy, held, a, b, ids, hidden)[1]
+            want = xk.lora_projection_backward(dy, xk.act_restore(held, dt), a, b, ids, hidden)[1]
+            assert torch.equal(got.isnan(), want.isnan()), (power, first)
+            bad = ((got != want) & ~want.isnan()).flatten().nonzero().flatten()
+            assert bad.numel() == 0, (power, first, bad.numel(), bad[:4].tolist(), got.flatten()[bad[:4]], want.flatten()[bad[:4]])

@@ -230,3 +230,19 @@ def test_lora_refuses_what_no_grid_holds(kw):
     assert _lora(**kw) == INVALID and "bad sizes" in _lib.last_error()
     grad = {{"ldb": "ldg"}.get(k, k): v for k, v in kw.items()}
     assert _lora_grad(**grad) == INVALID and "bad sizes" in _lib.last_error()
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_oracle_takes_8_bits_as_restored(dt):
+    """A largest value whose 8-bit neighbour passes the type's range: finite gradients."""
+    from oracle import tuning_ref as o
+
+    x = torch.ones(2, 40, dtype=dt)
+    x[0, 5] = torch.finfo(dt).max
+    held = o.act_checkpoint_ref(x)
+    rest = (torch.ones(1, 3, 40, dtype=dt), torch.ones(1, 8, 3, dtype=dt), torch.zeros(2, dtype=torch.int32),
+            torch.ones(2, 3))
+    dy = torch.full((2, 8), 2.0 ** -9, dtype=dt)
+    got = o.lora_projection_backward_ref(dy, held, *rest)
+    want = o.lora_projection_backward_ref(dy, o.act_restore_ref(held, dt), *rest)
+    assert all(torch.isfinite(t).all() for t in got) and all(torch.equal(p, q) for p, q in zip(got, want))
