@@ -52,7 +52,7 @@ def moe_router_backward_ref(gating_output, topk_ids, grad_weights=None, renormal
 
 def lora_projection_ref(x, lora_a, lora_b, adapter_ids, base=None, scaling=None, return_hidden=False):
     M, (L, r, _), N = x.shape[0], lora_a.shape, lora_b.shape[1]
-    out = torch.zeros(M, N, device=x.device) if base is None else base.float()
+    out = torch.zeros(M, N, device=x.device) if base is None else base.to(torch.float32, copy=True)
     hidden = torch.zeros(M, r, device=x.device)
     for i in range(L):
         m = torch.nonzero(adapter_ids == i).flatten()

@@ -246,3 +246,18 @@ def test_oracle_takes_8_bits_as_restored(dt):
     got = o.lora_projection_backward_ref(dy, held, *rest)
     want = o.lora_projection_backward_ref(dy, o.act_restore_ref(held, dt), *rest)
     assert all(torch.isfinite(t).all() for t in got) and all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("op", OPS)
+def test_oracle_leaves_its_inputs_alone(op):
+    """fp32 inputs, which a cast to fp32 does not copy, and every other point of the sweep."""
+    points = load_shape_sweep(all_specs()[op].shape_sweep)
+    for p in points + [{**q, "dtype": "fp32"} for q in points]:
+        f = input_gen.generate_inputs(op, p, 3, "cpu")
+        flat = [t for v in f.values() for t in (v if isinstance(v, tuple) else (v,)) if torch.is_tensor(t)]
+        before = [t.clone() for t in flat]
+        out = reference_callable(op)(**f)
+        assert all(torch.equal(t.view(torch.uint8) if t.dim() else t, b.view(torch.uint8) if b.dim() else b)
+                   for t, b in zip(flat, before)), p
+        outs = [out] if torch.is_tensor(out) else list(out)
+        assert not {t.data_ptr() for t in outs if t.numel()} & {t.data_ptr() for t in flat if t.numel()}, p
