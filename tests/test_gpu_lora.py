@@ -449,3 +449,56 @@ def test_backward_from_every_byte(K, dt, dev):
             assert torch.equal(got.isnan(), want.isnan()), (power, first)
             bad = ((got != want) & ~want.isnan()).flatten().nonzero().flatten()
             assert bad.numel() == 0, (power, first, bad.numel(), bad[:4].tolist(), got.flatten()[bad[:4]], want.flatten()[bad[:4]])
+
+
+@pytest.mark.parametrize("M", [2, 300])
+@pytest.mark.parametrize("r", [1, 20, 40, 100])
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_infinite_hidden_keeps_its_sign(M, r, dt, dev):
+    """Infinities of either sign in one column of x, weights that are nowhere 0 or infinite
+    where they meet them: infinities of the formula's signs, no NaN."""
+    K, N = 72, 40
+    a = torch.zeros(1, r, K, dtype=dt, device="cuda")
+    a[:, :, 0] = 1
+    b = torch.ones(1, N, r, dtype=dt, device="cuda")
+    b[:, 1::2] = -1
+    x = torch.ones(M, K, dtype=dt, device="cuda")
+    x[0, 0], x[1, 0] = float("inf"), float("-inf")
+    ids = torch.zeros(M, dtype=torch.int32, device="cuda")
+    out, hidden = xk.lora_projection(x, a, b, ids, return_hidden=True)
+    sign = b[0, :, 0]
+    assert torch.equal(hidden[0], torch.full_like(hidden[0], float("inf"))) and torch.equal(hidden[1], -hidden[0])
+    assert torch.equal(out[0], sign * float("inf")) and torch.equal(out[1], -sign * float("inf"))
+    assert torch.equal(out[2:], (r * sign).expand(M - 2, N))
+
+
+@pytest.mark.parametrize("M", [3, 300])
+@pytest.mark.parametrize("r", [1, 20, 40, 100])
+def test_hidden_past_bf16s_range(M, r, dev):
+    """An h and a g between bf16's largest value and fp32's, times 2^-2: finite, as in 32 bits."""
+    K, N, top = 64, 48, 2.0 ** 127
+    big = torch.tensor([1.5 * top, 0.498046875 * top]).to(BF)  # both exact; their sum rounds to 2^128 in bf16
+    assert torch.isfinite(big.float().sum()) and torch.isinf(big.float().sum().to(BF))
+    a, b = torch.zeros(1, r, K, dtype=BF), torch.zeros(1, N, r, dtype=BF)
+    a[0, 0, :2], b[0, :, 0] = 1, 0.25
+    a[0, 0, 2:] = 0.25
+    x = torch.zeros(M, K, dtype=BF)
+    x[0, :2], x[1, :2] = big, -big
+    ids = torch.zeros(M, dtype=torch.int32)
+    x, a, b, ids = (t.cuda() for t in (x, a, b, ids))
+    out, hidden = xk.lora_projection(x, a, b, ids, return_hidden=True)
+    want, h, bound, hb = lora_ref(x, a, b, ids)
+    check(hidden, h, hb, "hidden")
+    check(out, want, bound, "out")
+    b[0, :2, 0] = 1  # g = big[0] + big[1]
+    dy = torch.zeros(M, N, dtype=BF, device="cuda")
+    dy[0, :2], dy[2 % M, 2:] = big.cuda(), 0.5
+    hidden[0] = 0  # (as x: a product with grad_out that stays finite)
+    x[:2] = 0.25
+    hidden[1, 0] = float(big.float().sum())  # times grad_out of 0.25
+    dy[1, 4] = 0.25
+    a[0, 0] = 0.25
+    got = xk.lora_projection_backward(dy, x, a, b, ids, hidden)
+    want, bounds = lora_grad_ref(dy, x, a, b, ids, hidden)
+    for name, g, w, bd in zip(("grad_x", "grad_a", "grad_b"), got, want, bounds):
+        check(g, w, bd, name)

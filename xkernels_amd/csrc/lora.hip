@@ -127,18 +127,17 @@ __device__ __forceinline__ typename mm<T>::frag zero_frag() {
   for (int i = 0; i < int(sizeof(T)) / 2; ++i) reinterpret_cast<u32x4*>(&f)[i] = u32x4{0, 0, 0, 0};
   return f;
 }
-// What hi leaves of v; 0 where hi is infinite or NaN and says it all.
-__device__ __forceinline__ float rest_of(float v, float hi) {
-  const float rest = v - hi;
-  return fabsf(rest) <= 3.4028234663852886e38f ? rest : 0.f;
-}
-
+// v as hi + lo. Where v rounds to an infinity hi is bf16's largest value, so that a finite v
+// leaves the difference to lo, and an infinity itself. (By its bits: limits in registers
+// cost the expansion of up to 16 ranks 12 bytes a lane of scratch.)
 __device__ __forceinline__ bf16x8 split_part(const float* v, bool low) {
   bf16x8 f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const __bf16 hi = static_cast<__bf16>(v[i]);
-    f[i] = low ? static_cast<__bf16>(rest_of(v[i], static_cast<float>(hi))) : hi;
+    uint16_t bits = __builtin_bit_cast(uint16_t, static_cast<__bf16>(v[i]));
+    bits -= (bits & 0x7FFFu) == 0x7F80u;
+    const __bf16 hi = __builtin_bit_cast(__bf16, bits);
+    f[i] = low ? static_cast<__bf16>(v[i] - static_cast<float>(hi)) : hi;
   }
   return f;
 }
