@@ -298,3 +298,22 @@ def test_counts_of_several_ranks(E, dev):
     got = torch.cat([xk.moe_router_backward(z[p], ids[p], grad_weights=u[p], grad_loss=gl, counts=counts, tokens=tokens,
                                             mask=mask[p]) for p in parts])
     check(got, want, bound)
+
+
+@pytest.mark.parametrize("M,E,k", [(300000, 600, 1), (1100000, 520, 2), (1 << 22, 48, 2), (1 << 26, 6, 1)])
+def test_sums_over_many_rows(M, E, k, dev):
+    """Equal logits: a probability of 1 / E is added M times, each time with the same rounding.
+    The loss is 1 whatever the ids. A lane's 64 additions, 4 lanes', 8 waves', 8 planes' and 8
+    parts' sums in 32 bits are off by half a step (2^-24) each at most, as are 1 / E, a plane, a
+    part and the loss; what lies beyond is added in 64 bits. None of it grows with M."""
+    off = (64 + 2 + 8 + 8 + 8 + 4) * 2.0 ** -24
+    z = torch.zeros(M, E, dtype=torch.bfloat16, device="cuda")
+    ids = (torch.arange(M * k, device="cuda", dtype=torch.int64) * 7 % E).view(M, k).int()
+    st = xk.moe_balance_loss(z, ids)
+    assert int(st.tokens) == M and int(st.counts.sum()) == M * k
+    assert abs(float(st.loss) - 1) <= off, float(st.loss) - 1
+    mask = torch.ones(M, dtype=torch.bool, device="cuda")
+    mask[::3] = False
+    half = xk.moe_balance_loss(z, ids, mask=mask)
+    assert int(half.tokens) == int(mask.sum())
+    assert abs(float(half.loss) - 1) <= off, float(half.loss) - 1

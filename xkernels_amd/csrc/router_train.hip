@@ -13,8 +13,10 @@
 // values in, and out in the backward) and launches for small ones. The forward
 // keeps each workgroup's column sums in registers over its rows and leaves one
 // plane of sums and counts per workgroup; a second launch adds the planes in
-// order, so results do not depend on scheduling (counts are whole numbers; the
-// probabilities' sums have a fixed order). The backward forms p again rather than
+// order, eights of them in 64 bits, so results do not depend on scheduling (counts are whole
+// numbers; the probabilities' sums have a fixed order). No sum in 32 bits is longer
+// than kLaneRows: a term that is always the same rounds the same way every time, and
+// the error would grow with the batch. The backward forms p again rather than
 // read it: M * E exponentials cost less than M * E more values from memory.
 // Up to kOneWgRows rows the forward is one workgroup and one launch.
 #include <algorithm>
@@ -30,7 +32,8 @@ constexpr int kOneWg = 1024;        // threads of the one workgroup of a small b
 constexpr int64_t kOneWgRows = 256; // rows up to which it is one workgroup's work
 constexpr int kFastExperts = 512, kFastTopk = 16;
 constexpr int kGradWgs = 1024;      // most workgroups of the gradient: each forms the counts' mean once
-constexpr int kPlanes = 512;        // most workgroups of the forward: 16 waves a CU
+constexpr int kPlanes = 512;        // workgroups of the forward: 16 waves a CU, more past 2^20 rows
+constexpr int kLaneRows = 64;       // most rows of a 16-lane row of the forward
 
 __device__ __forceinline__ float row_max(float x) {
   row_steps([&](auto from) { x = fmaxf(x, __uint_as_float(from(__float_as_uint(x)))); });
@@ -218,7 +221,7 @@ balance_finish(int planes, int64_t E, int64_t k, BalanceScratch s, float* __rest
   __shared__ int lds_rows[kOneWg / 64];
   const int tid = threadIdx.x, col = tid & 15, part = tid >> 4;
   const int64_t e = int64_t(blockIdx.x) * 16 + col;
-  float p = 0.f;
+  double p = 0.0;
   int c = 0;
   for (int g0 = part; g0 < planes; g0 += kParts * kAhead) {
     float pv[kAhead];
@@ -230,13 +233,15 @@ balance_finish(int planes, int64_t E, int64_t k, BalanceScratch s, float* __rest
       pv[j] = in ? s.sums[int64_t(g) * E + e] : 0.f;
       cv[j] = in && !COUNTED ? s.cnt[int64_t(g) * E + e] : 0;
     }
+    float eight = 0.f;
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
-      p += pv[j];
+      eight += pv[j];
       c += cv[j];
     }
+    p += double(eight);
   }
-  lds_p[part][col] = p;
+  lds_p[part][col] = float(p);
   lds_c[part][col] = c;
   int rows = 0;
   for (int g = tid; g < planes; g += kOneWg) rows += s.rows[g];
@@ -250,16 +255,21 @@ balance_finish(int planes, int64_t E, int64_t k, BalanceScratch s, float* __rest
   for (int w = 0; w < kOneWg / 64; ++w) T += lds_rows[w];
   double dot = 0.0;
   if (tid < 16 && e < E) {
-    float ps = 0.f;
+    double ps = 0.0;
     int cs = 0;
-#pragma unroll 16
-    for (int i = 0; i < kParts; ++i) {
-      ps += lds_p[i][col];
-      cs += lds_c[i][col];
+#pragma unroll 2
+    for (int i = 0; i < kParts; i += 8) {
+      float eight = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        eight += lds_p[i + j][col];
+        cs += lds_c[i + j][col];
+      }
+      ps += double(eight);
     }
     if (COUNTED) cs = counts[e];
     else counts[e] = cs;
-    dot = double(cs) * double(ps);
+    dot = double(cs) * ps;
   }
 #pragma unroll
   for (int off = 8; off >= 1; off >>= 1) dot += __shfl_xor(dot, off);
@@ -305,7 +315,8 @@ row_stats(const T* __restrict__ logits, const uint8_t* __restrict__ mask, int64_
   }
 }
 
-// Column sums: a thread per expert, a plane per part of the rows.
+// Column sums: a thread per expert, a plane per part of the rows, in 64 bits (a part may
+// be long).
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 balance_columns(const T* __restrict__ logits, const int32_t* __restrict__ ids, const uint8_t* __restrict__ mask,
@@ -313,19 +324,19 @@ balance_columns(const T* __restrict__ logits, const int32_t* __restrict__ ids, c
                 int32_t* __restrict__ counts) {
   const int64_t e = int64_t(blockIdx.x) * kThreads + threadIdx.x;
   const int64_t first = int64_t(blockIdx.y) * rows_per_plane, end = min(M, first + rows_per_plane);
-  float sum = 0.f;
+  double sum = 0.0;
   int rows = 0;
   for (int64_t row = first; row < end; ++row) {
     if (mask != nullptr && mask[row] == 0) continue;
     ++rows;
-    if (e < E) sum += expf(logit_at<T>(logits + row * E + e) - s.stat[2 * row]) * s.stat[2 * row + 1];
+    if (e < E) sum += double(expf(logit_at<T>(logits + row * E + e) - s.stat[2 * row]) * s.stat[2 * row + 1]);
     if (blockIdx.x == 0)
       for (int64_t j = threadIdx.x; j < k; j += kThreads) {
         const int id = ids[row * k + j];
         if (id >= 0 && id < E) atomicAdd(&counts[id], 1);
       }
   }
-  if (e < E) s.sums[int64_t(blockIdx.y) * E + e] = sum;
+  if (e < E) s.sums[int64_t(blockIdx.y) * E + e] = float(sum);
   if (blockIdx.x == 0 && threadIdx.x == 0) s.rows[blockIdx.y] = rows;
 }
 
@@ -538,7 +549,8 @@ router_grad_any(const T* __restrict__ logits, int64_t M, int64_t E, int64_t k, R
 }
 
 int planes_for(int64_t M, int64_t E) {
-  if (E <= kFastExperts) return int(std::min<int64_t>(kPlanes, cdiv(M, kRowThreads / 16)));
+  if (E <= kFastExperts)
+    return int(std::max(std::min<int64_t>(kPlanes, cdiv(M, kRowThreads / 16)), cdiv(M, kRowThreads / 16 * kLaneRows)));
   return int(std::max<int64_t>(1, std::min<int64_t>(64, cdiv(M, 16))));
 }
 int64_t up(int64_t x) { return (x + 255) / 256 * 256; }
