@@ -317,3 +317,23 @@ def test_sums_over_many_rows(M, E, k, dev):
     half = xk.moe_balance_loss(z, ids, mask=mask)
     assert int(half.tokens) == int(mask.sum())
     assert abs(float(half.loss) - 1) <= off, float(half.loss) - 1
+
+
+@pytest.mark.parametrize("E,k", [(48, 4), (384, 8), (511, 4), (600, 4), (40, 20)])
+def test_counts_past_24_bits(E, k, dev):
+    """Counts summed over many batches: near 2^28, a few apart. What the gradient takes is their
+    distance from the mean, which is as exact as that of small counts."""
+    z, ids, _, _ = _case(70, E, k, torch.float32, seed=E)
+    g = torch.Generator().manual_seed(k)
+    counts = (2 ** 28 + torch.randint(-40, 41, (E,), generator=g)).int()
+    T = 2 ** 30
+    gl = torch.tensor(1e9, device="cuda")
+    got = xk.moe_router_backward(z, ids, grad_loss=gl, counts=counts.cuda(),
+                                 tokens=torch.tensor(T, dtype=torch.int32, device="cuda"))
+    z64 = z.double().cpu()
+    p, delta = torch.softmax(z64, 1), softmax_delta(z64)
+    c = counts.double() - counts.double().mean()
+    pc = (p @ c).unsqueeze(1)
+    f = 1e9 * E / (float(T) * T * k)
+    size = (c - pc).abs() + c.abs() + (p @ c.abs()).unsqueeze(1)
+    check(got, f * p * (c - pc), f * p * (3 * delta + 16 * F32) * size)

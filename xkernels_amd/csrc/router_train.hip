@@ -54,6 +54,21 @@ __device__ __forceinline__ float wave_sum(float x) {
   return x;
 }
 
+// (exact for whole numbers, as the counts are)
+__device__ __forceinline__ double row_sum(double x) {
+  row_steps([&](auto from) {
+    const uint64_t b = __double_as_longlong(x);
+    const uint64_t lo = from(uint32_t(b)), hi = from(uint32_t(b >> 32));
+    x += __longlong_as_double(hi << 32 | lo);
+  });
+  return x;
+}
+__device__ __forceinline__ double wave_sum(double x) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off);
+  return x;
+}
+
 template <typename T> __device__ __forceinline__ T to_out(float f);
 template <> __device__ __forceinline__ uint16_t to_out<uint16_t>(float f) { return f32_to_bf16(f); }
 template <> __device__ __forceinline__ _Float16 to_out<_Float16>(float f) { return _Float16(f); }
@@ -372,7 +387,8 @@ __device__ __forceinline__ void put_row(const float* p, T* row, int i16) {
 }
 
 // The counts less their mean: as p sums to 1, c_i - sum p c is the same of either,
-// and near-uniform counts (as a balanced router has) no longer cancel. A row's
+// and near-uniform counts (as a balanced router has) no longer cancel. The difference
+// is formed in 64 bits: counts summed over many batches have more than fp32's 24. A row's
 // gradient goes through LDS on its way out: the selected experts' slots, on the lane
 // of their number, put their values there, and whole pieces leave.
 //
@@ -383,21 +399,22 @@ __global__ void __launch_bounds__(kThreads)
 router_grad_rows(const T* __restrict__ logits, int64_t M, int E, int k, RouterGrad a, T* __restrict__ grad) {
   constexpr int N = PIECES * 8, ROW = PIECES * 128;
   __shared__ __attribute__((aligned(16))) T rows_lds[kThreads / 16][ROW];
-  __shared__ __attribute__((aligned(16))) float counted[ROW];
+  __shared__ union { int count; float over; } experts[ROW];  // the counts, then less their mean
   const int tid = threadIdx.x, i16 = tid & 15;
   const bool with_loss = a.grad_loss != nullptr, with_weights = a.grad_weights != nullptr;
   T* mine = rows_lds[tid >> 4];
-  for (int e = tid; e < ROW; e += kThreads) counted[e] = with_loss && e < E ? float(a.counts[e]) : 0.f;
+  for (int e = tid; e < ROW; e += kThreads) experts[e].count = with_loss && e < E ? a.counts[e] : 0;
   __syncthreads();
-  float c[N], mean = 0.f;
+  double mean = 0.0;
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    c[j] = counted[((j >> 3) * 16 + i16) * 8 + (j & 7)];
-    mean += c[j];
-  }
-  mean = row_sum(mean) / float(E);
+  for (int j = 0; j < N; ++j) mean += double(experts[((j >> 3) * 16 + i16) * 8 + (j & 7)].count);
+  mean = row_sum(mean) / double(E);
+  __syncthreads();
+  for (int e = tid; e < ROW; e += kThreads) experts[e].over = float(double(experts[e].count) - mean);
+  __syncthreads();
+  float c[N];
 #pragma unroll
-  for (int j = 0; j < N; ++j) c[j] -= mean;
+  for (int j = 0; j < N; ++j) c[j] = experts[((j >> 3) * 16 + i16) * 8 + (j & 7)].over;
   const float factor = loss_factor(a, M, E, k);
   for (int64_t row = int64_t(blockIdx.x) * (kThreads / 16) + (tid >> 4); row < M;
        row += int64_t(gridDim.x) * (kThreads / 16)) {
@@ -449,7 +466,7 @@ router_grad_rows(const T* __restrict__ logits, int64_t M, int E, int k, RouterGr
           const int other = __shfl(id, (tid & 48) + l);
           if (other == id) add += v;
         }
-        if (id >= 0) mine[id] = to_out<T>((with_loss ? p_id * fmaf(factor, counted[id] - mean - pc, -q) : -p_id * q) + add);
+        if (id >= 0) mine[id] = to_out<T>((with_loss ? p_id * fmaf(factor, experts[id].over - pc, -q) : -p_id * q) + add);
       }
     } else {
 #pragma unroll
@@ -483,11 +500,12 @@ __global__ void __launch_bounds__(kThreads)
 router_grad_any(const T* __restrict__ logits, int64_t M, int64_t E, int64_t k, RouterGrad a, T* __restrict__ grad) {
   const int lane = threadIdx.x & 63;
   const bool with_loss = a.grad_loss != nullptr;
-  float mean = 0.f;
+  double mean = 0.0;
   if (with_loss) {
-    for (int64_t e = lane; e < E; e += 64) mean += float(a.counts[e]);
-    mean = wave_sum(mean) / float(E);
+    for (int64_t e = lane; e < E; e += 64) mean += double(a.counts[e]);
+    mean = wave_sum(mean) / double(E);
   }
+  auto over = [&](int64_t e) { return float(double(a.counts[e]) - mean); };
   const float factor = loss_factor(a, M, E, k);
   for (int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6); row < M; row += int64_t(gridDim.x) * 4) {
     const T* g = logits + row * E;
@@ -504,7 +522,7 @@ router_grad_any(const T* __restrict__ logits, int64_t M, int64_t E, int64_t k, R
     auto prob = [&](int64_t e) { return expf(logit_at<T>(g + e) - mx) / sum; };
     float pc = 0.f, q = 0.f, ps = 0.f, wu = 0.f, top = -__builtin_inff();
     if (with_loss) {
-      for (int64_t e = lane; e < E; e += 64) pc += prob(e) * (float(a.counts[e]) - mean);
+      for (int64_t e = lane; e < E; e += 64) pc += prob(e) * over(e);
       pc = wave_sum(pc);
     }
     if (a.grad_weights != nullptr) {
@@ -531,7 +549,7 @@ router_grad_any(const T* __restrict__ logits, int64_t M, int64_t E, int64_t k, R
     }
     auto base = [&](int64_t e) {
       const float pe = prob(e);
-      return (with_loss ? factor * pe * (float(a.counts[e]) - mean - pc) : 0.f) - pe * q;
+      return (with_loss ? factor * pe * (over(e) - pc) : 0.f) - pe * q;
     };
     for (int64_t e = lane; e < E; e += 64) out[e] = to_out<T>(base(e));
     if (a.grad_weights == nullptr) continue;
