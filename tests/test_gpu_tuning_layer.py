@@ -130,3 +130,42 @@ def test_tuning_step(dev):
             a -= 0.1 * ga
             b -= 0.1 * gb
             gate -= 0.1 * gg
+
+
+def test_calls_outside_autograd_say_so(dev, monkeypatch):
+    """The forwards warn in grad mode, once each, and give the same values; wrapped or under
+    no_grad they are silent."""
+    import warnings
+
+    from xkernels_amd.moe import hip_tuning
+
+    monkeypatch.setattr(hip_tuning, "_told", set())
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(9, 64, generator=g).to(BF).cuda()
+    a, b = torch.randn(2, 4, 64, generator=g).to(BF).cuda(), torch.randn(2, 32, 4, generator=g).to(BF).cuda()
+    ids = torch.randint(0, 2, (9,), generator=g, dtype=torch.int32).cuda()
+    z = torch.randn(9, 16, generator=g).cuda()
+    top = torch.topk(z, 2, 1).indices.int()
+    sc = torch.ones(2, device="cuda")
+    base = torch.zeros(9, 32, dtype=BF, device="cuda")
+    calls = {"lora_projection": lambda: (xk.lora_projection(x, a, b, ids, base=base, scaling=sc),),
+             "moe_balance_loss": lambda: tuple(xk.moe_balance_loss(z, top)),
+             "act_checkpoint": lambda: tuple(t.view(torch.uint8) for t in xk.act_checkpoint(x))}
+    want = {k: f() for k, f in calls.items()}
+    for t in (x, a, z):
+        t.requires_grad_()
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        with torch.no_grad():
+            for f in calls.values():
+                f()
+        Adapters.apply(x, a, b, base, ids, sc).sum().backward()
+        Router.apply(z, 2, torch.ones(9, dtype=torch.bool, device="cuda"))[2].backward()
+    assert a.grad is not None and z.grad is not None
+    for name, f in calls.items():
+        with pytest.warns(RuntimeWarning, match=name):
+            got = f()
+        assert all(torch.equal(p, q) for p, q in zip(got, want[name]))
+        with warnings.catch_warnings():
+            warnings.simplefilter("error")
+            f()

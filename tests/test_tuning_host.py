@@ -261,3 +261,18 @@ def test_oracle_leaves_its_inputs_alone(op):
                    for t, b in zip(flat, before)), p
         outs = [out] if torch.is_tensor(out) else list(out)
         assert not {t.data_ptr() for t in outs if t.numel()} & {t.data_ptr() for t in flat if t.numel()}, p
+
+
+def test_no_gradient_is_said_once(monkeypatch):
+    """One warning an op."""
+    import warnings
+
+    from xkernels_amd.moe import hip_tuning as h
+
+    monkeypatch.setattr(h, "_told", set())
+    for op in ("one", "other"):
+        with pytest.warns(RuntimeWarning, match=f"{op} records no autograd graph"):
+            h._no_graph(op)
+        with warnings.catch_warnings():
+            warnings.simplefilter("error")
+            h._no_graph(op)

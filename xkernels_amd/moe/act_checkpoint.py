@@ -23,7 +23,8 @@ def act_checkpoint(x: torch.Tensor, *, backend: Backend | str = "auto") -> ActCh
     """``x [M, K]`` (bf16, fp16 or fp32) in 8 bits. A block's scale is the least power of two
     with which none of its finite values passes 448; values round to nearest even
     (2^-4 of a value, or of the block's largest over 2^14 for the smallest). Infinities
-    and NaN become NaN."""
+    and NaN become NaN. No autograd graph is recorded (a warning, once, where ``x`` requires
+    a gradient)."""
     return dispatch("act_checkpoint", x, backend=backend)
 
 

@@ -31,7 +31,8 @@ def moe_balance_loss(
     ``loss = E / (T^2 top_k) * sum_e counts[e] * sum_m softmax(gating_output)[m, e]`` over
     the ``T`` rows that ``mask [M]`` (true: counts) leaves; 1 for a perfectly balanced
     router. ``gating_output [M, E]`` bf16, fp16 or fp32; ``topk_ids [M, top_k]`` as
-    ``topk_softmax`` gives them (ids outside ``[0, E)`` count nowhere). Deterministic.
+    ``topk_softmax`` gives them (ids outside ``[0, E)`` count nowhere). Deterministic. No
+    autograd graph is recorded (a warning, once, where the logits require a gradient).
     """
     return dispatch("moe_balance_loss", gating_output, topk_ids, mask=mask, backend=backend)
 

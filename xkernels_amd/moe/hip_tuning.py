@@ -8,6 +8,7 @@ Nothing synchronises, so every call may be captured into a HIP graph.
 """
 from __future__ import annotations
 
+import warnings
 from functools import lru_cache
 
 import torch
@@ -37,6 +38,21 @@ def _device(op: str, first: torch.Tensor, *others: torch.Tensor | None) -> int:
         if t is not None and t.get_device() != i:
             _need_gpu(op, first, t)
     return i
+
+
+_told: set[str] = set()
+_recording = torch.is_grad_enabled
+
+
+def _no_graph(op: str) -> None:
+    """Says, once an op, that a call which autograd would be expected to record (``_recording``, and
+    an input requires a gradient) is not. Under no_grad, and in the forward of an
+    autograd.Function, which runs without it, there is nothing to say."""
+    if op not in _told:
+        _told.add(op)
+        warnings.warn(f"{op} records no autograd graph: its result carries no gradient to inputs that require one. "
+                      "Call it and its backward in a torch.autograd.Function, or under torch.no_grad() if none is "
+                      "wanted", RuntimeWarning, stacklevel=5)
 
 
 def _stream(i: int) -> int:
@@ -112,6 +128,8 @@ def moe_balance_loss_hip(gating_output: torch.Tensor, topk_ids: torch.Tensor,
     i = _device(op, gating_output, topk_ids, mask)
     if i != _current_device():
         return _elsewhere(i, moe_balance_loss_hip, gating_output, topk_ids, mask)
+    if gating_output.requires_grad and _recording():
+        _no_graph(op)
     dt = _code(op, gating_output)
     M, E, k, g, ids, on = _router_args(op, gating_output, topk_ids, mask)
     loss = g.new_empty((), dtype=torch.float32)
@@ -183,6 +201,9 @@ def lora_projection_hip(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Ten
     i = _device(op, x, lora_a, lora_b, adapter_ids, base, scaling)
     if i != _current_device():
         return _elsewhere(i, lora_projection_hip, x, lora_a, lora_b, adapter_ids, base, scaling, return_hidden)
+    if (x.requires_grad or lora_a.requires_grad or lora_b.requires_grad
+            or (base is not None and base.requires_grad)) and _recording():
+        _no_graph(op)
     dt = _code(op, x, _LORA_DT)
     if x.dim() != 2:
         raise RuntimeError(f"{op}: x must be [M, K], got {list(x.shape)}")
@@ -254,6 +275,8 @@ def act_checkpoint_hip(x: torch.Tensor) -> ActCheckpoint:
     i = _device(op, x)
     if i != _current_device():
         return _elsewhere(i, act_checkpoint_hip, x)
+    if x.requires_grad and _recording():
+        _no_graph(op)
     dt = _code(op, x)
     if x.dim() != 2 or x.shape[1] == 0:
         raise RuntimeError(f"{op}: x must be [M, K], K >= 1, got {list(x.shape)}")

@@ -28,7 +28,8 @@ def lora_projection(
     [L, N, r]``, one dtype (bf16 or fp32); ``scaling [L]`` fp32; up to 1,024 adapters of
     rank up to 128 (adapters of smaller ranks filled up with zeros). ``return_hidden``
     adds ``x[m] @ lora_a[a].T`` (fp32 ``[M, r]``), which the backward takes.
-    Rows do not mix: what is not finite in one stays there.
+    Rows do not mix: what is not finite in one stays there. No autograd graph is recorded
+    (a warning, once, where an input requires a gradient).
     """
     return dispatch("lora_projection", x, lora_a, lora_b, adapter_ids, base=base, scaling=scaling,
                     return_hidden=return_hidden, backend=backend)
