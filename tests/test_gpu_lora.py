@@ -502,3 +502,18 @@ def test_hidden_past_bf16s_range(M, r, dev):
     want, bounds = lora_grad_ref(dy, x, a, b, ids, hidden)
     for name, g, w, bd in zip(("grad_x", "grad_a", "grad_b"), got, want, bounds):
         check(g, w, bd, name)
+
+
+@pytest.mark.parametrize("M", [200, 300, 5000])
+@pytest.mark.parametrize("N", [64, 47])
+@pytest.mark.parametrize("r", [16, 128])
+def test_small_products_beside_a_large_base(M, N, r, dev):
+    """fp32 products each below half a step of the base: their sum, which is not, counts."""
+    ids = torch.zeros(M, dtype=torch.int32, device="cuda")
+    x = torch.ones(M, 8, device="cuda")
+    a = torch.full((1, r, 8), 2.0 ** -3, device="cuda")
+    b = torch.full((1, N, r), 0.9 * 2.0 ** -25, device="cuda")
+    base = torch.ones(M, N, device="cuda")
+    out = xk.lora_projection(x, a, b, ids, base=base)
+    want, _, bound, _ = lora_ref(x, a, b, ids, base)
+    check(out, want, bound)

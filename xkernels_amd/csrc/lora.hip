@@ -743,6 +743,7 @@ lora_expand(Rows rows, Ranks h, const T* __restrict__ b, int wide, const float* 
   constexpr int RP = RT * 16, HP = RP + 4, PER = 16 / sizeof(T), BN = 16 * PER;
   constexpr int PPR = RP / PER, WP = RP + PER, NW = BN * PPR / kThreads;  // pieces of a weight row, its pitch, pieces a thread
   constexpr int kWeightBytes = 2 * BN * WP * sizeof(T), kHiddenBytes = kTile * HP * 4;
+  constexpr bool kBaseFirst = sizeof(T) == 2;
   typedef rank_blocks<T, RT> rb;
   __shared__ int tile_rows[kTile];
   __shared__ __attribute__((aligned(16))) unsigned char lds[kWeightBytes > kHiddenBytes ? kWeightBytes : kHiddenBytes];
@@ -834,15 +835,21 @@ lora_expand(Rows rows, Ranks h, const T* __restrict__ b, int wide, const float* 
       put_weights(buf);
       if (n0 + BN < c1) fetch_weights(n0 + BN);
       lds_sync();  // one a round: a buffer is written again two rounds on
-      f32x4 acc[PER];  // from the base on
+      // bf16: from the base on (what its 24 bits lose of small products is far below the
+      // result's half step); fp32: the base last, as no later rounding hides that loss
+      f32x4 acc[PER];
+      u32x4 bc[kBaseFirst ? 1 : 4];
 #pragma unroll
       for (int t = 0; t < PER; ++t) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const T bv = reinterpret_cast<const T*>(&bn[i])[t];
-          acc[t][i] = io<T>::load(&bv);
+          acc[t][i] = kBaseFirst ? io<T>::load(&bv) : 0.f;
         }
       }
+      if constexpr (!kBaseFirst)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bc[i] = bn[i];
       if (n0 + BN < c1) fetch_base(n0 + BN);
 #pragma unroll
       for (int t = 0; t < PER; ++t)
@@ -857,7 +864,11 @@ lora_expand(Rows rows, Ranks h, const T* __restrict__ b, int wide, const float* 
         if (!in[i]) continue;
         u32x4 o;
 #pragma unroll
-        for (int t = 0; t < PER; ++t) io<T>::store(reinterpret_cast<T*>(&o) + t, acc[t][i]);
+        for (int t = 0; t < PER; ++t) {
+          float v = acc[t][i];
+          if constexpr (!kBaseFirst) v += __uint_as_float(bc[i][t]);
+          io<T>::store(reinterpret_cast<T*>(&o) + t, v);
+        }
         if constexpr (VEC) {
           if (n0 + col < c1) *reinterpret_cast<u32x4*>(orow[i] + n0) = o;
         } else {
