@@ -337,3 +337,26 @@ def test_counts_past_24_bits(E, k, dev):
     f = 1e9 * E / (float(T) * T * k)
     size = (c - pc).abs() + c.abs() + (p @ c.abs()).unsqueeze(1)
     check(got, f * p * (c - pc), f * p * (3 * delta + 16 * F32) * size)
+
+
+@pytest.mark.parametrize("M,E", [(40, 100), (300, 384), (40, 700)])
+@pytest.mark.parametrize("renorm", [True, False])
+def test_probabilities_below_the_least_normal_number(M, E, renorm, dev):
+    """Logits 85 to 110 below their row's largest: probabilities down to fp32's least step (2^-149)
+    and past it, and gradients that are theirs alone."""
+    g = torch.Generator().manual_seed(E)
+    z = -85 - 25 * torch.rand(M, E, generator=g)
+    z[:, 0] = 0
+    ids = torch.stack([torch.randperm(E - 1, generator=g)[:4] + 1 for _ in range(M)]).int()
+    ids[::2, 1] = 0
+    u = torch.randn(M, 4, generator=g)
+    z, ids, u = z.cuda(), ids.cuda(), u.cuda()
+    st = _check_loss(z, ids, None)
+    gl = torch.tensor(0.7, device="cuda")
+    got = xk.moe_router_backward(z, ids, grad_weights=u, renormalize=renorm, grad_loss=gl, counts=st.counts)
+    want, bound = router_grad_ref(z, ids, u, renorm, gl, st.counts)
+    check(got, want, bound + 8 * 2.0 ** -149)  # (each of a value's few factors and sums has that step)
+    # alone: the plain weights' gradient is the probability times u and its distance from the rest
+    got = xk.moe_router_backward(z, ids, grad_weights=u, renormalize=renorm)
+    want, bound = router_grad_ref(z, ids, u, renorm)
+    check(got, want, bound + 8 * 2.0 ** -149)

@@ -74,15 +74,16 @@ template <> __device__ __forceinline__ uint16_t to_out<uint16_t>(float f) { retu
 template <> __device__ __forceinline__ _Float16 to_out<_Float16>(float f) { return _Float16(f); }
 template <> __device__ __forceinline__ float to_out<float>(float f) { return f; }
 
-// e^x for x <= 0 or NaN, to 2 steps of fp32: 2^(x log2 e) by v_exp_f32, what the
-// product and log2 e in 24 bits leave over (c, and 1.33e-8 x after the factor ln 2)
-// carried over as a factor. Results below the least normal number are 0.
+// e^x for x <= 0 or NaN, to 2 steps of fp32 and to fp32's least step: 2^(x log2 e) as
+// 2^n 2^f, n the nearest whole number (the low bits of a sum with 1.5 * 2^23) and f what
+// is left, with log2 e in two parts, by v_exp_f32 (whose own results below the least
+// normal number would be 0).
 __device__ __forceinline__ float exp_neg(float x) {
-  x = x < -104.f ? -104.f : x;
-  const float a = x * 1.44269502f;
-  const float c = fmaf(x, 1.44269502f, -a);
-  const float e = __builtin_amdgcn_exp2f(a);
-  return fmaf(e, fmaf(c, 0.693147181f, x * 1.33497587e-8f), e);
+  x = __builtin_elementwise_maximum(x, -104.f);  // (NaN stays)
+  constexpr float kWhole = 12582912.f;
+  const float t = fmaf(x, 1.44269502f, kWhole);
+  const float f = fmaf(x, 1.92596303e-8f, fmaf(x, 1.44269502f, kWhole - t));
+  return __builtin_ldexpf(__builtin_amdgcn_exp2f(f), int(__float_as_uint(t) - __float_as_uint(kWhole)));
 }
 
 // A row on its 16 lanes: lane i holds the 8-expert pieces i, i + 16, ...; z the logits
@@ -548,8 +549,7 @@ router_grad_any(const T* __restrict__ logits, int64_t M, int64_t E, int64_t k, R
       }
     }
     auto base = [&](int64_t e) {
-      const float pe = prob(e);
-      return (with_loss ? factor * pe * (over(e) - pc) : 0.f) - pe * q;
+      return prob(e) * (with_loss ? fmaf(factor, over(e) - pc, -q) : -q);
     };
     for (int64_t e = lane; e < E; e += 64) out[e] = to_out<T>(base(e));
     if (a.grad_weights == nullptr) continue;
