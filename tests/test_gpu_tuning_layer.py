@@ -169,3 +169,45 @@ def test_calls_outside_autograd_say_so(dev, monkeypatch):
         with warnings.catch_warnings():
             warnings.simplefilter("error")
             f()
+
+
+@pytest.mark.parametrize("renorm", [True, False])
+def test_router_gradient_through_the_experts(renorm, dev):
+    """The router's weights get their gradient from the experts themselves: a slot's is the output's
+    gradient times that slot's expert output, which the fused op gives for the slot alone."""
+    from tests._tuning_ref import gamma, router_grad_ref
+
+    M, E, N, K, k = 70, 16, 192, 256, 4
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(M, K, generator=g).to(BF).cuda()
+    z = torch.randn(M, E, generator=g).cuda()
+    experts = _weights(E, N, K, 5)
+    gy = torch.randn(M, N, generator=g).cuda()
+    w, ids = xk.topk_softmax(z, k, renormalize=renorm)
+    st = xk.moe_balance_loss(z, ids)
+    one = torch.ones(M, 1, device="cuda")
+    slots = [xk.fused_moe_int4_w4a16(x, *experts, ids[:, j:j + 1].contiguous(), one) for j in range(k)]
+    gw = torch.stack([(gy * o.float()).sum(1) for o in slots], 1)
+    gl = torch.tensor(0.01, device="cuda")
+    got = xk.moe_router_backward(z, ids, grad_weights=gw, renormalize=renorm, grad_loss=gl, counts=st.counts)
+    # in 64 bits, from the dequantised weights
+    W = dequant_w4a16(*experts).double().cpu()
+    o64 = torch.stack([torch.einsum("mk,mnk->mn", x.double().cpu(), W[ids[:, j].long().cpu()]) for j in range(k)], 1)
+    mag = torch.stack([torch.einsum("mk,mnk->mn", x.double().cpu().abs(), W[ids[:, j].long().cpu()].abs())
+                       for j in range(k)], 1)
+    gy64 = gy.double().cpu().unsqueeze(1)
+    u64 = (gy64 * o64).sum(2)
+    # a slot's output: fp32 sums over K, half a step of bf16 (and of the slot's own sum over one slot);
+    # their products' fp32 sum over N
+    off_o = 2 * half_step(BF) * o64.abs() + gamma(K) * mag
+    off_u = (gy64.abs() * (off_o + gamma(N) * o64.abs())).sum(2)
+    check(gw, u64, off_u, "grad_weights")
+    want, bound = router_grad_ref(z, ids, u64, renorm, gl, st.counts)
+    p = torch.softmax(z.double().cpu(), 1)
+    pj = p.gather(1, ids.long().cpu())
+    wj = pj / pj.sum(1, keepdim=True) if renorm else pj
+    mean = (wj * off_u).sum(1, keepdim=True)
+    bound = bound.scatter_add(1, ids.long().cpu(), wj * (off_u + mean if renorm else off_u))
+    if not renorm:
+        bound = bound + p * mean
+    check(got, want, bound, "logits")
