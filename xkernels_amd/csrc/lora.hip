@@ -8,7 +8,9 @@
 // A [L, r, K], B [L, N, r].
 //
 // A row's r values cost 2 r (K + N) operations against K + 2 N values of traffic:
-// HBM bound for every r taken here (up to 128). So each kernel reads its long rows
+// bf16 is HBM bound for every r taken here (up to 128), fp32, with an eighth of the
+// operations a second, to about r = 90 (4,096 x 4,096 -> 4,096, r = 128: 157 us for 216 MB
+// and 56 us of products). So each kernel reads its long rows
 // once, in 16-byte pieces straight into MFMA operands, and the adapters' weights,
 // which many rows share, come from L2.
 //
@@ -20,8 +22,9 @@
 //
 // Precision: bf16 operands, fp32 sums. What stands between two products (h, g) is
 // kept in fp32 and enters the second product as the bf16 pair hi + lo (2^-17
-// relative): an operand of 16 ranks fills half of an MFMA's 32 contraction
-// places, so the pair costs no further instruction. fp32 tensors run on fp32 MFMAs.
+// relative, where a bf16 result rounds by 2^-8): an operand of 16 ranks fills half of
+// an MFMA's 32 contraction places, so the pair costs no further instruction. fp32
+// tensors run on fp32 MFMAs.
 //
 // Times beside the kernels are of single launches on one MI355X, whose device copies
 // run at 5.1 TB/s (1 GiB) to 7 (within the last level's cache).
@@ -43,7 +46,9 @@ constexpr int kTile = 64;      // rows of a sorted tile
 constexpr int kFewTile = 16;   // rows of a tile that a workgroup finds itself
 constexpr int kFew = 256;      // rows up to which they do (a thread per row)
 constexpr int kMaxRank = 128;
-// Workgroups of a CU that the registers and LDS of their ranks' tiles of 16 allow.
+// Workgroups of a CU asked of the compiler, and counted on by Shares. The unaligned bf16
+// forms get there by spilling: 36 bytes a lane for RT = 1, 12 for RT = 4 (4,096 x 4,097 ->
+// 2,881, r = 16: 21 us, aligned 12).
 template <int RT> constexpr int kExpandPlaces = RT == 1 ? 4 : RT <= 4 ? 3 : 2;
 // The same of the weight gradients (fp32, 24 adapters of rank 8 on 2,422 rows, 6,552 and
 // 7,168 columns: 53 us with three, 65 with two).
@@ -253,7 +258,9 @@ __device__ __forceinline__ int few_tile(const Rows& a, int j, int* rows) {
 
 // ----------------------------------------------------------------- sort ----
 // A stable sort of the rows by adapter into tiles: 5.5 us for 300 rows, 6 for 4,096,
-// 9.5 for 16,384, with the weights' transposes 10; chains of dependent steps. Group L holds the rows without an
+// 9.7 for 16,384, with the weights' transposes 10; chains of dependent steps. Past
+// kOneLaunchRows every workgroup walks all parts' counts: 131,072 rows 4.8 + 7.5 us with
+// 32 adapters, 4.6 + 56 with 1,024 (128 parts of 1,025). Group L holds the rows without an
 // adapter. A workgroup places rounds of 1,024 rows of its part of the batch; what
 // lies before it, and the groups' sizes, it counts itself over the whole batch (64 KB
 // of ids at 16,384 rows, from L2: one launch where counting apart needs two) up to
@@ -476,7 +483,7 @@ lora_prepare(const int32_t* __restrict__ ids, int64_t M, int L, int64_t part, in
 // M = 8,192, K = 4,096, r = 16 17.7 us (67 MB, 3.8 TB/s), 4,096 x 7,168, r = 32 14.8
 // (59 MB, 4.0), 16,384 x 2,048, r = 64 31 (2.2; 22 where the launch before wrote its
 // 235 MB past the caches). A second round of x on its way, or twice the slices,
-// measured the same.
+// measured the same. fp32: 4,096 x 7,168, r = 32 35 (117 MB, 3.4), 8,192 x 4,096, r = 16 58.
 template <typename T> constexpr int kStepK = 256 / sizeof(T);  // contraction values a round
 
 template <typename T, int RT, bool VEC>
@@ -734,8 +741,10 @@ __device__ __forceinline__ void copy_rows(const int* tile_rows, int n_rows, int6
 // for right after a store. `out` may be `base`: a lane's values of it are read before
 // they are written, and no other lane uses them.
 //
-// HBM bound: M = 16,384, N = 7,168, r = 64 with a base 100 us (470 MB, 4.7 TB/s; a copy
-// of as much 87), r = 32 without one 51 (235 MB, 4.6), 4,096 x 4,096, r = 32 19 (67 MB).
+// HBM bound: M = 16,384, N = 7,168, r = 64 with a base 101 us (470 MB, 4.7 TB/s; a copy
+// of as much 87), r = 32 without one 53 (235 MB, 4.4). 4,096 x 4,096, r = 32 19 (67 MB,
+// 3.5 TB/s, where copies of that size run at 6.9: a tile's chunks begin with its ranks'
+// planes). fp32 35 (134 MB, 3.8).
 template <typename T, int RT, bool VEC>
 __global__ void __launch_bounds__(kThreads, kExpandPlaces<RT>)
 lora_expand(Rows rows, Ranks h, const T* __restrict__ b, int wide, const float* __restrict__ scaling,
@@ -975,9 +984,9 @@ lora_expand_few(Rows rows, Ranks h, const T* __restrict__ b, int wide, const flo
 // fall on distinct banks.
 //
 // Both gradients in one launch. HBM, two workgroups a CU (their sums and two tiles of
-// rows fill the registers): M = 8,192, K = 7,168, N = 4,096, r = 16 44 us (184 MB, 4.2 TB/s),
-// 16,384 x (7,168 of 8 bits + 2,048), r = 32 49 to 57 (184 MB, 3.2 to 3.8); 300 rows of
-// 2 x 2,880, r = 8 5.2.
+// rows fill the registers): M = 8,192, K = 7,168, N = 4,096, r = 16 43 us (184 MB, 4.3 TB/s;
+// fp32 99, 369 MB, 3.7), 16,384 x (7,168 of 8 bits + 2,048), r = 32 49 to 57 (184 MB, 3.2 to
+// 3.8); 300 rows of 2 x 2,880, r = 8 5.3.
 struct Side {
   const void* packed;      // [positions / 32, parts, RT, 64 lanes, 8] of T: u as operands
   const void* v;           // [M, C] of T, or e4m3 bytes with `scales`

@@ -21,8 +21,9 @@ class ActCheckpoint(NamedTuple):
 
 def act_checkpoint(x: torch.Tensor, *, backend: Backend | str = "auto") -> ActCheckpoint:
     """``x [M, K]`` (bf16, fp16 or fp32) in 8 bits. A block's scale is the least power of two
-    with which none of its finite values passes 448; values round to nearest even
-    (2^-4 of a value, or of the block's largest over 2^14 for the smallest). Infinities
+    with which none of its finite values passes 448; values round to nearest even, off by at
+    most 2^-4 of themselves or, the small ones, 2^-17 of the block's largest (2^-137 where
+    that largest is below 2^-119: the least scale). Infinities
     and NaN become NaN. No autograd graph is recorded (a warning, once, where ``x`` requires
     a gradient)."""
     return dispatch("act_checkpoint", x, backend=backend)

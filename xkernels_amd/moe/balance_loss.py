@@ -51,8 +51,9 @@ def moe_router_backward(
 ) -> torch.Tensor:
     """Gradient of the logits ``[M, E]`` (in their dtype) in one pass, from ``grad_weights
     [M, top_k]`` (of ``topk_softmax``'s weights, called with the same ``renormalize``),
-    ``grad_loss`` (of ``moe_balance_loss``, with its ``counts`` and ``tokens``; the counts
-    are constants) or both. Rows that ``mask`` leaves out get zeros.
+    ``grad_loss`` (of ``moe_balance_loss``, with its ``counts`` and ``tokens``, or sums of
+    them over parts of a batch, int32; the counts are constants) or both. Rows that ``mask``
+    leaves out get zeros.
     """
     return dispatch("moe_router_backward", gating_output, topk_ids, grad_weights=grad_weights,
                     renormalize=renormalize, grad_loss=grad_loss, counts=counts, tokens=tokens, mask=mask,
