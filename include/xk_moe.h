@@ -326,6 +326,59 @@ int xk_act_checkpoint(const void* x, int32_t dtype, int64_t ldx, int64_t M, int6
 int xk_act_restore(const uint8_t* values, const uint8_t* scales, int64_t M, int64_t K,
                    int32_t dtype, void* out, hipStream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * The dense gated feed-forward block beside the routed experts, in 16 bits:
+ *   g = x Wg^T, u = x Wu^T, h = silu(min(g, L)) * clamp(u, -L, L), out = h W2^T
+ * x [M, hidden] with rows ldx apart, w13 [2 ispp, hidden] (rows gate, then up) and
+ * w2 [hidden, ispp] contiguous, out [M, hidden] contiguous, one dtype (bf16 | fp16);
+ * swiglu_limit L <= 0: no clamp. gate_up [M, 2 ispp] (nullable) receives g and u, rounded
+ * to dtype but never across the limit. fp32 sums; h is rounded to dtype. x, w13 and w2
+ * are 16-byte aligned, ldx a multiple of 8 where hidden is, and at most 2,000,000;
+ * hidden <= 1,000,000, ispp <= 500,000, M < 2^29. workspace is 256-byte aligned.
+ * ------------------------------------------------------------------------- */
+int64_t xk_gated_ffn_workspace_bytes(int64_t M, int64_t hidden, int64_t ispp);
+int xk_gated_ffn(const void* x, int32_t dtype, int64_t ldx, int64_t M, int64_t hidden,
+                 const void* w13, const void* w2, int64_t ispp, float swiglu_limit, void* out,
+                 void* gate_up, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* Gradients of the above for grad_out [M, hidden] (rows ldg apart, as x): grad_x [M, hidden],
+ * grad_w13 [2 ispp, hidden], grad_w2 [hidden, ispp] of dtype, contiguous. gate_up as the
+ * forward left it, or NULL: computed again (`recompute` of the size query). The clamps pass the
+ * gradient where g <= L and |u| <= L. M = 0 gives weights' gradients of zero. */
+int64_t xk_gated_ffn_backward_workspace_bytes(int64_t M, int64_t hidden, int64_t ispp,
+                                              int32_t recompute);
+int xk_gated_ffn_backward(const void* grad_out, int32_t dtype, int64_t ldg, const void* x,
+                          int64_t ldx, int64_t M, int64_t hidden, const void* w13,
+                          const void* w2, int64_t ispp, const void* gate_up,
+                          float swiglu_limit, void* grad_x, void* grad_w13, void* grad_w2,
+                          void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Values in MXFP4, the format of xk_moe_mxfp4's weights: e2m1 codes, two a byte (the lower
+ * k in the low half), with one e8m0 byte for each 32 of a row, value = e2m1 *
+ * 2^(byte - 127). A row of K values is ceil(K / 32) whole blocks: codes [M, 16 ceil(K /
+ * 32)] (the last block filled up with zeros), scales [M, ceil(K / 32)]. The scale is the
+ * least power of two with which no value of the block passes 6, values round to nearest
+ * even; a block with an infinity or a NaN gets byte 255, NaN (which xk_moe_mxfp4 reads as 0).
+ * x [M, K] bf16 | fp32 | fp16 with rows ldx apart, K <= 2^22. Restored values that
+ * would pass the output type's largest finite value become that.
+ * ------------------------------------------------------------------------- */
+int xk_mxfp4_quantize(const void* x, int32_t dtype, int64_t ldx, int64_t M, int64_t K,
+                      uint8_t* codes, uint8_t* scales, hipStream_t stream);
+int xk_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K,
+                        int32_t dtype, void* out, hipStream_t stream);
+
+/* out [M, N] = x W^T (+ bias [N]) of MXFP4 operands in fp32 sums, rounded to out_dtype (bf16
+ * | fp32 | fp16; bias of it, nullable). w_codes and w_scales as above for [N, K]. x: values
+ * [M, K] of dtype with rows ldx apart, which are quantised as above first, or, with
+ * x_scales, codes of the same format (dtype and ldx unused). Codes are 16-byte
+ * aligned, scales 4-byte; K and N <= 1,000,000, M < 2^29. workspace is 256-byte aligned. */
+int64_t xk_mxfp4_linear_workspace_bytes(int64_t M, int64_t K, int64_t N);
+int xk_mxfp4_linear(const void* x, int32_t dtype, int64_t ldx, const uint8_t* x_scales,
+                    int64_t M, int64_t K, const uint8_t* w_codes, const uint8_t* w_scales,
+                    int64_t N, const void* bias, void* out, int32_t out_dtype,
+                    void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -5,7 +5,8 @@ Public ops (same names and signatures as ``xkernels``):
 ``moe_sum_reduce``, ``topk_softmax``; without a counterpart there, for tuning and
 serving over the frozen experts: ``moe_balance_loss``, ``moe_router_backward``,
 ``lora_projection``, ``lora_projection_backward``, ``act_checkpoint``,
-``act_restore``; harness: ``find_impl``, ``verify``, ``verify_parity``,
+``act_restore``; the dense block beside the experts: ``gated_ffn``,
+``gated_ffn_backward``, ``mxfp4_quantize``, ``mxfp4_dequantize``, ``mxfp4_linear``; harness: ``find_impl``, ``verify``, ``verify_parity``,
 ``backend_diagnostics``. The ops run hand-written HIP kernels from
 ``libxk_moe.so``; they raise if the library is missing or the tensors are not on
 the GPU.
@@ -19,10 +20,13 @@ from .moe import (
     MoeAlignWorkspace,
     MoeInt4Workspace,
     MoeMxfp4Workspace,
+    Mxfp4,
     act_checkpoint,
     act_restore,
     fused_moe_int4_w4a16,
     fused_moe_mxfp4,
+    gated_ffn,
+    gated_ffn_backward,
     lora_projection,
     lora_projection_backward,
     make_mxfp4_moe_weights,
@@ -31,6 +35,9 @@ from .moe import (
     moe_balance_loss,
     moe_router_backward,
     moe_sum_reduce,
+    mxfp4_dequantize,
+    mxfp4_linear,
+    mxfp4_quantize,
     topk_softmax,
 )
 from .retrieval import find_impl
@@ -42,6 +49,7 @@ __all__ = [
     "moe_align_block_size", "moe_sum_reduce", "topk_softmax", "make_w4a16_weights", "make_mxfp4_moe_weights",
     "moe_balance_loss", "moe_router_backward", "BalanceLoss", "lora_projection", "lora_projection_backward",
     "act_checkpoint", "act_restore", "ActCheckpoint",
+    "gated_ffn", "gated_ffn_backward", "mxfp4_quantize", "mxfp4_dequantize", "mxfp4_linear", "Mxfp4",
     "MoeAlignWorkspace", "MoeInt4Workspace", "MoeMxfp4Workspace", "find_impl", "verify",
     "verify_parity", "__version__",
 ]

@@ -97,6 +97,23 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "xk_act_checkpoint": (ctypes.c_int, [_p, _i32, _i64, _i64, _i64, _p, _p, _p]),
     "xk_act_restore": (ctypes.c_int, [_p, _p, _i64, _i64, _i32, _p, _p]),
+    "xk_gated_ffn_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "xk_gated_ffn": (
+        ctypes.c_int,
+        [_p, _i32, _i64, _i64, _i64, _p, _p, _i64, _f32, _p, _p, _p, _i64, _p],
+    ),
+    "xk_gated_ffn_backward_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32]),
+    "xk_gated_ffn_backward": (
+        ctypes.c_int,
+        [_p, _i32, _i64, _p, _i64, _i64, _i64, _p, _p, _i64, _p, _f32, _p, _p, _p, _p, _i64, _p],
+    ),
+    "xk_mxfp4_quantize": (ctypes.c_int, [_p, _i32, _i64, _i64, _i64, _p, _p, _p]),
+    "xk_mxfp4_dequantize": (ctypes.c_int, [_p, _p, _i64, _i64, _i32, _p, _p]),
+    "xk_mxfp4_linear_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "xk_mxfp4_linear": (
+        ctypes.c_int,
+        [_p, _i32, _i64, _p, _i64, _i64, _p, _p, _i64, _p, _p, _i32, _p, _i64, _p],
+    ),
 }
 
 _LIB: ctypes.CDLL | None = None

@@ -20,7 +20,8 @@ LIB = LIB_DIR / "libxk_moe.so"
 ARCH = "gfx950"
 
 SOURCES = ["capi.hip", "align.hip", "reduce.hip", "int4_gemm.hip", "int4_stream.hip", "int4_prefill.hip", "tile_gemm.hip", "small_batch.hip", "mxfp4_gemm.hip", "topk_softmax.hip",
-           "router_train.hip", "lora.hip", "mx8.hip", "capi_tuning.hip"]
+           "router_train.hip", "lora.hip", "mx8.hip", "capi_tuning.hip",
+           "gated_ffn.hip", "mx4.hip", "mxfp4_linear.hip", "capi_dense.hip"]
 
 # Packed-fp32 VALU ops are disabled for every device pass: the compiler must not
 # form v_pk_{add,mul,fma}_f32 from float code.

@@ -1,0 +1,313 @@
+// The gated feed-forward block in 16 bits and its gradients:
+//   g = x Wg^T, u = x Wu^T, h = silu(min(g, L)) clamp(u, -L, L), out = h W2^T
+//   dh = dy W2, gc = min(g, L), uc = clamp(u, -L, L), s = 1 / (1 + e^-gc)
+//   dg = dh uc s (1 + gc (1 - s)) [g <= L],  du = dh gc s [|u| <= L]
+//   dx = [dg du] W13,  dW13 = [dg du]^T x,  dW2 = dy^T h
+// Each product is one launch of the tile kernel; the activation runs in the epilogue of
+// the gate/up product, its gradient in that of dh. h, dg and du are rounded to the
+// type once, as operands of the next product: their roundings add up like those of the
+// outputs themselves.
+#include <algorithm>
+
+#include "dense_tile.h"
+
+namespace xk {
+namespace {
+
+using namespace dense;
+
+int64_t pad8(int64_t n) { return (n + 7) & ~int64_t(7); }
+int64_t aligned(int64_t bytes) { return (bytes + 255) & ~int64_t(255); }
+
+template <Form F> struct num;
+template <> struct num<Form::kBf16> {
+  typedef uint16_t type;
+  __device__ __forceinline__ static float get(uint16_t b) { return bf16_to_f32(b); }
+  __device__ __forceinline__ static uint16_t put(float f) { return f32_to_bf16(f); }
+};
+template <> struct num<Form::kFp16> {
+  typedef _Float16 type;
+  __device__ __forceinline__ static float get(_Float16 h) { return float(h); }
+  __device__ __forceinline__ static _Float16 put(float f) { return _Float16(f); }
+};
+
+// 4 consecutive values, of which n (any number) are within the row.
+template <typename T> struct four { T v[4]; };
+template <typename T> __device__ __forceinline__ void store_four(T* p, const four<T>& v, int64_t n) {
+  if (n >= 4) {
+    store_unaligned(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if (i < n) p[i] = v.v[i];
+  }
+}
+template <typename T> __device__ __forceinline__ four<T> load_four(const T* p, int64_t n) {
+  four<T> v;
+  if (n >= 4) {
+    v = load_unaligned<four<T>>(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v.v[i] = i < n ? p[i] : T(0);
+  }
+  return v;
+}
+
+// out[m, n] in the type.
+template <Form F> struct Store {
+  typename num<F>::type* out;
+  int64_t ld, M, N;
+  template <int WT, int XT>
+  __device__ __forceinline__ void operator()(const f32x4 (&acc)[WT][XT], int64_t m, int64_t n, int lane) const {
+    typedef typename num<F>::type T;
+    n += (lane >> 4) * 4;
+#pragma unroll
+    for (int b = 0; b < XT; ++b) {
+      const int64_t row = m + b * 16 + (lane & 15);
+      if (row >= M) continue;
+#pragma unroll
+      for (int a = 0; a < WT; ++a) {
+        four<T> v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v.v[i] = num<F>::put(acc[a][b][i]);
+        store_four(out + row * ld + n + a * 16, v, N - n - a * 16);
+      }
+    }
+  }
+};
+
+// A sum as gate_up holds it: rounded to the type, but never over the limit or back onto it,
+// so that the gradient passes where the sum itself let it.
+template <Form F> __device__ __forceinline__ typename num<F>::type held(float v, float limit) {
+  typedef typename num<F>::type T;
+  const T r = num<F>::put(v);
+  if (limit > 0.f) {
+    const bool past = fabsf(v) > limit, r_past = fabsf(num<F>::get(r)) > limit;
+    if (past != r_past && v == v) {  // one step away from zero, or towards it
+      const uint16_t b = __builtin_bit_cast(uint16_t, r);
+      return __builtin_bit_cast(T, uint16_t(past ? b + 1 : b - 1));
+    }
+  }
+  return r;
+}
+
+__device__ __forceinline__ float sigmoid(float g) { return 1.0f / (1.0f + __expf(-g)); }
+// min(g, L) and clamp(u, -L, L); NaN stays NaN
+__device__ __forceinline__ float below(float g, float limit) { return limit > 0.f && g > limit ? limit : g; }
+__device__ __forceinline__ float within(float u, float limit) {
+  return limit > 0.f && fabsf(u) > limit ? copysignf(limit, u) : u;
+}
+
+// h = silu(g) u, in rows ldh apart whose places past the I columns are zeros, and
+// gate_up [M, 2 I] (either may be null).
+template <Form F> struct Gate {
+  typename num<F>::type *h, *gate_up;
+  int64_t ldh, M, I;
+  float limit;
+  template <int WT, int XT>
+  __device__ __forceinline__ void operator()(const f32x4 (&acc)[WT][XT], int64_t m, int64_t n, int lane) const {
+    typedef typename num<F>::type T;
+    n += (lane >> 4) * 4;
+#pragma unroll
+    for (int b = 0; b < XT; ++b) {
+      const int64_t row = m + b * 16 + (lane & 15);
+      if (row >= M) continue;
+#pragma unroll
+      for (int a = 0; a < WT / 2; ++a) {
+        const int64_t j = n + a * 16;
+        four<T> g, u, v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float gs = acc[a][b][i], us = acc[a + WT / 2][b][i];
+          g.v[i] = held<F>(gs, limit);
+          u.v[i] = held<F>(us, limit);
+          const float gc = below(gs, limit), uc = within(us, limit);
+          v.v[i] = j + i < I ? num<F>::put(gc * sigmoid(gc) * uc) : T(0);
+        }
+        if (h != nullptr) store_four(h + row * ldh + j, v, ldh - j);
+        if (gate_up != nullptr) {
+          store_four(gate_up + row * 2 * I + j, g, I - j);
+          store_four(gate_up + row * 2 * I + I + j, u, I - j);
+        }
+      }
+    }
+  }
+};
+
+// From dh and gate_up [M, 2 I]: d [M, 2 I] = [dg du] and h [M, I], rows ldd and ldh apart with
+// zeros behind them.
+template <Form F> struct GateGrad {
+  const typename num<F>::type* gate_up;
+  typename num<F>::type *d, *h;
+  int64_t ldd, ldh, M, I;
+  float limit;
+  template <int WT, int XT>
+  __device__ __forceinline__ void operator()(const f32x4 (&acc)[WT][XT], int64_t m, int64_t n, int lane) const {
+    typedef typename num<F>::type T;
+    n += (lane >> 4) * 4;
+#pragma unroll
+    for (int b = 0; b < XT; ++b) {
+      const int64_t row = m + b * 16 + (lane & 15);
+      if (row >= M) continue;
+#pragma unroll
+      for (int a = 0; a < WT; ++a) {
+        const int64_t j = n + a * 16;
+        if (j >= I) continue;
+        const four<T> g = load_four(gate_up + row * 2 * I + j, I - j);
+        const four<T> u = load_four(gate_up + row * 2 * I + I + j, I - j);
+        four<T> dg, du, v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float gs = num<F>::get(g.v[i]), us = num<F>::get(u.v[i]), dh = acc[a][b][i];
+          const float gc = below(gs, limit), uc = within(us, limit), s = sigmoid(gc);
+          const bool on_g = !(limit > 0.f && gs > limit), on_u = !(limit > 0.f && fabsf(us) > limit);
+          dg.v[i] = num<F>::put(on_g ? dh * uc * s * (1.0f + gc * (1.0f - s)) : 0.f);
+          du.v[i] = num<F>::put(on_u ? dh * gc * s : 0.f);
+          v.v[i] = j + i < I ? num<F>::put(gc * s * uc) : T(0);
+        }
+        store_four(d + row * ldd + j, dg, I - j);
+        store_four(d + row * ldd + I + j, du, I - j);
+        store_four(h + row * ldh + j, v, ldh - j);
+        if (j + 4 >= I) {
+          for (int64_t c = 2 * I; c < ldd; ++c) d[row * ldd + c] = T(0);
+          for (int64_t c = j + 4; c < ldh; ++c) h[row * ldh + c] = T(0);
+        }
+      }
+    }
+  }
+};
+
+// Rows of n values, ld apart, to rows of n8 = pad8(n) with zeros behind them.
+__global__ void __launch_bounds__(256)
+pad_rows(const uint16_t* __restrict__ src, int64_t ld, int64_t rows, int64_t n, int64_t n8, uint16_t* __restrict__ dst) {
+  const int64_t pieces = n8 / 8, total = rows * pieces;
+  for (int64_t q = int64_t(blockIdx.x) * 256 + threadIdx.x; q < total; q += int64_t(gridDim.x) * 256) {
+    const int64_t row = q / pieces, k = (q - row * pieces) * 8;
+    const uint16_t* s = src + row * ld + k;
+    __attribute__((aligned(16))) uint16_t v[8];
+    if (k + 8 <= n) {
+      __builtin_memcpy(v, s, 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = k + i < n ? s[i] : uint16_t(0);
+    }
+    *reinterpret_cast<u32x4*>(dst + row * n8 + k) = *reinterpret_cast<const u32x4*>(v);
+  }
+}
+
+// A matrix [rows, n] of 16-bit values, rows ld apart, whose rows start at 16 bytes.
+struct Matrix {
+  const void* p;
+  int64_t rows, n, ld;
+  Side of_k() const { return Side{static_cast<const char*>(p), ld * 2, rows, nullptr, 0}; }
+  // its columns as the rows of an operand
+  Side columns() const { return Side{static_cast<const char*>(p), ld * 2, pad8(n), nullptr, 0}; }
+};
+
+// Takes the matrix as it is, or, where its width keeps rows from 16 bytes, as a copy with wider rows.
+Matrix take(const void* p, int64_t rows, int64_t n, int64_t ld, char*& ws, hipStream_t stream) {
+  if (n % 8 == 0) return Matrix{p, rows, n, ld};
+  const int64_t n8 = pad8(n);
+  uint16_t* to = reinterpret_cast<uint16_t*>(ws);
+  ws += aligned(rows * n8 * 2);
+  if (rows > 0) {
+    const int grid = int(std::min<int64_t>(cdiv(rows * n8 / 8, 256), 256 * 32));
+    hipLaunchKernelGGL(pad_rows, dim3(grid), dim3(256), 0, stream, static_cast<const uint16_t*>(p), ld, rows, n, n8, to);
+  }
+  return Matrix{to, rows, n, n8};
+}
+int64_t taken_bytes(int64_t rows, int64_t n) { return n % 8 == 0 ? 0 : aligned(rows * pad8(n) * 2); }
+
+// out = X W^T of k values a row
+Product product(const Side& x, const Side& w, int64_t M, int64_t N, int64_t k8, int64_t k_rows) {
+  Product p{};
+  p.x = x;
+  p.w = w;
+  p.M = M;
+  p.N = N;
+  p.k_bytes = k8 * 2;
+  p.k_rows = k_rows;
+  p.chunks = int(cdiv(std::max(k8, k_rows), 64));
+  return p;
+}
+
+template <Form F> void gate_up_product(const Matrix& x, const Matrix& w13, const Gate<F>& epi, hipStream_t stream) {
+  const int64_t I = epi.I;
+  launch_tile<F, Lay::kRowsOfK, Lay::kRowsOfK, 128, 128, 64, 64, true>(
+      product(x.of_k(), w13.of_k(), x.rows, I, pad8(x.n), 0), epi, stream);
+}
+
+template <Form F>
+int forward(const void* x, int64_t ldx, int64_t M, int64_t H, const void* w13, const void* w2, int64_t I, float limit,
+            void* out, void* gate_up, void* workspace, hipStream_t stream) {
+  typedef typename num<F>::type T;
+  char* ws = static_cast<char*>(workspace);
+  T* h = reinterpret_cast<T*>(ws);
+  ws += aligned(M * pad8(I) * 2);
+  const Matrix xm = take(x, M, H, ldx, ws, stream), m13 = take(w13, 2 * I, H, H, ws, stream),
+               m2 = take(w2, H, I, I, ws, stream);
+  const Matrix hm{h, M, I, pad8(I)};
+  gate_up_product<F>(xm, m13, Gate<F>{h, static_cast<T*>(gate_up), hm.ld, M, I, limit}, stream);
+  launch_tile<F, Lay::kRowsOfK, Lay::kRowsOfK, 128, 128, 64, 64, false>(
+      product(hm.of_k(), m2.of_k(), M, H, pad8(I), 0), Store<F>{static_cast<T*>(out), H, M, H}, stream);
+  XK_CHECK_LAUNCH("gated_ffn");
+  return XK_OK;
+}
+
+template <Form F>
+int backward(const void* dy, int64_t ldg, const void* x, int64_t ldx, int64_t M, int64_t H, const void* w13,
+             const void* w2, int64_t I, const void* gate_up, float limit, void* dx, void* dw13, void* dw2,
+             void* workspace, hipStream_t stream) {
+  typedef typename num<F>::type T;
+  char* ws = static_cast<char*>(workspace);
+  T* h = reinterpret_cast<T*>(ws);
+  ws += aligned(M * pad8(I) * 2);
+  T* d = reinterpret_cast<T*>(ws);
+  ws += aligned(M * pad8(2 * I) * 2);
+  const Matrix xm = take(x, M, H, ldx, ws, stream), m13 = take(w13, 2 * I, H, H, ws, stream),
+               m2 = take(w2, H, I, I, ws, stream), gm = take(dy, M, H, ldg, ws, stream);
+  const Matrix hm{h, M, I, pad8(I)}, dm{d, M, 2 * I, pad8(2 * I)};
+  if (M > 0) {
+    if (gate_up == nullptr) {
+      gate_up_product<F>(xm, m13, Gate<F>{nullptr, reinterpret_cast<T*>(ws), 0, M, I, limit}, stream);
+      gate_up = ws;
+    }
+    launch_tile<F, Lay::kRowsOfK, Lay::kColumns, 128, 128, 64, 64, false>(
+        product(gm.of_k(), m2.columns(), M, I, pad8(H), H),
+        GateGrad<F>{static_cast<const T*>(gate_up), d, h, dm.ld, hm.ld, M, I, limit}, stream);
+    launch_tile<F, Lay::kRowsOfK, Lay::kColumns, 128, 128, 64, 64, false>(
+        product(dm.of_k(), m13.columns(), M, H, pad8(2 * I), 2 * I), Store<F>{static_cast<T*>(dx), H, M, H}, stream);
+  }
+  launch_tile<F, Lay::kColumns, Lay::kColumns, 128, 128, 64, 64, false>(
+      product(dm.columns(), xm.columns(), 2 * I, H, 0, M), Store<F>{static_cast<T*>(dw13), H, 2 * I, H}, stream);
+  launch_tile<F, Lay::kColumns, Lay::kColumns, 128, 128, 64, 64, false>(
+      product(gm.columns(), hm.columns(), H, I, 0, M), Store<F>{static_cast<T*>(dw2), I, H, I}, stream);
+  XK_CHECK_LAUNCH("gated_ffn_backward");
+  return XK_OK;
+}
+
+}  // namespace
+
+int64_t gated_ffn_workspace_bytes(int64_t M, int64_t H, int64_t I) {
+  return aligned(M * pad8(I) * 2) + taken_bytes(M, H) + taken_bytes(2 * I, H) + taken_bytes(H, I);
+}
+int64_t gated_ffn_backward_workspace_bytes(int64_t M, int64_t H, int64_t I, int recompute) {
+  return gated_ffn_workspace_bytes(M, H, I) + aligned(M * pad8(2 * I) * 2) + taken_bytes(M, H) +
+         (recompute ? aligned(M * 2 * I * 2) : 0);
+}
+
+int launch_gated_ffn(const void* x, int dtype, int64_t ldx, int64_t M, int64_t H, const void* w13, const void* w2,
+                     int64_t I, float limit, void* out, void* gate_up, void* ws, hipStream_t stream) {
+  return dtype == XK_DT_BF16 ? forward<Form::kBf16>(x, ldx, M, H, w13, w2, I, limit, out, gate_up, ws, stream)
+                             : forward<Form::kFp16>(x, ldx, M, H, w13, w2, I, limit, out, gate_up, ws, stream);
+}
+
+int launch_gated_ffn_backward(const void* dy, int dtype, int64_t ldg, const void* x, int64_t ldx, int64_t M, int64_t H,
+                              const void* w13, const void* w2, int64_t I, const void* gate_up, float limit, void* dx,
+                              void* dw13, void* dw2, void* ws, hipStream_t stream) {
+  return dtype == XK_DT_BF16
+             ? backward<Form::kBf16>(dy, ldg, x, ldx, M, H, w13, w2, I, gate_up, limit, dx, dw13, dw2, ws, stream)
+             : backward<Form::kFp16>(dy, ldg, x, ldx, M, H, w13, w2, I, gate_up, limit, dx, dw13, dw2, ws, stream);
+}
+
+}  // namespace xk
