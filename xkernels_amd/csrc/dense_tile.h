@@ -4,17 +4,26 @@
 //   * Operands lie k-contiguous (kRowsOfK: [rows, k], as activations and weights do) or
 //     k by k (kColumns: [k, rows], as both operands of a weight's gradient do). Either
 //     way a chunk of 128 bytes of k a row (64 values of 16 bits, 256 of 4) comes to LDS
-//     by direct loads of 16 bytes a lane, double buffered.
+//     by direct loads of 16 bytes a lane.
 //   * LDS holds kRowsOfK chunks as rows of 8 pieces of 16 bytes, permuted by the row's
 //     low bits; an operand of v_mfma 16x16x32 (16 bits) or 16x16x128 (4 bits) is one
 //     ds_read_b128 either way, so the three formats share every address. kColumns chunks
 //     lie as [64 k][rows], units of 16 rows permuted by k, and are read through the
-//     transposing ds_read_b64_tr_b16.
+//     transposing ds_read_b64_tr_b16. Neither has bank conflicts.
+//   * A wave owns 64 rows x BN / 2 (or BN / 4) columns. While it multiplies one half of a
+//     chunk it reads the other half's fragments, W's into the registers that are done
+//     with, so the matrix unit waits for LDS only behind a barrier, of which there is one a
+//     chunk; and it issues the loads of later chunks between the products. X has three
+//     places in LDS and W two (160 KB at 256 x 256), so loads stay in flight across the
+//     barrier.
 //   * The W side is the MFMA's first operand, so a lane's four sums are consecutive n of
 //     one m, which the epilogue writes together.
 //   * Past a tensor's end the buffer loads give zeros; a row's last chunk, where it is
-//     short, is cut off lane by lane.
+//     short, is cut off lane by lane. Behind the last chunk the loop loads nothing in the
+//     same way, so it has one form.
 #pragma once
+
+#include <algorithm>
 
 #include "int4_common.h"
 
@@ -27,8 +36,8 @@ enum class Lay { kRowsOfK, kColumns };
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kChunk = 128;     // bytes of k a row and chunk
-constexpr int kCut = 1 << 30;   // added to an offset: past every buffer's end (records stay below)
+constexpr int kChunk = 128;    // bytes of k a row and chunk: two MFMAs'
+constexpr int kCut = 1 << 30;  // added to an offset: past every buffer's end (records stay below)
 
 // One side of the product, as the kernel reads it.
 struct Side {
@@ -43,133 +52,143 @@ __device__ __forceinline__ uint32_t records(int64_t bytes) {
   return bytes <= 0 ? 0u : uint32_t(bytes < kCut ? bytes : int64_t(kCut));
 }
 
-// 4-byte form of dma_16: lane i's 4 bytes land at lds + 4 i.
-__device__ __forceinline__ void dma_4(i32x4 rsrc, const void* lds, int voff, int soff) {
-  const uint32_t m0 = uniform(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)));
+// Direct-to-LDS loads: lane i's 16 (4) bytes from voff + soff land at LDS address `lds` + 16 i
+// (4 i), zeros where they are past the buffer. Inline assembly, as dma_16 is, with the
+// LDS address as the number that it is. The kernel waits for them itself.
+__device__ __forceinline__ void to_lds_16(i32x4 rsrc, uint32_t lds, int voff, int soff) {
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :
+               : "s"(uniform(lds)), "v"(voff), "s"(rsrc), "s"(uniform(soff))
+               : "memory", "m0");
+}
+__device__ __forceinline__ void to_lds_4(i32x4 rsrc, uint32_t lds, int voff, int soff) {
   asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, %3 offen lds"
                :
-               : "s"(m0), "v"(voff), "s"(rsrc), "s"(uniform(soff))
+               : "s"(uniform(lds)), "v"(voff), "s"(rsrc), "s"(uniform(soff))
                : "memory", "m0");
 }
 
-// Which row of an operand lies in LDS row r of a tile that starts at r0.
-struct Straight {
-  static constexpr bool kPaired = false;
-};
-// Gate and up rows of one weight [2 half, k]: of each wave's WAVE rows the first half are gate
-// rows, the other the up rows of the same columns, so both sums of a column meet in a lane.
-template <int WAVE> struct Paired {
-  static constexpr bool kPaired = true;
-  static constexpr int kWave = WAVE;
+// Chunks [first, end) of `all` that a launch's slice works on.
+struct Range {
+  int first, end, all;
 };
 
-template <Form F, Lay L, int ROWS, int WAVES, typename MAP = Straight> struct Loader {
+// Loads one side's chunks. PAIR: the rows of W are gate and up rows of one weight [2 half, k]: of
+// each PAIR rows in LDS (a wave's) the first half are gate rows, the other the up rows of
+// the same columns, so both sums of a column meet in a lane. 0: rows as they come.
+template <Form F, Lay L, int ROWS, int WAVES, int PAIR = 0> struct Loader {
   static constexpr int kBytes = ROWS * kChunk;
   static constexpr int kInstr = ROWS * kChunk / 1024 / WAVES;  // loads of 1 KiB a wave and chunk
   static constexpr int kPitch = L == Lay::kRowsOfK ? kChunk : 2 * ROWS;
   static constexpr int kKRows = 64;  // k of a kColumns chunk
-  static_assert(kInstr >= 1, "a wave loads 1 KiB at a time");
-  static_assert(L == Lay::kRowsOfK || (F != Form::kFp4 && ROWS >= 128), "kColumns: 16 bits, 8 units a row");
+  static_assert(kInstr * 1024 * WAVES == kBytes, "a wave loads 1 KiB at a time");
+  static_assert(L == Lay::kRowsOfK || (F != Form::kFp4 && kInstr == 4 && (ROWS == 256 || ROWS == 128)), "kColumns: 16 bits");
 
+  i32x4 rsrc, up;     // up: PAIR's up rows; kColumns: 4 k further
+  int soff;           // kRowsOfK: k of the chunk. kColumns: the descriptor moves on
+  int left;           // kRowsOfK: pieces of 16 bytes left of a row. kColumns: chunks left,
+  uint32_t last;      // and the records of the last one
   const char* base;
-  const char* base2;  // Paired: the up rows
-  int64_t left, left2, step;
-  int off[kInstr], piece;
+  int64_t step;
+  // kColumns: a lane's places 4 k apart differ by no more than that
+  static constexpr int kBit = ROWS == 256 ? 2 : 1;  // of i, that says which of the two
+  static constexpr int kOff = L == Lay::kRowsOfK ? kInstr : kInstr / 2;
+  int off[kOff], piece;
 
-  // `half`: Paired: the rows of a half.
-  // `extent`: the side's k, in bytes of a row (kRowsOfK) or a number (kColumns)
-  __device__ __forceinline__ void init(const Side& s, int64_t r0, int64_t extent, int64_t k0, int wave, int lane,
+  // `extent`: the side's k, in bytes of a row (kRowsOfK) or a number (kColumns); `half`: PAIR's.
+  __device__ __forceinline__ void init(const Side& s, int64_t r0, int64_t extent, Range c, int wave, int lane,
                                        int64_t half = 0) {
     if constexpr (L == Lay::kRowsOfK) {
       piece = (lane & 7) ^ (lane >> 3);
-      base = s.p + r0 * s.ld + k0 * kChunk;
-      const int64_t rows = MAP::kPaired ? half : s.rows;
-      left = (rows - 1 - r0) * s.ld + extent - k0 * kChunk;
-      if constexpr (MAP::kPaired) {
-        base2 = base + half * s.ld;
-        left2 = left;
-      }
-      step = kChunk;
+      // (a row past the last starts past the end, whatever the chunk)
+      const uint32_t n = records(((PAIR ? half : s.rows) - 1 - r0) * s.ld + extent);
+      rsrc = make_rsrc(s.p + r0 * s.ld, n);
+      if constexpr (PAIR != 0) up = make_rsrc(s.p + (r0 + half) * s.ld, n);
+      soff = c.first * kChunk;
+      left = min(int(extent >> 4), c.end * 8) - c.first * 8;
 #pragma unroll
       for (int i = 0; i < kInstr; ++i) {
         int row = (wave * kInstr + i) * 8 + (lane >> 3);
-        if constexpr (MAP::kPaired) row = row / MAP::kWave * (MAP::kWave / 2) + row % (MAP::kWave / 2);
+        if constexpr (PAIR != 0) row = row / PAIR * (PAIR / 2) + row % (PAIR / 2);
         off[i] = int(row * s.ld) + piece * 16;
       }
     } else {
-      piece = 0;
-      base = s.p + r0 * 2 + k0 * kKRows * s.ld;
-      left = (extent - 1 - k0 * kKRows) * s.ld + (s.rows - r0) * 2;
+      piece = soff = 0;
+      base = s.p + r0 * 2 + int64_t(c.first) * kKRows * s.ld;
       step = kKRows * s.ld;
+      // (all that a chunk before the tensor's last reads lies before the tensor's end)
+      left = c.end - c.first;
+      last = c.end < c.all ? uint32_t(kCut)
+                           : records((extent - 1 - int64_t(c.end - 1) * kKRows) * s.ld + (s.rows - r0) * 2);
+      describe();
 #pragma unroll
-      for (int i = 0; i < kInstr; ++i) {
+      for (int j = 0; j < kOff; ++j) {
+        const int i = kBit == 2 ? j : 2 * j;
         const int at = ((wave * kInstr + i) * 64 + lane) * 16, k = at / kPitch, unit = at % kPitch / 32;
-        off[i] = int(k * s.ld) + (unit ^ flip(k)) * 32 + (at & 16);
+        off[j] = int(k * s.ld) + (unit ^ flip(k)) * 32 + (at & 16);
       }
     }
+  }
+  __device__ __forceinline__ void describe() {
+    const uint32_t n = left > 1 ? uint32_t(kCut) : left == 1 ? last : 0u, four = uint32_t(4 * step / kKRows);
+    rsrc = make_rsrc(base, n);
+    up = make_rsrc(base + four, n > four ? n - four : 0u);
   }
   // which way the 32-byte units of k are permuted: the 8 k of a half wave's transposing read
   // (0 .. 3 and 8 .. 11 of 16) fall on all banks
   __device__ __forceinline__ static int flip(int k) { return (k & 3) | ((k >> 1) & 4); }
 
-  // Issues the next chunk's loads to `lds`; `cut` (kRowsOfK): pieces left of a short chunk, else 8.
-  __device__ __forceinline__ void issue(char* lds, int wave, int cut) {
-    const i32x4 r = make_rsrc(base, records(left));
-    i32x4 r2;
-    if constexpr (MAP::kPaired) r2 = make_rsrc(base2, records(left2));
-#pragma unroll
-    for (int i = 0; i < kInstr; ++i) {
-      int o = off[i];
-      if (L == Lay::kRowsOfK && cut < 8) o |= piece >= cut ? kCut : 0;
-      char* at = lds + (wave * kInstr + i) * 1024;
-      if constexpr (MAP::kPaired) {
-        const bool up = (wave * kInstr + i) * 8 % MAP::kWave >= MAP::kWave / 2;
-        dma_16(up ? r2 : r, at, o, 0);
-      } else {
-        dma_16(r, at, o, 0);
-      }
+  // Load i of the next chunk to the wave's place in LDS.
+  __device__ __forceinline__ void issue(uint32_t lds, int wave, int i) {
+    if constexpr (L == Lay::kColumns) {
+      to_lds_16(i & kBit ? up : rsrc, lds + i * 1024, off[kBit == 2 ? i & 1 : i >> 1], 0);
+      return;
     }
-    base += step;
-    left -= step;
-    if constexpr (MAP::kPaired) {
-      base2 += step;
-      left2 -= step;
+    const int o = off[i < kOff ? i : 0] | (piece >= left ? kCut : 0);
+    if (PAIR != 0 && (wave * kInstr + i) * 8 % (PAIR ? PAIR : 1) >= PAIR / 2) to_lds_16(up, lds + i * 1024, o, soff);
+    else to_lds_16(rsrc, lds + i * 1024, o, soff);
+  }
+  __device__ __forceinline__ void advance() {
+    if constexpr (L == Lay::kRowsOfK) {
+      soff += kChunk;
+      left -= 8;
+    } else {
+      base += step;
+      --left;
+      describe();
     }
   }
 };
 
-// The scales of an MXFP4 operand: 8 bytes a row and chunk.
+// The scales of an MXFP4 operand: 8 bytes a row and chunk, in loads of 256 bytes for 32 rows.
 template <int ROWS, int WAVES> struct ScaleLoader {
   static constexpr int kBytes = ROWS * 8;
-  static constexpr int kTotal = ROWS / 32;  // loads of 256 bytes
-  static constexpr int kInstr = (kTotal + WAVES - 1) / WAVES;
-  const uint8_t* base;
-  int64_t left;
-  int off[kInstr], word;
-  __device__ __forceinline__ void init(const Side& s, int64_t r0, int64_t blocks, int64_t k0, int wave, int lane) {
+  static constexpr int kLoads = ROWS / 32;
+  static_assert(kLoads <= WAVES, "at most a load a wave");
+  i32x4 rsrc;
+  int soff, off, word, left;
+  __device__ __forceinline__ void init(const Side& s, int64_t r0, int64_t blocks, Range c, int wave, int lane) {
     word = lane & 1;
-    base = s.s + r0 * s.lds + k0 * 8;
-    left = (s.rows - 1 - r0) * s.lds + (blocks + 3) / 4 * 4 - k0 * 8;
-#pragma unroll
-    for (int i = 0; i < kInstr; ++i) off[i] = int(((wave * kInstr + i) * 32 + (lane >> 1)) * s.lds) + word * 4;
+    rsrc = make_rsrc(s.s + r0 * s.lds, records((s.rows - 1 - r0) * s.lds + (blocks + 3) / 4 * 4));
+    off = int((wave * 32 + (lane >> 1)) * s.lds) + word * 4;
+    soff = c.first * 8;
+    left = min(int((blocks + 3) >> 2), c.end * 2) - c.first * 2;
   }
-  // `cut`: words left of a short chunk, else 2
-  __device__ __forceinline__ void issue(char* lds, int wave, int cut) {
-    const i32x4 r = make_rsrc(base, records(left));
-#pragma unroll
-    for (int i = 0; i < kInstr; ++i)
-      if (wave * kInstr + i < kTotal) dma_4(r, lds + (wave * kInstr + i) * 256, off[i] | (word >= cut ? kCut : 0), 0);
-    base += 8;
-    left -= 8;
+  __device__ __forceinline__ void issue(uint32_t lds, int wave) {
+    if (wave < kLoads) to_lds_4(rsrc, lds, off | (word >= left ? kCut : 0), soff);
+    soff += 8;
+    left -= 2;
   }
 };
 
-// One operand fragment: 16 rows, step s of 2 of a chunk.
+// One operand fragment: 16 rows, step S of 2 of a chunk.
 template <Form F, Lay L, int ROWS> struct Reader {
   static constexpr int kPitch = L == Lay::kRowsOfK ? kChunk : 2 * ROWS;
-  int at0, at1;  // kRowsOfK: of each step; kColumns: at0, to which a fragment's unit is xored
+  int at0, at1;  // kRowsOfK: of each step; kColumns: of a unit's first byte, and the way units are permuted
+  int unit;
   __device__ __forceinline__ void init(int row0, int lane) {
     const int c = lane & 15, q = lane >> 4;
+    unit = row0 >> 4;
     if constexpr (L == Lay::kRowsOfK) {
       // 16 bits: step s reads piece 4 s + q, 4 bits: block 2 q + s (any order of k will do that
       // both operands share)
@@ -177,18 +196,22 @@ template <Form F, Lay L, int ROWS> struct Reader {
       at0 = (row0 + c) * kChunk + ((p0 ^ (c & 7)) << 4);
       at1 = (row0 + c) * kChunk + ((p1 ^ (c & 7)) << 4);
     } else {
-      at0 = (8 * q + (c >> 2)) * kPitch + (((row0 >> 4) ^ ((c >> 2) | (q & 1) << 2)) << 5) + (c & 3) * 8;
-      at1 = 0;
+      at0 = (8 * q + (c >> 2)) * kPitch + (c & 3) * 8;
+      at1 = ((c >> 2) | (q & 1) << 2) << 5;
     }
   }
-  // fragment t (row0 + 16 t .. + 15); row0 is a multiple of 16 times the wave's fragments
-  __device__ __forceinline__ u32x4 read(const char* lds, int t, int s) const {
+  // Keeps the compiler from holding every fragment's address in registers over the loop.
+  __device__ __forceinline__ void forget() {
+    if constexpr (L == Lay::kColumns) asm volatile("" : "+v"(at1));
+  }
+  // fragment t: rows row0 + 16 t .. + 15
+  template <int S> __device__ __forceinline__ u32x4 read(const char* lds, int t) const {
     if constexpr (L == Lay::kRowsOfK) {
-      return *reinterpret_cast<const u32x4*>(lds + (s ? at1 : at0) + t * 16 * kChunk);
+      return *reinterpret_cast<const u32x4*>(lds + (S ? at1 : at0) + t * 16 * kChunk);
     } else {
       typedef short s4 __attribute__((ext_vector_type(4)));
       typedef __attribute__((address_space(3))) s4 lds_s4;
-      const char* p = lds + (at0 ^ (t << 5)) + s * 32 * kPitch;
+      const char* p = lds + at0 + (((unit + t) << 5) ^ at1) + S * 32 * kPitch;
       const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)p);
       const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + 4 * kPitch));
       return __builtin_bit_cast(u32x4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -211,21 +234,21 @@ template <int S> __device__ __forceinline__ f32x4 mma4(u32x4 w, uint32_t ws, u32
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, S, int(ws), S, int(xs));
 }
 
-// What a launch works on. Grid: tiles of the product, one after the other.
+// What a launch works on.
 struct Product {
   Side x, w;
-  int64_t M, N;      // N: of the output's columns (Paired: those of a half)
+  int64_t M, N;      // N: of the output's columns (pairs: those of a half)
   int64_t k_bytes;   // of a row of a kRowsOfK side (a multiple of 16)
   int64_t k_rows;    // of a kColumns side: the number of k
   int64_t blocks;    // MXFP4: blocks of a row
   int chunks;        // of k
-  int tiles_m, tiles_n;
+  int tiles_m, tiles_n, slices;
 };
 
 // Tile `id` of the launch: XCD i (workgroups go round the 8 of them) takes a run of
 // consecutive tiles, ordered in bands of kBand row tiles, so that its 4 MB of L2 sees few
 // rows of X and W at a time.
-constexpr int kBand = 8;
+constexpr int kBand = 4;
 __device__ __forceinline__ void tile_of(int id, int total, int tiles_m, int tiles_n, int& tm, int& tn) {
   const int xcd = id & 7, local = id >> 3, share = total >> 3, rest = total & 7;
   const int t = xcd * share + min(xcd, rest) + local;
@@ -235,101 +258,303 @@ __device__ __forceinline__ void tile_of(int id, int total, int tiles_m, int tile
   tm = band * kBand + in - tn * height;
 }
 
-// EPI: struct with `template <int WT, int XT> void operator()(const f32x4 (&acc)[WT][XT], int64_t m, int64_t n, int lane)`:
-// the sums of the wave's rows m .. and columns n .. (fragment t of either side 16 t further, Paired: n of
-// the gate's first half of the fragments).
-template <Form F, Lay LX, Lay LW, int BM, int BN, int WM, int WN, bool PAIRED, typename EPI>
-__global__ void __launch_bounds__(BM / WM * (BN / WN) * 64)
+// EPI: struct with `void operator()(int64_t m, int64_t n, f32x4 v)`, the sums of row m and columns n .. n + 3, or,
+// for pairs, `void operator()(int64_t m, int64_t j, f32x4 g, f32x4 u)`; either may lie past the output's
+// last column, not its last row. n and j are multiples of 4. blockIdx.y is the slice of k.
+template <Form F, Lay LX, Lay LW, int BM, int BN, int WAVES_N, bool PAIRED, typename EPI>
+__global__ void __launch_bounds__(BM / 64 * WAVES_N * 64)
 dense_tile(Product p, EPI epi) {
-  constexpr int WAVES = BM / WM * (BN / WN), XT = WM / 16, WT = WN / 16;
+  constexpr int WAVES = BM / 64 * WAVES_N, WN = BN / WAVES_N, XT = 4, WT = WN / 16;
   constexpr bool FP4 = F == Form::kFp4;
+  // (224 columns are loaded as 256: whole loads for every wave)
+  constexpr int W_ROWS = BN == 224 ? 256 : BN;
+  static_assert(!PAIRED || BN == W_ROWS, "pairs: whole tiles");
   using XLoad = Loader<F, LX, BM, WAVES>;
-  using WLoad = Loader<F, LW, BN, WAVES, std::conditional_t<PAIRED, Paired<WN>, Straight>>;
+  using WLoad = Loader<F, LW, W_ROWS, WAVES, PAIRED ? WN : 0>;
   using XScale = ScaleLoader<BM, WAVES>;
-  using WScale = ScaleLoader<BN, WAVES>;
-  constexpr int STAGE = XLoad::kBytes + WLoad::kBytes + (FP4 ? XScale::kBytes + WScale::kBytes : 0);
-  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
+  using WScale = ScaleLoader<W_ROWS, WAVES>;
+  // X lies in three places in turn, W in two: while chunk c is read, W of c + 1 and X of c + 1
+  // and c + 2 are on their way, so the loads never run dry. (4 bits: the scales leave X two.)
+  constexpr int XRING = FP4 ? 2 : 3, XI = XLoad::kInstr, WI = WLoad::kInstr;
+  constexpr int W_AT = XRING * XLoad::kBytes, S_AT = W_AT + 2 * WLoad::kBytes;
+  constexpr int SCALES = FP4 ? XScale::kBytes + WScale::kBytes : 0;
+  __shared__ __attribute__((aligned(1024))) char lds[S_AT + 2 * SCALES];
   const int lane = threadIdx.x & 63, wave = uniform(int(threadIdx.x) >> 6);
-  const int wn = wave % (BN / WN), wm = wave / (BN / WN);
+  const int wn = wave % WAVES_N, wm = wave / WAVES_N;
   int tm, tn;
   tile_of(blockIdx.x, gridDim.x, p.tiles_m, p.tiles_n, tm, tn);
   const int64_t m0 = int64_t(tm) * BM, n0 = int64_t(tn) * (PAIRED ? BN / 2 : BN);
+  const int y = blockIdx.y, share = p.chunks / p.slices, rest = p.chunks - share * p.slices;
+  Range range;
+  range.first = y * share + min(y, rest);
+  range.end = range.first + share + (y < rest);
+  range.all = p.chunks;
 
   XLoad xl;
   WLoad wl;
-  xl.init(p.x, m0, LX == Lay::kRowsOfK ? p.k_bytes : p.k_rows, 0, wave, lane);
-  wl.init(p.w, n0, LW == Lay::kRowsOfK ? p.k_bytes : p.k_rows, 0, wave, lane, p.N);
+  xl.init(p.x, m0, LX == Lay::kRowsOfK ? p.k_bytes : p.k_rows, range, wave, lane);
+  wl.init(p.w, n0, LW == Lay::kRowsOfK ? p.k_bytes : p.k_rows, range, wave, lane, p.N);
   XScale xsl;
   WScale wsl;
   if constexpr (FP4) {
-    xsl.init(p.x, m0, p.blocks, 0, wave, lane);
-    wsl.init(p.w, n0, p.blocks, 0, wave, lane);
+    xsl.init(p.x, m0, p.blocks, range, wave, lane);
+    wsl.init(p.w, n0, p.blocks, range, wave, lane);
   }
-  auto issue = [&](int i) __attribute__((always_inline)) {
-    char* at = lds + (i & 1) * STAGE;
-    const int64_t left = LX == Lay::kRowsOfK ? p.k_bytes - int64_t(i) * kChunk : kChunk;
-    const int cut = left < kChunk ? int(left >> 4) : 8;
-    xl.issue(at, wave, cut);
-    wl.issue(at + XLoad::kBytes, wave, cut);
-    if constexpr (FP4) {
-      const int words = left < kChunk ? int((p.blocks - int64_t(i) * 8 + 3) >> 2) : 2;
-      xsl.issue(at + XLoad::kBytes + WLoad::kBytes, wave, words);
-      wsl.issue(at + XLoad::kBytes + WLoad::kBytes + XScale::kBytes, wave, words);
-    }
+  // the next loads' places
+  const uint32_t lds0 = uniform(uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds)));
+  const uint32_t x_to = lds0 + wave * XI * 1024, w_to = lds0 + W_AT + wave * WI * 1024, s_to = lds0 + S_AT + wave * 256;
+  int x_at = 0, w_at = 0, s_at = 0;
+  auto issue_x = [&](int i) __attribute__((always_inline)) { xl.issue(x_to + x_at, wave, i); };
+  auto issue_w = [&](int i) __attribute__((always_inline)) { wl.issue(w_to + w_at, wave, i); };
+  auto issue_s = [&]() __attribute__((always_inline)) {
+    xsl.issue(s_to + s_at, wave);
+    wsl.issue(s_to + s_at + XScale::kBytes, wave);
+    s_at ^= SCALES;
+  };
+  auto next_x = [&]() __attribute__((always_inline)) {
+    xl.advance();
+    x_at = x_at == (XRING - 1) * XLoad::kBytes ? 0 : x_at + XLoad::kBytes;
+  };
+  auto next_w = [&]() __attribute__((always_inline)) {
+    wl.advance();
+    w_at = WLoad::kBytes - w_at;
   };
   Reader<F, LX, BM> xr;
-  Reader<F, LW, BN> wr;
-  xr.init(wm * WM, lane);
+  Reader<F, LW, W_ROWS> wr;
+  xr.init(wm * 64, lane);
   wr.init(wn * WN, lane);
+  const int sx_at = S_AT + (wm * 64 + (lane & 15)) * 8 + (lane >> 4) * 2,
+            sw_at = S_AT + XScale::kBytes + (wn * WN + (lane & 15)) * 8 + (lane >> 4) * 2;
 
   f32x4 acc[WT][XT];
 #pragma unroll
   for (int a = 0; a < WT; ++a)
 #pragma unroll
     for (int b = 0; b < XT; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // Fragments of the step at hand and, as its W fragments are used up, of the next. W's last one
+  // has places of its own in both steps, so that every read is out well before a barrier.
+  constexpr int KEEP = WT - 1;
+  u32x4 wf[KEEP], we[2], xf[2][XT];
+  uint32_t ws[WT], xs[XT], xsn[XT];
+  int cx = 0, cw = 0, cs = 0;  // where the chunk to read lies
 
-  if (p.chunks > 0) issue(0);
-  for (int i = 0; i < p.chunks; ++i) {
-    // chunk i has landed, and every wave has read chunk i - 1, whose place chunk i + 1 takes
-    XK_WAIT_VMCNT(0);
-    lds_sync();
-    if (i + 1 < p.chunks) issue(i + 1);
-    const char* xb = lds + (i & 1) * STAGE;
-    const char* wb = xb + XLoad::kBytes;
-    uint32_t xs[XT], ws[WT];
-    if constexpr (FP4) {
-      const char* sb = wb + WLoad::kBytes + (lane & 15) * 8 + (lane >> 4) * 2;
+  // Step S of the chunk in registers, while step 1 - S is read: of the same chunk (S = 0), or of
+  // the next one (S = 1); W of the chunk after that (S = 1) and X of one more (S = 0) go out.
+  auto step = [&](auto STEP, auto READ, auto MATH) __attribute__((always_inline)) {
+    constexpr int s = decltype(STEP)::value, n = 1 - s;
+    constexpr bool read = decltype(READ)::value, math = decltype(MATH)::value;
+    const char* xb = lds + cx;
+    const char* wb = lds + W_AT + cw;
+    auto w_of = [&](int a) __attribute__((always_inline)) -> u32x4& { return a < KEEP ? wf[a] : we[s]; };
+    if constexpr (read) {
+      xr.forget();
+      wr.forget();
 #pragma unroll
-      for (int b = 0; b < XT; ++b) xs[b] = *reinterpret_cast<const uint16_t*>(sb + (wm * WM + b * 16) * 8);
+      for (int b = 0; b < XT; ++b) xf[n][b] = xr.template read<n>(xb, b);
+      if constexpr (FP4 && n == 0) {
 #pragma unroll
-      for (int a = 0; a < WT; ++a)
-        ws[a] = *reinterpret_cast<const uint16_t*>(sb + XScale::kBytes + (wn * WN + a * 16) * 8);
+        for (int b = 0; b < XT; ++b) xsn[b] = *reinterpret_cast<const uint16_t*>(lds + cs + sx_at + b * 128);
+      }
+      we[n] = wr.template read<n>(wb, KEEP);
     }
-    static_for<2>([&](auto S) __attribute__((always_inline)) {
-      constexpr int s = decltype(S)::value;
-      u32x4 wf[WT], xf[XT];
 #pragma unroll
-      for (int a = 0; a < WT; ++a) wf[a] = wr.read(wb, a, s);
+    for (int a = 0; a < WT; ++a) {
+      if constexpr (math) {
 #pragma unroll
-      for (int b = 0; b < XT; ++b) xf[b] = xr.read(xb, b, s);
-#pragma unroll
-      for (int b = 0; b < XT; ++b)
-#pragma unroll
-        for (int a = 0; a < WT; ++a) {
-          if constexpr (FP4) acc[a][b] = mma4<s>(wf[a], ws[a], xf[b], xs[b], acc[a][b]);
-          else acc[a][b] = mma<F>(wf[a], xf[b], acc[a][b]);
+        for (int b = 0; b < XT; ++b) {
+          if constexpr (FP4) acc[a][b] = mma4<s>(w_of(a), ws[a], xf[s][b], xs[b], acc[a][b]);
+          else acc[a][b] = mma<F>(w_of(a), xf[s][b], acc[a][b]);
         }
-    });
+      }
+      if constexpr (read && s == 1) {
+        if (FP4 && a == 0) issue_s();
+#pragma unroll
+        for (int i = a * WI / WT; i < (a + 1) * WI / WT; ++i) issue_w(i);
+      }
+      if constexpr (read && s == (XRING == 2)) {
+#pragma unroll
+        for (int i = a * XI / WT; i < (a + 1) * XI / WT; ++i) issue_x(i);
+      }
+      if constexpr (read) {
+        if (a < KEEP) wf[a] = wr.template read<n>(wb, a);
+        if constexpr (FP4 && n == 0) ws[a] = *reinterpret_cast<const uint16_t*>(lds + cs + sw_at + a * 128);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (FP4 && read && n == 0) {
+#pragma unroll
+      for (int b = 0; b < XT; ++b) xs[b] = xsn[b];
+    }
+    if constexpr (read && s == 1) next_w();
+    if constexpr (read && s == (XRING == 2)) next_x();
+  };
+  // Behind it: all of the next chunk has landed, for every wave, and every wave has read the
+  // one before it.
+  auto publish = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_sched_barrier(0);
+    XK_WAIT_VMCNT(XRING == 2 ? 0 : XI);
+    lds_sync();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto turn = [&]() __attribute__((always_inline)) {  // to the next chunk's places
+    cx = cx == (XRING - 1) * XLoad::kBytes ? 0 : cx + XLoad::kBytes;
+    cw = WLoad::kBytes - cw;
+    cs ^= SCALES;
+  };
+  constexpr std::integral_constant<int, 0> S0{};
+  constexpr std::integral_constant<int, 1> S1{};
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
+  const int C = range.end - range.first;
+  if (C > 0) {
+#pragma unroll
+    for (int i = 0; i < XI; ++i) issue_x(i);
+    next_x();
+#pragma unroll
+    for (int i = 0; i < WI; ++i) issue_w(i);
+    next_w();
+    if constexpr (FP4) issue_s();
+    if constexpr (XRING == 3) {
+#pragma unroll
+      for (int i = 0; i < XI; ++i) issue_x(i);
+      next_x();
+    }
+    publish();
+    // chunk c's turn: step 1 of c - 1 and step 0 of c, reading both steps of c
+    step(S1, yes, no);
+    step(S0, yes, yes);
+    publish();
+    turn();
+    for (int c = 1; c < C; ++c) {
+      step(S1, yes, yes);
+      step(S0, yes, yes);
+      publish();
+      turn();
+    }
+    step(S1, no, yes);
+    XK_WAIT_VMCNT(0);  // no load may land in what is another workgroup's LDS by then
   }
-  epi(acc, m0 + wm * WM, n0 + wn * (PAIRED ? WN / 2 : WN), lane);
+
+  const int64_t m = m0 + wm * 64 + (lane & 15), n = n0 + wn * (PAIRED ? WN / 2 : WN) + (lane >> 4) * 4;
+#pragma unroll
+  for (int b = 0; b < XT; ++b) {
+    if (m + b * 16 >= p.M) continue;
+    if constexpr (PAIRED) {
+#pragma unroll
+      for (int a = 0; a < WT / 2; ++a) epi(m + b * 16, n + a * 16, acc[a][b], acc[a + WT / 2][b]);
+    } else {
+#pragma unroll
+      for (int a = 0; a < WT; ++a) epi(m + b * 16, n + a * 16, acc[a][b]);
+    }
+  }
 }
 
-template <Form F, Lay LX, Lay LW, int BM, int BN, int WM, int WN, bool PAIRED, typename EPI>
-void launch_tile(Product p, const EPI& epi, hipStream_t stream) {
+// ---------------------------------------------------------------- launches ----
+
+// How a product is cut up.
+struct Plan {
+  int cols;    // of a tile: 256 or 224 (with 256 rows), 128 (with 128)
+  int slices;  // of k, whose sums another launch adds up
+};
+
+// The cheapest of the tiles and slices, in microseconds as measured (16 bits; MXFP4):
+//   * 256 x 256, a workgroup a CU: 1.47 (2.6) a chunk, however many CUs are busy
+//     (8192 x 4096 x 7168: 333 us; 4096 x 4096 x 7168 in 4 bits: 74);
+//   * 256 x 224 takes 0.96 of that, and fewer rounds where it divides the columns better
+//     (8192 x 7168 x 4096, 4 rounds of either: 369 us, with 256 x 256 384);
+//   * 128 x 128: two workgroups a CU 0.88 (1.7) a chunk each, one alone 0.75 (0.8)
+//     (8192 x 4096 x 7168: 392 us; 512 x 4096 x 4096: 53 us, where 256 x 256 takes 97);
+//   * slices of k, where 128 x 128 tiles leave CUs idle: another launch, 3 us, and the slices'
+//     sums written and read at 3 TB/s (64 x 4096 x 4096: 1 slice 50 us, 8 slices 11 and 4).
+// `paired`: N columns of gate and N of up.
+inline Plan plan_tiles(bool fp4, int64_t M, int64_t N, int64_t chunks, bool paired) {
+  const int64_t cols = paired ? 2 * N : N;
+  const double big = fp4 ? 2.6 : 1.47, two = fp4 ? 1.7 : 0.88, one = fp4 ? 0.8 : 0.75;
+  auto rounds = [&](int64_t bm, int64_t bn, int64_t places) { return double(cdiv(cdiv(M, bm) * cdiv(cols, bn), places)); };
+  Plan best{256, 1};
+  double least = 4 + rounds(256, 256, 256) * big * chunks;
+  auto offer = [&](int c, int s, double us) {
+    if (us < least) {
+      least = us;
+      best = Plan{c, s};
+    }
+  };
+  if (!paired) offer(224, 1, 4 + rounds(256, 224, 256) * 0.96 * big * chunks);
+  const int64_t tiles = cdiv(M, 128) * cdiv(cols, 128);
+  for (int s = 1; s == 1 || (tiles * s <= 512 && 2 * s <= chunks && s <= 32); s *= 2) {
+    const double each = double(cdiv(chunks, s));
+    const double us = 3 + (tiles * s <= 256 ? one * each : double(cdiv(tiles * s, 512)) * two * each);
+    offer(128, s, us + (s > 1 ? 3 + s * M * cols * 4 / 3e6 : 0));
+  }
+  return best;
+}
+
+// The slices' sums: planes [M, ld] in fp32, pairs' gate columns from 0, the up columns from ld / 2.
+struct Partial {
+  float* p;
+  int64_t ld, M, N;  // N rounded up to 4
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, f32x4 v) const {
+    if (n < N) *reinterpret_cast<f32x4*>(p + (int64_t(blockIdx.y) * M + m) * ld + n) = v;
+  }
+  __device__ __forceinline__ void operator()(int64_t m, int64_t j, f32x4 g, f32x4 u) const {
+    float* at = p + (int64_t(blockIdx.y) * M + m) * ld + j;
+    if (j >= N) return;
+    *reinterpret_cast<f32x4*>(at) = g;
+    *reinterpret_cast<f32x4*>(at + ld / 2) = u;
+  }
+};
+inline int64_t round4(int64_t n) { return (n + 3) & ~int64_t(3); }
+inline int64_t partial_bytes(const Plan& plan, int64_t M, int64_t N, bool paired) {
+  return plan.slices > 1 ? plan.slices * M * round4(N) * (paired ? 2 : 1) * 4 : 0;
+}
+
+// Adds the slices up, in their order, for the epilogue.
+template <bool PAIRED, typename EPI>
+__global__ void __launch_bounds__(256)
+dense_finish(Partial part, int slices, EPI epi) {
+  const int64_t pieces = part.N / 4, total = part.M * pieces, plane = part.M * part.ld;
+  for (int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x; t < total; t += int64_t(gridDim.x) * 256) {
+    const int64_t m = t / pieces, n = (t - m * pieces) * 4;
+    const float* at = part.p + m * part.ld + n;
+    f32x4 v = *reinterpret_cast<const f32x4*>(at), u = {};
+    if constexpr (PAIRED) u = *reinterpret_cast<const f32x4*>(at + part.ld / 2);
+    for (int s = 1; s < slices; ++s) {
+      v += *reinterpret_cast<const f32x4*>(at + s * plane);
+      if constexpr (PAIRED) u += *reinterpret_cast<const f32x4*>(at + s * plane + part.ld / 2);
+    }
+    if constexpr (PAIRED) epi(m, n, v, u);
+    else epi(m, n, v);
+  }
+}
+
+template <Form F, Lay LX, Lay LW, int BM, int BN, bool PAIRED, typename EPI>
+void launch_cut(Product p, const EPI& epi, hipStream_t stream) {
+  constexpr int kWavesN = 2;
   p.tiles_m = int(cdiv(p.M, BM));
   p.tiles_n = int(cdiv(p.N, PAIRED ? BN / 2 : BN));
-  auto* fn = &dense_tile<F, LX, LW, BM, BN, WM, WN, PAIRED, EPI>;
-  hipLaunchKernelGGL(fn, dim3(p.tiles_m * p.tiles_n), dim3(BM / WM * (BN / WN) * 64), 0, stream, p, epi);
+  auto* fn = &dense_tile<F, LX, LW, BM, BN, kWavesN, PAIRED, EPI>;
+  hipLaunchKernelGGL(fn, dim3(p.tiles_m * p.tiles_n, p.slices), dim3(BM / 64 * kWavesN * 64), 0, stream, p, epi);
+}
+
+// The product with its epilogue; `scratch` holds partial_bytes (16-byte aligned).
+template <Form F, Lay LX, Lay LW, bool PAIRED, typename EPI>
+void launch_tiles(Product p, const EPI& epi, void* scratch, hipStream_t stream) {
+  const Plan plan = plan_tiles(F == Form::kFp4, p.M, p.N, p.chunks, PAIRED);
+  p.slices = plan.slices;
+  if (plan.slices > 1) {
+    const int64_t n = round4(p.N);
+    const Partial part{static_cast<float*>(scratch), PAIRED ? 2 * n : n, p.M, n};
+    launch_cut<F, LX, LW, 128, 128, PAIRED>(p, part, stream);
+    const int64_t total = p.M * (n / 4);
+    hipLaunchKernelGGL((dense_finish<PAIRED, EPI>), dim3(int(std::min<int64_t>(cdiv(total, 256), 256 * 16))), dim3(256),
+                       0, stream, part, plan.slices, epi);
+  } else if (plan.cols == 128) {
+    launch_cut<F, LX, LW, 128, 128, PAIRED>(p, epi, stream);
+  } else if (plan.cols == 224) {
+    if constexpr (!PAIRED) launch_cut<F, LX, LW, 256, 224, false>(p, epi, stream);
+  } else {
+    launch_cut<F, LX, LW, 256, 256, PAIRED>(p, epi, stream);
+  }
 }
 
 }  // namespace dense

@@ -3,13 +3,13 @@
 //   dh = dy W2, gc = min(g, L), uc = clamp(u, -L, L), s = 1 / (1 + e^-gc)
 //   dg = dh uc s (1 + gc (1 - s)) [g <= L],  du = dh gc s [|u| <= L]
 //   dx = [dg du] W13,  dW13 = [dg du]^T x,  dW2 = dy^T h
-// Each product is one launch of the tile kernel; the activation runs in the epilogue of
-// the gate/up product, its gradient in that of dh. h, dg and du are rounded to the
-// type once, as operands of the next product: their roundings add up like those of the
-// outputs themselves.
+// Each product is a launch of the tile kernel (two with slices of k), or, for up to 16 tokens,
+// of the kernel for few rows; the activation runs in the epilogue of the gate/up product,
+// its gradient in that of dh. h, dg and du are rounded to the type once, as operands of
+// the next product: their roundings add up like those of the outputs themselves.
 #include <algorithm>
 
-#include "dense_tile.h"
+#include "dense_rows.h"
 
 namespace xk {
 namespace {
@@ -56,23 +56,12 @@ template <typename T> __device__ __forceinline__ four<T> load_four(const T* p, i
 // out[m, n] in the type.
 template <Form F> struct Store {
   typename num<F>::type* out;
-  int64_t ld, M, N;
-  template <int WT, int XT>
-  __device__ __forceinline__ void operator()(const f32x4 (&acc)[WT][XT], int64_t m, int64_t n, int lane) const {
-    typedef typename num<F>::type T;
-    n += (lane >> 4) * 4;
+  int64_t ld, N;
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, f32x4 sum) const {
+    four<typename num<F>::type> v;
 #pragma unroll
-    for (int b = 0; b < XT; ++b) {
-      const int64_t row = m + b * 16 + (lane & 15);
-      if (row >= M) continue;
-#pragma unroll
-      for (int a = 0; a < WT; ++a) {
-        four<T> v;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v.v[i] = num<F>::put(acc[a][b][i]);
-        store_four(out + row * ld + n + a * 16, v, N - n - a * 16);
-      }
-    }
+    for (int i = 0; i < 4; ++i) v.v[i] = num<F>::put(sum[i]);
+    store_four(out + m * ld + n, v, N - n);
   }
 };
 
@@ -102,34 +91,27 @@ __device__ __forceinline__ float within(float u, float limit) {
 // gate_up [M, 2 I] (either may be null).
 template <Form F> struct Gate {
   typename num<F>::type *h, *gate_up;
-  int64_t ldh, M, I;
+  int64_t ldh, I;
   float limit;
-  template <int WT, int XT>
-  __device__ __forceinline__ void operator()(const f32x4 (&acc)[WT][XT], int64_t m, int64_t n, int lane) const {
+  __device__ __forceinline__ void operator()(int64_t m, int64_t j, f32x4 gs, f32x4 us) const {
     typedef typename num<F>::type T;
-    n += (lane >> 4) * 4;
+    four<T> g, u, v;
 #pragma unroll
-    for (int b = 0; b < XT; ++b) {
-      const int64_t row = m + b * 16 + (lane & 15);
-      if (row >= M) continue;
-#pragma unroll
-      for (int a = 0; a < WT / 2; ++a) {
-        const int64_t j = n + a * 16;
-        four<T> g, u, v;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float gs = acc[a][b][i], us = acc[a + WT / 2][b][i];
-          g.v[i] = held<F>(gs, limit);
-          u.v[i] = held<F>(us, limit);
-          const float gc = below(gs, limit), uc = within(us, limit);
-          v.v[i] = j + i < I ? num<F>::put(gc * sigmoid(gc) * uc) : T(0);
-        }
-        if (h != nullptr) store_four(h + row * ldh + j, v, ldh - j);
-        if (gate_up != nullptr) {
-          store_four(gate_up + row * 2 * I + j, g, I - j);
-          store_four(gate_up + row * 2 * I + I + j, u, I - j);
-        }
-      }
+    for (int i = 0; i < 4; ++i) {
+      g.v[i] = held<F>(gs[i], limit);
+      u.v[i] = held<F>(us[i], limit);
+      const float gc = below(gs[i], limit), uc = within(us[i], limit);
+      v.v[i] = j + i < I ? num<F>::put(gc * sigmoid(gc) * uc) : T(0);
+    }
+    if (j >= I) return;
+    if (h != nullptr) {
+      store_four(h + m * ldh + j, v, ldh - j);
+      if (j + 4 >= I)
+        for (int64_t c = j + 4; c < ldh; ++c) h[m * ldh + c] = T(0);
+    }
+    if (gate_up != nullptr) {
+      store_four(gate_up + m * 2 * I + j, g, I - j);
+      store_four(gate_up + m * 2 * I + I + j, u, I - j);
     }
   }
 };
@@ -139,40 +121,29 @@ template <Form F> struct Gate {
 template <Form F> struct GateGrad {
   const typename num<F>::type* gate_up;
   typename num<F>::type *d, *h;
-  int64_t ldd, ldh, M, I;
+  int64_t ldd, ldh, I;
   float limit;
-  template <int WT, int XT>
-  __device__ __forceinline__ void operator()(const f32x4 (&acc)[WT][XT], int64_t m, int64_t n, int lane) const {
+  __device__ __forceinline__ void operator()(int64_t m, int64_t j, f32x4 dh) const {
     typedef typename num<F>::type T;
-    n += (lane >> 4) * 4;
+    if (j >= I) return;
+    const four<T> g = load_four(gate_up + m * 2 * I + j, I - j);
+    const four<T> u = load_four(gate_up + m * 2 * I + I + j, I - j);
+    four<T> dg, du, v;
 #pragma unroll
-    for (int b = 0; b < XT; ++b) {
-      const int64_t row = m + b * 16 + (lane & 15);
-      if (row >= M) continue;
-#pragma unroll
-      for (int a = 0; a < WT; ++a) {
-        const int64_t j = n + a * 16;
-        if (j >= I) continue;
-        const four<T> g = load_four(gate_up + row * 2 * I + j, I - j);
-        const four<T> u = load_four(gate_up + row * 2 * I + I + j, I - j);
-        four<T> dg, du, v;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float gs = num<F>::get(g.v[i]), us = num<F>::get(u.v[i]), dh = acc[a][b][i];
-          const float gc = below(gs, limit), uc = within(us, limit), s = sigmoid(gc);
-          const bool on_g = !(limit > 0.f && gs > limit), on_u = !(limit > 0.f && fabsf(us) > limit);
-          dg.v[i] = num<F>::put(on_g ? dh * uc * s * (1.0f + gc * (1.0f - s)) : 0.f);
-          du.v[i] = num<F>::put(on_u ? dh * gc * s : 0.f);
-          v.v[i] = j + i < I ? num<F>::put(gc * s * uc) : T(0);
-        }
-        store_four(d + row * ldd + j, dg, I - j);
-        store_four(d + row * ldd + I + j, du, I - j);
-        store_four(h + row * ldh + j, v, ldh - j);
-        if (j + 4 >= I) {
-          for (int64_t c = 2 * I; c < ldd; ++c) d[row * ldd + c] = T(0);
-          for (int64_t c = j + 4; c < ldh; ++c) h[row * ldh + c] = T(0);
-        }
-      }
+    for (int i = 0; i < 4; ++i) {
+      const float gs = num<F>::get(g.v[i]), us = num<F>::get(u.v[i]);
+      const float gc = below(gs, limit), uc = within(us, limit), s = sigmoid(gc);
+      const bool on_g = !(limit > 0.f && gs > limit), on_u = !(limit > 0.f && fabsf(us) > limit);
+      dg.v[i] = num<F>::put(on_g ? dh[i] * uc * s * (1.0f + gc * (1.0f - s)) : 0.f);
+      du.v[i] = num<F>::put(on_u ? dh[i] * gc * s : 0.f);
+      v.v[i] = j + i < I ? num<F>::put(gc * s * uc) : T(0);
+    }
+    store_four(d + m * ldd + j, dg, I - j);
+    store_four(d + m * ldd + I + j, du, I - j);
+    store_four(h + m * ldh + j, v, ldh - j);
+    if (j + 4 >= I) {
+      for (int64_t c = 2 * I; c < ldd; ++c) d[m * ldd + c] = T(0);
+      for (int64_t c = j + 4; c < ldh; ++c) h[m * ldh + c] = T(0);
     }
   }
 };
@@ -218,7 +189,9 @@ Matrix take(const void* p, int64_t rows, int64_t n, int64_t ld, char*& ws, hipSt
 }
 int64_t taken_bytes(int64_t rows, int64_t n) { return n % 8 == 0 ? 0 : aligned(rows * pad8(n) * 2); }
 
-// out = X W^T of k values a row
+int64_t chunks_of(int64_t k) { return cdiv(k, 64); }
+
+// out = X W^T of k8 values a row of a side that lies so, k_rows of one that does not
 Product product(const Side& x, const Side& w, int64_t M, int64_t N, int64_t k8, int64_t k_rows) {
   Product p{};
   p.x = x;
@@ -227,29 +200,31 @@ Product product(const Side& x, const Side& w, int64_t M, int64_t N, int64_t k8, 
   p.N = N;
   p.k_bytes = k8 * 2;
   p.k_rows = k_rows;
-  p.chunks = int(cdiv(std::max(k8, k_rows), 64));
+  p.chunks = int(chunks_of(std::max(k8, k_rows)));
   return p;
 }
-
-template <Form F> void gate_up_product(const Matrix& x, const Matrix& w13, const Gate<F>& epi, hipStream_t stream) {
-  const int64_t I = epi.I;
-  launch_tile<F, Lay::kRowsOfK, Lay::kRowsOfK, 128, 128, 64, 64, true>(
-      product(x.of_k(), w13.of_k(), x.rows, I, pad8(x.n), 0), epi, stream);
-}
+Rows rows_of(const void* p, int64_t rows, int64_t ld) { return Rows{static_cast<const char*>(p), ld * 2, rows, nullptr, 0}; }
 
 template <Form F>
 int forward(const void* x, int64_t ldx, int64_t M, int64_t H, const void* w13, const void* w2, int64_t I, float limit,
             void* out, void* gate_up, void* workspace, hipStream_t stream) {
   typedef typename num<F>::type T;
+  constexpr Lay R = Lay::kRowsOfK;
   char* ws = static_cast<char*>(workspace);
   T* h = reinterpret_cast<T*>(ws);
-  ws += aligned(M * pad8(I) * 2);
-  const Matrix xm = take(x, M, H, ldx, ws, stream), m13 = take(w13, 2 * I, H, H, ws, stream),
-               m2 = take(w2, H, I, I, ws, stream);
-  const Matrix hm{h, M, I, pad8(I)};
-  gate_up_product<F>(xm, m13, Gate<F>{h, static_cast<T*>(gate_up), hm.ld, M, I, limit}, stream);
-  launch_tile<F, Lay::kRowsOfK, Lay::kRowsOfK, 128, 128, 64, 64, false>(
-      product(hm.of_k(), m2.of_k(), M, H, pad8(I), 0), Store<F>{static_cast<T*>(out), H, M, H}, stream);
+  const int64_t ldh = pad8(I);
+  ws += aligned(M * ldh * 2);
+  const Gate<F> gate{h, static_cast<T*>(gate_up), ldh, I, limit};
+  const Store<F> store{static_cast<T*>(out), H, H};
+  if (M <= kFewRows) {
+    launch_rows<F, void, true>(rows_of(x, M, ldx), rows_of(w13, 2 * I, H), M, I, H, 0, gate, stream);
+    launch_rows<F, void, false>(rows_of(h, M, ldh), rows_of(w2, H, I), M, H, I, 0, store, stream);
+  } else {
+    const Matrix xm = take(x, M, H, ldx, ws, stream), m13 = take(w13, 2 * I, H, H, ws, stream),
+                 m2 = take(w2, H, I, I, ws, stream), hm{h, M, I, ldh};
+    launch_tiles<F, R, R, true>(product(xm.of_k(), m13.of_k(), M, I, pad8(H), 0), gate, ws, stream);
+    launch_tiles<F, R, R, false>(product(hm.of_k(), m2.of_k(), M, H, ldh, 0), store, ws, stream);
+  }
   XK_CHECK_LAUNCH("gated_ffn");
   return XK_OK;
 }
@@ -259,6 +234,7 @@ int backward(const void* dy, int64_t ldg, const void* x, int64_t ldx, int64_t M,
              const void* w2, int64_t I, const void* gate_up, float limit, void* dx, void* dw13, void* dw2,
              void* workspace, hipStream_t stream) {
   typedef typename num<F>::type T;
+  constexpr Lay R = Lay::kRowsOfK, C = Lay::kColumns;
   char* ws = static_cast<char*>(workspace);
   T* h = reinterpret_cast<T*>(ws);
   ws += aligned(M * pad8(I) * 2);
@@ -269,31 +245,44 @@ int backward(const void* dy, int64_t ldg, const void* x, int64_t ldx, int64_t M,
   const Matrix hm{h, M, I, pad8(I)}, dm{d, M, 2 * I, pad8(2 * I)};
   if (M > 0) {
     if (gate_up == nullptr) {
-      gate_up_product<F>(xm, m13, Gate<F>{nullptr, reinterpret_cast<T*>(ws), 0, M, I, limit}, stream);
       gate_up = ws;
+      ws += aligned(M * 2 * I * 2);
+      const Gate<F> gate{nullptr, static_cast<T*>(const_cast<void*>(gate_up)), 0, I, limit};
+      launch_tiles<F, R, R, true>(product(xm.of_k(), m13.of_k(), M, I, pad8(H), 0), gate, ws, stream);
     }
-    launch_tile<F, Lay::kRowsOfK, Lay::kColumns, 128, 128, 64, 64, false>(
-        product(gm.of_k(), m2.columns(), M, I, pad8(H), H),
-        GateGrad<F>{static_cast<const T*>(gate_up), d, h, dm.ld, hm.ld, M, I, limit}, stream);
-    launch_tile<F, Lay::kRowsOfK, Lay::kColumns, 128, 128, 64, 64, false>(
-        product(dm.of_k(), m13.columns(), M, H, pad8(2 * I), 2 * I), Store<F>{static_cast<T*>(dx), H, M, H}, stream);
+    const GateGrad<F> grad{static_cast<const T*>(gate_up), d, h, dm.ld, hm.ld, I, limit};
+    launch_tiles<F, R, C, false>(product(gm.of_k(), m2.columns(), M, I, pad8(H), H), grad, ws, stream);
+    launch_tiles<F, R, C, false>(product(dm.of_k(), m13.columns(), M, H, pad8(2 * I), 2 * I),
+                                 Store<F>{static_cast<T*>(dx), H, H}, ws, stream);
   }
-  launch_tile<F, Lay::kColumns, Lay::kColumns, 128, 128, 64, 64, false>(
-      product(dm.columns(), xm.columns(), 2 * I, H, 0, M), Store<F>{static_cast<T*>(dw13), H, 2 * I, H}, stream);
-  launch_tile<F, Lay::kColumns, Lay::kColumns, 128, 128, 64, 64, false>(
-      product(gm.columns(), hm.columns(), H, I, 0, M), Store<F>{static_cast<T*>(dw2), I, H, I}, stream);
+  launch_tiles<F, C, C, false>(product(dm.columns(), xm.columns(), 2 * I, H, 0, M), Store<F>{static_cast<T*>(dw13), H, H},
+                               ws, stream);
+  launch_tiles<F, C, C, false>(product(gm.columns(), hm.columns(), H, I, 0, M), Store<F>{static_cast<T*>(dw2), I, I}, ws,
+                               stream);
   XK_CHECK_LAUNCH("gated_ffn_backward");
   return XK_OK;
+}
+
+// the slices' sums of a product of k values
+int64_t sums_bytes(int64_t M, int64_t N, int64_t k, bool paired) {
+  return M > 0 ? aligned(partial_bytes(plan_tiles(false, M, N, chunks_of(k), paired), M, N, paired)) : 0;
 }
 
 }  // namespace
 
 int64_t gated_ffn_workspace_bytes(int64_t M, int64_t H, int64_t I) {
-  return aligned(M * pad8(I) * 2) + taken_bytes(M, H) + taken_bytes(2 * I, H) + taken_bytes(H, I);
+  const int64_t h = aligned(M * pad8(I) * 2);
+  if (M <= kFewRows) return h;
+  return h + taken_bytes(M, H) + taken_bytes(2 * I, H) + taken_bytes(H, I) +
+         std::max(sums_bytes(M, I, pad8(H), true), sums_bytes(M, H, pad8(I), false));
 }
 int64_t gated_ffn_backward_workspace_bytes(int64_t M, int64_t H, int64_t I, int recompute) {
-  return gated_ffn_workspace_bytes(M, H, I) + aligned(M * pad8(2 * I) * 2) + taken_bytes(M, H) +
-         (recompute ? aligned(M * 2 * I * 2) : 0);
+  const int64_t k1 = pad8(H), k2 = pad8(2 * I);
+  int64_t sums = std::max(std::max(sums_bytes(M, I, k1, false), sums_bytes(M, H, k2, false)),
+                          std::max(sums_bytes(2 * I, H, M, false), sums_bytes(H, I, M, false)));
+  if (recompute) sums = std::max(sums, sums_bytes(M, I, k1, true)) + aligned(M * 2 * I * 2);
+  return aligned(M * pad8(I) * 2) + aligned(M * k2 * 2) + taken_bytes(M, H) * 2 + taken_bytes(2 * I, H) +
+         taken_bytes(H, I) + sums;
 }
 
 int launch_gated_ffn(const void* x, int dtype, int64_t ldx, int64_t M, int64_t H, const void* w13, const void* w2,

@@ -1,11 +1,10 @@
 // The product of two MXFP4 operands: out[m, n] = sum over blocks b of 2^(sx + sw) times the
 // block's sum of e2m1 products (+ bias[n]), in fp32 on the scaled matrix instructions,
-// rounded once. Activations that come in 16 or 32 bits are quantised first, in a pass
-// of their own.
+// rounded once. Up to 16 rows are one launch, which quantises activations in 16 or 32 bits as it
+// reads them; of more rows they are quantised first, in a pass of their own.
 #include <algorithm>
 
-#include "dense_tile.h"
-#include "mx4.h"
+#include "dense_rows.h"
 
 namespace xk {
 
@@ -36,33 +35,20 @@ template <> struct val<float> {
 template <typename T> struct Store {
   T* out;
   const T* bias;
-  int64_t M, N;
-  template <int WT, int XT>
-  __device__ __forceinline__ void operator()(const f32x4 (&acc)[WT][XT], int64_t m, int64_t n, int lane) const {
-    struct four { T v[4]; };
-    n += (lane >> 4) * 4;
+  int64_t N;
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, f32x4 sum) const {
+    struct four { T v[4]; } v;
+    const int64_t left = N - n;
+    T* to = out + m * N + n;
 #pragma unroll
-    for (int a = 0; a < WT; ++a) {
-      const int64_t left = N - n - a * 16;
-      float add[4];
+    for (int i = 0; i < 4; ++i)
+      v.v[i] = val<T>::put(bias != nullptr && i < left ? sum[i] + val<T>::get(bias[n + i]) : sum[i]);
+    if (left >= 4) {
+      store_unaligned(to, v);
+    } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) add[i] = bias != nullptr && i < left ? val<T>::get(bias[n + a * 16 + i]) : 0.f;
-#pragma unroll
-      for (int b = 0; b < XT; ++b) {
-        const int64_t row = m + b * 16 + (lane & 15);
-        if (row >= M) continue;
-        T* to = out + row * N + n + a * 16;
-        four v;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v.v[i] = val<T>::put(acc[a][b][i] + add[i]);
-        if (left >= 4) {
-          store_unaligned(to, v);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 3; ++i)
-            if (i < left) to[i] = v.v[i];
-        }
-      }
+      for (int i = 0; i < 3; ++i)
+        if (i < left) to[i] = v.v[i];
     }
   }
 };
@@ -87,48 +73,81 @@ const uint8_t* take_scales(const uint8_t* s, int64_t rows, int64_t blocks, char*
   return to;
 }
 
-template <typename T>
-void typed(const Product& p, const void* bias, void* out, hipStream_t stream) {
-  launch_tile<Form::kFp4, Lay::kRowsOfK, Lay::kRowsOfK, 128, 128, 64, 64, false>(
-      p, Store<T>{static_cast<T*>(out), static_cast<const T*>(bias), p.M, p.N}, stream);
+struct Call {
+  const void* x;
+  int dtype;
+  int64_t ldx;
+  const uint8_t* x_scales;
+  int64_t M, K;
+  const uint8_t *codes, *scales;
+  int64_t N;
+};
+
+template <typename T> int typed(const Call& c, const Store<T>& store, char* ws, hipStream_t stream) {
+  const int64_t blocks = cdiv(c.K, kMx4Block), lds = pad4(blocks);
+  const char* codes = reinterpret_cast<const char*>(c.codes);
+  if (c.M <= kFewRows) {
+    const Rows w{codes, blocks * 16, c.N, c.scales, blocks};
+    const Rows x{static_cast<const char*>(c.x), c.x_scales ? blocks * 16 : c.ldx * (c.dtype == XK_DT_FP32 ? 4 : 2), c.M,
+                 c.x_scales, blocks};
+    if (c.x_scales != nullptr)
+      launch_rows<Form::kFp4, void, false>(x, w, c.M, c.N, blocks, 0, store, stream);
+    else if (c.dtype == XK_DT_BF16)
+      launch_rows<Form::kFp4, uint16_t, false>(x, w, c.M, c.N, blocks, c.K, store, stream);
+    else if (c.dtype == XK_DT_FP16)
+      launch_rows<Form::kFp4, _Float16, false>(x, w, c.M, c.N, blocks, c.K, store, stream);
+    else
+      launch_rows<Form::kFp4, float, false>(x, w, c.M, c.N, blocks, c.K, store, stream);
+    return XK_OK;
+  }
+  const char* xc = static_cast<const char*>(c.x);
+  const uint8_t* xs;
+  if (c.x_scales == nullptr) {
+    uint8_t* to = reinterpret_cast<uint8_t*>(ws);
+    ws += aligned(c.M * blocks * 16);
+    uint8_t* s = reinterpret_cast<uint8_t*>(ws);
+    ws += aligned(c.M * lds);
+    if (int rc = launch_mxfp4_quantize(c.x, c.dtype, c.ldx, c.M, c.K, to, s, lds, stream)) return rc;
+    xc = reinterpret_cast<const char*>(to);
+    xs = s;
+  } else {
+    xs = take_scales(c.x_scales, c.M, blocks, ws, stream);
+  }
+  const uint8_t* wsc = take_scales(c.scales, c.N, blocks, ws, stream);
+  Product p{};
+  p.x = Side{xc, blocks * 16, c.M, xs, lds};
+  p.w = Side{codes, blocks * 16, c.N, wsc, lds};
+  p.M = c.M;
+  p.N = c.N;
+  p.k_bytes = blocks * 16;
+  p.blocks = blocks;
+  p.chunks = int(cdiv(blocks, 8));
+  launch_tiles<Form::kFp4, Lay::kRowsOfK, Lay::kRowsOfK, false>(p, store, ws, stream);
+  return XK_OK;
 }
 
 }  // namespace
 
 int64_t mxfp4_linear_workspace_bytes(int64_t M, int64_t K, int64_t N) {
+  if (M <= kFewRows) return 0;
   const int64_t blocks = cdiv(K, kMx4Block), lds = pad4(blocks);
-  return aligned(M * blocks * 16) + aligned(M * lds) + (lds == blocks ? 0 : aligned(N * lds));
+  return aligned(M * blocks * 16) + aligned(M * lds) + (lds == blocks ? 0 : aligned(N * lds)) +
+         partial_bytes(plan_tiles(true, M, N, cdiv(blocks, 8), false), M, N, false);
 }
 
 int launch_mxfp4_linear(const void* x, int dtype, int64_t ldx, const uint8_t* x_scales, int64_t M, int64_t K,
                         const uint8_t* codes, const uint8_t* scales, int64_t N, const void* bias, void* out,
                         int out_dtype, void* workspace, hipStream_t stream) {
-  const int64_t blocks = cdiv(K, kMx4Block), lds = pad4(blocks);
+  const Call c{x, dtype, ldx, x_scales, M, K, codes, scales, N};
   char* ws = static_cast<char*>(workspace);
-  const uint8_t *xc = static_cast<const uint8_t*>(x), *xs;
-  if (x_scales == nullptr) {
-    uint8_t* c = reinterpret_cast<uint8_t*>(ws);
-    ws += aligned(M * blocks * 16);
-    uint8_t* s = reinterpret_cast<uint8_t*>(ws);
-    ws += aligned(M * lds);
-    if (int rc = launch_mxfp4_quantize(x, dtype, ldx, M, K, c, s, lds, stream)) return rc;
-    xc = c;
-    xs = s;
-  } else {
-    xs = take_scales(x_scales, M, blocks, ws, stream);
-  }
-  const uint8_t* wsc = take_scales(scales, N, blocks, ws, stream);
-  Product p{};
-  p.x = Side{reinterpret_cast<const char*>(xc), blocks * 16, M, xs, lds};
-  p.w = Side{reinterpret_cast<const char*>(codes), blocks * 16, N, wsc, lds};
-  p.M = M;
-  p.N = N;
-  p.k_bytes = blocks * 16;
-  p.blocks = blocks;
-  p.chunks = int(cdiv(blocks, 8));
-  if (out_dtype == XK_DT_BF16) typed<uint16_t>(p, bias, out, stream);
-  else if (out_dtype == XK_DT_FP16) typed<_Float16>(p, bias, out, stream);
-  else typed<float>(p, bias, out, stream);
+  int rc;
+  if (out_dtype == XK_DT_BF16)
+    rc = typed(c, Store<uint16_t>{static_cast<uint16_t*>(out), static_cast<const uint16_t*>(bias), N}, ws, stream);
+  else if (out_dtype == XK_DT_FP16)
+    rc = typed(c, Store<_Float16>{static_cast<_Float16*>(out), static_cast<const _Float16*>(bias), N}, ws, stream);
+  else
+    rc = typed(c, Store<float>{static_cast<float*>(out), static_cast<const float*>(bias), N}, ws, stream);
+  if (rc) return rc;
   XK_CHECK_LAUNCH("mxfp4_linear");
   return XK_OK;
 }
