@@ -258,9 +258,11 @@ __device__ __forceinline__ void tile_of(int id, int total, int tiles_m, int tile
   tm = band * kBand + in - tn * height;
 }
 
-// EPI: struct with `void operator()(int64_t m, int64_t n, f32x4 v)`, the sums of row m and columns n .. n + 3, or,
-// for pairs, `void operator()(int64_t m, int64_t j, f32x4 g, f32x4 u)`; either may lie past the output's
-// last column, not its last row. n and j are multiples of 4. blockIdx.y is the slice of k.
+// EPI: struct with `template <bool WHOLE> void put(int64_t m, int64_t n, f32x4 v)`, the sums of row m and columns
+// n .. n + 3, or, for pairs, `put(int64_t m, int64_t j, f32x4 g, f32x4 u)`; n and j are multiples of 4. WHOLE: they
+// lie within the output, else they may lie past its last column (not its last row): a tile's
+// checks cost more than its stores (16384 x 7168 x 2048 in 4 bits: 293 us with them in every
+// tile, 194 without). blockIdx.y is the slice of k.
 template <Form F, Lay LX, Lay LW, int BM, int BN, int WAVES_N, bool PAIRED, typename EPI>
 __global__ void __launch_bounds__(BM / 64 * WAVES_N * 64)
 dense_tile(Product p, EPI epi) {
@@ -436,17 +438,19 @@ dense_tile(Product p, EPI epi) {
   }
 
   const int64_t m = m0 + wm * 64 + (lane & 15), n = n0 + wn * (PAIRED ? WN / 2 : WN) + (lane >> 4) * 4;
+  auto put_all = [&](auto WHOLE) __attribute__((always_inline)) {
+    constexpr bool whole = decltype(WHOLE)::value;
 #pragma unroll
-  for (int b = 0; b < XT; ++b) {
-    if (m + b * 16 >= p.M) continue;
-    if constexpr (PAIRED) {
+    for (int a = 0; a < (PAIRED ? WT / 2 : WT); ++a)
 #pragma unroll
-      for (int a = 0; a < WT / 2; ++a) epi(m + b * 16, n + a * 16, acc[a][b], acc[a + WT / 2][b]);
-    } else {
-#pragma unroll
-      for (int a = 0; a < WT; ++a) epi(m + b * 16, n + a * 16, acc[a][b]);
-    }
-  }
+      for (int b = 0; b < XT; ++b) {
+        if (!whole && m + b * 16 >= p.M) continue;
+        if constexpr (PAIRED) epi.template put<whole>(m + b * 16, n + a * 16, acc[a][b], acc[a + WT / 2][b]);
+        else epi.template put<whole>(m + b * 16, n + a * 16, acc[a][b]);
+      }
+  };
+  if (m0 + BM <= p.M && n0 + (PAIRED ? BN / 2 : BN) <= p.N) put_all(std::true_type{});
+  else put_all(std::false_type{});
 }
 
 // ---------------------------------------------------------------- launches ----
@@ -493,12 +497,12 @@ inline Plan plan_tiles(bool fp4, int64_t M, int64_t N, int64_t chunks, bool pair
 struct Partial {
   float* p;
   int64_t ld, M, N;  // N rounded up to 4
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, f32x4 v) const {
-    if (n < N) *reinterpret_cast<f32x4*>(p + (int64_t(blockIdx.y) * M + m) * ld + n) = v;
+  template <bool WHOLE> __device__ __forceinline__ void put(int64_t m, int64_t n, f32x4 v) const {
+    if (WHOLE || n < N) *reinterpret_cast<f32x4*>(p + (int64_t(blockIdx.y) * M + m) * ld + n) = v;
   }
-  __device__ __forceinline__ void operator()(int64_t m, int64_t j, f32x4 g, f32x4 u) const {
+  template <bool WHOLE> __device__ __forceinline__ void put(int64_t m, int64_t j, f32x4 g, f32x4 u) const {
     float* at = p + (int64_t(blockIdx.y) * M + m) * ld + j;
-    if (j >= N) return;
+    if (!WHOLE && j >= N) return;
     *reinterpret_cast<f32x4*>(at) = g;
     *reinterpret_cast<f32x4*>(at + ld / 2) = u;
   }
@@ -522,8 +526,8 @@ dense_finish(Partial part, int slices, EPI epi) {
       v += *reinterpret_cast<const f32x4*>(at + s * plane);
       if constexpr (PAIRED) u += *reinterpret_cast<const f32x4*>(at + s * plane + part.ld / 2);
     }
-    if constexpr (PAIRED) epi(m, n, v, u);
-    else epi(m, n, v);
+    if constexpr (PAIRED) epi.template put<false>(m, n, v, u);
+    else epi.template put<false>(m, n, v);
   }
 }
 

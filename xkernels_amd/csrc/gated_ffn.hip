@@ -57,11 +57,11 @@ template <typename T> __device__ __forceinline__ four<T> load_four(const T* p, i
 template <Form F> struct Store {
   typename num<F>::type* out;
   int64_t ld, N;
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, f32x4 sum) const {
+  template <bool WHOLE> __device__ __forceinline__ void put(int64_t m, int64_t n, f32x4 sum) const {
     four<typename num<F>::type> v;
 #pragma unroll
     for (int i = 0; i < 4; ++i) v.v[i] = num<F>::put(sum[i]);
-    store_four(out + m * ld + n, v, N - n);
+    store_four(out + m * ld + n, v, WHOLE ? 4 : N - n);
   }
 };
 
@@ -93,25 +93,25 @@ template <Form F> struct Gate {
   typename num<F>::type *h, *gate_up;
   int64_t ldh, I;
   float limit;
-  __device__ __forceinline__ void operator()(int64_t m, int64_t j, f32x4 gs, f32x4 us) const {
+  template <bool WHOLE> __device__ __forceinline__ void put(int64_t m, int64_t j, f32x4 gs, f32x4 us) const {
     typedef typename num<F>::type T;
+    if (!WHOLE && j >= I) return;
     four<T> g, u, v;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       g.v[i] = held<F>(gs[i], limit);
       u.v[i] = held<F>(us[i], limit);
       const float gc = below(gs[i], limit), uc = within(us[i], limit);
-      v.v[i] = j + i < I ? num<F>::put(gc * sigmoid(gc) * uc) : T(0);
+      v.v[i] = WHOLE || j + i < I ? num<F>::put(gc * sigmoid(gc) * uc) : T(0);
     }
-    if (j >= I) return;
     if (h != nullptr) {
-      store_four(h + m * ldh + j, v, ldh - j);
-      if (j + 4 >= I)
+      store_four(h + m * ldh + j, v, WHOLE ? 4 : ldh - j);
+      if (!WHOLE && j + 4 >= I)
         for (int64_t c = j + 4; c < ldh; ++c) h[m * ldh + c] = T(0);
     }
     if (gate_up != nullptr) {
-      store_four(gate_up + m * 2 * I + j, g, I - j);
-      store_four(gate_up + m * 2 * I + I + j, u, I - j);
+      store_four(gate_up + m * 2 * I + j, g, WHOLE ? 4 : I - j);
+      store_four(gate_up + m * 2 * I + I + j, u, WHOLE ? 4 : I - j);
     }
   }
 };
@@ -123,11 +123,12 @@ template <Form F> struct GateGrad {
   typename num<F>::type *d, *h;
   int64_t ldd, ldh, I;
   float limit;
-  __device__ __forceinline__ void operator()(int64_t m, int64_t j, f32x4 dh) const {
+  template <bool WHOLE> __device__ __forceinline__ void put(int64_t m, int64_t j, f32x4 dh) const {
     typedef typename num<F>::type T;
-    if (j >= I) return;
-    const four<T> g = load_four(gate_up + m * 2 * I + j, I - j);
-    const four<T> u = load_four(gate_up + m * 2 * I + I + j, I - j);
+    if (!WHOLE && j >= I) return;
+    const int64_t left = WHOLE ? 4 : I - j;
+    const four<T> g = load_four(gate_up + m * 2 * I + j, left);
+    const four<T> u = load_four(gate_up + m * 2 * I + I + j, left);
     four<T> dg, du, v;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -136,12 +137,12 @@ template <Form F> struct GateGrad {
       const bool on_g = !(limit > 0.f && gs > limit), on_u = !(limit > 0.f && fabsf(us) > limit);
       dg.v[i] = num<F>::put(on_g ? dh[i] * uc * s * (1.0f + gc * (1.0f - s)) : 0.f);
       du.v[i] = num<F>::put(on_u ? dh[i] * gc * s : 0.f);
-      v.v[i] = j + i < I ? num<F>::put(gc * s * uc) : T(0);
+      v.v[i] = WHOLE || i < left ? num<F>::put(gc * s * uc) : T(0);
     }
-    store_four(d + m * ldd + j, dg, I - j);
-    store_four(d + m * ldd + I + j, du, I - j);
-    store_four(h + m * ldh + j, v, ldh - j);
-    if (j + 4 >= I) {
+    store_four(d + m * ldd + j, dg, left);
+    store_four(d + m * ldd + I + j, du, left);
+    store_four(h + m * ldh + j, v, WHOLE ? 4 : ldh - j);
+    if (j + 4 >= I) {  // (the last columns of a whole tile may be a row's last)
       for (int64_t c = 2 * I; c < ldd; ++c) d[m * ldd + c] = T(0);
       for (int64_t c = j + 4; c < ldh; ++c) h[m * ldh + c] = T(0);
     }

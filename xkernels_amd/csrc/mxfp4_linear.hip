@@ -32,17 +32,17 @@ template <> struct val<float> {
   __device__ __forceinline__ static float put(float f) { return f; }
 };
 
-template <typename T> struct Store {
+template <typename T, bool BIAS> struct Store {
   T* out;
   const T* bias;
   int64_t N;
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, f32x4 sum) const {
+  template <bool WHOLE> __device__ __forceinline__ void put(int64_t m, int64_t n, f32x4 sum) const {
     struct four { T v[4]; } v;
-    const int64_t left = N - n;
+    const int64_t left = WHOLE ? 4 : N - n;
     T* to = out + m * N + n;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      v.v[i] = val<T>::put(bias != nullptr && i < left ? sum[i] + val<T>::get(bias[n + i]) : sum[i]);
+      v.v[i] = val<T>::put(BIAS && (WHOLE || i < left) ? sum[i] + val<T>::get(bias[n + i]) : sum[i]);
     if (left >= 4) {
       store_unaligned(to, v);
     } else {
@@ -83,7 +83,7 @@ struct Call {
   int64_t N;
 };
 
-template <typename T> int typed(const Call& c, const Store<T>& store, char* ws, hipStream_t stream) {
+template <typename EPI> int cut(const Call& c, const EPI& store, char* ws, hipStream_t stream) {
   const int64_t blocks = cdiv(c.K, kMx4Block), lds = pad4(blocks);
   const char* codes = reinterpret_cast<const char*>(c.codes);
   if (c.M <= kFewRows) {
@@ -126,6 +126,12 @@ template <typename T> int typed(const Call& c, const Store<T>& store, char* ws, 
   return XK_OK;
 }
 
+template <typename T> int typed(const Call& c, void* out, const void* bias, char* ws, hipStream_t stream) {
+  T* o = static_cast<T*>(out);
+  const T* b = static_cast<const T*>(bias);
+  return b != nullptr ? cut(c, Store<T, true>{o, b, c.N}, ws, stream) : cut(c, Store<T, false>{o, b, c.N}, ws, stream);
+}
+
 }  // namespace
 
 int64_t mxfp4_linear_workspace_bytes(int64_t M, int64_t K, int64_t N) {
@@ -140,13 +146,9 @@ int launch_mxfp4_linear(const void* x, int dtype, int64_t ldx, const uint8_t* x_
                         int out_dtype, void* workspace, hipStream_t stream) {
   const Call c{x, dtype, ldx, x_scales, M, K, codes, scales, N};
   char* ws = static_cast<char*>(workspace);
-  int rc;
-  if (out_dtype == XK_DT_BF16)
-    rc = typed(c, Store<uint16_t>{static_cast<uint16_t*>(out), static_cast<const uint16_t*>(bias), N}, ws, stream);
-  else if (out_dtype == XK_DT_FP16)
-    rc = typed(c, Store<_Float16>{static_cast<_Float16*>(out), static_cast<const _Float16*>(bias), N}, ws, stream);
-  else
-    rc = typed(c, Store<float>{static_cast<float*>(out), static_cast<const float*>(bias), N}, ws, stream);
+  const int rc = out_dtype == XK_DT_BF16   ? typed<uint16_t>(c, out, bias, ws, stream)
+                 : out_dtype == XK_DT_FP16 ? typed<_Float16>(c, out, bias, ws, stream)
+                                           : typed<float>(c, out, bias, ws, stream);
   if (rc) return rc;
   XK_CHECK_LAUNCH("mxfp4_linear");
   return XK_OK;
