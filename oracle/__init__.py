@@ -2,7 +2,8 @@
 
 ``torch_ref``: pure-torch restatement of the reference backend (also the
 REFERENCE backend the test harness registers). ``tuning_ref``: the same for the ops
-for tuning and serving over the frozen experts. ``c_oracle``: independent
+for tuning and serving over the frozen experts. ``dense_ref``: for the dense block
+beside them. ``c_oracle``: independent
 plain-C restatement (moe_oracle.c, built by ``make -C oracle``) used as a second
 oracle and as the benchmark's CPU baseline. Only tests/, __graft_entry__.smoke()
 and bench.py's cpu_baseline may import this package; the product package

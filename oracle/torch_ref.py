@@ -265,7 +265,8 @@ def register_reference_backends() -> None:
     register("topk_softmax", Backend.REFERENCE)(topk_softmax_ref)
     for path, fn in SPEC_REFERENCES.items():
         bind_reference(path, fn)
+    from .dense_ref import DENSE_REFERENCES
     from .tuning_ref import TUNING_REFERENCES
 
-    for kernel, fn in TUNING_REFERENCES.items():
+    for kernel, fn in {**TUNING_REFERENCES, **DENSE_REFERENCES}.items():
         register(kernel, Backend.REFERENCE)(fn)

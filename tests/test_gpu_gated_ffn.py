@@ -9,6 +9,16 @@ from tests._dense_ref import ffn_grad_ref, ffn_ref
 from tests._tuning_ref import check
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _nan_in_free_memory():
+    """What the allocator hands out next holds NaN: scratch that is read before it is written shows."""
+    if torch.cuda.is_available():
+        for n in (1 << 12, 1 << 18, 1 << 22, 1 << 25):
+            torch.full((n,), float("nan"), device="cuda")
+
+
 BF, FP16 = torch.bfloat16, torch.float16
 
 

@@ -80,7 +80,8 @@ template <Form F> __device__ __forceinline__ typename num<F>::type held(float v,
   return r;
 }
 
-__device__ __forceinline__ float sigmoid(float g) { return 1.0f / (1.0f + __expf(-g)); }
+// (the reciprocal is within a step of fp32, as a division is; of an infinity it is 0)
+__device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
 // min(g, L) and clamp(u, -L, L); NaN stays NaN
 __device__ __forceinline__ float below(float g, float limit) { return limit > 0.f && g > limit ? limit : g; }
 __device__ __forceinline__ float within(float u, float limit) {

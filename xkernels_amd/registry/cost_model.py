@@ -100,6 +100,28 @@ def _act_checkpoint(p: dict[str, Any]) -> tuple[int, int]:
     return 2 * M * K, M * (K * (dtype_bytes(p.get("dtype", "bf16")) + 1) + -(-K // 32))
 
 
+def _gated_ffn(p: dict[str, Any]) -> tuple[int, int]:
+    M, H, I = (int(p[x]) for x in ("M", "hidden", "ispp"))
+    return 6 * M * H * I, dtype_bytes(p.get("dtype", "bf16")) * (2 * M * H + 3 * H * I)
+
+
+def _gated_ffn_backward(p: dict[str, Any]) -> tuple[int, int]:
+    M, H, I = (int(p[x]) for x in ("M", "hidden", "ispp"))
+    kept = bool(p.get("kept"))
+    return (12 if kept else 16) * M * H * I, dtype_bytes(p.get("dtype", "bf16")) * (3 * M * H + 6 * H * I + 2 * M * I * kept)
+
+
+def _mxfp4_quantize(p: dict[str, Any]) -> tuple[int, int]:
+    M, K = int(p["M"]), int(p["K"])
+    return 2 * M * K, M * (K * dtype_bytes(p.get("dtype", "bf16")) + 17 * -(-K // 32))
+
+
+def _mxfp4_linear(p: dict[str, Any]) -> tuple[int, int]:
+    M, K, N = (int(p[x]) for x in ("M", "K", "N"))
+    ab = dtype_bytes(p.get("dtype", "bf16"))
+    return 2 * M * N * K, ab * (M * (K + N) + N * bool(p.get("bias"))) + N * 17 * -(-K // 32)
+
+
 _MODELS: dict[str, Callable[[dict[str, Any]], tuple[int, int]]] = {
     "moe_int4_w4a16@1.0.0": _moe_int4_w4a16,
     "moe_sum_reduce@1.0.0": _moe_sum_reduce,
@@ -111,6 +133,11 @@ _MODELS: dict[str, Callable[[dict[str, Any]], tuple[int, int]]] = {
     "lora_projection_backward@1.0.0": _lora_projection_backward,
     "act_checkpoint@1.0.0": _act_checkpoint,
     "act_restore@1.0.0": _act_checkpoint,
+    "gated_ffn@1.0.0": _gated_ffn,
+    "gated_ffn_backward@1.0.0": _gated_ffn_backward,
+    "mxfp4_quantize@1.0.0": _mxfp4_quantize,
+    "mxfp4_dequantize@1.0.0": _mxfp4_quantize,
+    "mxfp4_linear@1.0.0": _mxfp4_linear,
 }
 
 

@@ -130,6 +130,46 @@ def _act_restore(p: dict[str, Any], seed: int, device: str) -> dict[str, Any]:
     return {"held": _held(x), "dtype": to_torch_dtype(p["dtype"])}
 
 
+def _gated_ffn(p: dict[str, Any], seed: int, device: str) -> dict[str, Any]:
+    dt = to_torch_dtype(p["dtype"])
+    M, H, I = (int(p[x]) for x in ("M", "hidden", "ispp"))
+    return {"x": _randn(device, torch.float32, M, H, seed=seed).to(dt),
+            "w13": (_randn(device, torch.float32, 2 * I, H, seed=seed + 1) / H ** 0.5).to(dt),
+            "w2": (_randn(device, torch.float32, H, I, seed=seed + 2) / I ** 0.5).to(dt),
+            "swiglu_limit": float(p["limit"]) if p.get("limit") else None}
+
+
+def _gated_ffn_backward(p: dict[str, Any], seed: int, device: str) -> dict[str, Any]:
+    f = _gated_ffn(p, seed, device)
+    M, dt = int(p["M"]), f["x"].dtype
+    gate_up = _randn(device, torch.float32, M, f["w13"].shape[0], seed=seed + 4).to(dt) if p.get("kept") else None
+    grad = _randn(device, torch.float32, M, f["x"].shape[1], seed=seed + 3).to(dt)
+    return {"grad_out": grad, "x": f["x"], "w13": f["w13"], "w2": f["w2"], "gate_up": gate_up,
+            "swiglu_limit": f["swiglu_limit"]}
+
+
+def _mxfp4(rows: int, K: int, seed: int, device: str):
+    """Any valid codes, with scales about 1."""
+    from ..moe.mxfp4_linear import Mxfp4
+
+    g = torch.Generator(device=device).manual_seed(seed)
+    nb = -(-K // 32)
+    return Mxfp4(torch.randint(0, 256, (rows, 16 * nb), generator=g, device=device, dtype=torch.uint8),
+                 torch.randint(124, 129, (rows, nb), generator=g, device=device, dtype=torch.uint8))
+
+
+def _mxfp4_dequantize(p: dict[str, Any], seed: int, device: str) -> dict[str, Any]:
+    return {"held": _mxfp4(int(p["M"]), int(p["K"]), seed, device), "dtype": to_torch_dtype(p["dtype"])}
+
+
+def _mxfp4_linear(p: dict[str, Any], seed: int, device: str) -> dict[str, Any]:
+    dt = to_torch_dtype(p["dtype"])
+    M, K, N = (int(p[x]) for x in ("M", "K", "N"))
+    bias = _randn(device, torch.float32, N, seed=seed + 2).to(dt) if p.get("bias") else None
+    return {"x": (_randn(device, torch.float32, M, K, seed=seed) / K ** 0.5).to(dt),
+            "weight": _mxfp4(N, K, seed + 1, device), "bias": bias}
+
+
 _GENERATORS: dict[str, Callable[[dict, int, str], dict[str, Any]]] = {
     "moe_sum_reduce@1.0.0": _moe_sum_reduce,
     "moe_align_block_size@1.0.0": _moe_align_block_size,
@@ -142,6 +182,11 @@ _GENERATORS: dict[str, Callable[[dict, int, str], dict[str, Any]]] = {
     "lora_projection_backward@1.0.0": _lora_projection_backward,
     "act_checkpoint@1.0.0": _act_checkpoint,
     "act_restore@1.0.0": _act_restore,
+    "gated_ffn@1.0.0": _gated_ffn,
+    "gated_ffn_backward@1.0.0": _gated_ffn_backward,
+    "mxfp4_quantize@1.0.0": _act_checkpoint,
+    "mxfp4_dequantize@1.0.0": _mxfp4_dequantize,
+    "mxfp4_linear@1.0.0": _mxfp4_linear,
 }
 
 
