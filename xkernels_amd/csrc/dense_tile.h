@@ -16,6 +16,8 @@
 //     chunk; and it issues the loads of later chunks between the products. X has three
 //     places in LDS and W two (160 KB at 256 x 256), so loads stay in flight across the
 //     barrier.
+//   * A workgroup stays for tile after tile and sends for the next one's first chunks before
+//     it writes a tile out.
 //   * The W side is the MFMA's first operand, so a lane's four sums are consecutive n of
 //     one m, which the epilogue writes together.
 //   * Past a tensor's end the buffer loads give zeros; a row's last chunk, where it is
@@ -68,10 +70,15 @@ __device__ __forceinline__ void to_lds_4(i32x4 rsrc, uint32_t lds, int voff, int
                : "memory", "m0");
 }
 
-// Chunks [first, end) of `all` that a launch's slice works on.
+// Chunks [first, end) of `all` that a slice of k has.
 struct Range {
   int first, end, all;
 };
+__device__ __forceinline__ Range range_of(int slice, int slices, int chunks) {
+  const int share = chunks / slices, rest = chunks - share * slices;
+  const int first = slice * share + min(slice, rest);
+  return Range{first, first + share + (slice < rest), chunks};
+}
 
 // Loads one side's chunks. PAIR: the rows of W are gate and up rows of one weight [2 half, k]: of
 // each PAIR rows in LDS (a wave's) the first half are gate rows, the other the up rows of
@@ -242,13 +249,16 @@ struct Product {
   int64_t k_rows;    // of a kColumns side: the number of k
   int64_t blocks;    // MXFP4: blocks of a row
   int chunks;        // of k
-  int tiles_m, tiles_n, slices;
+  // Tiles from `full` on are cut into `slices` of k, whose sums go to `sums` for dense_finish.
+  int tiles_m, tiles_n, full, slices;
+  f32x4* sums;
 };
 
 // Tile `id` of the launch: XCD i (workgroups go round the 8 of them) takes a run of
 // consecutive tiles, ordered in bands of kBand row tiles, so that its 4 MB of L2 sees few
 // rows of X and W at a time.
 constexpr int kBand = 4;
+constexpr int kWavesN = 2;  // side by side in a tile's columns
 __device__ __forceinline__ void tile_of(int id, int total, int tiles_m, int tiles_n, int& tm, int& tn) {
   const int xcd = id & 7, local = id >> 3, share = total >> 3, rest = total & 7;
   const int t = xcd * share + min(xcd, rest) + local;
@@ -262,11 +272,11 @@ __device__ __forceinline__ void tile_of(int id, int total, int tiles_m, int tile
 // n .. n + 3, or, for pairs, `put(int64_t m, int64_t j, f32x4 g, f32x4 u)`; n and j are multiples of 4. WHOLE: they
 // lie within the output, else they may lie past its last column (not its last row): a tile's
 // checks cost more than its stores (16384 x 7168 x 2048 in 4 bits: 293 us with them in every
-// tile, 194 without). blockIdx.y is the slice of k.
-template <Form F, Lay LX, Lay LW, int BM, int BN, int WAVES_N, bool PAIRED, typename EPI>
-__global__ void __launch_bounds__(BM / 64 * WAVES_N * 64)
+// tile, 194 without).
+template <Form F, Lay LX, Lay LW, int BM, int BN, bool DEEP, bool PAIRED, typename EPI>
+__global__ void __launch_bounds__(BM / 64 * kWavesN * 64)
 dense_tile(Product p, EPI epi) {
-  constexpr int WAVES = BM / 64 * WAVES_N, WN = BN / WAVES_N, XT = 4, WT = WN / 16;
+  constexpr int WAVES = BM / 64 * kWavesN, WN = BN / kWavesN, XT = 4, WT = WN / 16;
   constexpr bool FP4 = F == Form::kFp4;
   // (224 columns are loaded as 256: whole loads for every wave)
   constexpr int W_ROWS = BN == 224 ? 256 : BN;
@@ -275,33 +285,49 @@ dense_tile(Product p, EPI epi) {
   using WLoad = Loader<F, LW, W_ROWS, WAVES, PAIRED ? WN : 0>;
   using XScale = ScaleLoader<BM, WAVES>;
   using WScale = ScaleLoader<W_ROWS, WAVES>;
-  // X lies in three places in turn, W in two: while chunk c is read, W of c + 1 and X of c + 1
-  // and c + 2 are on their way, so the loads never run dry. (4 bits: the scales leave X two.)
-  constexpr int XRING = FP4 ? 2 : 3, XI = XLoad::kInstr, WI = WLoad::kInstr;
-  constexpr int W_AT = XRING * XLoad::kBytes, S_AT = W_AT + 2 * WLoad::kBytes;
+  // X lies in XRING places in turn, W in WRING: while chunk c is read, the chunks up to c + WRING - 1
+  // and, of X, c + XRING - 1 are on their way, so the loads never run dry. 256 rows: 3 and 2
+  // (4 bits: the scales leave 2 and 2); DEEP, for a workgroup alone on its CU: 5 and 5 (4 and 4).
+  constexpr int XRING = DEEP ? (FP4 ? 4 : 5) : FP4 ? 2 : 3, WRING = DEEP ? XRING : 2;
+  constexpr int XI = XLoad::kInstr, WI = WLoad::kInstr;
+  static_assert(XRING == WRING || XRING == WRING + 1, "the order of loads that publish() counts on");
+  constexpr int W_AT = XRING * XLoad::kBytes, S_AT = W_AT + WRING * WLoad::kBytes;
   constexpr int SCALES = FP4 ? XScale::kBytes + WScale::kBytes : 0;
-  __shared__ __attribute__((aligned(1024))) char lds[S_AT + 2 * SCALES];
+  __shared__ __attribute__((aligned(1024))) char lds[S_AT + WRING * SCALES];
   const int lane = threadIdx.x & 63, wave = uniform(int(threadIdx.x) >> 6);
-  const int wn = wave % WAVES_N, wm = wave / WAVES_N;
-  int tm, tn;
-  tile_of(blockIdx.x, gridDim.x, p.tiles_m, p.tiles_n, tm, tn);
-  const int64_t m0 = int64_t(tm) * BM, n0 = int64_t(tn) * (PAIRED ? BN / 2 : BN);
-  const int y = blockIdx.y, share = p.chunks / p.slices, rest = p.chunks - share * p.slices;
-  Range range;
-  range.first = y * share + min(y, rest);
-  range.end = range.first + share + (y < rest);
-  range.all = p.chunks;
-
+  const int wn = wave % kWavesN, wm = wave / kWavesN;
   XLoad xl;
   WLoad wl;
-  xl.init(p.x, m0, LX == Lay::kRowsOfK ? p.k_bytes : p.k_rows, range, wave, lane);
-  wl.init(p.w, n0, LW == Lay::kRowsOfK ? p.k_bytes : p.k_rows, range, wave, lane, p.N);
   XScale xsl;
   WScale wsl;
-  if constexpr (FP4) {
-    xsl.init(p.x, m0, p.blocks, range, wave, lane);
-    wsl.init(p.w, n0, p.blocks, range, wave, lane);
-  }
+  int64_t m0, n0;
+  int C, part;  // chunks, and which of the slices' sums (-1: a whole tile)
+  // the lane's number, for what is worked out between tiles and not to be held during one
+  auto lane_again = [&]() __attribute__((always_inline)) {
+    int l = threadIdx.x & 63;
+    asm volatile("" : "+v"(l));
+    return l;
+  };
+  auto open = [&](int job) __attribute__((always_inline)) {
+    const int lane = lane_again();
+    Range range{0, p.chunks, p.chunks};
+    part = job - p.full;
+    if (part >= 0) {
+      job = p.full + part / p.slices;
+      range = range_of(part % p.slices, p.slices, p.chunks);
+    }
+    C = range.end - range.first;
+    int tm, tn;
+    tile_of(job, p.tiles_m * p.tiles_n, p.tiles_m, p.tiles_n, tm, tn);
+    m0 = int64_t(tm) * BM;
+    n0 = int64_t(tn) * (PAIRED ? BN / 2 : BN);
+    xl.init(p.x, m0, LX == Lay::kRowsOfK ? p.k_bytes : p.k_rows, range, wave, lane);
+    wl.init(p.w, n0, LW == Lay::kRowsOfK ? p.k_bytes : p.k_rows, range, wave, lane, p.N);
+    if constexpr (FP4) {
+      xsl.init(p.x, m0, p.blocks, range, wave, lane);
+      wsl.init(p.w, n0, p.blocks, range, wave, lane);
+    }
+  };
   // the next loads' places
   const uint32_t lds0 = uniform(uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds)));
   const uint32_t x_to = lds0 + wave * XI * 1024, w_to = lds0 + W_AT + wave * WI * 1024, s_to = lds0 + S_AT + wave * 256;
@@ -311,7 +337,7 @@ dense_tile(Product p, EPI epi) {
   auto issue_s = [&]() __attribute__((always_inline)) {
     xsl.issue(s_to + s_at, wave);
     wsl.issue(s_to + s_at + XScale::kBytes, wave);
-    s_at ^= SCALES;
+    s_at = s_at == (WRING - 1) * SCALES ? 0 : s_at + SCALES;
   };
   auto next_x = [&]() __attribute__((always_inline)) {
     xl.advance();
@@ -319,7 +345,7 @@ dense_tile(Product p, EPI epi) {
   };
   auto next_w = [&]() __attribute__((always_inline)) {
     wl.advance();
-    w_at = WLoad::kBytes - w_at;
+    w_at = w_at == (WRING - 1) * WLoad::kBytes ? 0 : w_at + WLoad::kBytes;
   };
   Reader<F, LX, BM> xr;
   Reader<F, LW, W_ROWS> wr;
@@ -329,19 +355,15 @@ dense_tile(Product p, EPI epi) {
             sw_at = S_AT + XScale::kBytes + (wn * WN + (lane & 15)) * 8 + (lane >> 4) * 2;
 
   f32x4 acc[WT][XT];
-#pragma unroll
-  for (int a = 0; a < WT; ++a)
-#pragma unroll
-    for (int b = 0; b < XT; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
   // Fragments of the step at hand and, as its W fragments are used up, of the next. W's last one
   // has places of its own in both steps, so that every read is out well before a barrier.
-  constexpr int KEEP = WT - 1;
+  constexpr int KEEP = WT - 1, XLATE = XRING == 2;  // (two places of X: its loads go out as early as W's)
   u32x4 wf[KEEP], we[2], xf[2][XT];
   uint32_t ws[WT], xs[XT], xsn[XT];
   int cx = 0, cw = 0, cs = 0;  // where the chunk to read lies
 
   // Step S of the chunk in registers, while step 1 - S is read: of the same chunk (S = 0), or of
-  // the next one (S = 1); W of the chunk after that (S = 1) and X of one more (S = 0) go out.
+  // the next one (S = 1); a later chunk of W (S = 1) and of X (S = 0) go out.
   auto step = [&](auto STEP, auto READ, auto MATH) __attribute__((always_inline)) {
     constexpr int s = decltype(STEP)::value, n = 1 - s;
     constexpr bool read = decltype(READ)::value, math = decltype(MATH)::value;
@@ -373,7 +395,7 @@ dense_tile(Product p, EPI epi) {
 #pragma unroll
         for (int i = a * WI / WT; i < (a + 1) * WI / WT; ++i) issue_w(i);
       }
-      if constexpr (read && s == (XRING == 2)) {
+      if constexpr (read && s == XLATE) {
 #pragma unroll
         for (int i = a * XI / WT; i < (a + 1) * XI / WT; ++i) issue_x(i);
       }
@@ -388,176 +410,231 @@ dense_tile(Product p, EPI epi) {
       for (int b = 0; b < XT; ++b) xs[b] = xsn[b];
     }
     if constexpr (read && s == 1) next_w();
-    if constexpr (read && s == (XRING == 2)) next_x();
+    if constexpr (read && s == XLATE) next_x();
   };
   // Behind it: all of the next chunk has landed, for every wave, and every wave has read the
   // one before it.
   auto publish = [&]() __attribute__((always_inline)) {
     __builtin_amdgcn_sched_barrier(0);
-    XK_WAIT_VMCNT(XRING == 2 ? 0 : XI);
+    constexpr int CHUNK = XI + WI + (FP4 ? 2 : 0);  // (a wave without a load of scales waits for more)
+    XK_WAIT_VMCNT((WRING - 2) * CHUNK + (XRING > WRING ? XI : 0));
     lds_sync();
     __builtin_amdgcn_sched_barrier(0);
   };
   auto turn = [&]() __attribute__((always_inline)) {  // to the next chunk's places
     cx = cx == (XRING - 1) * XLoad::kBytes ? 0 : cx + XLoad::kBytes;
-    cw = WLoad::kBytes - cw;
-    cs ^= SCALES;
+    cw = cw == (WRING - 1) * WLoad::kBytes ? 0 : cw + WLoad::kBytes;
+    if constexpr (FP4) cs = cs == (WRING - 1) * SCALES ? 0 : cs + SCALES;
   };
   constexpr std::integral_constant<int, 0> S0{};
   constexpr std::integral_constant<int, 1> S1{};
   constexpr std::true_type yes{};
   constexpr std::false_type no{};
-  const int C = range.end - range.first;
-  if (C > 0) {
+  auto send = [&]() __attribute__((always_inline)) {  // a tile's first chunks
+    x_at = w_at = s_at = 0;
 #pragma unroll
-    for (int i = 0; i < XI; ++i) issue_x(i);
-    next_x();
+    for (int r = 0; r < WRING - 1; ++r) {
+      if constexpr (FP4) issue_s();
 #pragma unroll
-    for (int i = 0; i < WI; ++i) issue_w(i);
-    next_w();
-    if constexpr (FP4) issue_s();
-    if constexpr (XRING == 3) {
+      for (int i = 0; i < WI; ++i) issue_w(i);
+      next_w();
 #pragma unroll
       for (int i = 0; i < XI; ++i) issue_x(i);
       next_x();
     }
-    publish();
-    // chunk c's turn: step 1 of c - 1 and step 0 of c, reading both steps of c
-    step(S1, yes, no);
-    step(S0, yes, yes);
-    publish();
-    turn();
-    for (int c = 1; c < C; ++c) {
-      step(S1, yes, yes);
+    if constexpr (XRING > WRING) {
+#pragma unroll
+      for (int i = 0; i < XI; ++i) issue_x(i);
+      next_x();
+    }
+  };
+  const int jobs = p.full + (p.tiles_m * p.tiles_n - p.full) * p.slices;
+  int job = blockIdx.x;
+  open(job);
+  send();
+  while (true) {
+#pragma unroll
+    for (int a = 0; a < WT; ++a)
+#pragma unroll
+      for (int b = 0; b < XT; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    cx = cw = cs = 0;
+    if (C > 0) {
+      publish();
+      // chunk c's turn: step 1 of c - 1 and step 0 of c, reading both steps of c
+      step(S1, yes, no);
       step(S0, yes, yes);
       publish();
       turn();
-    }
-    step(S1, no, yes);
-    XK_WAIT_VMCNT(0);  // no load may land in what is another workgroup's LDS by then
-  }
-
-  const int64_t m = m0 + wm * 64 + (lane & 15), n = n0 + wn * (PAIRED ? WN / 2 : WN) + (lane >> 4) * 4;
-  auto put_all = [&](auto WHOLE) __attribute__((always_inline)) {
-    constexpr bool whole = decltype(WHOLE)::value;
-#pragma unroll
-    for (int a = 0; a < (PAIRED ? WT / 2 : WT); ++a)
-#pragma unroll
-      for (int b = 0; b < XT; ++b) {
-        if (!whole && m + b * 16 >= p.M) continue;
-        if constexpr (PAIRED) epi.template put<whole>(m + b * 16, n + a * 16, acc[a][b], acc[a + WT / 2][b]);
-        else epi.template put<whole>(m + b * 16, n + a * 16, acc[a][b]);
+      for (int c = 1; c < C; ++c) {
+        step(S1, yes, yes);
+        step(S0, yes, yes);
+        publish();
+        turn();
       }
-  };
-  if (m0 + BM <= p.M && n0 + (PAIRED ? BN / 2 : BN) <= p.N) put_all(std::true_type{});
-  else put_all(std::false_type{});
+      step(S1, no, yes);
+    }
+    // the loads of nothing have landed: they are the wave's own, as are the places of the next
+    // ones (and at the end the LDS may be another workgroup's)
+    XK_WAIT_VMCNT(0);
+    const int l = lane_again(), done = part;
+    const int64_t m = m0 + wm * 64, n = n0 + wn * (PAIRED ? WN / 2 : WN);
+    const bool whole_tile = m0 + BM <= p.M && n0 + (PAIRED ? BN / 2 : BN) <= p.N;
+    job += gridDim.x;
+    if (job < jobs) {
+      open(job);
+      send();
+    }
+    // Up to 4 fragments of 16 rows at a time go through LDS (the wave's part of X's last place, which
+    // no load is bound for yet) and come back row by row: whole pieces of a row leave together,
+    // and the epilogue's code is there once for 16 of its calls. Pieces are permuted by the row.
+    f32x4* own = reinterpret_cast<f32x4*>(lds + (XRING - 1) * XLoad::kBytes + wave * 4096);
+    static_assert(XLoad::kBytes == WAVES * 4096, "4 KB of an X place a wave");
+    auto put_all = [&](auto WHOLE) __attribute__((always_inline)) {
+      constexpr bool whole = decltype(WHOLE)::value;
+      constexpr int STRIDE = PAIRED ? 2 : 4;  // fragments of columns a time
+#pragma unroll
+      for (int a0 = 0; a0 < (PAIRED ? WT / 2 : WT); a0 += STRIDE)
+#pragma unroll
+        for (int b = 0; b < XT; ++b) {
+          const int c = l & 15, q = l >> 4;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int a = PAIRED ? a0 + (e & 1) + (e >> 1) * (WT / 2) : a0 + e;
+            if (a < WT) own[c * 16 + ((e * 4 + q) ^ c)] = acc[a][b];
+          }
+          wave_lds_fence();
+          constexpr int LANES = PAIRED ? 8 : 16;  // to a row
+          const int unit = l & (LANES - 1);
+          const int64_t col = n + a0 * 16 + unit * 4;
+#pragma unroll 1
+          for (int row = l / LANES; row < 16; row += 64 / LANES) {
+            const int64_t at = m + b * 16 + row;
+            if ((!whole && at >= p.M) || (!PAIRED && unit >= (WT - a0) * 4)) continue;
+            const f32x4 v = own[row * 16 + (unit ^ row)];
+            if constexpr (PAIRED) epi.template put<whole>(at, col, v, own[row * 16 + ((unit + 8) ^ row)]);
+            else epi.template put<whole>(at, col, v);
+          }
+          wave_lds_fence();
+        }
+    };
+    if (done >= 0) {
+      f32x4* to = p.sums + (int64_t(done) * WAVES + wave) * (WT * XT * 64) + l;
+#pragma unroll
+      for (int a = 0; a < WT; ++a)
+#pragma unroll
+        for (int b = 0; b < XT; ++b) to[(a * XT + b) * 64] = acc[a][b];
+    } else if (whole_tile) {
+      put_all(yes);
+    } else {
+      put_all(no);
+    }
+    if (job >= jobs) break;
+  }
+}
+
+// Adds up the slices of tiles full .., in their order, for the epilogue: a workgroup a wave's
+// 16 columns (pairs: both 16s) x 64 rows.
+template <int BM, int BN, bool PAIRED, typename EPI>
+__global__ void __launch_bounds__(256)
+dense_finish(Product p, EPI epi) {
+  constexpr int WAVES = BM / 64 * kWavesN, WN = BN / kWavesN, XT = 4, WT = WN / 16, AT = PAIRED ? WT / 2 : WT;
+  const int lane = threadIdx.x & 63, b = threadIdx.x >> 6;
+  const int a = blockIdx.x % AT, wave = blockIdx.x / AT % WAVES, rest = blockIdx.x / AT / WAVES;
+  const int wn = wave % kWavesN, wm = wave / kWavesN;
+  int tm, tn;
+  tile_of(p.full + rest, p.tiles_m * p.tiles_n, p.tiles_m, p.tiles_n, tm, tn);
+  const int64_t m = int64_t(tm) * BM + wm * 64 + b * 16 + (lane & 15);
+  const int64_t n = int64_t(tn) * (PAIRED ? BN / 2 : BN) + wn * (PAIRED ? WN / 2 : WN) + a * 16 + (lane >> 4) * 4;
+  if (m >= p.M) return;
+  constexpr int64_t plane = int64_t(WAVES) * WT * XT * 64;
+  const f32x4* at = p.sums + int64_t(rest) * p.slices * plane + (int64_t(wave) * WT + a) * XT * 64 + b * 64 + lane;
+  f32x4 v = *at, u = {};
+  if constexpr (PAIRED) u = at[WT / 2 * XT * 64];
+  for (int s = 1; s < p.slices; ++s) {
+    v += at[s * plane];
+    if constexpr (PAIRED) u += at[s * plane + WT / 2 * XT * 64];
+  }
+  if constexpr (PAIRED) epi.template put<false>(m, n, v, u);
+  else epi.template put<false>(m, n, v);
 }
 
 // ---------------------------------------------------------------- launches ----
 
 // How a product is cut up.
 struct Plan {
-  int cols;    // of a tile: 256 or 224 (with 256 rows), 128 (with 128)
-  int slices;  // of k, whose sums another launch adds up
+  int rows, cols;  // of a tile
+  int full;        // tiles that are not cut; a multiple of the workgroups at a time
+  int slices;      // of k, that the other tiles are cut into
+  int64_t rest;    // the other tiles
 };
+inline int64_t sums_bytes(const Plan& plan) {
+  return plan.slices > 1 ? plan.rest * plan.slices * plan.rows * plan.cols * 4 : 0;
+}
 
 // The cheapest of the tiles and slices, in microseconds as measured (16 bits; MXFP4):
-//   * 256 x 256, a workgroup a CU: 1.47 (2.6) a chunk, however many CUs are busy
-//     (8192 x 4096 x 7168: 333 us; 4096 x 4096 x 7168 in 4 bits: 74);
+//   * 256 x 256, a workgroup a CU: 1.47 (2.3) a chunk, however many CUs are busy
+//     (8192 x 4096 x 7168: 333 us; 4096 x 4096 x 7168 in 4 bits: 67);
 //   * 256 x 224 takes 0.96 of that, and fewer rounds where it divides the columns better
-//     (8192 x 7168 x 4096, 4 rounds of either: 369 us, with 256 x 256 384);
-//   * 128 x 128: two workgroups a CU 0.88 (1.7) a chunk each, one alone 0.75 (0.8)
-//     (8192 x 4096 x 7168: 392 us; 512 x 4096 x 4096: 53 us, where 256 x 256 takes 97);
-//   * slices of k, where 128 x 128 tiles leave CUs idle: another launch, 3 us, and the slices'
-//     sums written and read at 3 TB/s (64 x 4096 x 4096: 1 slice 50 us, 8 slices 11 and 4).
-// `paired`: N columns of gate and N of up.
+//     (8192 x 7168 x 4096, 4 rounds of either: 376 us, with 256 x 256 391);
+//   * 128 x 128: two workgroups a CU 0.88 (1.7) a chunk each, one alone 0.55 (0.62), with more
+//     places in LDS (8192 x 4096 x 7168: 392 us; 512 x 4096 x 4096: 39 us, where 256 x 256 takes 98);
+//   * slices of k, for all tiles where they leave CUs idle or for those of the last round: the
+//     sums written and read at 3 TB/s, and another launch of 5 us (64 x 4096 x 4096: 30 us, with 8
+//     slices 11 and 4).
 inline Plan plan_tiles(bool fp4, int64_t M, int64_t N, int64_t chunks, bool paired) {
   const int64_t cols = paired ? 2 * N : N;
-  const double big = fp4 ? 2.6 : 1.47, two = fp4 ? 1.7 : 0.88, one = fp4 ? 0.8 : 0.75;
-  auto rounds = [&](int64_t bm, int64_t bn, int64_t places) { return double(cdiv(cdiv(M, bm) * cdiv(cols, bn), places)); };
-  Plan best{256, 1};
-  double least = 4 + rounds(256, 256, 256) * big * chunks;
-  auto offer = [&](int c, int s, double us) {
-    if (us < least) {
-      least = us;
-      best = Plan{c, s};
+  const double big = fp4 ? 2.3 : 1.47, two = fp4 ? 1.7 : 0.88, one = fp4 ? 0.62 : 0.55;
+  Plan best{};
+  double least = 1e300;
+  auto offer = [&](int bm, int bn, int64_t places, double chunk, double alone) {
+    const int64_t tiles = cdiv(M, bm) * cdiv(cols, bn), full = tiles / places * places, rest = tiles - full;
+    for (int s = 1; s <= 32 && (s == 1 || (rest * s <= places && 2 * s <= chunks)); s *= 2) {
+      const double each = rest == 0 ? 0 : full == 0 && rest * s <= 256 ? alone : chunk;
+      Plan plan{bm, bn, int(s > 1 ? full : tiles), s, s > 1 ? rest : 0};
+      const double us = 4 + double(full / places) * chunk * chunks + each * double(cdiv(chunks, s)) +
+                        (s > 1 ? 5 + sums_bytes(plan) / 3e6 : 0);
+      if (us < least) {
+        least = us;
+        best = plan;
+      }
     }
   };
-  if (!paired) offer(224, 1, 4 + rounds(256, 224, 256) * 0.96 * big * chunks);
-  const int64_t tiles = cdiv(M, 128) * cdiv(cols, 128);
-  for (int s = 1; s == 1 || (tiles * s <= 512 && 2 * s <= chunks && s <= 32); s *= 2) {
-    const double each = double(cdiv(chunks, s));
-    const double us = 3 + (tiles * s <= 256 ? one * each : double(cdiv(tiles * s, 512)) * two * each);
-    offer(128, s, us + (s > 1 ? 3 + s * M * cols * 4 / 3e6 : 0));
-  }
+  offer(256, 256, 256, big, big);
+  if (!paired) offer(256, 224, 256, 0.96 * big, 0.96 * big);
+  offer(128, 128, 512, two, one);
   return best;
 }
 
-// The slices' sums: planes [M, ld] in fp32, pairs' gate columns from 0, the up columns from ld / 2.
-struct Partial {
-  float* p;
-  int64_t ld, M, N;  // N rounded up to 4
-  template <bool WHOLE> __device__ __forceinline__ void put(int64_t m, int64_t n, f32x4 v) const {
-    if (WHOLE || n < N) *reinterpret_cast<f32x4*>(p + (int64_t(blockIdx.y) * M + m) * ld + n) = v;
-  }
-  template <bool WHOLE> __device__ __forceinline__ void put(int64_t m, int64_t j, f32x4 g, f32x4 u) const {
-    float* at = p + (int64_t(blockIdx.y) * M + m) * ld + j;
-    if (!WHOLE && j >= N) return;
-    *reinterpret_cast<f32x4*>(at) = g;
-    *reinterpret_cast<f32x4*>(at + ld / 2) = u;
-  }
-};
-inline int64_t round4(int64_t n) { return (n + 3) & ~int64_t(3); }
-inline int64_t partial_bytes(const Plan& plan, int64_t M, int64_t N, bool paired) {
-  return plan.slices > 1 ? plan.slices * M * round4(N) * (paired ? 2 : 1) * 4 : 0;
-}
-
-// Adds the slices up, in their order, for the epilogue.
-template <bool PAIRED, typename EPI>
-__global__ void __launch_bounds__(256)
-dense_finish(Partial part, int slices, EPI epi) {
-  const int64_t pieces = part.N / 4, total = part.M * pieces, plane = part.M * part.ld;
-  for (int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x; t < total; t += int64_t(gridDim.x) * 256) {
-    const int64_t m = t / pieces, n = (t - m * pieces) * 4;
-    const float* at = part.p + m * part.ld + n;
-    f32x4 v = *reinterpret_cast<const f32x4*>(at), u = {};
-    if constexpr (PAIRED) u = *reinterpret_cast<const f32x4*>(at + part.ld / 2);
-    for (int s = 1; s < slices; ++s) {
-      v += *reinterpret_cast<const f32x4*>(at + s * plane);
-      if constexpr (PAIRED) u += *reinterpret_cast<const f32x4*>(at + s * plane + part.ld / 2);
-    }
-    if constexpr (PAIRED) epi.template put<false>(m, n, v, u);
-    else epi.template put<false>(m, n, v);
-  }
-}
-
-template <Form F, Lay LX, Lay LW, int BM, int BN, bool PAIRED, typename EPI>
-void launch_cut(Product p, const EPI& epi, hipStream_t stream) {
-  constexpr int kWavesN = 2;
+template <Form F, Lay LX, Lay LW, int BM, int BN, bool DEEP, bool PAIRED, typename EPI>
+void launch_cut(Product p, int64_t places, const EPI& epi, hipStream_t stream) {
   p.tiles_m = int(cdiv(p.M, BM));
   p.tiles_n = int(cdiv(p.N, PAIRED ? BN / 2 : BN));
-  auto* fn = &dense_tile<F, LX, LW, BM, BN, kWavesN, PAIRED, EPI>;
-  hipLaunchKernelGGL(fn, dim3(p.tiles_m * p.tiles_n, p.slices), dim3(BM / 64 * kWavesN * 64), 0, stream, p, epi);
+  const int64_t rest = int64_t(p.tiles_m) * p.tiles_n - p.full, jobs = p.full + rest * p.slices;
+  hipLaunchKernelGGL((dense_tile<F, LX, LW, BM, BN, DEEP, PAIRED, EPI>), dim3(int(std::min(jobs, places))),
+                     dim3(BM / 64 * kWavesN * 64), 0, stream, p, epi);
+  if (rest > 0)
+    hipLaunchKernelGGL((dense_finish<BM, BN, PAIRED, EPI>),
+                       dim3(int(rest * (BM / 64 * kWavesN) * (BN / kWavesN / 16 / (PAIRED ? 2 : 1)))), dim3(256), 0, stream,
+                       p, epi);
 }
 
-// The product with its epilogue; `scratch` holds partial_bytes (16-byte aligned).
+// The product with its epilogue; `scratch` (16-byte aligned) holds the plan's sums_bytes.
 template <Form F, Lay LX, Lay LW, bool PAIRED, typename EPI>
 void launch_tiles(Product p, const EPI& epi, void* scratch, hipStream_t stream) {
   const Plan plan = plan_tiles(F == Form::kFp4, p.M, p.N, p.chunks, PAIRED);
+  p.full = plan.full;
   p.slices = plan.slices;
-  if (plan.slices > 1) {
-    const int64_t n = round4(p.N);
-    const Partial part{static_cast<float*>(scratch), PAIRED ? 2 * n : n, p.M, n};
-    launch_cut<F, LX, LW, 128, 128, PAIRED>(p, part, stream);
-    const int64_t total = p.M * (n / 4);
-    hipLaunchKernelGGL((dense_finish<PAIRED, EPI>), dim3(int(std::min<int64_t>(cdiv(total, 256), 256 * 16))), dim3(256),
-                       0, stream, part, plan.slices, epi);
-  } else if (plan.cols == 128) {
-    launch_cut<F, LX, LW, 128, 128, PAIRED>(p, epi, stream);
+  p.sums = static_cast<f32x4*>(scratch);
+  if (plan.rows == 128) {
+    // deep where every workgroup has a CU to itself
+    if (plan.full + plan.rest * plan.slices <= 256)
+      launch_cut<F, LX, LW, 128, 128, true, PAIRED>(p, 256, epi, stream);
+    else
+      launch_cut<F, LX, LW, 128, 128, false, PAIRED>(p, 512, epi, stream);
   } else if (plan.cols == 224) {
-    if constexpr (!PAIRED) launch_cut<F, LX, LW, 256, 224, false>(p, epi, stream);
+    if constexpr (!PAIRED) launch_cut<F, LX, LW, 256, 224, false, false>(p, 256, epi, stream);
   } else {
-    launch_cut<F, LX, LW, 256, 256, PAIRED>(p, epi, stream);
+    launch_cut<F, LX, LW, 256, 256, false, PAIRED>(p, 256, epi, stream);
   }
 }
 

@@ -150,22 +150,34 @@ template <Form F> struct GateGrad {
   }
 };
 
-// Rows of n values, ld apart, to rows of n8 = pad8(n) with zeros behind them.
-__global__ void __launch_bounds__(256)
-pad_rows(const uint16_t* __restrict__ src, int64_t ld, int64_t rows, int64_t n, int64_t n8, uint16_t* __restrict__ dst) {
-  const int64_t pieces = n8 / 8, total = rows * pieces;
-  for (int64_t q = int64_t(blockIdx.x) * 256 + threadIdx.x; q < total; q += int64_t(gridDim.x) * 256) {
+// Up to 4 matrices of n values a row, ld apart, to rows of n8 = pad8(n) with zeros behind them.
+struct Copies {
+  const uint16_t* src[4];
+  uint16_t* dst[4];
+  int64_t ld[4], n[4], end[4];  // end: in pieces of 8, of the copies up to this one
+  int count = 0;
+};
+__global__ void __launch_bounds__(256) pad_rows(Copies c) {
+  for (int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x; t < c.end[c.count - 1]; t += int64_t(gridDim.x) * 256) {
+    int i = 0;
+    while (t >= c.end[i]) ++i;
+    const int64_t q = i ? t - c.end[i - 1] : t, n = c.n[i], pieces = (n + 7) / 8;
     const int64_t row = q / pieces, k = (q - row * pieces) * 8;
-    const uint16_t* s = src + row * ld + k;
+    const uint16_t* s = c.src[i] + row * c.ld[i] + k;
     __attribute__((aligned(16))) uint16_t v[8];
     if (k + 8 <= n) {
       __builtin_memcpy(v, s, 16);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = k + i < n ? s[i] : uint16_t(0);
+      for (int j = 0; j < 8; ++j) v[j] = k + j < n ? s[j] : uint16_t(0);
     }
-    *reinterpret_cast<u32x4*>(dst + row * n8 + k) = *reinterpret_cast<const u32x4*>(v);
+    *reinterpret_cast<u32x4*>(c.dst[i] + q * 8) = *reinterpret_cast<const u32x4*>(v);
   }
+}
+void launch_copies(const Copies& c, hipStream_t stream) {
+  if (c.count == 0) return;
+  const int grid = int(std::min<int64_t>(cdiv(c.end[c.count - 1], 256), 256 * 32));
+  hipLaunchKernelGGL(pad_rows, dim3(grid), dim3(256), 0, stream, c);
 }
 
 // A matrix [rows, n] of 16-bit values, rows ld apart, whose rows start at 16 bytes.
@@ -178,16 +190,17 @@ struct Matrix {
 };
 
 // Takes the matrix as it is, or, where its width keeps rows from 16 bytes, as a copy with wider rows.
-Matrix take(const void* p, int64_t rows, int64_t n, int64_t ld, char*& ws, hipStream_t stream) {
-  if (n % 8 == 0) return Matrix{p, rows, n, ld};
+Matrix take(const void* p, int64_t rows, int64_t n, int64_t ld, char*& ws, Copies& copies) {
+  if (n % 8 == 0 || rows == 0) return Matrix{p, rows, n, ld};
   const int64_t n8 = pad8(n);
-  uint16_t* to = reinterpret_cast<uint16_t*>(ws);
+  const int i = copies.count++;
+  copies.src[i] = static_cast<const uint16_t*>(p);
+  copies.dst[i] = reinterpret_cast<uint16_t*>(ws);
+  copies.ld[i] = ld;
+  copies.n[i] = n;
+  copies.end[i] = rows * (n8 / 8) + (i ? copies.end[i - 1] : 0);
   ws += aligned(rows * n8 * 2);
-  if (rows > 0) {
-    const int grid = int(std::min<int64_t>(cdiv(rows * n8 / 8, 256), 256 * 32));
-    hipLaunchKernelGGL(pad_rows, dim3(grid), dim3(256), 0, stream, static_cast<const uint16_t*>(p), ld, rows, n, n8, to);
-  }
-  return Matrix{to, rows, n, n8};
+  return Matrix{copies.dst[i], rows, n, n8};
 }
 int64_t taken_bytes(int64_t rows, int64_t n) { return n % 8 == 0 ? 0 : aligned(rows * pad8(n) * 2); }
 
@@ -222,8 +235,10 @@ int forward(const void* x, int64_t ldx, int64_t M, int64_t H, const void* w13, c
     launch_rows<F, void, true>(rows_of(x, M, ldx), rows_of(w13, 2 * I, H), M, I, H, 0, gate, stream);
     launch_rows<F, void, false>(rows_of(h, M, ldh), rows_of(w2, H, I), M, H, I, 0, store, stream);
   } else {
-    const Matrix xm = take(x, M, H, ldx, ws, stream), m13 = take(w13, 2 * I, H, H, ws, stream),
-                 m2 = take(w2, H, I, I, ws, stream), hm{h, M, I, ldh};
+    Copies copies;
+    const Matrix xm = take(x, M, H, ldx, ws, copies), m13 = take(w13, 2 * I, H, H, ws, copies),
+                 m2 = take(w2, H, I, I, ws, copies), hm{h, M, I, ldh};
+    launch_copies(copies, stream);
     launch_tiles<F, R, R, true>(product(xm.of_k(), m13.of_k(), M, I, pad8(H), 0), gate, ws, stream);
     launch_tiles<F, R, R, false>(product(hm.of_k(), m2.of_k(), M, H, ldh, 0), store, ws, stream);
   }
@@ -242,8 +257,10 @@ int backward(const void* dy, int64_t ldg, const void* x, int64_t ldx, int64_t M,
   ws += aligned(M * pad8(I) * 2);
   T* d = reinterpret_cast<T*>(ws);
   ws += aligned(M * pad8(2 * I) * 2);
-  const Matrix xm = take(x, M, H, ldx, ws, stream), m13 = take(w13, 2 * I, H, H, ws, stream),
-               m2 = take(w2, H, I, I, ws, stream), gm = take(dy, M, H, ldg, ws, stream);
+  Copies copies;
+  const Matrix xm = take(x, M, H, ldx, ws, copies), m13 = take(w13, 2 * I, H, H, ws, copies),
+               m2 = take(w2, H, I, I, ws, copies), gm = take(dy, M, H, ldg, ws, copies);
+  launch_copies(copies, stream);
   const Matrix hm{h, M, I, pad8(I)}, dm{d, M, 2 * I, pad8(2 * I)};
   if (M > 0) {
     if (gate_up == nullptr) {
@@ -266,8 +283,8 @@ int backward(const void* dy, int64_t ldg, const void* x, int64_t ldx, int64_t M,
 }
 
 // the slices' sums of a product of k values
-int64_t sums_bytes(int64_t M, int64_t N, int64_t k, bool paired) {
-  return M > 0 ? aligned(partial_bytes(plan_tiles(false, M, N, chunks_of(k), paired), M, N, paired)) : 0;
+int64_t sums_of(int64_t M, int64_t N, int64_t k, bool paired) {
+  return M > 0 ? aligned(sums_bytes(plan_tiles(false, M, N, chunks_of(k), paired))) : 0;
 }
 
 }  // namespace
@@ -276,13 +293,13 @@ int64_t gated_ffn_workspace_bytes(int64_t M, int64_t H, int64_t I) {
   const int64_t h = aligned(M * pad8(I) * 2);
   if (M <= kFewRows) return h;
   return h + taken_bytes(M, H) + taken_bytes(2 * I, H) + taken_bytes(H, I) +
-         std::max(sums_bytes(M, I, pad8(H), true), sums_bytes(M, H, pad8(I), false));
+         std::max(sums_of(M, I, pad8(H), true), sums_of(M, H, pad8(I), false));
 }
 int64_t gated_ffn_backward_workspace_bytes(int64_t M, int64_t H, int64_t I, int recompute) {
   const int64_t k1 = pad8(H), k2 = pad8(2 * I);
-  int64_t sums = std::max(std::max(sums_bytes(M, I, k1, false), sums_bytes(M, H, k2, false)),
-                          std::max(sums_bytes(2 * I, H, M, false), sums_bytes(H, I, M, false)));
-  if (recompute) sums = std::max(sums, sums_bytes(M, I, k1, true)) + aligned(M * 2 * I * 2);
+  int64_t sums = std::max(std::max(sums_of(M, I, k1, false), sums_of(M, H, k2, false)),
+                          std::max(sums_of(2 * I, H, M, false), sums_of(H, I, M, false)));
+  if (recompute) sums = std::max(sums, sums_of(M, I, k1, true)) + aligned(M * 2 * I * 2);
   return aligned(M * pad8(I) * 2) + aligned(M * k2 * 2) + taken_bytes(M, H) * 2 + taken_bytes(2 * I, H) +
          taken_bytes(H, I) + sums;
 }

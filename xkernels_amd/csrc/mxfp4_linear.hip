@@ -138,7 +138,7 @@ int64_t mxfp4_linear_workspace_bytes(int64_t M, int64_t K, int64_t N) {
   if (M <= kFewRows) return 0;
   const int64_t blocks = cdiv(K, kMx4Block), lds = pad4(blocks);
   return aligned(M * blocks * 16) + aligned(M * lds) + (lds == blocks ? 0 : aligned(N * lds)) +
-         partial_bytes(plan_tiles(true, M, N, cdiv(blocks, 8), false), M, N, false);
+         sums_bytes(plan_tiles(true, M, N, cdiv(blocks, 8), false));
 }
 
 int launch_mxfp4_linear(const void* x, int dtype, int64_t ldx, const uint8_t* x_scales, int64_t M, int64_t K,
