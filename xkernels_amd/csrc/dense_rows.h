@@ -167,8 +167,7 @@ dense_rows(Rows x, Rows w, int64_t M, int64_t N, int64_t K, int64_t x_values, EP
     for (int v = 1; v < kRowWaves; ++v) t += sums[v][at];
     return t;
   };
-  if constexpr (PAIRED) epi.template put<false>(int64_t(c), n0 + q * 4, total(lane), total(lane + 32));
-  else epi.template put<false>(int64_t(c), n0 + q * 4, total(lane));
+  finish<EPI, PAIRED>(epi.spot(0, n0), c, q * 4, total(lane), PAIRED ? total((lane + 32) & 63) : f32x4{});
 }
 
 // More rows are cheaper in tiles with slices of k (32 x 4096 x 4096: 10 and 4 us, where two row

@@ -268,11 +268,14 @@ __device__ __forceinline__ void tile_of(int id, int total, int tiles_m, int tile
   tm = band * kBand + in - tn * height;
 }
 
-// EPI: struct with `template <bool WHOLE> void put(int64_t m, int64_t n, f32x4 v)`, the sums of row m and columns
-// n .. n + 3, or, for pairs, `put(int64_t m, int64_t j, f32x4 g, f32x4 u)`; n and j are multiples of 4. WHOLE: they
-// lie within the output, else they may lie past its last column (not its last row): a tile's
-// checks cost more than its stores (16384 x 7168 x 2048 in 4 bits: 293 us with them in every
-// tile, 194 without).
+// EPI: a struct whose `spot(m, n)` gives, for a wave's first row and column (pairs: of a half), a struct with
+// `template <bool WHOLE> void put(int row, int col, f32x4 v)`: the sums of row m + row and columns
+// n + col .. + 3, or, for pairs, `put(row, col, f32x4 g, f32x4 u)`; col is a multiple of 4, row and col are
+// below 256. WHOLE: they lie within the output, else they may lie past its last column (not its
+// last row). Addresses come from the wave's place and 32-bit offsets, and whole tiles have no checks:
+// a tile's epilogue is code that nothing hides (16384 x 7168 x 2048 in 4 bits: 293 us with checks
+// in every tile, 194 without). With EPI::kFetches, put takes a last argument, what
+// `fetch<WHOLE>(row, col)` read from memory for it: the tile kernel calls that ahead.
 template <Form F, Lay LX, Lay LW, int BM, int BN, bool DEEP, bool PAIRED, typename EPI>
 __global__ void __launch_bounds__(BM / 64 * kWavesN * 64)
 dense_tile(Product p, EPI epi) {
@@ -477,7 +480,8 @@ dense_tile(Product p, EPI epi) {
     // ones (and at the end the LDS may be another workgroup's)
     XK_WAIT_VMCNT(0);
     const int l = lane_again(), done = part;
-    const int64_t m = m0 + wm * 64, n = n0 + wn * (PAIRED ? WN / 2 : WN);
+    const int rows_left = int(min(p.M - m0 - wm * 64, int64_t(64)));
+    const auto spot = epi.spot(m0 + wm * 64, n0 + wn * (PAIRED ? WN / 2 : WN));
     const bool whole_tile = m0 + BM <= p.M && n0 + (PAIRED ? BN / 2 : BN) <= p.N;
     job += gridDim.x;
     if (job < jobs) {
@@ -486,36 +490,72 @@ dense_tile(Product p, EPI epi) {
     }
     // Up to 4 fragments of 16 rows at a time go through LDS (the wave's part of X's last place, which
     // no load is bound for yet) and come back row by row: whole pieces of a row leave together,
-    // and the epilogue's code is there once for 16 of its calls. Pieces are permuted by the row.
+    // and the epilogue's code is there once for 16 of its calls (code that runs once comes from
+    // memory: the checked form of GateGrad, unrolled, took a 128 x 128 tile 20 us). Pieces are
+    // permuted by the row.
     f32x4* own = reinterpret_cast<f32x4*>(lds + (XRING - 1) * XLoad::kBytes + wave * 4096);
     static_assert(XLoad::kBytes == WAVES * 4096, "4 KB of an X place a wave");
     auto put_all = [&](auto WHOLE) __attribute__((always_inline)) {
       constexpr bool whole = decltype(WHOLE)::value;
-      constexpr int STRIDE = PAIRED ? 2 : 4;  // fragments of columns a time
+      constexpr int AT = PAIRED ? WT / 2 : WT, STRIDE = PAIRED ? 2 : 4;  // fragments of columns, and at a time
+      constexpr int LANES = PAIRED ? 8 : 16, ROWS = 64 / LANES;          // to a row, and rows of a wave at a time
+      constexpr int TIMES = (AT + STRIDE - 1) / STRIDE * XT;
+      const int unit = l & (LANES - 1);
+      auto stage = [&](int t) __attribute__((always_inline)) {
+        const int a0 = t / XT * STRIDE, b = t % XT, c = l & 15, q = l >> 4;
 #pragma unroll
-      for (int a0 = 0; a0 < (PAIRED ? WT / 2 : WT); a0 += STRIDE)
-#pragma unroll
-        for (int b = 0; b < XT; ++b) {
-          const int c = l & 15, q = l >> 4;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int a = PAIRED ? a0 + (e & 1) + (e >> 1) * (WT / 2) : a0 + e;
-            if (a < WT) own[c * 16 + ((e * 4 + q) ^ c)] = acc[a][b];
-          }
-          wave_lds_fence();
-          constexpr int LANES = PAIRED ? 8 : 16;  // to a row
-          const int unit = l & (LANES - 1);
-          const int64_t col = n + a0 * 16 + unit * 4;
-#pragma unroll 1
-          for (int row = l / LANES; row < 16; row += 64 / LANES) {
-            const int64_t at = m + b * 16 + row;
-            if ((!whole && at >= p.M) || (!PAIRED && unit >= (WT - a0) * 4)) continue;
-            const f32x4 v = own[row * 16 + (unit ^ row)];
-            if constexpr (PAIRED) epi.template put<whole>(at, col, v, own[row * 16 + ((unit + 8) ^ row)]);
-            else epi.template put<whole>(at, col, v);
-          }
-          wave_lds_fence();
+        for (int e = 0; e < 4; ++e) {
+          const int a = PAIRED ? a0 + (e & 1) + (e >> 1) * (WT / 2) : a0 + e;
+          if (a < WT) own[c * 16 + ((e * 4 + q) ^ c)] = acc[a][b];
         }
+        wave_lds_fence();
+      };
+      // whether the lane has something to write in row `row` of turn t
+      auto holds = [&](int t, int row) __attribute__((always_inline)) {
+        return (whole || t % XT * 16 + row < rows_left) && (PAIRED || unit < (WT - t / XT * STRIDE) * 4);
+      };
+      if constexpr (EPI::kFetches) if constexpr (whole) {
+        static_assert(!PAIRED, "no pairs with values of memory");
+        decltype(spot.template fetch<whole>(0, 0)) held[2][16 / ROWS];
+        auto fetch = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+          for (int r = 0; r < 16 / ROWS; ++r) {
+            const int row = l / LANES + r * ROWS;
+            if (holds(t, row)) held[t & 1][r] = spot.template fetch<whole>(t % XT * 16 + row, t / XT * STRIDE * 16 + unit * 4);
+          }
+        };
+        fetch(0);
+#pragma unroll
+        for (int t = 0; t < TIMES; ++t) {
+          if (t + 1 < TIMES) fetch(t + 1);
+          stage(t);
+#pragma unroll
+          for (int r = 0; r < 16 / ROWS; ++r) {
+            const int row = l / LANES + r * ROWS;
+            if (holds(t, row))
+              spot.template put<whole>(t % XT * 16 + row, t / XT * STRIDE * 16 + unit * 4, own[row * 16 + (unit ^ row)],
+                                       held[t & 1][r]);
+          }
+          wave_lds_fence();
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        return;
+      }
+#pragma unroll
+      for (int t = 0; t < TIMES; ++t) {
+        stage(t);
+        const int col = t / XT * STRIDE * 16 + unit * 4;
+#pragma unroll 1
+        for (int row = l / LANES; row < 16; row += ROWS) {
+          if (!holds(t, row)) continue;
+          const int at = t % XT * 16 + row;
+          const f32x4 v = own[row * 16 + (unit ^ row)];
+          if constexpr (PAIRED) spot.template put<whole>(at, col, v, own[row * 16 + ((unit + 8) ^ row)]);
+          else if constexpr (EPI::kFetches) spot.template put<whole>(at, col, v, spot.template fetch<whole>(at, col));
+          else spot.template put<whole>(at, col, v);
+        }
+        wave_lds_fence();
+      }
     };
     if (done >= 0) {
       f32x4* to = p.sums + (int64_t(done) * WAVES + wave) * (WT * XT * 64) + l;
@@ -532,20 +572,29 @@ dense_tile(Product p, EPI epi) {
   }
 }
 
+// One group of sums to the epilogue, outside the tile kernel.
+template <typename EPI, bool PAIRED, typename SPOT>
+__device__ __forceinline__ void finish(const SPOT& spot, int row, int col, f32x4 v, f32x4 u) {
+  if constexpr (PAIRED) spot.template put<false>(row, col, v, u);
+  else if constexpr (EPI::kFetches) spot.template put<false>(row, col, v, spot.template fetch<false>(row, col));
+  else spot.template put<false>(row, col, v);
+}
+
 // Adds up the slices of tiles full .., in their order, for the epilogue: a workgroup a wave's
 // 16 columns (pairs: both 16s) x 64 rows.
 template <int BM, int BN, bool PAIRED, typename EPI>
 __global__ void __launch_bounds__(256)
 dense_finish(Product p, EPI epi) {
   constexpr int WAVES = BM / 64 * kWavesN, WN = BN / kWavesN, XT = 4, WT = WN / 16, AT = PAIRED ? WT / 2 : WT;
-  const int lane = threadIdx.x & 63, b = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, b = uniform(int(threadIdx.x) >> 6);
   const int a = blockIdx.x % AT, wave = blockIdx.x / AT % WAVES, rest = blockIdx.x / AT / WAVES;
   const int wn = wave % kWavesN, wm = wave / kWavesN;
   int tm, tn;
   tile_of(p.full + rest, p.tiles_m * p.tiles_n, p.tiles_m, p.tiles_n, tm, tn);
-  const int64_t m = int64_t(tm) * BM + wm * 64 + b * 16 + (lane & 15);
-  const int64_t n = int64_t(tn) * (PAIRED ? BN / 2 : BN) + wn * (PAIRED ? WN / 2 : WN) + a * 16 + (lane >> 4) * 4;
-  if (m >= p.M) return;
+  const int64_t m = int64_t(tm) * BM + wm * 64 + b * 16;
+  const int64_t n = int64_t(tn) * (PAIRED ? BN / 2 : BN) + wn * (PAIRED ? WN / 2 : WN) + a * 16;
+  const int row = lane & 15, col = (lane >> 4) * 4;
+  if (m + row >= p.M) return;
   constexpr int64_t plane = int64_t(WAVES) * WT * XT * 64;
   const f32x4* at = p.sums + int64_t(rest) * p.slices * plane + (int64_t(wave) * WT + a) * XT * 64 + b * 64 + lane;
   f32x4 v = *at, u = {};
@@ -554,8 +603,7 @@ dense_finish(Product p, EPI epi) {
     v += at[s * plane];
     if constexpr (PAIRED) u += at[s * plane + WT / 2 * XT * 64];
   }
-  if constexpr (PAIRED) epi.template put<false>(m, n, v, u);
-  else epi.template put<false>(m, n, v);
+  finish<EPI, PAIRED>(epi.spot(m, n), row, col, v, u);
 }
 
 // ---------------------------------------------------------------- launches ----
@@ -576,14 +624,14 @@ inline int64_t sums_bytes(const Plan& plan) {
 //     (8192 x 4096 x 7168: 333 us; 4096 x 4096 x 7168 in 4 bits: 67);
 //   * 256 x 224 takes 0.96 of that, and fewer rounds where it divides the columns better
 //     (8192 x 7168 x 4096, 4 rounds of either: 376 us, with 256 x 256 391);
-//   * 128 x 128: two workgroups a CU 0.88 (1.7) a chunk each, one alone 0.55 (0.62), with more
+//   * 128 x 128: two workgroups a CU 0.88 (1.7) a chunk each, one alone 0.75, with more
 //     places in LDS (8192 x 4096 x 7168: 392 us; 512 x 4096 x 4096: 39 us, where 256 x 256 takes 98);
 //   * slices of k, for all tiles where they leave CUs idle or for those of the last round: the
-//     sums written and read at 3 TB/s, and another launch of 5 us (64 x 4096 x 4096: 30 us, with 8
+//     sums written and read at 3 TB/s, and another launch of 4 us (64 x 4096 x 4096: 30 us, with 8
 //     slices 11 and 4).
 inline Plan plan_tiles(bool fp4, int64_t M, int64_t N, int64_t chunks, bool paired) {
   const int64_t cols = paired ? 2 * N : N;
-  const double big = fp4 ? 2.3 : 1.47, two = fp4 ? 1.7 : 0.88, one = fp4 ? 0.62 : 0.55;
+  const double big = fp4 ? 2.3 : 1.47, two = fp4 ? 1.7 : 0.88, one = 0.75;
   Plan best{};
   double least = 1e300;
   auto offer = [&](int bm, int bn, int64_t places, double chunk, double alone) {
@@ -592,7 +640,7 @@ inline Plan plan_tiles(bool fp4, int64_t M, int64_t N, int64_t chunks, bool pair
       const double each = rest == 0 ? 0 : full == 0 && rest * s <= 256 ? alone : chunk;
       Plan plan{bm, bn, int(s > 1 ? full : tiles), s, s > 1 ? rest : 0};
       const double us = 4 + double(full / places) * chunk * chunks + each * double(cdiv(chunks, s)) +
-                        (s > 1 ? 5 + sums_bytes(plan) / 3e6 : 0);
+                        (s > 1 ? 4 + sums_bytes(plan) / 3e6 : 0);
       if (us < least) {
         least = us;
         best = plan;

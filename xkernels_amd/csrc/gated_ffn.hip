@@ -55,98 +55,140 @@ template <typename T> __device__ __forceinline__ four<T> load_four(const T* p, i
 
 // out[m, n] in the type.
 template <Form F> struct Store {
-  typename num<F>::type* out;
+  static constexpr bool kFetches = false;
+  typedef typename num<F>::type T;
+  T* out;
   int64_t ld, N;
-  template <bool WHOLE> __device__ __forceinline__ void put(int64_t m, int64_t n, f32x4 sum) const {
-    four<typename num<F>::type> v;
+  struct Spot {
+    T* out;
+    int ld, left;  // columns from the spot on
+    template <bool WHOLE> __device__ __forceinline__ void put(int row, int col, f32x4 sum) const {
+      four<T> v;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v.v[i] = num<F>::put(sum[i]);
-    store_four(out + m * ld + n, v, WHOLE ? 4 : N - n);
-  }
+      for (int i = 0; i < 4; ++i) v.v[i] = num<F>::put(sum[i]);
+      store_four(out + uint32_t(row * ld + col), v, WHOLE ? 4 : left - col);
+    }
+  };
+  __device__ __forceinline__ Spot spot(int64_t m, int64_t n) const { return Spot{out + m * ld + n, int(ld), int(N - n)}; }
 };
+
+// The activation's parts. `limit` is an infinity where there is none.
+__device__ __forceinline__ bool past(float v, float limit) { return v > limit; }  // (NaN is not)
+// min(g, L) and clamp(u, -L, L); NaN stays NaN
+__device__ __forceinline__ float below(float g, float limit) { return past(g, limit) ? limit : g; }
+__device__ __forceinline__ float within(float u, float limit) { return past(fabsf(u), limit) ? copysignf(limit, u) : u; }
+// (the reciprocal is within a step of fp32, as a division is; of an infinity it is 0)
+__device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
 
 // A sum as gate_up holds it: rounded to the type, but never over the limit or back onto it,
 // so that the gradient passes where the sum itself let it.
 template <Form F> __device__ __forceinline__ typename num<F>::type held(float v, float limit) {
   typedef typename num<F>::type T;
   const T r = num<F>::put(v);
-  if (limit > 0.f) {
-    const bool past = fabsf(v) > limit, r_past = fabsf(num<F>::get(r)) > limit;
-    if (past != r_past && v == v) {  // one step away from zero, or towards it
+  if (limit < __builtin_inff()) {
+    const bool over = past(fabsf(v), limit), r_over = past(fabsf(num<F>::get(r)), limit);
+    if (over != r_over) {  // one step away from zero, or towards it
       const uint16_t b = __builtin_bit_cast(uint16_t, r);
-      return __builtin_bit_cast(T, uint16_t(past ? b + 1 : b - 1));
+      return __builtin_bit_cast(T, uint16_t(over ? b + 1 : b - 1));
     }
   }
   return r;
 }
 
-// (the reciprocal is within a step of fp32, as a division is; of an infinity it is 0)
-__device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
-// min(g, L) and clamp(u, -L, L); NaN stays NaN
-__device__ __forceinline__ float below(float g, float limit) { return limit > 0.f && g > limit ? limit : g; }
-__device__ __forceinline__ float within(float u, float limit) {
-  return limit > 0.f && fabsf(u) > limit ? copysignf(limit, u) : u;
-}
-
 // h = silu(g) u, in rows ldh apart whose places past the I columns are zeros, and
 // gate_up [M, 2 I] (either may be null).
 template <Form F> struct Gate {
-  typename num<F>::type *h, *gate_up;
+  static constexpr bool kFetches = false;
+  typedef typename num<F>::type T;
+  T *h, *gate_up;
   int64_t ldh, I;
   float limit;
-  template <bool WHOLE> __device__ __forceinline__ void put(int64_t m, int64_t j, f32x4 gs, f32x4 us) const {
-    typedef typename num<F>::type T;
-    if (!WHOLE && j >= I) return;
-    four<T> g, u, v;
+  struct Spot {
+    T *h, *g, *u;
+    int ldh, ldg, left;
+    float limit;
+    template <bool WHOLE> __device__ __forceinline__ void put(int row, int col, f32x4 gs, f32x4 us) const {
+      if (!WHOLE && col >= left) return;
+      if (h != nullptr) {
+        four<T> v;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      g.v[i] = held<F>(gs[i], limit);
-      u.v[i] = held<F>(us[i], limit);
-      const float gc = below(gs[i], limit), uc = within(us[i], limit);
-      v.v[i] = WHOLE || j + i < I ? num<F>::put(gc * sigmoid(gc) * uc) : T(0);
+        for (int i = 0; i < 4; ++i) {
+          const float gc = below(gs[i], limit), uc = within(us[i], limit);
+          v.v[i] = WHOLE || col + i < left ? num<F>::put(gc * sigmoid(gc) * uc) : T(0);
+        }
+        T* at = h + uint32_t(row * ldh + col);
+        store_unaligned(at, v);  // (rows end at a multiple of 8)
+        if (!WHOLE && col + 4 >= left && (left & 7) <= 4 && (left & 7) > 0) store_unaligned(at + 4, four<T>{});
+      }
+      if (g != nullptr) {
+        four<T> gr, ur;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          gr.v[i] = held<F>(gs[i], limit);
+          ur.v[i] = held<F>(us[i], limit);
+        }
+        const uint32_t at = uint32_t(row * ldg + col);
+        store_four(g + at, gr, WHOLE ? 4 : left - col);
+        store_four(u + at, ur, WHOLE ? 4 : left - col);
+      }
     }
-    if (h != nullptr) {
-      store_four(h + m * ldh + j, v, WHOLE ? 4 : ldh - j);
-      if (!WHOLE && j + 4 >= I)
-        for (int64_t c = j + 4; c < ldh; ++c) h[m * ldh + c] = T(0);
-    }
-    if (gate_up != nullptr) {
-      store_four(gate_up + m * 2 * I + j, g, WHOLE ? 4 : I - j);
-      store_four(gate_up + m * 2 * I + I + j, u, WHOLE ? 4 : I - j);
-    }
+  };
+  __device__ __forceinline__ Spot spot(int64_t m, int64_t j) const {
+    T* g = gate_up == nullptr ? nullptr : gate_up + m * 2 * I + j;
+    return Spot{h == nullptr ? nullptr : h + m * ldh + j, g, g + I, int(ldh), int(2 * I), int(I - j), limit};
   }
 };
 
 // From dh and gate_up [M, 2 I]: d [M, 2 I] = [dg du] and h [M, I], rows ldd and ldh apart with
 // zeros behind them.
 template <Form F> struct GateGrad {
-  const typename num<F>::type* gate_up;
-  typename num<F>::type *d, *h;
+  static constexpr bool kFetches = true;
+  typedef typename num<F>::type T;
+  const T* gate_up;
+  T *d, *h;
   int64_t ldd, ldh, I;
   float limit;
-  template <bool WHOLE> __device__ __forceinline__ void put(int64_t m, int64_t j, f32x4 dh) const {
-    typedef typename num<F>::type T;
-    if (!WHOLE && j >= I) return;
-    const int64_t left = WHOLE ? 4 : I - j;
-    const four<T> g = load_four(gate_up + m * 2 * I + j, left);
-    const four<T> u = load_four(gate_up + m * 2 * I + I + j, left);
-    four<T> dg, du, v;
+  struct Kept {
+    four<T> g, u;
+  };
+  struct Spot {
+    const T *g, *u;
+    T *dg, *du, *h;
+    int ldg, ldd, ldh, left;
+    float limit;
+    template <bool WHOLE> __device__ __forceinline__ Kept fetch(int row, int col) const {
+      const uint32_t at = uint32_t(row * ldg + col);
+      return Kept{load_four(g + at, WHOLE ? 4 : left - col), load_four(u + at, WHOLE ? 4 : left - col)};
+    }
+    template <bool WHOLE> __device__ __forceinline__ void put(int row, int col, f32x4 dh, const Kept& kept) const {
+      if (!WHOLE && col >= left) return;
+      four<T> gr, ur, v;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float gs = num<F>::get(g.v[i]), us = num<F>::get(u.v[i]);
-      const float gc = below(gs, limit), uc = within(us, limit), s = sigmoid(gc);
-      const bool on_g = !(limit > 0.f && gs > limit), on_u = !(limit > 0.f && fabsf(us) > limit);
-      dg.v[i] = num<F>::put(on_g ? dh[i] * uc * s * (1.0f + gc * (1.0f - s)) : 0.f);
-      du.v[i] = num<F>::put(on_u ? dh[i] * gc * s : 0.f);
-      v.v[i] = WHOLE || i < left ? num<F>::put(gc * s * uc) : T(0);
+      for (int i = 0; i < 4; ++i) {
+        const float gs = num<F>::get(kept.g.v[i]), us = num<F>::get(kept.u.v[i]);
+        const bool g_over = past(gs, limit), u_over = past(fabsf(us), limit);
+        const float gc = g_over ? limit : gs, uc = u_over ? copysignf(limit, us) : us;
+        const float s = sigmoid(gc), silu = gc * s, slope = fmaf(silu, 1.0f - s, s);
+        gr.v[i] = num<F>::put(g_over ? 0.f : dh[i] * uc * slope);
+        ur.v[i] = num<F>::put(u_over ? 0.f : dh[i] * silu);
+        v.v[i] = WHOLE || col + i < left ? num<F>::put(silu * uc) : T(0);
+      }
+      const uint32_t at = uint32_t(row * ldd + col);
+      store_four(dg + at, gr, WHOLE ? 4 : left - col);
+      store_four(du + at, ur, WHOLE ? 4 : left - col);
+      T* hat = h + uint32_t(row * ldh + col);
+      store_unaligned(hat, v);  // (rows end at a multiple of 8)
+      if (col + 4 >= left) {    // a row's last columns: the zeros behind them
+        if ((left & 7) <= 4 && (left & 7) > 0) store_unaligned(hat + 4, four<T>{});
+        T* end = du + uint32_t(row * ldd + left);
+        for (int c = 0; c < ldd - ldg; ++c) end[c] = T(0);
+      }
     }
-    store_four(d + m * ldd + j, dg, left);
-    store_four(d + m * ldd + I + j, du, left);
-    store_four(h + m * ldh + j, v, WHOLE ? 4 : ldh - j);
-    if (j + 4 >= I) {  // (the last columns of a whole tile may be a row's last)
-      for (int64_t c = 2 * I; c < ldd; ++c) d[m * ldd + c] = T(0);
-      for (int64_t c = j + 4; c < ldh; ++c) h[m * ldh + c] = T(0);
-    }
+  };
+  __device__ __forceinline__ Spot spot(int64_t m, int64_t j) const {
+    const T* g = gate_up + m * 2 * I + j;
+    T* dg = d + m * ldd + j;
+    return Spot{g, g + I, dg, dg + I, h + m * ldh + j, int(2 * I), int(ldd), int(ldh), int(I - j), limit};
   }
 };
 
@@ -225,6 +267,7 @@ int forward(const void* x, int64_t ldx, int64_t M, int64_t H, const void* w13, c
             void* out, void* gate_up, void* workspace, hipStream_t stream) {
   typedef typename num<F>::type T;
   constexpr Lay R = Lay::kRowsOfK;
+  limit = limit > 0.f ? limit : __builtin_inff();
   char* ws = static_cast<char*>(workspace);
   T* h = reinterpret_cast<T*>(ws);
   const int64_t ldh = pad8(I);
@@ -252,6 +295,7 @@ int backward(const void* dy, int64_t ldg, const void* x, int64_t ldx, int64_t M,
              void* workspace, hipStream_t stream) {
   typedef typename num<F>::type T;
   constexpr Lay R = Lay::kRowsOfK, C = Lay::kColumns;
+  limit = limit > 0.f ? limit : __builtin_inff();
   char* ws = static_cast<char*>(workspace);
   T* h = reinterpret_cast<T*>(ws);
   ws += aligned(M * pad8(I) * 2);

@@ -33,23 +33,36 @@ template <> struct val<float> {
 };
 
 template <typename T, bool BIAS> struct Store {
+  static constexpr bool kFetches = BIAS;
   T* out;
   const T* bias;
   int64_t N;
-  template <bool WHOLE> __device__ __forceinline__ void put(int64_t m, int64_t n, f32x4 sum) const {
-    struct four { T v[4]; } v;
-    const int64_t left = WHOLE ? 4 : N - n;
-    T* to = out + m * N + n;
+  struct Spot {
+    T* out;
+    const T* bias;
+    int ld, left;  // columns from the spot on
+    template <bool WHOLE> __device__ __forceinline__ f32x4 fetch(int, int col) const {
+      f32x4 v;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      v.v[i] = val<T>::put(BIAS && (WHOLE || i < left) ? sum[i] + val<T>::get(bias[n + i]) : sum[i]);
-    if (left >= 4) {
-      store_unaligned(to, v);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 3; ++i)
-        if (i < left) to[i] = v.v[i];
+      for (int i = 0; i < 4; ++i) v[i] = WHOLE || col + i < left ? val<T>::get(bias[col + i]) : 0.f;
+      return v;
     }
+    template <bool WHOLE> __device__ __forceinline__ void put(int row, int col, f32x4 sum, f32x4 add = {}) const {
+      struct four { T v[4]; } v;
+      T* to = out + uint32_t(row * ld + col);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v.v[i] = val<T>::put(BIAS ? sum[i] + add[i] : sum[i]);
+      if (WHOLE || left - col >= 4) {
+        store_unaligned(to, v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+          if (col + i < left) to[i] = v.v[i];
+      }
+    }
+  };
+  __device__ __forceinline__ Spot spot(int64_t m, int64_t n) const {
+    return Spot{out + m * N + n, bias + n, int(N), int(N - n)};
   }
 };
 
