@@ -1,7 +1,7 @@
 // extern "C" entry points of the dense block beside the experts: the gated feed-forward
 // block and its gradients, MXFP4 quantisation and products (declared in
 // include/xk_moe.h). Arguments are checked here, before any launch.
-#include "common.h"
+#include "mx4.h"
 
 namespace xk {
 
@@ -12,8 +12,6 @@ int launch_gated_ffn(const void* x, int dtype, int64_t ldx, int64_t M, int64_t H
 int launch_gated_ffn_backward(const void* dy, int dtype, int64_t ldg, const void* x, int64_t ldx, int64_t M, int64_t H,
                               const void* w13, const void* w2, int64_t I, const void* gate_up, float limit, void* dx,
                               void* dw13, void* dw2, void* ws, hipStream_t stream);
-int launch_mxfp4_quantize(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, uint8_t* codes, uint8_t* scales,
-                          int64_t lds, hipStream_t stream);
 int launch_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, int dtype, void* out,
                             hipStream_t stream);
 int64_t mxfp4_linear_workspace_bytes(int64_t M, int64_t K, int64_t N);
@@ -116,7 +114,7 @@ int xk_mxfp4_quantize(const void* x, int32_t dtype, int64_t ldx, int64_t M, int6
   if (M == 0) return XK_OK;
   XK_REQUIRE(x && codes && scales, "mxfp4_quantize: null pointer");
   XK_REQUIRE(M == 1 || ldx >= K, "mxfp4_quantize: rows overlap (ldx)");
-  return launch_mxfp4_quantize(x, dtype, ldx, M, K, codes, scales, cdiv(K, 32), stream);
+  return launch_mxfp4_quantize(x, dtype, ldx, M, K, codes, scales, cdiv(K, 32), ScaleRows{}, stream);
 }
 
 int xk_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, int32_t dtype, void* out,

@@ -560,9 +560,11 @@ dense_tile(Product p, EPI epi) {
     if (done >= 0) {
       f32x4* to = p.sums + (int64_t(done) * WAVES + wave) * (WT * XT * 64) + l;
 #pragma unroll
-      for (int a = 0; a < WT; ++a)
+      for (int b = 0; b < XT; ++b) {
+        if (b * 16 >= rows_left) break;  // (rows past the last are not added up either)
 #pragma unroll
-        for (int b = 0; b < XT; ++b) to[(a * XT + b) * 64] = acc[a][b];
+        for (int a = 0; a < WT; ++a) to[(a * XT + b) * 64] = acc[a][b];
+      }
     } else if (whole_tile) {
       put_all(yes);
     } else {
@@ -627,8 +629,9 @@ inline int64_t sums_bytes(const Plan& plan) {
 //   * 128 x 128: two workgroups a CU 0.88 (1.7) a chunk each, one alone 0.75, with more
 //     places in LDS (8192 x 4096 x 7168: 392 us; 512 x 4096 x 4096: 39 us, where 256 x 256 takes 98);
 //   * slices of k, for all tiles where they leave CUs idle or for those of the last round: the
-//     sums written and read at 3 TB/s, and another launch of 4 us (64 x 4096 x 4096: 30 us, with 8
-//     slices 11 and 4).
+//     sums written and read at 3 TB/s, and another launch of 4 us and half a one for each slice
+//     (64 x 4096 x 4096: 30 us, with 8 slices 11 and 4; 64 x 4096 x 2048: 4 slices 11 and 4, 8 slices
+//     14 and 5); without them 3 us for results written by few workgroups.
 inline Plan plan_tiles(bool fp4, int64_t M, int64_t N, int64_t chunks, bool paired) {
   const int64_t cols = paired ? 2 * N : N;
   const double big = fp4 ? 2.3 : 1.47, two = fp4 ? 1.7 : 0.88, one = 0.75;
@@ -640,7 +643,8 @@ inline Plan plan_tiles(bool fp4, int64_t M, int64_t N, int64_t chunks, bool pair
       const double each = rest == 0 ? 0 : full == 0 && rest * s <= 256 ? alone : chunk;
       Plan plan{bm, bn, int(s > 1 ? full : tiles), s, s > 1 ? rest : 0};
       const double us = 4 + double(full / places) * chunk * chunks + each * double(cdiv(chunks, s)) +
-                        (s > 1 ? 4 + sums_bytes(plan) / 3e6 : 0);
+                        (s > 1 ? 4 + 0.5 * s + double(sums_bytes(plan)) * std::min<int64_t>(M, bm) / bm / 3e6 : 0) +
+                        (s == 1 && full == 0 && rest <= 256 ? 3 : 0);
       if (us < least) {
         least = us;
         best = plan;

@@ -45,4 +45,17 @@ __device__ __forceinline__ void mx4_unpack8(uint32_t w, float* v) {
   v[4] = c[0]; v[5] = c[1]; v[6] = d[0]; v[7] = d[1];
 }
 
+// Rows of `from` scales that are to lie `to` apart, filled up with 127 (no rows: nothing to do).
+struct ScaleRows {
+  const uint8_t* src = nullptr;
+  uint8_t* dst = nullptr;
+  int64_t rows = 0, from = 0, to = 0;
+};
+
+// Codes and scales (rows lds apart, filled up with 127) of x; in the same launch scales of another
+// operand are widened.
+int launch_mxfp4_quantize(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, uint8_t* codes, uint8_t* scales,
+                          int64_t lds, const ScaleRows& wide, hipStream_t stream);
+int launch_mxfp4_widen(const ScaleRows& a, const ScaleRows& b, hipStream_t stream);
+
 }  // namespace xk

@@ -1,9 +1,12 @@
 // Values to MXFP4 (format in mx4.h) and back.
 //
-// One pass each way, HBM bound: a lane owns half a block, 16 values, whose loads are 16
-// bytes each; the block's largest magnitude takes one lane exchange. A power of two as
-// scale makes the division exact, so the one rounding is the value's, to e2m1.
+// One pass each way, HBM bound. To 4 bits a lane owns half a block, 16 values, whose loads are 16
+// bytes each; the block's largest magnitude takes one lane exchange. Back, a lane owns 16
+// bytes of the result, so that a wave's stores are one run of 1 KB. A power of two as scale
+// makes the division exact, so the one rounding is the value's, to e2m1. Rows are told apart by
+// a division a lane, which whole blocks in rows without a gap do not need.
 #include <algorithm>
+#include <type_traits>
 
 #include "mx4.h"
 
@@ -39,27 +42,36 @@ template <typename T> __device__ __forceinline__ void load_piece(const T* p, int
     for (int i = 0; i < kPiece; ++i) v[i] = i < n ? p[i] : T(0);
   }
 }
-template <typename T> __device__ __forceinline__ void store_piece(T* p, int n, const T* v) {
-  if (n >= kPiece) {
-    __builtin_memcpy(p, v, kPiece * sizeof(T));
-  } else {
-#pragma unroll
-    for (int i = 0; i < kPiece; ++i)
-      if (i < n) p[i] = v[i];
+// Scales in rows of `to`, filled up with 127, from rows of `from` (see launch_mxfp4_quantize).
+__device__ __forceinline__ void widen(const ScaleRows& w, int64_t first, int64_t step) {
+  for (int64_t q = first; q < w.rows * w.to; q += step) {
+    const int64_t row = q / w.to, b = q - row * w.to;
+    w.dst[q] = b < w.from ? w.src[row * w.from + b] : 127;
   }
 }
 
+__global__ void __launch_bounds__(kThreads) mx4_widen_kernel(ScaleRows a, ScaleRows b) {
+  const int64_t first = int64_t(blockIdx.x) * kThreads + threadIdx.x, step = int64_t(gridDim.x) * kThreads;
+  widen(a, first, step);
+  widen(b, first, step);
+}
+
 // Half blocks are numbered row by row: both lanes of a block are always in the same round.
-// The scales' rows lie lds apart, the places behind the row's blocks are filled with 127.
-template <typename T>
+// The scales' rows lie lds apart, the places behind the row's blocks are filled with 127. FLAT: rows
+// without a gap of whole blocks, one after the other. U: a number that holds them all.
+// Workgroups from `own` on widen other scales.
+template <typename T, bool FLAT, typename U>
 __global__ void __launch_bounds__(kThreads)
-mx4_quantize_kernel(const T* __restrict__ x, int64_t ldx, int64_t M, int64_t K, int64_t blocks,
-                    uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int64_t lds) {
-  const int64_t halves = 2 * blocks, total = M * halves;
-  for (int64_t q = int64_t(blockIdx.x) * kThreads + threadIdx.x; q < total; q += int64_t(gridDim.x) * kThreads) {
-    const int64_t row = q / halves, half = q - row * halves;
-    const int64_t k0 = half * kPiece;
-    const int n = int(min(int64_t(kPiece), max(int64_t(0), K - k0)));
+mx4_quantize_kernel(const T* __restrict__ x, int64_t ldx, U total, int64_t K, U halves,
+                    uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int64_t lds, int own, ScaleRows wide) {
+  if (int(blockIdx.x) >= own) {
+    widen(wide, int64_t(blockIdx.x - own) * kThreads + threadIdx.x, int64_t(gridDim.x - own) * kThreads);
+    return;
+  }
+  for (U q = U(blockIdx.x) * kThreads + threadIdx.x; q < total; q += U(own) * kThreads) {
+    const U row = FLAT ? 0 : q / halves, half = q - row * halves;
+    const int64_t k0 = int64_t(half) * kPiece;
+    const int n = FLAT ? kPiece : int(min(int64_t(kPiece), max(int64_t(0), K - k0)));
     __attribute__((aligned(16))) T v[kPiece];
     load_piece(x + row * ldx + k0, n, v);
     float f[kPiece];
@@ -75,66 +87,102 @@ mx4_quantize_kernel(const T* __restrict__ x, int64_t ldx, int64_t M, int64_t K, 
 #pragma unroll
     for (int i = 0; i < kPiece; ++i) f[i] = byte == kMx4Nan ? 0.f : f[i] * inv;
     uint32_t w[2] = {mx4_pack8(f), mx4_pack8(f + 8)};
-    __builtin_memcpy(codes + q * 8, w, 8);
+    __builtin_memcpy(codes + int64_t(q) * 8, w, 8);
     if ((half & 1) == 0) scales[row * lds + half / 2] = uint8_t(byte);
-    if (half == halves - 1)
-      for (int64_t b = blocks; b < lds; ++b) scales[row * lds + b] = 127;
+    if (!FLAT && half == halves - 1)
+      for (int64_t b = halves / 2; b < lds; ++b) scales[row * lds + b] = 127;
   }
 }
 
-template <typename T>
+template <typename T, bool FLAT, typename U>
 __global__ void __launch_bounds__(kThreads)
-mx4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t M, int64_t K,
-                      int64_t blocks, T* __restrict__ out) {
-  const int64_t halves = 2 * blocks, total = M * halves;
-  for (int64_t q = int64_t(blockIdx.x) * kThreads + threadIdx.x; q < total; q += int64_t(gridDim.x) * kThreads) {
-    const int64_t row = q / halves, half = q - row * halves;
-    const int64_t k0 = half * kPiece;
-    const int n = int(min(int64_t(kPiece), K - k0));
+mx4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, U total, int64_t K,
+                      U pieces, T* __restrict__ out) {
+  constexpr int PER = 16 / sizeof(T);  // values of a lane
+  typedef std::conditional_t<PER == 8, uint32_t, uint16_t> W;
+  for (U q = U(blockIdx.x) * kThreads + threadIdx.x; q < total; q += U(gridDim.x) * kThreads) {
+    const U row = FLAT ? 0 : q / pieces, piece = q - row * pieces;
+    const int64_t k0 = int64_t(piece) * PER;
+    const int n = FLAT ? PER : int(min(int64_t(PER), K - k0));
     if (n <= 0) continue;
-    uint32_t w[2];
-    __builtin_memcpy(w, codes + q * 8, 8);
-    const float s = mx4_scale(scales[row * blocks + half / 2]);
-    float f[kPiece];
-    mx4_unpack8(w[0], f);
-    mx4_unpack8(w[1], f + 8);
-    __attribute__((aligned(16))) T v[kPiece];
+    const uint32_t w = load_unaligned<W>(codes + int64_t(q) * (PER / 2));
+    const float s = mx4_scale(scales[q / (kMx4Block / PER)]);
+    float f[8];
+    mx4_unpack8(w, f);
+    __attribute__((aligned(16))) T v[PER];
 #pragma unroll
-    for (int i = 0; i < kPiece; ++i) {
+    for (int i = 0; i < PER; ++i) {
       const float a = f[i] * s;
       const float c = fminf(fmaxf(a, -val<T>::kMax), val<T>::kMax);
       v[i] = val<T>::put(a == a ? c : a);
     }
-    store_piece(out + row * K + k0, n, v);
+    T* to = out + row * K + k0;
+    if (n == PER) {
+      __builtin_memcpy(to, v, 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER - 1; ++i)
+        if (i < n) to[i] = v[i];
+    }
   }
 }
 
 int grid_for(int64_t pieces) { return int(std::min<int64_t>(cdiv(pieces, kThreads), 256 * 64)); }
+// (a round of the grid past the last piece still fits)
+bool small(int64_t pieces) { return pieces < (int64_t(1) << 31); }
 
 template <typename T>
 void quantize_typed(const void* x, int64_t ldx, int64_t M, int64_t K, uint8_t* codes, uint8_t* scales, int64_t lds,
-                    hipStream_t stream) {
-  const int64_t blocks = cdiv(K, kMx4Block);
-  hipLaunchKernelGGL((mx4_quantize_kernel<T>), dim3(grid_for(M * 2 * blocks)), dim3(kThreads), 0, stream,
-                     static_cast<const T*>(x), ldx, M, K, blocks, codes, scales, lds);
+                    const ScaleRows& wide, hipStream_t stream) {
+  const int64_t blocks = cdiv(K, kMx4Block), total = M * 2 * blocks;
+  const int own = grid_for(total), more = wide.rows > 0 ? grid_for(cdiv(wide.rows * wide.to, 8)) : 0;
+  const dim3 grid(own + more), block(kThreads);
+  const T* p = static_cast<const T*>(x);
+  const bool flat = K % kMx4Block == 0 && (ldx == K || M == 1) && lds == blocks;
+  if (flat && small(total))
+    hipLaunchKernelGGL((mx4_quantize_kernel<T, true, uint32_t>), grid, block, 0, stream, p, ldx, uint32_t(total), K,
+                       uint32_t(2 * blocks), codes, scales, lds, own, wide);
+  else if (small(total))
+    hipLaunchKernelGGL((mx4_quantize_kernel<T, false, uint32_t>), grid, block, 0, stream, p, ldx, uint32_t(total), K,
+                       uint32_t(2 * blocks), codes, scales, lds, own, wide);
+  else
+    hipLaunchKernelGGL((mx4_quantize_kernel<T, false, int64_t>), grid, block, 0, stream, p, ldx, total, K, 2 * blocks,
+                       codes, scales, lds, own, wide);
 }
 
 template <typename T>
 void dequantize_typed(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, void* out,
                       hipStream_t stream) {
-  const int64_t blocks = cdiv(K, kMx4Block);
-  hipLaunchKernelGGL((mx4_dequantize_kernel<T>), dim3(grid_for(M * 2 * blocks)), dim3(kThreads), 0, stream, codes,
-                     scales, M, K, blocks, static_cast<T*>(out));
+  const int64_t pieces = cdiv(K, kMx4Block) * kMx4Block / (16 / int64_t(sizeof(T))), total = M * pieces;
+  const dim3 grid(grid_for(total)), block(kThreads);
+  T* to = static_cast<T*>(out);
+  if (K % kMx4Block == 0 && small(total))
+    hipLaunchKernelGGL((mx4_dequantize_kernel<T, true, uint32_t>), grid, block, 0, stream, codes, scales,
+                       uint32_t(total), K, uint32_t(pieces), to);
+  else if (small(total))
+    hipLaunchKernelGGL((mx4_dequantize_kernel<T, false, uint32_t>), grid, block, 0, stream, codes, scales,
+                       uint32_t(total), K, uint32_t(pieces), to);
+  else
+    hipLaunchKernelGGL((mx4_dequantize_kernel<T, false, int64_t>), grid, block, 0, stream, codes, scales, total, K,
+                       pieces, to);
 }
 
 }  // namespace
 
 int launch_mxfp4_quantize(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, uint8_t* codes, uint8_t* scales,
-                          int64_t lds, hipStream_t stream) {
-  if (dtype == XK_DT_BF16) quantize_typed<uint16_t>(x, ldx, M, K, codes, scales, lds, stream);
-  else if (dtype == XK_DT_FP16) quantize_typed<_Float16>(x, ldx, M, K, codes, scales, lds, stream);
-  else quantize_typed<float>(x, ldx, M, K, codes, scales, lds, stream);
+                          int64_t lds, const ScaleRows& wide, hipStream_t stream) {
+  if (dtype == XK_DT_BF16) quantize_typed<uint16_t>(x, ldx, M, K, codes, scales, lds, wide, stream);
+  else if (dtype == XK_DT_FP16) quantize_typed<_Float16>(x, ldx, M, K, codes, scales, lds, wide, stream);
+  else quantize_typed<float>(x, ldx, M, K, codes, scales, lds, wide, stream);
   XK_CHECK_LAUNCH("mxfp4_quantize");
+  return XK_OK;
+}
+
+int launch_mxfp4_widen(const ScaleRows& a, const ScaleRows& b, hipStream_t stream) {
+  if (a.rows + b.rows == 0) return XK_OK;
+  const int64_t pieces = cdiv(std::max(a.rows * a.to, b.rows * b.to), 8);
+  hipLaunchKernelGGL(mx4_widen_kernel, dim3(grid_for(pieces)), dim3(kThreads), 0, stream, a, b);
+  XK_CHECK_LAUNCH("mxfp4_widen");
   return XK_OK;
 }
 

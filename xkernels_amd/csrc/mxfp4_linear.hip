@@ -8,9 +8,6 @@
 
 namespace xk {
 
-int launch_mxfp4_quantize(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, uint8_t* codes, uint8_t* scales,
-                          int64_t lds, hipStream_t stream);
-
 namespace {
 
 using namespace dense;
@@ -66,24 +63,13 @@ template <typename T, bool BIAS> struct Store {
   }
 };
 
-// Scales whose rows do not start at 4 bytes, in rows that do.
-__global__ void __launch_bounds__(256)
-pad_scales(const uint8_t* __restrict__ src, int64_t rows, int64_t blocks, int64_t lds, uint8_t* __restrict__ dst) {
-  const int64_t total = rows * lds;
-  for (int64_t q = int64_t(blockIdx.x) * 256 + threadIdx.x; q < total; q += int64_t(gridDim.x) * 256) {
-    const int64_t row = q / lds, b = q - row * lds;
-    dst[q] = b < blocks ? src[row * blocks + b] : 127;
-  }
-}
-
-const uint8_t* take_scales(const uint8_t* s, int64_t rows, int64_t blocks, char*& ws, hipStream_t stream) {
+// Scales whose rows do not start at 4 bytes lie in rows that do (`rows` says which those are to be).
+const uint8_t* take_scales(const uint8_t* s, int64_t n, int64_t blocks, char*& ws, ScaleRows& rows) {
   const int64_t lds = pad4(blocks);
   if (lds == blocks) return s;
-  uint8_t* to = reinterpret_cast<uint8_t*>(ws);
-  ws += aligned(rows * lds);
-  const int grid = int(std::min<int64_t>(cdiv(rows * lds, 256), 256 * 32));
-  hipLaunchKernelGGL(pad_scales, dim3(grid), dim3(256), 0, stream, s, rows, blocks, lds, to);
-  return to;
+  rows = ScaleRows{s, reinterpret_cast<uint8_t*>(ws), n, blocks, lds};
+  ws += aligned(n * lds);
+  return rows.dst;
 }
 
 struct Call {
@@ -115,18 +101,22 @@ template <typename EPI> int cut(const Call& c, const EPI& store, char* ws, hipSt
   }
   const char* xc = static_cast<const char*>(c.x);
   const uint8_t* xs;
+  ScaleRows wide, x_wide;
+  const uint8_t* wsc = take_scales(c.scales, c.N, blocks, ws, wide);
+  int rc;
   if (c.x_scales == nullptr) {
     uint8_t* to = reinterpret_cast<uint8_t*>(ws);
     ws += aligned(c.M * blocks * 16);
     uint8_t* s = reinterpret_cast<uint8_t*>(ws);
     ws += aligned(c.M * lds);
-    if (int rc = launch_mxfp4_quantize(c.x, c.dtype, c.ldx, c.M, c.K, to, s, lds, stream)) return rc;
+    rc = launch_mxfp4_quantize(c.x, c.dtype, c.ldx, c.M, c.K, to, s, lds, wide, stream);
     xc = reinterpret_cast<const char*>(to);
     xs = s;
   } else {
-    xs = take_scales(c.x_scales, c.M, blocks, ws, stream);
+    xs = take_scales(c.x_scales, c.M, blocks, ws, x_wide);
+    rc = launch_mxfp4_widen(wide, x_wide, stream);
   }
-  const uint8_t* wsc = take_scales(c.scales, c.N, blocks, ws, stream);
+  if (rc) return rc;
   Product p{};
   p.x = Side{xc, blocks * 16, c.M, xs, lds};
   p.w = Side{codes, blocks * 16, c.N, wsc, lds};
