@@ -360,7 +360,7 @@ int xk_gated_ffn_backward(const void* grad_out, int32_t dtype, int64_t ldg, cons
  * 32)] (the last block filled up with zeros), scales [M, ceil(K / 32)]. The scale is the
  * least power of two with which no value of the block passes 6, values round to nearest
  * even; a block with an infinity or a NaN gets byte 255, NaN (which xk_moe_mxfp4 reads as 0).
- * x [M, K] bf16 | fp32 | fp16 with rows ldx apart, K <= 2^22. Restored values that
+ * x [M, K] bf16 | fp32 | fp16 with rows ldx apart, K <= 2^22, fewer than 2^33 values. Restored values that
  * would pass the output type's largest finite value become that.
  * ------------------------------------------------------------------------- */
 int xk_mxfp4_quantize(const void* x, int32_t dtype, int64_t ldx, int64_t M, int64_t K,
@@ -372,7 +372,8 @@ int xk_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t M, 
  * | fp32 | fp16; bias of it, nullable). w_codes and w_scales as above for [N, K]. x: values
  * [M, K] of dtype with rows ldx apart, which are quantised as above first, or, with
  * x_scales, codes of the same format (dtype and ldx unused). Codes are 16-byte
- * aligned, scales 4-byte; K and N <= 1,000,000, M < 2^29. workspace is 256-byte aligned. */
+ * aligned, scales 4-byte; K and N <= 1,000,000, M < 2^29, x of fewer than 2^33 values. workspace is
+ * 256-byte aligned. */
 int64_t xk_mxfp4_linear_workspace_bytes(int64_t M, int64_t K, int64_t N);
 int xk_mxfp4_linear(const void* x, int32_t dtype, int64_t ldx, const uint8_t* x_scales,
                     int64_t M, int64_t K, const uint8_t* w_codes, const uint8_t* w_scales,

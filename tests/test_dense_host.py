@@ -92,14 +92,14 @@ def test_ffn_backward_workspace():
 
 
 @pytest.mark.parametrize("args", [(P, 7, 32, 4, 32, P, P), (P, BF, 32, -1, 32, P, P), (P, BF, 32, 4, 0, P, P),
-                                  (P, BF, 32, 1 << 40, 32, P, P), (P, BF, 1 << 23, 4, (1 << 22) + 1, P, P),
+                                  (P, BF, 32, 1 << 40, 32, P, P), (P, BF, 32, 1 << 28, 32, P, P), (P, BF, 1 << 23, 4, (1 << 22) + 1, P, P),
                                   (None, BF, 32, 4, 32, P, P), (P, BF, 32, 4, 32, None, P), (P, BF, 32, 4, 32, P, None),
                                   (P, BF, 31, 4, 32, P, P)])
 def test_quantize_refuses(args):
     assert _rc("xk_mxfp4_quantize", *args, None) == INVALID and _lib.last_error()
 
 
-@pytest.mark.parametrize("args", [(P, P, 4, 32, 9, P), (P, P, -4, 32, BF, P), (P, P, 4, 0, BF, P), (None, P, 4, 32, BF, P),
+@pytest.mark.parametrize("args", [(P, P, 4, 32, 9, P), (P, P, -4, 32, BF, P), (P, P, 1 << 28, 1, BF, P), (P, P, 4, 0, BF, P), (None, P, 4, 32, BF, P),
                                   (P, None, 4, 32, BF, P), (P, P, 4, 32, BF, None)])
 def test_dequantize_refuses(args):
     assert _rc("xk_mxfp4_dequantize", *args, None) == INVALID and _lib.last_error()
@@ -111,7 +111,7 @@ def _linear(x=P, dtype=BF, ldx=64, xs=None, M=40, K=64, wc=P, ws=P, N=32, bias=N
 
 
 @pytest.mark.parametrize("kw", [dict(dtype=5), dict(odt=-1), dict(M=-1), dict(M=1 << 29), dict(K=0), dict(K=1000001),
-                                dict(N=0), dict(N=1000001), dict(M=(1 << 29) - 1, N=1000000), dict(x=None), dict(wc=None),
+                                dict(N=0), dict(N=1000001), dict(M=(1 << 29) - 1, N=1000000), dict(M=1 << 28, N=1), dict(x=None), dict(wc=None),
                                 dict(ws=None), dict(out=None), dict(ldx=63), dict(wc=P + 8), dict(ws=P + 2),
                                 dict(xs=P + 1, dtype=-1), dict(xs=P, x=P + 4), dict(scratch=P + 128)])
 def test_linear_refuses(kw):

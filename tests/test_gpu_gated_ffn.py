@@ -202,6 +202,27 @@ def test_two_streams(dev):
             assert all(torch.equal(s, t) for s, t in zip(p, q))
 
 
+def test_past_32_bits(dev):
+    """Rows behind 2^31 bytes of every long operand: the last ones as in a batch of their own, and the
+    weights' gradients of those alone."""
+    M, H, I, last = 540_000, 2048, 24, 300
+    _, w13, w2, dy = _inputs(1, H, I, BF, 7)
+    x = torch.zeros(M, H, dtype=BF, device="cuda")
+    dys = torch.zeros(M, H, dtype=BF, device="cuda")
+    xe, _, _, dye = _inputs(last, H, I, BF, 8)
+    x[-last:], dys[-last:] = xe, dye
+    out, gu = xk.gated_ffn(x, w13, w2, return_gate_up=True)
+    want, _, bound, _ = ffn_ref(xe, w13, w2)
+    check(out[-last:], want, bound)
+    assert not out[:-last].any()
+    got = xk.gated_ffn_backward(dys, x, w13, w2, gu)
+    ref, bounds = ffn_grad_ref(dye, xe, w13, w2)
+    check(got[0][-last:], ref[0], bounds[0])
+    assert not got[0][:-last].any()
+    for p, q, b in zip(got[1:], ref[1:], bounds[1:]):  # (the other rows' terms are zeros)
+        check(p, q, b)
+
+
 def test_refusals(dev):
     x, w13, w2, dy = _inputs(4, 64, 32, BF)
     gu = torch.zeros(4, 64, dtype=BF, device="cuda")

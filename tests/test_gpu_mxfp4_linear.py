@@ -177,6 +177,25 @@ def test_linear_not_finite(M, K, N, dev):
     assert got[~rows].isnan().all() and got[:, ~cols].isnan().all()
 
 
+def test_past_32_bits(dev):
+    """Rows behind 2^31 values and 2^31 bytes of codes: the last ones as in a batch of their own."""
+    M, K, N, last = 1_100_000, 4096, 40, 200
+    x = torch.zeros(M, K, dtype=BF, device="cuda")
+    end = _values((last, K), BF, 1)
+    x[-last:] = end
+    q, qe = xk.mxfp4_quantize(x), xk.mxfp4_quantize(end)
+    assert torch.equal(q.codes[-last:], qe.codes) and torch.equal(q.scales[-last:], qe.scales)
+    back = xk.mxfp4_dequantize(q)
+    assert torch.equal(back[-last:], xk.mxfp4_dequantize(qe)) and not back[:-last].any()
+    del back
+    w = xk.mxfp4_quantize(_values((N, K), BF, 2))
+    want, bound = linear_ref(mxfp4_values(qe), mxfp4_values(w))
+    for a in (x, q):
+        y = xk.mxfp4_linear(a, w, out_dtype=BF)
+        check(y[-last:], want, bound)
+        assert not y[:-last].any()
+
+
 def test_linear_odd_addresses(dev):
     x, held = _values((30, 224), BF, 1), xk.mxfp4_quantize(_values((50, 224), BF, 2))
     want = xk.mxfp4_linear(x, held)

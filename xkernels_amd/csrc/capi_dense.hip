@@ -23,7 +23,7 @@ namespace {
 
 // What the kernels' 32-bit offsets within a tile (256 rows) and the launches' grids hold.
 constexpr int64_t kMaxRows = int64_t(1) << 29, kMaxCols = 1000000, kMaxApart = 2000000;
-constexpr int64_t kMaxTiles = int64_t(1) << 30;
+constexpr int64_t kMaxTiles = int64_t(1) << 30, kMaxValues = int64_t(1) << 33;
 
 bool any_dtype(int dt) { return dt == XK_DT_BF16 || dt == XK_DT_FP32 || dt == XK_DT_FP16; }
 bool at(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
@@ -43,6 +43,14 @@ int check_ffn(const char* op, int dtype, int64_t M, int64_t H, int64_t I) {
   XK_REQUIRE(M >= 0 && M < kMaxRows && H >= 1 && H <= kMaxCols && I >= 1 && I <= kMaxCols / 2,
              "%s: bad sizes M=%lld hidden=%lld ispp=%lld", op, (long long)M, (long long)H, (long long)I);
   XK_REQUIRE(fits(M, H) && fits(M, I) && fits(2 * I, H), "%s: more tiles than a launch holds", op);
+  return XK_OK;
+}
+
+// values that are quantised or restored: the kernels number groups of 4 and more in 32 bits
+int check_values(const char* op, int64_t M, int64_t K) {
+  XK_REQUIRE(M >= 0 && M < (int64_t(1) << 33) && K >= 1 && K <= (int64_t(1) << 22), "%s: bad sizes M=%lld K=%lld", op,
+             (long long)M, (long long)K);
+  XK_REQUIRE(M * cdiv(K, 32) * 32 < kMaxValues, "%s: %lld x %lld values, 2^33 or more", op, (long long)M, (long long)K);
   return XK_OK;
 }
 
@@ -109,8 +117,7 @@ int xk_mxfp4_quantize(const void* x, int32_t dtype, int64_t ldx, int64_t M, int6
                       uint8_t* scales, hipStream_t stream) {
   clear_error();
   XK_REQUIRE(any_dtype(dtype), "mxfp4_quantize: dtype code %d is not bf16, fp32 or fp16", dtype);
-  XK_REQUIRE(M >= 0 && M < (int64_t(1) << 40) && K >= 1 && K <= (int64_t(1) << 22),
-             "mxfp4_quantize: bad sizes M=%lld K=%lld", (long long)M, (long long)K);
+  if (int rc = check_values("mxfp4_quantize", M, K)) return rc;
   if (M == 0) return XK_OK;
   XK_REQUIRE(x && codes && scales, "mxfp4_quantize: null pointer");
   XK_REQUIRE(M == 1 || ldx >= K, "mxfp4_quantize: rows overlap (ldx)");
@@ -121,8 +128,7 @@ int xk_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t M, 
                         hipStream_t stream) {
   clear_error();
   XK_REQUIRE(any_dtype(dtype), "mxfp4_dequantize: dtype code %d is not bf16, fp32 or fp16", dtype);
-  XK_REQUIRE(M >= 0 && M < (int64_t(1) << 40) && K >= 1 && K <= (int64_t(1) << 22),
-             "mxfp4_dequantize: bad sizes M=%lld K=%lld", (long long)M, (long long)K);
+  if (int rc = check_values("mxfp4_dequantize", M, K)) return rc;
   if (M == 0) return XK_OK;
   XK_REQUIRE(codes && scales && out, "mxfp4_dequantize: null pointer");
   return launch_mxfp4_dequantize(codes, scales, M, K, dtype, out, stream);
@@ -132,7 +138,7 @@ static int check_linear(int64_t M, int64_t K, int64_t N) {
   XK_REQUIRE(M >= 0 && M < kMaxRows && K >= 1 && K <= kMaxCols && N >= 1 && N <= kMaxCols,
              "mxfp4_linear: bad sizes M=%lld K=%lld N=%lld", (long long)M, (long long)K, (long long)N);
   XK_REQUIRE(fits(M, N), "mxfp4_linear: more tiles than a launch holds");
-  return XK_OK;
+  return check_values("mxfp4_linear", M, K);
 }
 
 int64_t xk_mxfp4_linear_workspace_bytes(int64_t M, int64_t K, int64_t N) {

@@ -58,18 +58,19 @@ __global__ void __launch_bounds__(kThreads) mx4_widen_kernel(ScaleRows a, ScaleR
 
 // Half blocks are numbered row by row: both lanes of a block are always in the same round.
 // The scales' rows lie lds apart, the places behind the row's blocks are filled with 127. FLAT: rows
-// without a gap of whole blocks, one after the other. U: a number that holds them all.
+// without a gap of whole blocks, one after the other. There are fewer than 2^31.
 // Workgroups from `own` on widen other scales.
-template <typename T, bool FLAT, typename U>
+template <typename T, bool FLAT>
 __global__ void __launch_bounds__(kThreads)
-mx4_quantize_kernel(const T* __restrict__ x, int64_t ldx, U total, int64_t K, U halves,
+mx4_quantize_kernel(const T* __restrict__ x, int64_t ldx, uint32_t total, int64_t K, uint32_t halves,
                     uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int64_t lds, int own, ScaleRows wide) {
   if (int(blockIdx.x) >= own) {
     widen(wide, int64_t(blockIdx.x - own) * kThreads + threadIdx.x, int64_t(gridDim.x - own) * kThreads);
     return;
   }
-  for (U q = U(blockIdx.x) * kThreads + threadIdx.x; q < total; q += U(own) * kThreads) {
-    const U row = FLAT ? 0 : q / halves, half = q - row * halves;
+  for (uint32_t q = blockIdx.x * kThreads + threadIdx.x; q < total; q += uint32_t(own) * kThreads) {
+    const uint32_t r = FLAT ? 0 : q / halves, half = q - r * halves;
+    const int64_t row = r;
     const int64_t k0 = int64_t(half) * kPiece;
     const int n = FLAT ? kPiece : int(min(int64_t(kPiece), max(int64_t(0), K - k0)));
     __attribute__((aligned(16))) T v[kPiece];
@@ -94,14 +95,15 @@ mx4_quantize_kernel(const T* __restrict__ x, int64_t ldx, U total, int64_t K, U 
   }
 }
 
-template <typename T, bool FLAT, typename U>
+template <typename T, bool FLAT>
 __global__ void __launch_bounds__(kThreads)
-mx4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, U total, int64_t K,
-                      U pieces, T* __restrict__ out) {
+mx4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, uint32_t total, int64_t K,
+                      uint32_t pieces, T* __restrict__ out) {
   constexpr int PER = 16 / sizeof(T);  // values of a lane
   typedef std::conditional_t<PER == 8, uint32_t, uint16_t> W;
-  for (U q = U(blockIdx.x) * kThreads + threadIdx.x; q < total; q += U(gridDim.x) * kThreads) {
-    const U row = FLAT ? 0 : q / pieces, piece = q - row * pieces;
+  for (uint32_t q = blockIdx.x * kThreads + threadIdx.x; q < total; q += gridDim.x * kThreads) {
+    const uint32_t r = FLAT ? 0 : q / pieces, piece = q - r * pieces;
+    const int64_t row = r;
     const int64_t k0 = int64_t(piece) * PER;
     const int n = FLAT ? PER : int(min(int64_t(PER), K - k0));
     if (n <= 0) continue;
@@ -128,8 +130,6 @@ mx4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restri
 }
 
 int grid_for(int64_t pieces) { return int(std::min<int64_t>(cdiv(pieces, kThreads), 256 * 64)); }
-// (a round of the grid past the last piece still fits)
-bool small(int64_t pieces) { return pieces < (int64_t(1) << 31); }
 
 template <typename T>
 void quantize_typed(const void* x, int64_t ldx, int64_t M, int64_t K, uint8_t* codes, uint8_t* scales, int64_t lds,
@@ -139,15 +139,12 @@ void quantize_typed(const void* x, int64_t ldx, int64_t M, int64_t K, uint8_t* c
   const dim3 grid(own + more), block(kThreads);
   const T* p = static_cast<const T*>(x);
   const bool flat = K % kMx4Block == 0 && (ldx == K || M == 1) && lds == blocks;
-  if (flat && small(total))
-    hipLaunchKernelGGL((mx4_quantize_kernel<T, true, uint32_t>), grid, block, 0, stream, p, ldx, uint32_t(total), K,
-                       uint32_t(2 * blocks), codes, scales, lds, own, wide);
-  else if (small(total))
-    hipLaunchKernelGGL((mx4_quantize_kernel<T, false, uint32_t>), grid, block, 0, stream, p, ldx, uint32_t(total), K,
+  if (flat)
+    hipLaunchKernelGGL((mx4_quantize_kernel<T, true>), grid, block, 0, stream, p, ldx, uint32_t(total), K,
                        uint32_t(2 * blocks), codes, scales, lds, own, wide);
   else
-    hipLaunchKernelGGL((mx4_quantize_kernel<T, false, int64_t>), grid, block, 0, stream, p, ldx, total, K, 2 * blocks,
-                       codes, scales, lds, own, wide);
+    hipLaunchKernelGGL((mx4_quantize_kernel<T, false>), grid, block, 0, stream, p, ldx, uint32_t(total), K,
+                       uint32_t(2 * blocks), codes, scales, lds, own, wide);
 }
 
 template <typename T>
@@ -156,15 +153,12 @@ void dequantize_typed(const uint8_t* codes, const uint8_t* scales, int64_t M, in
   const int64_t pieces = cdiv(K, kMx4Block) * kMx4Block / (16 / int64_t(sizeof(T))), total = M * pieces;
   const dim3 grid(grid_for(total)), block(kThreads);
   T* to = static_cast<T*>(out);
-  if (K % kMx4Block == 0 && small(total))
-    hipLaunchKernelGGL((mx4_dequantize_kernel<T, true, uint32_t>), grid, block, 0, stream, codes, scales,
-                       uint32_t(total), K, uint32_t(pieces), to);
-  else if (small(total))
-    hipLaunchKernelGGL((mx4_dequantize_kernel<T, false, uint32_t>), grid, block, 0, stream, codes, scales,
-                       uint32_t(total), K, uint32_t(pieces), to);
+  if (K % kMx4Block == 0)
+    hipLaunchKernelGGL((mx4_dequantize_kernel<T, true>), grid, block, 0, stream, codes, scales, uint32_t(total), K,
+                       uint32_t(pieces), to);
   else
-    hipLaunchKernelGGL((mx4_dequantize_kernel<T, false, int64_t>), grid, block, 0, stream, codes, scales, total, K,
-                       pieces, to);
+    hipLaunchKernelGGL((mx4_dequantize_kernel<T, false>), grid, block, 0, stream, codes, scales, uint32_t(total), K,
+                       uint32_t(pieces), to);
 }
 
 }  // namespace
