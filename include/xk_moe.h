@@ -331,8 +331,8 @@ int xk_act_restore(const uint8_t* values, const uint8_t* scales, int64_t M, int6
  *   g = x Wg^T, u = x Wu^T, h = silu(min(g, L)) * clamp(u, -L, L), out = h W2^T
  * x [M, hidden] with rows ldx apart, w13 [2 ispp, hidden] (rows gate, then up) and
  * w2 [hidden, ispp] contiguous, out [M, hidden] contiguous, one dtype (bf16 | fp16);
- * swiglu_limit L <= 0: no clamp. gate_up [M, 2 ispp] (nullable) receives g and u, rounded
- * to dtype but never across the limit. fp32 sums; h is rounded to dtype. x, w13 and w2
+ * swiglu_limit L <= 0: no clamp. gate_up fp32 [M, 2 ispp] (nullable) receives g and u.
+ * fp32 sums; h is rounded to dtype. x, w13 and w2
  * are 16-byte aligned, ldx a multiple of 8 where hidden is, and at most 2,000,000;
  * hidden <= 1,000,000, ispp <= 500,000, M < 2^29. workspace is 256-byte aligned.
  * ------------------------------------------------------------------------- */

@@ -21,7 +21,7 @@ def gated_ffn_ref(x, w13, w2, swiglu_limit=None, return_gate_up=False):
     gu = x.float() @ w13.float().t()
     g, u, _, _ = _clamped(gu, w2.shape[1], swiglu_limit)
     out = ((g * torch.sigmoid(g) * u) @ w2.float().t()).to(x.dtype)
-    return (out, gu.to(x.dtype)) if return_gate_up else out
+    return (out, gu) if return_gate_up else out
 
 
 def gated_ffn_backward_ref(grad_out, x, w13, w2, gate_up=None, swiglu_limit=None):

@@ -23,7 +23,7 @@ def _clamped(g, u, limit):
 
 
 def ffn_ref(x, w13, w2, limit=None):
-    """``(out, gate_up, bound of out, bound of gate_up)``, gate_up before its rounding."""
+    """``(out, gate_up, bound of out, bound of gate_up)``."""
     e, tiny = half_step(x.dtype), _tiny(x.dtype)
     x, w13, w2 = (t.double().cpu() for t in (x, w13, w2))
     H, I = w2.shape
@@ -49,7 +49,6 @@ def ffn_grad_ref(dy, x, w13, w2, limit=None):
     # a sum next to the limit may fall on its other side
     near = torch.zeros_like(gu) if limit is None else \
         (torch.cat(((g - limit).abs(), (u.abs() - limit).abs()), 1) <= 2 * off).double()
-    off = off + 2 * e * gu.abs() + tiny  # gate_up's rounding, a whole step where it would cross the limit
     og, ou = off[:, :I], off[:, I:]
     s = torch.sigmoid(gc)
     silu, slope = gc * s, s * (1 + gc * (1 - s))

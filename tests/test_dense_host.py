@@ -88,7 +88,7 @@ def test_ffn_backward_refuses(kw):
 def test_ffn_backward_workspace():
     assert _grad(ws_bytes=64) == WORKSPACE
     need = [_lib.query("xk_gated_ffn_backward_workspace_bytes", 4096, 512, 256, r) for r in (0, 1)]
-    assert need[1] >= need[0] + 4096 * 512 * 2
+    assert need[1] >= need[0] + 4096 * 512 * 4
 
 
 @pytest.mark.parametrize("args", [(P, 7, 32, 4, 32, P, P), (P, BF, 32, -1, 32, P, P), (P, BF, 32, 4, 0, P, P),

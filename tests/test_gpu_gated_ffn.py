@@ -42,8 +42,8 @@ def test_forward(M, H, I, dt, dev):
     limit = 2.5 if M % 2 else None
     out, gu = xk.gated_ffn(x, w13, w2, swiglu_limit=limit, return_gate_up=True)
     want, gu_want, bound, gu_bound = ffn_ref(x, w13, w2, limit)
-    step = torch.finfo(dt).eps / 2 * gu_want.abs() if limit else 0.0  # a sum kept off the limit
-    check(gu, gu_want, gu_bound + step, "gate_up")
+    assert gu.dtype == torch.float32
+    check(gu, gu_want, gu_bound, "gate_up")
     check(out, want, bound, "out")
     assert torch.equal(out, xk.gated_ffn(x, w13, w2, swiglu_limit=limit))
 
@@ -225,14 +225,14 @@ def test_past_32_bits(dev):
 
 def test_refusals(dev):
     x, w13, w2, dy = _inputs(4, 64, 32, BF)
-    gu = torch.zeros(4, 64, dtype=BF, device="cuda")
+    gu = torch.zeros(4, 64, device="cuda")
     bad = [lambda: xk.gated_ffn(x.float(), w13.float(), w2.float()), lambda: xk.gated_ffn(x, w13.half(), w2),
            lambda: xk.gated_ffn(x[0], w13, w2), lambda: xk.gated_ffn(x[:, :32], w13, w2),
            lambda: xk.gated_ffn(x, w13[:63], w2), lambda: xk.gated_ffn(x, w13, w2[:, :31]),
            lambda: xk.gated_ffn(x, w13, w2.cpu()), lambda: xk.gated_ffn(x, w13, w2, swiglu_limit=float("nan")),
            lambda: xk.gated_ffn_backward(dy[:3], x, w13, w2), lambda: xk.gated_ffn_backward(dy.half(), x, w13, w2),
            lambda: xk.gated_ffn_backward(dy, x, w13, w2, gu[:, :32]),
-           lambda: xk.gated_ffn_backward(dy, x, w13, w2, gu.float())]
+           lambda: xk.gated_ffn_backward(dy, x, w13, w2, gu[:3])]
     for call in bad:
         with pytest.raises(RuntimeError):
             call()

@@ -516,25 +516,28 @@ dense_tile(Product p, EPI epi) {
       };
       if constexpr (EPI::kFetches) if constexpr (whole) {
         static_assert(!PAIRED, "no pairs with values of memory");
-        decltype(spot.template fetch<whole>(0, 0)) held[2][16 / ROWS];
-        auto fetch = [&](int t) __attribute__((always_inline)) {
+        // two rows of a turn at a time, the next two's values on their way
+        constexpr int HALVES = 16 / ROWS / 2;
+        decltype(spot.template fetch<whole>(0, 0)) held[2][2];
+        auto fetch = [&](int h) __attribute__((always_inline)) {
 #pragma unroll
-          for (int r = 0; r < 16 / ROWS; ++r) {
-            const int row = l / LANES + r * ROWS;
-            if (holds(t, row)) held[t & 1][r] = spot.template fetch<whole>(t % XT * 16 + row, t / XT * STRIDE * 16 + unit * 4);
+          for (int r = 0; r < 2; ++r) {
+            const int t = h / HALVES, row = l / LANES + (h % HALVES * 2 + r) * ROWS;
+            if (holds(t, row)) held[h & 1][r] = spot.template fetch<whole>(t % XT * 16 + row, t / XT * STRIDE * 16 + unit * 4);
           }
         };
         fetch(0);
 #pragma unroll
-        for (int t = 0; t < TIMES; ++t) {
-          if (t + 1 < TIMES) fetch(t + 1);
-          stage(t);
+        for (int h = 0; h < TIMES * HALVES; ++h) {
+          const int t = h / HALVES;
+          if (h + 1 < TIMES * HALVES) fetch(h + 1);
+          if (h % HALVES == 0) stage(t);
 #pragma unroll
-          for (int r = 0; r < 16 / ROWS; ++r) {
-            const int row = l / LANES + r * ROWS;
+          for (int r = 0; r < 2; ++r) {
+            const int row = l / LANES + (h % HALVES * 2 + r) * ROWS;
             if (holds(t, row))
               spot.template put<whole>(t % XT * 16 + row, t / XT * STRIDE * 16 + unit * 4, own[row * 16 + (unit ^ row)],
-                                       held[t & 1][r]);
+                                       held[h & 1][r]);
           }
           wave_lds_fence();
           __builtin_amdgcn_sched_barrier(0);

@@ -24,8 +24,8 @@ def gated_ffn(
     ``x [M, hidden]`` (rows may lie apart), ``w13 [2 * ispp, hidden]`` (rows ``[gate; up]``),
     ``w2 [hidden, ispp]``, one dtype (bf16 or fp16); ``out [M, hidden]`` of it. fp32 sums; the
     activations between the projections are rounded to the dtype. ``return_gate_up`` adds
-    ``[M, 2 * ispp]``, ``g`` and ``u`` rounded to the dtype (never across the limit), which
-    spares the backward their product. Rows do not mix: what is not finite in one stays
+    ``[M, 2 * ispp]`` in fp32, the sums ``g`` and ``u``, which spare the backward their
+    product. Rows do not mix: what is not finite in one stays
     there. No autograd graph is recorded (a warning, once, where an input requires a gradient).
     """
     return dispatch("gated_ffn", x, w13, w2, swiglu_limit=swiglu_limit, return_gate_up=return_gate_up,

@@ -13,7 +13,7 @@ import torch
 from .. import _lib
 from .._backends import Backend
 from .._dispatch import register
-from .hip_backend import _ptr
+from .hip_backend import _contig, _ptr
 from .hip_tuning import _ANY_DT, _bytes, _code, _current_device, _device, _elsewhere, _no_graph, _recording, _rows, \
     _shape, _stream
 from .mxfp4_linear import Mxfp4
@@ -75,7 +75,7 @@ def gated_ffn_hip(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, swiglu_l
     limit = _limit(op, swiglu_limit)
     xr, ldx = _aligned_rows(x)
     out = x.new_empty((M, H))
-    gate_up = x.new_empty((M, 2 * I)) if return_gate_up else None
+    gate_up = x.new_empty((M, 2 * I), dtype=torch.float32) if return_gate_up else None
     nbytes = _bytes("xk_gated_ffn_workspace_bytes", M, H, I)
     ws = x.new_empty(nbytes, dtype=torch.uint8)
     _lib.call("xk_gated_ffn", xr.data_ptr(), dt, ldx, M, H, w13.data_ptr(), w2.data_ptr(), I, limit, out.data_ptr(),
@@ -89,12 +89,12 @@ def gated_ffn_backward_hip(grad_out: torch.Tensor, x: torch.Tensor, w13: torch.T
     i = _device(op, grad_out, x, w13, w2, gate_up)
     if i != _current_device():
         return _elsewhere(i, gated_ffn_backward_hip, grad_out, x, w13, w2, gate_up, swiglu_limit)
-    dt, M, H, I, w13, w2 = _ffn_args(op, x, w13, w2, grad_out, gate_up)
+    dt, M, H, I, w13, w2 = _ffn_args(op, x, w13, w2, grad_out)
     _shape(op, "grad_out", grad_out, (M, H))
     _shape(op, "gate_up", gate_up, (M, 2 * I))
     limit = _limit(op, swiglu_limit)
     (gr, ldg), (xr, ldx) = _aligned_rows(grad_out), _aligned_rows(x)
-    gu = None if gate_up is None else gate_up.contiguous()
+    gu = None if gate_up is None else _contig(gate_up, torch.float32)
     grad_x, grad_w13, grad_w2 = x.new_empty((M, H)), torch.empty_like(w13), torch.empty_like(w2)
     nbytes = _bytes("xk_gated_ffn_backward_workspace_bytes", M, H, I, int(gu is None))
     ws = x.new_empty(nbytes, dtype=torch.uint8)

@@ -108,7 +108,7 @@ def _gated_ffn(p: dict[str, Any]) -> tuple[int, int]:
 def _gated_ffn_backward(p: dict[str, Any]) -> tuple[int, int]:
     M, H, I = (int(p[x]) for x in ("M", "hidden", "ispp"))
     kept = bool(p.get("kept"))
-    return (12 if kept else 16) * M * H * I, dtype_bytes(p.get("dtype", "bf16")) * (3 * M * H + 6 * H * I + 2 * M * I * kept)
+    return (12 if kept else 16) * M * H * I, dtype_bytes(p.get("dtype", "bf16")) * (3 * M * H + 6 * H * I) + 8 * M * I * kept
 
 
 def _mxfp4_quantize(p: dict[str, Any]) -> tuple[int, int]:

@@ -142,7 +142,7 @@ def _gated_ffn(p: dict[str, Any], seed: int, device: str) -> dict[str, Any]:
 def _gated_ffn_backward(p: dict[str, Any], seed: int, device: str) -> dict[str, Any]:
     f = _gated_ffn(p, seed, device)
     M, dt = int(p["M"]), f["x"].dtype
-    gate_up = _randn(device, torch.float32, M, f["w13"].shape[0], seed=seed + 4).to(dt) if p.get("kept") else None
+    gate_up = _randn(device, torch.float32, M, f["w13"].shape[0], seed=seed + 4) if p.get("kept") else None
     grad = _randn(device, torch.float32, M, f["x"].shape[1], seed=seed + 3).to(dt)
     return {"grad_out": grad, "x": f["x"], "w13": f["w13"], "w2": f["w2"], "gate_up": gate_up,
             "swiglu_limit": f["swiglu_limit"]}
