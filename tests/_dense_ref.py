@@ -8,6 +8,7 @@ import torch
 
 from tests._tuning_ref import F32, gamma, half_step
 
+# (64-bit forms of the feed-forward block stay on their inputs' device)
 GRID = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], dtype=torch.float64)
 
 
@@ -25,7 +26,7 @@ def _clamped(g, u, limit):
 def ffn_ref(x, w13, w2, limit=None):
     """``(out, gate_up, bound of out, bound of gate_up)``."""
     e, tiny = half_step(x.dtype), _tiny(x.dtype)
-    x, w13, w2 = (t.double().cpu() for t in (x, w13, w2))
+    x, w13, w2 = (t.double() for t in (x, w13, w2))
     H, I = w2.shape
     gu, off = x @ w13.t(), gamma(H) * (x.abs() @ w13.abs().t())
     gc, uc, _, _ = _clamped(gu[:, :I], gu[:, I:], limit)
@@ -40,7 +41,7 @@ def ffn_ref(x, w13, w2, limit=None):
 def ffn_grad_ref(dy, x, w13, w2, limit=None):
     """``((dx, dW13, dW2), (their bounds))``."""
     e, tiny = half_step(x.dtype), _tiny(x.dtype)
-    dy, x, w13, w2 = (t.double().cpu() for t in (dy, x, w13, w2))
+    dy, x, w13, w2 = (t.double() for t in (dy, x, w13, w2))
     H, I = w2.shape
     M = x.shape[0]
     gu, off = x @ w13.t(), gamma(H) * (x.abs() @ w13.abs().t())

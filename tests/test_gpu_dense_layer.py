@@ -74,11 +74,11 @@ def test_training_step(M, dev):
     assert torch.equal(got[1], xk.gated_ffn_backward(dy, held, w13, w2, xk.gated_ffn(
         x, w13, w2, swiglu_limit=limit, return_gate_up=True)[1], swiglu_limit=limit)[1])
     # each held value is off by at most 2^-4 of itself or 2^-17 of its block's largest
-    off = x.abs().double().cpu() * 2.0 ** -4 + x.abs().double().cpu().amax() * 2.0 ** -17
-    gu = x.double().cpu() @ w13.double().cpu().t()
+    off = x.abs().double() * 2.0 ** -4 + x.abs().double().amax() * 2.0 ** -17
+    gu = x.double() @ w13.double().t()
     a, b = gu.chunk(2, 1)
     s = torch.sigmoid(a.clamp(max=limit))
-    dh = dy.double().cpu() @ w2.double().cpu()
+    dh = dy.double() @ w2.double()
     slope = (s * (1 + a.clamp(max=limit) * (1 - s))).abs()
     size = torch.cat((dh.abs() * b.abs().clamp(max=limit) * slope, dh.abs() * (a.clamp(max=limit) * s).abs()), 1)
     check(got[1], ref[1], bounds[1] * 1.1 + 1.02 * size.t() @ off)

@@ -61,6 +61,28 @@ def test_backward(M, H, I, dt, recompute, dev):
         check(p, q, b, name)
 
 
+# Sizes at which every tile and every way of cutting k is taken by one of the six products: 256 x 256 and
+# 256 x 224 tiles, two 128 x 128 ones to a CU, slices of all tiles and of a last round's.
+LARGE = [(2048, 2304, 3584), (8000, 1800, 1030), (2100, 4096, 2000), (4064, 1024, 3584), (4096, 7168, 256), (900, 2880, 1440),
+         (4090, 2080, 4100)]
+
+
+@pytest.mark.parametrize("M,H,I", LARGE)
+def test_large(M, H, I, dev):
+    x, w13, w2, dy = _inputs(M, H, I, BF, M)
+    out, gu = xk.gated_ffn(x, w13, w2, swiglu_limit=6.0, return_gate_up=True)
+    want, gu_want, bound, gu_bound = ffn_ref(x, w13, w2, 6.0)
+    check(gu, gu_want, gu_bound, "gate_up")
+    check(out, want, bound, "out")
+    del want, gu_want, bound, gu_bound
+    got = xk.gated_ffn_backward(dy, x, w13, w2, gu, swiglu_limit=6.0)
+    want, bounds = ffn_grad_ref(dy, x, w13, w2, 6.0)
+    for name, p, q, b in zip(("grad_x", "grad_w13", "grad_w2"), got, want, bounds):
+        check(p, q, b, name)
+    again = xk.gated_ffn_backward(dy, x, w13, w2, gu, swiglu_limit=6.0)
+    assert all(torch.equal(p, q) for p, q in zip(got, again))
+
+
 def test_gradient_against_differences(dev):
     """The gradients against differences of the 64-bit form along random directions."""
     x, w13, w2, dy = _inputs(40, 96, 48, BF, 5)
@@ -79,7 +101,7 @@ def test_gradient_against_differences(dev):
         plus[n], minus[n] = args[n] + 1e-5 * step, args[n] - 1e-5 * step
         slope = (value(plus) - value(minus)) / 2e-5
         mine = got[n].double().cpu()
-        off = ((bounds[n] + 2.0 ** -8 * mine.abs()) * step.abs()).sum() + 1e-6 * slope.abs() + 1e-6
+        off = ((bounds[n].cpu() + 2.0 ** -8 * mine.abs()) * step.abs()).sum() + 1e-6 * slope.abs() + 1e-6
         assert abs((mine * step).sum() - slope) <= off
 
 
@@ -151,7 +173,7 @@ def test_limits(dev):
             out, gu = xk.gated_ffn(x, w13, w2, swiglu_limit=L, return_gate_up=True)
             want, gw, bound, _ = ffn_ref(x, w13, w2, L)
             check(out, want, bound)
-            past = (gu[:, mine].double().cpu() > L) if gate else gu[:, mine].double().cpu().abs() > L
+            past = (gu[:, mine].double() > L) if gate else gu[:, mine].double().abs() > L
             assert torch.equal(past, gw[:, mine] > L if gate else gw[:, mine].abs() > L)
             for keep in (gu, None):
                 got = xk.gated_ffn_backward(dy, x, w13, w2, keep, swiglu_limit=L)

@@ -7,7 +7,7 @@ import torch
 
 import xkernels_amd as xk
 from tests._dense_ref import GRID, linear_ref, mxfp4_ref, mxfp4_values
-from tests._tuning_ref import check
+from tests._tuning_ref import check, gamma
 
 pytestmark = pytest.mark.gpu
 
@@ -148,6 +148,15 @@ def test_linear(M, K, N, dt, dev):
         assert xk.mxfp4_linear(xq, held).dtype == BF
         for out in TYPES:
             check(xk.mxfp4_linear(x, held, out_dtype=out), want, bound)
+
+
+@pytest.mark.parametrize("M,K,N", [(4096, 2048, 4096), (8000, 520, 7160), (2500, 1024, 5200), (1000, 7168, 1024), (4090, 512, 4100)])
+def test_linear_large(M, K, N, dev):
+    """Every tile and way of cutting k."""
+    x, w = xk.mxfp4_quantize(_values((M, K), BF, 1)), xk.mxfp4_quantize(_values((N, K), BF, 2) / K ** 0.5)
+    xv, wv = mxfp4_values(x).cuda(), mxfp4_values(w).cuda()
+    want = xv @ wv.t()
+    check(xk.mxfp4_linear(x, w), want, gamma(K) * (xv.abs() @ wv.abs().t()))
 
 
 def test_linear_far_scales(dev):

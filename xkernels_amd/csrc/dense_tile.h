@@ -171,7 +171,7 @@ template <Form F, Lay L, int ROWS, int WAVES, int PAIR = 0> struct Loader {
 template <int ROWS, int WAVES> struct ScaleLoader {
   static constexpr int kBytes = ROWS * 8;
   static constexpr int kLoads = ROWS / 32;
-  static_assert(kLoads <= WAVES, "at most a load a wave");
+  static_assert(kLoads == WAVES, "a load a wave");
   i32x4 rsrc;
   int soff, off, word, left;
   __device__ __forceinline__ void init(const Side& s, int64_t r0, int64_t blocks, Range c, int wave, int lane) {
@@ -181,8 +181,8 @@ template <int ROWS, int WAVES> struct ScaleLoader {
     soff = c.first * 8;
     left = min(int((blocks + 3) >> 2), c.end * 2) - c.first * 2;
   }
-  __device__ __forceinline__ void issue(uint32_t lds, int wave) {
-    if (wave < kLoads) to_lds_4(rsrc, lds, off | (word >= left ? kCut : 0), soff);
+  __device__ __forceinline__ void issue(uint32_t lds) {
+    to_lds_4(rsrc, lds, off | (word >= left ? kCut : 0), soff);
     soff += 8;
     left -= 2;
   }
@@ -338,8 +338,8 @@ dense_tile(Product p, EPI epi) {
   auto issue_x = [&](int i) __attribute__((always_inline)) { xl.issue(x_to + x_at, wave, i); };
   auto issue_w = [&](int i) __attribute__((always_inline)) { wl.issue(w_to + w_at, wave, i); };
   auto issue_s = [&]() __attribute__((always_inline)) {
-    xsl.issue(s_to + s_at, wave);
-    wsl.issue(s_to + s_at + XScale::kBytes, wave);
+    xsl.issue(s_to + s_at);
+    wsl.issue(s_to + s_at + XScale::kBytes);
     s_at = s_at == (WRING - 1) * SCALES ? 0 : s_at + SCALES;
   };
   auto next_x = [&]() __attribute__((always_inline)) {
@@ -419,7 +419,7 @@ dense_tile(Product p, EPI epi) {
   // one before it.
   auto publish = [&]() __attribute__((always_inline)) {
     __builtin_amdgcn_sched_barrier(0);
-    constexpr int CHUNK = XI + WI + (FP4 ? 2 : 0);  // (a wave without a load of scales waits for more)
+    constexpr int CHUNK = XI + WI + (FP4 ? 2 : 0);  // a wave's loads of a chunk
     XK_WAIT_VMCNT((WRING - 2) * CHUNK + (XRING > WRING ? XI : 0));
     lds_sync();
     __builtin_amdgcn_sched_barrier(0);

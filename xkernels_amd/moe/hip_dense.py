@@ -25,7 +25,8 @@ MAX_APART = 2_000_000  # values from row to row that the kernels' offsets hold
 
 def _aligned(t: torch.Tensor, n: int = 16) -> torch.Tensor:
     """Contiguous, from an address that the kernels' loads can start at."""
-    t = t.contiguous()
+    if not t.is_contiguous():
+        return t.contiguous()
     return t if t.data_ptr() % n == 0 else t.clone()
 
 
@@ -108,10 +109,10 @@ def gated_ffn_backward_hip(grad_out: torch.Tensor, x: torch.Tensor, w13: torch.T
 
 def _check_held(op: str, name: str, held) -> tuple[torch.Tensor, torch.Tensor]:
     c, s = held
-    if c.dtype != torch.uint8 or s.dtype != torch.uint8 or c.dim() < 1 or c.dim() != s.dim():
+    cs, ss = c.shape, s.shape
+    if c.dtype != torch.uint8 or s.dtype != torch.uint8 or len(ss) == 0 or cs[:-1] != ss[:-1] or cs[-1] != 16 * ss[-1]:
         raise RuntimeError(f"{op}: {name} must be uint8 codes [..., 16 * blocks] and uint8 scales [..., blocks], got "
-                           f"{c.dtype} {list(c.shape)}, {s.dtype} {list(s.shape)}")
-    _shape(op, f"{name}'s codes", c, (*s.shape[:-1], s.shape[-1] * 16))
+                           f"{c.dtype} {list(cs)}, {s.dtype} {list(ss)}")
     return _aligned(c), _aligned(s, 4)
 
 
@@ -188,10 +189,10 @@ def mxfp4_linear_hip(x: torch.Tensor | Mxfp4, weight: Mxfp4, bias: torch.Tensor 
         if bias.dtype != out_dtype:
             raise RuntimeError(f"{op}: bias is {bias.dtype}, the output {out_dtype}")
         bias = bias.contiguous()
-    nbytes = _bytes("xk_mxfp4_linear_workspace_bytes", M, K, N)
-    scratch = xr.new_empty(nbytes, dtype=torch.uint8)
+    nbytes = _bytes("xk_mxfp4_linear_workspace_bytes", M, K, N)  # 0 for few rows
+    scratch = xr.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _lib.call("xk_mxfp4_linear", xr.data_ptr(), dt, ldx, _ptr(x_scales), M, K, wc.data_ptr(), ws.data_ptr(), N,
-              _ptr(bias), out.data_ptr(), odt, scratch.data_ptr(), nbytes, _stream(i))
+              _ptr(bias), out.data_ptr(), odt, _ptr(scratch), nbytes, _stream(i))
     return out
 
 
