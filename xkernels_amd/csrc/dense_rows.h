@@ -78,7 +78,7 @@ template <Form F, typename SRC, bool PAIRED, typename EPI>
 __global__ void __launch_bounds__(kRowWaves * 64)
 dense_rows(Rows x, Rows w, int64_t M, int64_t N, int64_t K, int64_t x_values, EPI epi) {
   constexpr bool FP4 = F == Form::kFp4, QUANT = !std::is_void_v<SRC>;
-  constexpr int U = QUANT ? 2 : 4;  // chunks at a time
+  constexpr int MOST = QUANT ? 2 : 4;  // chunks at a time
   typedef std::conditional_t<QUANT, SRC, uint16_t> S;
   __shared__ f32x4 sums[kRowWaves][64];
   const int lane = threadIdx.x & 63, wave = uniform(int(threadIdx.x) >> 6), c = lane & 15, q = lane >> 4;
@@ -116,11 +116,12 @@ dense_rows(Rows x, Rows w, int64_t M, int64_t N, int64_t K, int64_t x_values, EP
   };
   int chunk = wave;
   // U chunks: all their loads, then their products
-  for (; chunk + (U - 1) * kRowWaves < full; chunk += U * kRowWaves) {
+  auto batch = [&](auto COUNT) __attribute__((always_inline)) {
+    constexpr int U = decltype(COUNT)::value;
     Blocks wv[U];
+    std::conditional_t<QUANT, Values<S>, Blocks> xv[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) load(wp, wsp, chunk + u * kRowWaves, wv[u]);
-    std::conditional_t<QUANT, Values<S>, Blocks> xv[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if constexpr (QUANT) load_values(xp, chunk + u * kRowWaves, xv[u]);
@@ -131,9 +132,12 @@ dense_rows(Rows x, Rows w, int64_t M, int64_t N, int64_t K, int64_t x_values, EP
       if constexpr (QUANT) math(wv[u], quantised(xv[u]));
       else math(wv[u], xv[u]);
     }
-  }
-  // what is left, a chunk at a time: whole ones and the short one
-  for (; chunk < all; chunk += kRowWaves) {
+    chunk += U * kRowWaves;
+  };
+  while (chunk + (MOST - 1) * kRowWaves < full) batch(std::integral_constant<int, MOST>{});
+  if (MOST > 2 && chunk + kRowWaves < full) batch(std::integral_constant<int, 2>{});
+  if (chunk < full) batch(std::integral_constant<int, 1>{});
+  if (chunk < all) {  // the row's short chunk
     Blocks wv, xv;
     const int64_t k = int64_t(chunk) * kChunk + q * 32;
     auto load_end = [&](const char* row, const uint8_t* s, Blocks& o) __attribute__((always_inline)) {
