@@ -78,7 +78,7 @@ template <Form F, typename SRC, bool PAIRED, typename EPI>
 __global__ void __launch_bounds__(kRowWaves * 64)
 dense_rows(Rows x, Rows w, int64_t M, int64_t N, int64_t K, int64_t x_values, EPI epi) {
   constexpr bool FP4 = F == Form::kFp4, QUANT = !std::is_void_v<SRC>;
-  constexpr int MOST = QUANT ? 2 : 4;  // chunks at a time
+  constexpr int MOST = QUANT ? 2 : 8;  // chunks at a time
   typedef std::conditional_t<QUANT, SRC, uint16_t> S;
   __shared__ f32x4 sums[kRowWaves][64];
   const int lane = threadIdx.x & 63, wave = uniform(int(threadIdx.x) >> 6), c = lane & 15, q = lane >> 4;
@@ -135,6 +135,7 @@ dense_rows(Rows x, Rows w, int64_t M, int64_t N, int64_t K, int64_t x_values, EP
     chunk += U * kRowWaves;
   };
   while (chunk + (MOST - 1) * kRowWaves < full) batch(std::integral_constant<int, MOST>{});
+  if (MOST > 4 && chunk + 3 * kRowWaves < full) batch(std::integral_constant<int, 4>{});
   if (MOST > 2 && chunk + kRowWaves < full) batch(std::integral_constant<int, 2>{});
   if (chunk < full) batch(std::integral_constant<int, 1>{});
   if (chunk < all) {  // the row's short chunk
