@@ -107,6 +107,9 @@ template <Form F, Lay L, int ROWS, int WAVES, int PAIR = 0> struct Loader {
                                        int64_t half = 0) {
     if constexpr (L == Lay::kRowsOfK) {
       piece = (lane & 7) ^ (lane >> 3);
+      // 4 bits: a lane of step s is to find block 2 q + s, whose scales lie together, where it finds
+      // piece 4 s + q of 16 bits
+      if constexpr (F == Form::kFp4) piece = (piece & 3) * 2 + (piece >> 2);
       // (a row past the last starts past the end, whatever the chunk)
       const uint32_t n = records(((PAIR ? half : s.rows) - 1 - r0) * s.ld + extent);
       rsrc = make_rsrc(s.p + r0 * s.ld, n);
@@ -188,7 +191,8 @@ template <int ROWS, int WAVES> struct ScaleLoader {
   }
 };
 
-// One operand fragment: 16 rows, step S of 2 of a chunk.
+// One operand fragment: 16 rows, step S of 2 of a chunk, of which lane group q has k = 32 S + 8 q .. + 7 (16 bits)
+// or block 2 q + S (4 bits; any order of k will do that both operands share).
 template <Form F, Lay L, int ROWS> struct Reader {
   static constexpr int kPitch = L == Lay::kRowsOfK ? kChunk : 2 * ROWS;
   int at0, at1;  // kRowsOfK: of each step; kColumns: of a unit's first byte, and the way units are permuted
@@ -197,11 +201,8 @@ template <Form F, Lay L, int ROWS> struct Reader {
     const int c = lane & 15, q = lane >> 4;
     unit = row0 >> 4;
     if constexpr (L == Lay::kRowsOfK) {
-      // 16 bits: step s reads piece 4 s + q, 4 bits: block 2 q + s (any order of k will do that
-      // both operands share)
-      const int p0 = F == Form::kFp4 ? 2 * q : q, p1 = F == Form::kFp4 ? 2 * q + 1 : 4 + q;
-      at0 = (row0 + c) * kChunk + ((p0 ^ (c & 7)) << 4);
-      at1 = (row0 + c) * kChunk + ((p1 ^ (c & 7)) << 4);
+      at0 = (row0 + c) * kChunk + ((q ^ (c & 7)) << 4);
+      at1 = (row0 + c) * kChunk + (((4 + q) ^ (c & 7)) << 4);
     } else {
       at0 = (8 * q + (c >> 2)) * kPitch + (c & 3) * 8;
       at1 = ((c >> 2) | (q & 1) << 2) << 5;
