@@ -83,6 +83,22 @@ def test_large(M, H, I, dev):
     assert all(torch.equal(p, q) for p, q in zip(got, again))
 
 
+# Rows of a few values, with lengths a little past whole chunks of 64: the tile's columns are many rows of the
+# operand, and nothing behind its last row may be read, let alone count.
+@pytest.mark.parametrize("M,H,I", [(65, 8, 8), (129, 8, 24), (66, 24, 8), (193, 16, 33), (321, 40, 72), (130, 65, 65)])
+def test_narrow(M, H, I, dev):
+    x, w13, w2, dy = _inputs(M, H, I, BF, M)
+    want, bounds = ffn_grad_ref(dy, x, w13, w2, None)
+    padded = []
+    for t in (x, w13, w2, dy):  # each before a stretch of NaN
+        held = torch.full((t.numel() + 4096,), float("nan"), dtype=t.dtype, device=t.device)
+        held[:t.numel()] = t.reshape(-1)
+        padded.append(held[:t.numel()].view_as(t))
+    x, w13, w2, dy = padded
+    for name, p, q, b in zip(("grad_x", "grad_w13", "grad_w2"), xk.gated_ffn_backward(dy, x, w13, w2), want, bounds):
+        check(p, q, b, name)
+
+
 def test_gradient_against_differences(dev):
     """The gradients against differences of the 64-bit form along random directions."""
     x, w13, w2, dy = _inputs(40, 96, 48, BF, 5)

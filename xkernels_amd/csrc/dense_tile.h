@@ -70,14 +70,14 @@ __device__ __forceinline__ void to_lds_4(i32x4 rsrc, uint32_t lds, int voff, int
                : "memory", "m0");
 }
 
-// Chunks [first, end) of `all` that a slice of k has.
+// Chunks [first, end) of a slice of k.
 struct Range {
-  int first, end, all;
+  int first, end;
 };
 __device__ __forceinline__ Range range_of(int slice, int slices, int chunks) {
   const int share = chunks / slices, rest = chunks - share * slices;
   const int first = slice * share + min(slice, rest);
-  return Range{first, first + share + (slice < rest), chunks};
+  return Range{first, first + share + (slice < rest)};
 }
 
 // Loads one side's chunks. PAIR: the rows of W are gate and up rows of one weight [2 half, k]: of
@@ -94,7 +94,7 @@ template <Form F, Lay L, int ROWS, int WAVES, int PAIR = 0> struct Loader {
   i32x4 rsrc, up;     // up: PAIR's up rows; kColumns: 4 k further
   int soff;           // kRowsOfK: k of the chunk. kColumns: the descriptor moves on
   int left;           // kRowsOfK: pieces of 16 bytes left of a row. kColumns: chunks left,
-  uint32_t last;      // and the records of the last one
+  uint32_t last;      // and the bytes from the last one's start to the tensor's end
   const char* base;
   int64_t step;
   // kColumns: a lane's places 4 k apart differ by no more than that
@@ -126,10 +126,8 @@ template <Form F, Lay L, int ROWS, int WAVES, int PAIR = 0> struct Loader {
       piece = soff = 0;
       base = s.p + r0 * 2 + int64_t(c.first) * kKRows * s.ld;
       step = kKRows * s.ld;
-      // (all that a chunk before the tensor's last reads lies before the tensor's end)
       left = c.end - c.first;
-      last = c.end < c.all ? uint32_t(kCut)
-                           : records((extent - 1 - int64_t(c.end - 1) * kKRows) * s.ld + (s.rows - r0) * 2);
+      last = records((extent - 1 - int64_t(c.end - 1) * kKRows) * s.ld + (s.rows - r0) * 2);
       describe();
 #pragma unroll
       for (int j = 0; j < kOff; ++j) {
@@ -140,7 +138,10 @@ template <Form F, Lay L, int ROWS, int WAVES, int PAIR = 0> struct Loader {
     }
   }
   __device__ __forceinline__ void describe() {
-    const uint32_t n = left > 1 ? uint32_t(kCut) : left == 1 ? last : 0u, four = uint32_t(4 * step / kKRows);
+    // (a chunk with two more behind it reads nothing past the end: of its last k at most 512 bytes from the
+    // tile's first row on, and 64 k and more follow, of 16 bytes at least)
+    const uint32_t four = uint32_t(4 * step / kKRows),
+                   n = left > 2 ? uint32_t(kCut) : left == 2 ? min(last + uint32_t(step), uint32_t(kCut)) : left == 1 ? last : 0u;
     rsrc = make_rsrc(base, n);
     up = make_rsrc(base + four, n > four ? n - four : 0u);
   }
@@ -314,7 +315,7 @@ dense_tile(Product p, EPI epi) {
   };
   auto open = [&](int job) __attribute__((always_inline)) {
     const int lane = lane_again();
-    Range range{0, p.chunks, p.chunks};
+    Range range{0, p.chunks};
     part = job - p.full;
     if (part >= 0) {
       job = p.full + part / p.slices;
