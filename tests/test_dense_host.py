@@ -201,3 +201,9 @@ def test_mxfp4_oracle():
     a, w = torch.randn(6, 64), o.mxfp4_quantize_ref(torch.randn(5, 64))
     want, _ = linear_ref(mxfp4_ref(a)[0], mxfp4_values(w), a[0, :5])
     torch.testing.assert_close(o.mxfp4_linear_ref(a, w, a[0, :5]).double(), want, rtol=1e-5, atol=1e-5)
+
+
+def test_linear_weight_without_scales_is_refused():
+    codes = torch.zeros(8, 32, dtype=torch.uint8)
+    with pytest.raises(RuntimeError, match="Mxfp4"):
+        xk.mxfp4_linear(torch.zeros(2, 64), codes, backend="hip")

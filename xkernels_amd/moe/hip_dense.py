@@ -160,6 +160,8 @@ def mxfp4_linear_hip(x: torch.Tensor | Mxfp4, weight: Mxfp4, bias: torch.Tensor 
     op = "mxfp4_linear"
     quantised = isinstance(x, tuple)
     xt, x_scales = x if quantised else (x, None)
+    if not isinstance(weight, tuple):
+        raise RuntimeError(f"{op}: weight must be an Mxfp4 (codes, scales), got {type(weight).__name__}")
     i = _device(op, xt, x_scales, *weight, bias)
     if i != _current_device():
         return _elsewhere(i, mxfp4_linear_hip, x, weight, bias, out_dtype)
