@@ -23,8 +23,9 @@ def _clamped(g, u, limit):
     return g.clamp(max=limit), u.clamp(-limit, limit), (g <= limit).double(), (u.abs() <= limit).double()
 
 
-def ffn_ref(x, w13, w2, limit=None):
-    """``(out, gate_up, bound of out, bound of gate_up)``."""
+def ffn_ref(x, w13, w2, limit=None, pair=False):
+    """``(out, gate_up, bound of out, bound of gate_up)``; ``pair``: the activations are held with what
+    their rounding left, rounded itself (off by a half step of a half step), in a sum of twice the terms."""
     e, tiny = half_step(x.dtype), _tiny(x.dtype)
     x, w13, w2 = (t.double() for t in (x, w13, w2))
     H, I = w2.shape
@@ -33,9 +34,9 @@ def ffn_ref(x, w13, w2, limit=None):
     s = torch.sigmoid(gc)
     h = gc * s * uc
     h_off = 1.1 * uc.abs() * off[:, :I] + (gc * s).abs() * off[:, I:] + (gc.abs() + 16) * F32 * h.abs()
-    h_off = h_off * (1 + e) + e * h.abs() + tiny
-    out = h @ w2.t()
-    return out, gu, (h_off * (1 + gamma(I)) + gamma(I) * h.abs()) @ w2.abs().t(), off
+    h_off = h_off * (1 + e) + (e * e if pair else e) * h.abs() + tiny
+    out, n = h @ w2.t(), 2 * I if pair else I
+    return out, gu, (h_off * (1 + gamma(n)) + gamma(n) * (1 + e) * h.abs()) @ w2.abs().t(), off
 
 
 def ffn_grad_ref(dy, x, w13, w2, limit=None):

@@ -83,6 +83,14 @@ def test_large(M, H, I, dev):
     assert all(torch.equal(p, q) for p, q in zip(got, again))
 
 
+@pytest.mark.parametrize("dt", [BF, FP16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("M,H,I", [(1, 1024, 2048), (2, 520, 65), (7, 96, 1001), (16, 256, 4100), (3, 8, 1)])
+def test_few_tokens_keep_what_rounding_leaves(M, H, I, dt, dev):
+    x, w13, w2, _ = _inputs(M, H, I, dt, M + 2)
+    want, _, bound, _ = ffn_ref(x, w13, w2, 8.0, pair=True)
+    check(xk.gated_ffn(x, w13, w2, swiglu_limit=8.0), want, bound, "out")
+
+
 # Rows of a few values, with lengths a little past whole chunks of 64: the tile's columns are many rows of the
 # operand, and nothing behind its last row may be read, let alone count.
 @pytest.mark.parametrize("M,H,I", [(65, 8, 8), (129, 8, 24), (66, 24, 8), (193, 16, 33), (321, 40, 72), (130, 65, 65)])

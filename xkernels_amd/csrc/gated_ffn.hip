@@ -6,7 +6,9 @@
 // Each product is a launch of the tile kernel (two with slices of k), or, for up to 16 tokens,
 // of the kernel for few rows; the activation runs in the epilogue of the gate/up product,
 // its gradient in that of dh. h, dg and du are rounded to the type once, as operands of
-// the next product: their roundings add up like those of the outputs themselves.
+// the next product: their roundings add up like those of the outputs themselves (in bf16 outputs are 2.3e-3
+// from 64 bits, their own rounding is 1.7e-3 of that). Up to 16 tokens the forward keeps what
+// h's rounding left as well, for the kernel that has room for it.
 #include <algorithm>
 
 #include "dense_rows.h"
@@ -91,29 +93,37 @@ __device__ __forceinline__ f32x4 load_sums(const float* p, int n) {
 // gate_up [M, 2 I] (either may be null). The sums are kept in fp32: rounded, they would add their
 // errors to every gradient (dW2 then is 3.4e-3 off, with them as they are 2.3e-3, the result's own
 // rounding alone 1.7e-3; the time of a step of 8,192 tokens does not show it).
-template <Form F> struct Gate {
+// LOW: what h's rounding left lies `low` values behind it.
+template <Form F, bool LOW = false> struct Gate {
   static constexpr bool kFetches = false;
   typedef typename num<F>::type T;
   T* h;
   float* gate_up;
   int64_t ldh, I;
   float limit;
+  int64_t low = 0;
   struct Spot {
     T* h;
     float *g, *u;
     int ldh, ldg, left;
     float limit;
+    int64_t low;
     template <bool WHOLE> __device__ __forceinline__ void put(int row, int col, f32x4 gs, f32x4 us) const {
       if (!WHOLE && col >= left) return;
       if (h != nullptr) {
-        four<T> v;
+        four<T> v, rest;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float gc = below(gs[i], limit), uc = within(us[i], limit);
-          v.v[i] = WHOLE || col + i < left ? num<F>::put(gc * sigmoid(gc) * uc) : T(0);
+          const float gc = below(gs[i], limit), uc = within(us[i], limit), a = gc * sigmoid(gc) * uc;
+          v.v[i] = WHOLE || col + i < left ? num<F>::put(a) : T(0);
+          if constexpr (LOW) {  // (of a value past the type's finite ones nothing is left)
+            const float off = a - num<F>::get(v.v[i]);
+            rest.v[i] = col + i < left && fabsf(off) < 1e38f ? num<F>::put(off) : T(0);
+          }
         }
         T* at = h + uint32_t(row * ldh + col);
         store_unaligned(at, v);  // (rows end at a multiple of 8)
+        if constexpr (LOW) store_unaligned(at + low, rest);
         if (!WHOLE && col + 4 >= left && (left & 7) <= 4 && (left & 7) > 0) store_unaligned(at + 4, four<T>{});
       }
       if (g != nullptr) {
@@ -125,7 +135,7 @@ template <Form F> struct Gate {
   };
   __device__ __forceinline__ Spot spot(int64_t m, int64_t j) const {
     float* g = gate_up == nullptr ? nullptr : gate_up + m * 2 * I + j;
-    return Spot{h == nullptr ? nullptr : h + m * ldh + j, g, g + I, int(ldh), int(2 * I), int(I - j), limit};
+    return Spot{h == nullptr ? nullptr : h + m * ldh + j, g, g + I, int(ldh), int(2 * I), int(I - j), limit, low};
   }
 };
 
@@ -261,13 +271,17 @@ int forward(const void* x, int64_t ldx, int64_t M, int64_t H, const void* w13, c
   char* ws = static_cast<char*>(workspace);
   T* h = reinterpret_cast<T*>(ws);
   const int64_t ldh = pad8(I);
-  ws += aligned(M * ldh * 2);
-  const Gate<F> gate{h, static_cast<float*>(gate_up), ldh, I, limit};
   const Store<F> store{static_cast<T*>(out), H, H};
   if (M <= kFewRows) {
+    const int64_t low = M * ldh;
+    const Gate<F, true> gate{h, static_cast<float*>(gate_up), ldh, I, limit, low};
+    Rows hr = rows_of(h, M, ldh);
+    hr.low = low * 2;
     launch_rows<F, void, true>(rows_of(x, M, ldx), rows_of(w13, 2 * I, H), M, I, H, 0, gate, stream);
-    launch_rows<F, void, false>(rows_of(h, M, ldh), rows_of(w2, H, I), M, H, I, 0, store, stream);
+    launch_rows<F, Both, false>(hr, rows_of(w2, H, I), M, H, I, 0, store, stream);
   } else {
+    ws += aligned(M * ldh * 2);
+    const Gate<F> gate{h, static_cast<float*>(gate_up), ldh, I, limit};
     Copies copies;
     const Matrix xm = take(x, M, H, ldx, ws, copies), m13 = take(w13, 2 * I, H, H, ws, copies),
                  m2 = take(w2, H, I, I, ws, copies), hm{h, M, I, ldh};
@@ -324,7 +338,7 @@ int64_t sums_of(int64_t M, int64_t N, int64_t k, bool paired) {
 }  // namespace
 
 int64_t gated_ffn_workspace_bytes(int64_t M, int64_t H, int64_t I) {
-  const int64_t h = aligned(M * pad8(I) * 2);
+  const int64_t h = aligned(M * pad8(I) * (M <= kFewRows ? 4 : 2));
   if (M <= kFewRows) return h;
   return h + taken_bytes(M, H) + taken_bytes(2 * I, H) + taken_bytes(H, I) +
          std::max(sums_of(M, I, pad8(H), true), sums_of(M, H, pad8(I), false));
