@@ -84,7 +84,7 @@ def test_large(M, H, I, dev):
 
 
 @pytest.mark.parametrize("dt", [BF, FP16], ids=["bf16", "fp16"])
-@pytest.mark.parametrize("M,H,I", [(1, 1024, 2048), (2, 520, 65), (7, 96, 1001), (16, 256, 4100), (3, 8, 1)])
+@pytest.mark.parametrize("M,H,I", [(1, 1024, 2048), (2, 520, 65), (7, 96, 1001), (8, 256, 4100), (3, 8, 1)])
 def test_few_tokens_keep_what_rounding_leaves(M, H, I, dt, dev):
     x, w13, w2, _ = _inputs(M, H, I, dt, M + 2)
     want, _, bound, _ = ffn_ref(x, w13, w2, 8.0, pair=True)

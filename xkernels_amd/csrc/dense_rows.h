@@ -9,8 +9,12 @@
 //     theirs go nowhere.
 //   * Rows start at any address; only a row's last, short chunk is read by the value.
 //   * MXFP4: activations in 16 or 32 bits are quantised on the way, a lane its blocks.
-//   * 16 bits: X may be a pair of values, a value and what its rounding left, which costs nothing where
-//     the weights' bytes are what counts (one token, 7168 x 2048: 18.9 us either way).
+//   * Up to 8 rows X may be pairs of values, each with what its rounding left, as rows 8 to 15 of
+//     the same operands: no more loads and products. (7168 x 2048, weights from memory: one token 21.3
+//     -> 21.7 us, 8 tokens 24.5 -> 26.5; with the rest as an operand of its own 23.0 and 27.5, and 16 tokens
+//     28.8 -> 32.9.)
+//   * The order of a turn's loads and products is the compiler's, which takes 62 registers: all loads ahead of the
+//     products take 154, and fewer waves, and were slower (23.0 -> 24.6 us).
 #pragma once
 
 #include "dense_tile.h"
@@ -22,7 +26,7 @@ namespace dense {
 constexpr int kRowWaves = 8;
 
 // Where rows' values lie: `ld` bytes apart, of MXFP4 codes with scales, or of values to quantise, or
-// of pairs, whose second parts lie `low` bytes behind the first ones.
+// of pairs, whose second parts lie `low` bytes behind the first ones (0: no pairs).
 struct Rows {
   const char* p;
   int64_t ld, rows;
@@ -75,14 +79,13 @@ template <typename SRC> __device__ __forceinline__ Blocks quantised(const Values
   return r;
 }
 
-struct Both {};
-// F: of W. SRC: void where X is of F too, Both where it is pairs, else the type of values that are quantised.
+// F: of W. SRC: void where X is of F too, else the type of values that are quantised.
 // K: 16-bit values, or MXFP4 blocks, of a row; `x_values`: the values of a row that are quantised.
 template <Form F, typename SRC, bool PAIRED, typename EPI>
 __global__ void __launch_bounds__(kRowWaves * 64)
 dense_rows(Rows x, Rows w, int64_t M, int64_t N, int64_t K, int64_t x_values, EPI epi) {
-  constexpr bool FP4 = F == Form::kFp4, BOTH = std::is_same_v<SRC, Both>, QUANT = !std::is_void_v<SRC> && !BOTH;
-  constexpr int MOST = QUANT ? 2 : BOTH ? 4 : 8;  // chunks at a time
+  constexpr bool FP4 = F == Form::kFp4, QUANT = !std::is_void_v<SRC>;
+  constexpr int MOST = QUANT ? 2 : 8;  // chunks at a time
   typedef std::conditional_t<QUANT, SRC, uint16_t> S;
   __shared__ f32x4 sums[kRowWaves][64];
   const int lane = threadIdx.x & 63, wave = uniform(int(threadIdx.x) >> 6), c = lane & 15, q = lane >> 4;
@@ -91,8 +94,9 @@ dense_rows(Rows x, Rows w, int64_t M, int64_t N, int64_t K, int64_t x_values, EP
   const int64_t wr = PAIRED ? min(n0 + (c & 7), N - 1) + (c >= 8 ? N : 0) : min(n0 + c, N - 1);
   const char* wp = w.p + wr * w.ld;
   const uint8_t* wsp = FP4 ? w.s + wr * w.lds : nullptr;
-  const int64_t xr = min(int64_t(c), M - 1);
-  const char* xp = x.p + xr * x.ld;
+  const bool both = x.low != 0;
+  const int64_t xr = min(int64_t(both ? c & 7 : c), M - 1);
+  const char* xp = x.p + xr * x.ld + (c >= 8 ? x.low : 0);
   const uint8_t* xsp = FP4 && !QUANT ? x.s + xr * x.lds : nullptr;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 
@@ -124,20 +128,17 @@ dense_rows(Rows x, Rows w, int64_t M, int64_t N, int64_t K, int64_t x_values, EP
     constexpr int U = decltype(COUNT)::value;
     Blocks wv[U];
     std::conditional_t<QUANT, Values<S>, Blocks> xv[U];
-    Blocks xl[BOTH ? U : 1];
 #pragma unroll
     for (int u = 0; u < U; ++u) load(wp, wsp, chunk + u * kRowWaves, wv[u]);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if constexpr (QUANT) load_values(xp, chunk + u * kRowWaves, xv[u]);
       else load(xp, xsp, chunk + u * kRowWaves, xv[u]);
-      if constexpr (BOTH) load(xp + x.low, xsp, chunk + u * kRowWaves, xl[u]);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if constexpr (QUANT) math(wv[u], quantised(xv[u]));
       else math(wv[u], xv[u]);
-      if constexpr (BOTH) math(wv[u], xl[u]);
     }
     chunk += U * kRowWaves;
   };
@@ -168,10 +169,6 @@ dense_rows(Rows x, Rows w, int64_t M, int64_t N, int64_t K, int64_t x_values, EP
       load_end(xp, xsp, xv);
     }
     math(wv, xv);
-    if constexpr (BOTH) {
-      load_end(xp + x.low, xsp, xv);
-      math(wv, xv);
-    }
   }
 
   sums[wave][lane] = acc;
@@ -183,12 +180,14 @@ dense_rows(Rows x, Rows w, int64_t M, int64_t N, int64_t K, int64_t x_values, EP
     for (int v = 1; v < kRowWaves; ++v) t += sums[v][at];
     return t;
   };
-  finish<EPI, PAIRED>(epi.spot(0, n0), c, q * 4, total(lane), PAIRED ? total((lane + 32) & 63) : f32x4{});
+  f32x4 t = total(lane);
+  if (both) t += total(lane + 8);
+  finish<EPI, PAIRED>(epi.spot(0, n0), c, q * 4, t, PAIRED ? total((lane + 32) & 63) : f32x4{});
 }
 
 // More rows are cheaper in tiles with slices of k (32 x 4096 x 4096: 10 and 4 us, where two row
 // tiles here took 15).
-constexpr int64_t kFewRows = 16;
+constexpr int64_t kFewRows = 16, kPairRows = 8;
 
 template <Form F, typename SRC, bool PAIRED, typename EPI>
 void launch_rows(const Rows& x, const Rows& w, int64_t M, int64_t N, int64_t K, int64_t x_values, const EPI& epi,

@@ -630,7 +630,8 @@ inline int64_t sums_bytes(const Plan& plan) {
   return plan.slices > 1 ? plan.rest * plan.slices * plan.rows * plan.cols * 4 : 0;
 }
 
-// The cheapest of the tiles and slices, in microseconds as measured (16 bits; MXFP4):
+// The cheapest of the tiles and slices, in microseconds as measured (16 bits; MXFP4; the 16-bit
+// figures with loads spread over whole steps: the present order takes 2 to 6 % off):
 //   * 256 x 256, a workgroup a CU: 1.47 (2.3) a chunk, however many CUs are busy
 //     (8192 x 4096 x 7168: 333 us; 4096 x 4096 x 7168 in 4 bits: 67);
 //   * 256 x 224 takes 0.96 of that, and fewer rounds where it divides the columns better

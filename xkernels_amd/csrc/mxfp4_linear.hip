@@ -1,7 +1,12 @@
 // The product of two MXFP4 operands: out[m, n] = sum over blocks b of 2^(sx + sw) times the
 // block's sum of e2m1 products (+ bias[n]), in fp32 on the scaled matrix instructions,
 // rounded once. Up to 16 rows are one launch, which quantises activations in 16 or 32 bits as it
-// reads them; of more rows they are quantised first, in a pass of their own.
+// reads them; of more rows they are quantised first, in a pass of their own: tiles that did it would
+// read four times the bytes, once for every column of tiles.
+//
+// bf16 in and out, the quantising pass included: one row 7168 -> 4096 8.4 us (its launch; 16 MB), 4,096 rows
+// 73 to 77 (3.1 to 3.3 PFLOP/s; the way from L2 to LDS, the matrix unit is busy half the time), 16,384 rows
+// 2048 -> 7168 171 to 178 (2.8; tiles of 8 chunks, 235 MB of results).
 #include <algorithm>
 
 #include "dense_rows.h"
