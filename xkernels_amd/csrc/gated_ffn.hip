@@ -11,8 +11,8 @@
 // h's rounding left as well, in operand rows that would be empty: outputs are 1.7e-3 off.
 //
 // bf16, 7168 x 2048: one token 19 us (88 MB at 4.6 TB/s, two launches), 4,096 tokens 279 to 292 (1.24 to 1.29
-// PFLOP/s, power and the way from L2 to LDS), forward and gradients of 8,192 tokens 1,755 to 1,827
-// (1.18 to 1.23); 64 tokens of 4096 x 2048 29 us, in four dependent launches.
+// PFLOP/s, power and the way from L2 to LDS), forward and gradients of 8,192 tokens 1,749 to 1,827
+// (1.18 to 1.24); 64 tokens of 4096 x 2048 29 us, in four dependent launches.
 #include <algorithm>
 
 #include "dense_rows.h"
