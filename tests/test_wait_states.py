@@ -1,6 +1,7 @@
 """The built library's gfx950 code, disassembled: direct-to-LDS loads are written in inline assembly, in
 which the compiler adds no wait states. A load of that kind needs one behind the scalar write of M0, which
-holds its LDS address."""
+holds its LDS address, and, as every load, five behind a vector instruction that wrote a scalar register it
+reads (a value made uniform, or one brought back from where registers had run out)."""
 from __future__ import annotations
 
 import re
@@ -84,3 +85,25 @@ def test_wait_states_behind_m0():
     assert loads
     bad = [(a, b[-1]) for a, b in loads if _since(b, lambda line: re.match(r"s_\w+ m0,", line)) < 1]
     assert not bad, f"{len(bad)} of {len(loads)} loads directly behind a write of M0, the first: {bad[0]}"
+
+
+def _scalars(text: str) -> set[str]:
+    """The scalar registers that operands name."""
+    found = {"vcc"} if "vcc" in text else set()
+    for first, last, one in re.findall(r"\bs\[(\d+):(\d+)\]|\bs(\d+)\b", text):
+        found |= {f"s{n}" for n in (range(int(first), int(last) + 1) if first else (int(one),))}
+    return found
+
+
+def _written_by_vector(line: str) -> set[str]:
+    """The scalar registers that a vector instruction writes (its first or, of a carry, second operand)."""
+    name, _, operands = line.partition(" ")
+    if not name.startswith("v_"):
+        return set()
+    return _scalars(",".join(operands.split(",")[:2 if "_co_" in name or "div_scale" in name else 1]))
+
+
+def test_wait_states_behind_scalars_of_vector_instructions():
+    loads = _loads()
+    bad = [(a, b) for a, b in loads if _since(b, lambda line: _written_by_vector(line) & _scalars(a)) < 5]
+    assert not bad, f"{len(bad)} of {len(loads)} loads, the first: {bad[0]}"

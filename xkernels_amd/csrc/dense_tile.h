@@ -55,16 +55,16 @@ __device__ __forceinline__ uint32_t records(int64_t bytes) {
 }
 
 // Direct-to-LDS loads: lane i's 16 (4) bytes from voff + soff land at LDS address `lds` + 16 i
-// (4 i), zeros where they are past the buffer. Inline assembly with its wait state, as dma_16 is,
+// (4 i), zeros where they are past the buffer. Inline assembly with its wait states, as dma_16 is,
 // and the LDS address as the number that it is. The kernel waits for them itself.
 __device__ __forceinline__ void to_lds_16(i32x4 rsrc, uint32_t lds, int voff, int soff) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
                : "s"(uniform(lds)), "v"(voff), "s"(rsrc), "s"(uniform(soff))
                : "memory", "m0");
 }
 __device__ __forceinline__ void to_lds_4(i32x4 rsrc, uint32_t lds, int voff, int soff) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, %3 offen lds"
                :
                : "s"(uniform(lds)), "v"(voff), "s"(rsrc), "s"(uniform(soff))
                : "memory", "m0");

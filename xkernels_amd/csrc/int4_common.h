@@ -36,11 +36,12 @@ __device__ __forceinline__ i32x4 make_rsrc(const void* base, uint32_t bytes) {
 // at lds + 16 i. Issued as inline assembly so that the compiler does not make
 // unrelated LDS reads wait for it; the kernel waits for these loads itself
 // (XK_WAIT_VMCNT) before it reads the buffer. Lanes out of the buffer's range
-// land zeros. The load reads M0 (its LDS address) as written before only after a wait
-// state, which the compiler does not put into assembly that it is given.
+// land zeros. The load needs one wait state behind the write of M0 (its LDS address),
+// and five behind a vector instruction that wrote its scalar operands (uniform()'s, or
+// a spilled register's return); the compiler puts none into assembly that it is given.
 __device__ __forceinline__ void dma_16(i32x4 rsrc, const void* lds, int voff, int soff) {
   const uint32_t m0 = uniform(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)));
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
                : "s"(m0), "v"(voff), "s"(rsrc), "s"(uniform(soff))
                : "memory", "m0");
