@@ -181,7 +181,11 @@ dense_rows(Rows x, Rows w, int64_t M, int64_t N, int64_t K, int64_t x_values, EP
     return t;
   };
   f32x4 t = total(lane);
-  if (both) t += total(lane + 8);
+  if (both) {  // (what is not finite comes from the first parts or from W, which has it in both sums)
+    const f32x4 rest = total(lane + 8);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = fabsf(t[i]) < __builtin_inff() ? t[i] + rest[i] : t[i];
+  }
   finish<EPI, PAIRED>(epi.spot(0, n0), c, q * 4, t, PAIRED ? total((lane + 32) & 63) : f32x4{});
 }
 
