@@ -24,9 +24,9 @@ class Mxfp4(NamedTuple):
 
 def mxfp4_quantize(x: torch.Tensor, *, backend: Backend | str = "auto") -> Mxfp4:
     """``x [..., K]`` (bf16, fp16 or fp32) in 4 bits. A block's scale is the least power of two
-    with which none of its values passes 6; values round to nearest even, off by at most a
-    sixth of themselves or, below the scale, a quarter of it. A block with an infinity or a
-    NaN becomes NaN. No autograd graph is recorded (a warning, once, where ``x`` requires a
+    with which none of its values passes 6; values round to nearest even, off by at most a fifth of
+    themselves or, below the scale, a quarter of it. A block with an infinity or a NaN becomes
+    NaN. No autograd graph is recorded (a warning, once, where ``x`` requires a
     gradient)."""
     return dispatch("mxfp4_quantize", x, backend=backend)
 
