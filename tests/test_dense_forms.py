@@ -2,6 +2,8 @@
 tested with, on the CPU."""
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 import xkernels_amd as xk
@@ -21,3 +23,12 @@ def test_mxfp4_error():
     row[0, :4] = torch.tensor([6.0, 5.0, 2.5, 1.25])
     assert o._values(*o.mxfp4_quantize_ref(row))[0, :4].tolist() == [6.0, 4.0, 2.0, 1.0]
     assert "off by at most a fifth of" in " ".join(xk.mxfp4_quantize.__doc__.split())
+
+
+def test_the_least_limits_still_clamp():
+    """A limit that fp32 would hold as 0, which means none."""
+    from xkernels_amd.moe.hip_dense import _limit
+
+    for limit in (5e-324, 1e-50, 2.0 ** -150, 2.0 ** -149, 1e-40, 7.0):
+        assert 0 < ctypes.c_float(_limit("gated_ffn", limit)).value <= max(limit, 2.0 ** -149) * 1.001
+    assert [_limit("gated_ffn", v) for v in (None, 0.0, -1.0, -5e-324)] == [0.0] * 4

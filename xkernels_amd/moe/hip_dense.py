@@ -21,6 +21,7 @@ from .mxfp4_linear import Mxfp4
 _FFN_DT = {torch.bfloat16: _lib.XK_DT_BF16, torch.float16: _lib.XK_DT_FP16}
 BLOCK = 32
 MAX_APART = 2_000_000  # values from row to row that the kernels' offsets hold
+LEAST = 2.0 ** -149  # of fp32's positive numbers (a limit of 0 means none)
 
 
 def _aligned(t: torch.Tensor, n: int = 16) -> torch.Tensor:
@@ -61,7 +62,7 @@ def _limit(op: str, limit: float | None) -> float:
     limit = 0.0 if limit is None else float(limit)
     if limit != limit:
         raise RuntimeError(f"{op}: swiglu_limit is NaN")
-    return max(limit, 0.0)
+    return max(limit, LEAST) if limit > 0 else 0.0
 
 
 def gated_ffn_hip(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, swiglu_limit: float | None = None,
