@@ -332,7 +332,8 @@ int xk_act_restore(const uint8_t* values, const uint8_t* scales, int64_t M, int6
  * x [M, hidden] with rows ldx apart, w13 [2 ispp, hidden] (rows gate, then up) and
  * w2 [hidden, ispp] contiguous, out [M, hidden] contiguous, one dtype (bf16 | fp16);
  * swiglu_limit L <= 0: no clamp. gate_up fp32 [M, 2 ispp] (nullable) receives g and u.
- * fp32 sums; h is rounded to dtype. x, w13 and w2
+ * fp32 sums; h is rounded to dtype (M <= 8: held as two values of it), in fp16 to an infinity
+ * past 65,504. x, w13 and w2
  * are 16-byte aligned, ldx a multiple of 8 where hidden is, and at most 2,000,000;
  * hidden <= 1,000,000, ispp <= 500,000, M < 2^29. workspace is 256-byte aligned.
  * ------------------------------------------------------------------------- */
@@ -344,7 +345,9 @@ int xk_gated_ffn(const void* x, int32_t dtype, int64_t ldx, int64_t M, int64_t h
 /* Gradients of the above for grad_out [M, hidden] (rows ldg apart, as x): grad_x [M, hidden],
  * grad_w13 [2 ispp, hidden], grad_w2 [hidden, ispp] of dtype, contiguous. gate_up as the
  * forward left it, or NULL: computed again (`recompute` of the size query). The clamps pass the
- * gradient where g <= L and |u| <= L. M = 0 gives weights' gradients of zero. */
+ * gradient where g <= L and |u| <= L. fp32 sums; h and the gradients of g and u are rounded to
+ * dtype between the products (fp16: infinities past 65,504, 0 below 3e-8). M = 0 gives weights'
+ * gradients of zero. */
 int64_t xk_gated_ffn_backward_workspace_bytes(int64_t M, int64_t hidden, int64_t ispp,
                                               int32_t recompute);
 int xk_gated_ffn_backward(const void* grad_out, int32_t dtype, int64_t ldg, const void* x,

@@ -636,8 +636,9 @@ inline int64_t sums_bytes(const Plan& plan) {
 //     (8192 x 4096 x 7168: 333 us; 4096 x 4096 x 7168 in 4 bits: 67);
 //   * 256 x 224 takes 0.96 of that, and fewer rounds where it divides the columns better
 //     (8192 x 7168 x 4096, 4 rounds of either: 376 us, with 256 x 256 391);
-//   * 128 x 128: two workgroups a CU 0.88 (1.7) a chunk each, one alone 0.75, with more
-//     places in LDS (8192 x 4096 x 7168: 392 us; 512 x 4096 x 4096: 39 us, where 256 x 256 takes 98);
+//   * 128 x 128: two workgroups a CU 0.88 (1.7) a chunk each, one alone 0.75 (0.77), with more
+//     places in LDS (8192 x 4096 x 7168: 392 us; 512 x 4096 x 4096: 39 us, where 256 x 256 takes 98; 2048 x 2048 in
+//     4 bits, 28 chunks 28.6 us, 8 chunks 13.2);
 //   * slices of k, for all tiles where they leave CUs idle or for those of the last round: the
 //     sums written and read at 3 TB/s, and another launch of 4 us and half a one for each slice
 //     (64 x 4096 x 4096: 30 us, with 8 slices 11 and 4; 64 x 4096 x 2048: 4 slices 11 and 4, 8 slices

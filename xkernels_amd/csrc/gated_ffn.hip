@@ -8,9 +8,11 @@
 // its gradient in that of dh. h, dg and du are rounded to the type once, as operands of
 // the next product: their roundings add up like those of the outputs themselves (in bf16 outputs are 2.3e-3
 // from 64 bits, their own rounding is 1.7e-3 of that). Up to 8 tokens the forward keeps what
-// h's rounding left as well, in operand rows that would be empty: outputs are 1.7e-3 off.
+// h's rounding left as well, in operand rows that would be empty: outputs are 1.7e-3 off. In
+// fp16 all this is so within its range: h, dg and du past 65,504 are infinities, below 6e-5 they lose bits.
 //
-// bf16, 7168 x 2048: one token 19 us (88 MB at 4.6 TB/s, two launches), 4,096 tokens 279 to 292 (1.24 to 1.29
+// bf16, 7168 x 2048: one token 22 us with the weights from memory (88 MB at 4.1 TB/s, two launches; 19 to 20 in calls
+// on the same weights, parts of which are in caches then), 4,096 tokens 279 to 292 (1.24 to 1.29
 // PFLOP/s, power and the way from L2 to LDS), forward and gradients of 8,192 tokens 1,749 to 1,827
 // (1.18 to 1.24); 64 tokens of 4096 x 2048 29 us, in four dependent launches.
 #include <algorithm>

@@ -5,8 +5,9 @@
 // read four times the bytes, once for every column of tiles.
 //
 // bf16 in and out, the quantising pass included: one row 7168 -> 4096 8.4 us (its launch; 16 MB), 4,096 rows
-// 73 to 78 (3.1 to 3.3 PFLOP/s; the way from L2 to LDS, the matrix unit is busy half the time), 16,384 rows
-// 2048 -> 7168 171 to 178 (2.8; tiles of 8 chunks, 235 MB of results).
+// 73 to 78 (3.1 to 3.3 PFLOP/s; the way from L2 to LDS: the scales leave X two places there, as W has, so a
+// chunk's barrier waits for every load, and the matrix unit is busy half the time), 16,384 rows 2048 -> 7168
+// 171 to 178 (2.8; tiles of 8 chunks, 235 MB of results).
 #include <algorithm>
 
 #include "dense_rows.h"

@@ -26,8 +26,8 @@ def mxfp4_quantize(x: torch.Tensor, *, backend: Backend | str = "auto") -> Mxfp4
     """``x [..., K]`` (bf16, fp16 or fp32) in 4 bits. A block's scale is the least power of two
     with which none of its values passes 6; values round to nearest even, off by at most a fifth of
     themselves or, below the scale, a quarter of it. A block with an infinity or a NaN becomes
-    NaN. No autograd graph is recorded (a warning, once, where ``x`` requires a
-    gradient)."""
+    NaN. K is at most 2^22, a call has fewer than 2^33 values. No autograd graph is recorded (a
+    warning, once, where ``x`` requires a gradient)."""
     return dispatch("mxfp4_quantize", x, backend=backend)
 
 
